@@ -649,6 +649,133 @@ gdn_status gdn_attn_forward(gdn_kv* kv, int32_t layer, const uint16_t* q_full, i
 gdn_status gdn_kv_read(gdn_kv* kv, int32_t layer, int32_t slot, uint16_t* k_out, uint16_t* v_out,
                        void* stream);
 
+/* ------------------------------------------------------------------------
+ * The decoder layer's sparse MLP half (qwen3_5.rs:226-311, SwitchMlp :102-160,
+ * SharedExpert :164-222): routing to experts, the experts' 4-bit products, and
+ * the norms around a block. Every call allocates nothing, launches kernels
+ * only and may be captured in a HIP graph.
+ * ------------------------------------------------------------------------ */
+#define GDN_MOE_SOFTMAX 0
+#define GDN_MOE_SIGMOID 1
+
+typedef struct gdn_moe_route_desc {
+  int32_t num_experts;  /* E routed experts, 1 .. 1024                            */
+  int32_t top_k;        /* 1 .. min(E, 32)                                        */
+  int32_t score;        /* GDN_MOE_SOFTMAX or GDN_MOE_SIGMOID                     */
+  int32_t num_groups;   /* divides E, at most 64; 1: no groups                    */
+  int32_t top_groups;   /* groups whose experts stay, 1 .. num_groups             */
+  int32_t group_top;    /* a group's score is the sum of its best 1 or 2 scores   */
+  int32_t renorm;       /* weights of the chosen experts sum to one before scale  */
+  float scale;          /* factor on the routed experts' weights                  */
+  int32_t num_shared;   /* experts E .. E + num_shared - 1 that every token takes, 0 .. 8 */
+  int32_t shared_gate;  /* 1: logit E of a row is their gate (weight sigmoid of it),
+                           0: weight 1                                            */
+  int32_t logits_f32;   /* logits are f32 rather than bf16                        */
+} gdn_moe_route_desc;
+
+/* Choose every token's experts. Row t of logits (T rows, logits_stride elements
+ * apart, E or more columns, E + 1 with shared_gate) holds a logit per expert;
+ * -inf and NaN take an expert out, +inf counts as the largest finite value.
+ * An expert's score is its softmax over the row or its sigmoid, plus bias [E]
+ * f32 (or NULL) for the choice alone; a bias of -inf or NaN takes the expert
+ * out. With num_groups > 1 only experts of the top_groups best groups stay (a
+ * group's score adds the scores it has; a group without any never stays). The
+ * top_k best scores are chosen in descending order, ties to the lowest index;
+ * scores that a bias or a sum of two enters are formed and compared in 64 bits,
+ * others by the logits themselves. ids [T, top_k + num_shared] and weights (f32)
+ * receive the chosen experts and their softmax or sigmoid (without the bias),
+ * renormalised over the chosen if asked for, times scale; where fewer than
+ * top_k are there, id -1 and weight 0. The shared experts follow. Runs on the
+ * current device. */
+gdn_status gdn_moe_route(const gdn_moe_route_desc* desc, const void* logits,
+                         int64_t logits_stride, int32_t T, const float* bias, int32_t* ids,
+                         float* weights, void* stream);
+
+/* The experts: for every token t and column j with expert e = ids[t, j] inside
+ * [0, E),
+ *   out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
+ * each product on MLX 4-bit weights (group 64: scales * q + biases). A column
+ * whose id is outside [0, E) adds nothing; a token without any gets zeros. An
+ * id may appear in several columns of a token. */
+typedef struct gdn_moe gdn_moe;
+
+/* One set of experts, appended to the layer's in order: MLX-format arrays of
+ * `experts` matrices each, gate and up [inner, hidden], down [hidden, inner]
+ * (w uint32 [.., K/8], scales and biases bf16 [.., K/64]). */
+typedef struct gdn_moe_part {
+  int32_t experts;
+  const uint32_t* gate_w;
+  const uint16_t* gate_scales;
+  const uint16_t* gate_biases;
+  const uint32_t* up_w;
+  const uint16_t* up_scales;
+  const uint16_t* up_biases;
+  const uint32_t* down_w;
+  const uint16_t* down_scales;
+  const uint16_t* down_biases;
+} gdn_moe_part;
+
+/* Repack the parts' weights (for example the routed experts, then the shared
+ * one) into one layer of E = sum(experts) <= 4096 on `device`, which owns its
+ * copy (the size of the sources). The sources are only read and may be freed
+ * once this returns (it synchronises `stream`). hidden and inner are multiples
+ * of 128 up to 8192; bits 4, group_size 64. */
+gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const gdn_moe_part* parts,
+                          int32_t group_size, int32_t bits, int32_t device, void* stream,
+                          gdn_moe** out);
+gdn_status gdn_moe_destroy(gdn_moe* moe);
+gdn_status gdn_moe_dims(const gdn_moe* moe, int32_t* hidden, int32_t* inner, int32_t* experts);
+
+/* Bytes of device workspace that gdn_moe_forward needs for calls of up to T
+ * tokens and k columns (non-decreasing in both; bounded: larger calls go in
+ * passes of 262,144 / k tokens). */
+gdn_status gdn_moe_workspace_bytes(const gdn_moe* moe, int32_t T, int32_t k, size_t* bytes);
+
+/* x [T, x_stride] bf16 -> out [T, out_stride] bf16 over the first hidden
+ * columns (others untouched). x: 16-byte aligned, x_stride >= hidden and a
+ * multiple of 8; out: 8-byte aligned, out_stride >= hidden and a multiple of
+ * 4; ids and weights [T, k], k <= 64. workspace: the caller's, 256-byte
+ * aligned, at least gdn_moe_workspace_bytes(T, k); its contents do not matter
+ * before or after, but calls that share one (captured graphs' replays too)
+ * must be ordered. out must not overlap x. T >= 0. */
+gdn_status gdn_moe_forward(const gdn_moe* moe, const uint16_t* x, int64_t x_stride, int32_t T,
+                           int32_t k, const int32_t* ids, const float* weights, uint16_t* out,
+                           int64_t out_stride, void* workspace, size_t workspace_bytes,
+                           void* stream);
+
+/* The seam behind and before a block in general form (gdn_add_rms_norm is the
+ * decoder's own): over n rows
+ *   b      = post_w ? x * rsqrt(mean(x^2) + post_eps) * post_w : x
+ *   h_out  = h + scale * gate * b
+ *   hn     = h_out * rsqrt(mean(h_out^2) + pre_eps) * pre_w
+ * in f32, h_out and hn each rounded once from the f32 values. The block's
+ * output x, the gate, hn and the weights are bf16; h and h_out are bf16, or
+ * f32 with h_f32. Row strides are in elements. */
+#define GDN_GATE_NONE 0
+#define GDN_GATE_ROW 1     /* gate[i * gate_stride], one value a row               */
+#define GDN_GATE_ELEMENT 2 /* gate[i * gate_stride + c]; stride 0: one row for all */
+typedef struct gdn_block_norm_desc {
+  int32_t hidden;       /* multiple of 8, 8 .. 16384                             */
+  int32_t h_f32;
+  int32_t gate;         /* GDN_GATE_*                                             */
+  int32_t gate_sigmoid; /* the gate enters through a sigmoid                      */
+  int32_t unit_offset;  /* norm weights are stored as offsets from one            */
+  float scale;
+  float post_eps;
+  float pre_eps;
+} gdn_block_norm_desc;
+
+/* post_w NULL: no norm of x. pre_w and hn both NULL: no norm of h_out. h_out
+ * may be h, and hn may be x, each with the same stride; other overlaps are not
+ * allowed. Rows are 16-byte aligned with strides that are multiples of 8 and
+ * at least hidden, the weights 16-byte aligned; so is an element gate (its
+ * stride may be 0). Runs on the current device. */
+gdn_status gdn_block_norm(const gdn_block_norm_desc* desc, int32_t n, const void* h,
+                          int64_t h_stride, const uint16_t* x, int64_t x_stride,
+                          const uint16_t* post_w, const uint16_t* gate, int64_t gate_stride,
+                          const uint16_t* pre_w, void* h_out, int64_t h_out_stride, uint16_t* hn,
+                          int64_t hn_stride, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

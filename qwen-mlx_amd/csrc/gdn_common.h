@@ -392,6 +392,73 @@ hipError_t launch_attn(const AttnArgs& a);
 hipError_t launch_kv_gather(const uint16_t* pages, const int32_t* prow, int Hkv, int64_t len,
                             uint16_t* k_out, uint16_t* v_out, hipStream_t s);
 
+// The sparse MLP half (gdn_moe.hip) and the block norm (gdn_norm.hip).
+struct MoeRouteArgs {
+  gdn_moe_route_desc d;
+  const void* logits;      // [T, stride] bf16 or f32
+  int64_t stride;
+  int T;
+  const float* bias;       // [E] or null
+  int32_t* ids;            // [T, top_k + num_shared]
+  float* weights;
+  hipStream_t stream;
+};
+hipError_t launch_moe_route(const MoeRouteArgs& a);
+
+// Packed matrices of all experts, rows in 16-row fragments, k in stages of 128
+// (two groups of 64): weights [expert][fragment][stage][64 lanes] u32x4 in
+// qlinear's nibble order, and {scales, biases} [expert][fragment][stage][16 rows]
+// as two dwords (a bf16 pair, one per group, each).
+struct MoePackArgs {
+  const uint32_t* w;       // [experts, n, k / 8]
+  const uint16_t* s;       // [experts, n, k / 64]
+  const uint16_t* b;
+  int experts, n, k;
+  int frags, fmul, fofs;   // fragment f of the part goes to fmul * f + fofs of frags
+  void* wp;                // of the first expert of the part
+  uint2* sb;
+  hipStream_t stream;
+};
+hipError_t launch_moe_pack(const MoePackArgs& a);
+
+struct MoeArgs {
+  int hidden, inner, experts;
+  const void* w1;          // gate and up fragments in turn
+  const uint2* sb1;
+  const void* w2;          // down
+  const uint2* sb2;
+  const uint16_t* x;       // [T, xs]
+  int64_t xs;
+  int T, k;
+  const int32_t* ids;      // [T, k]
+  const float* weights;
+  uint16_t* out;           // [T, os]
+  int64_t os;
+  void* workspace;         // moe_workspace_bytes(hidden, inner, experts, T, k)
+  hipStream_t stream;
+};
+// Tokens of one pass over the experts; larger calls go in pieces.
+int moe_pass_tokens(int k, int64_t x_stride);
+size_t moe_workspace_bytes(int hidden, int inner, int experts, int T, int k);
+hipError_t launch_moe(const MoeArgs& a);
+
+struct BlockNormArgs {
+  gdn_block_norm_desc d;
+  const void* h;
+  void* h_out;
+  const uint16_t* x;       // the block's output rows
+  int64_t h_stride, h_out_stride, x_stride;
+  const uint16_t* post_w;
+  const uint16_t* gate;
+  int64_t gate_stride;
+  const uint16_t* pre_w;
+  uint16_t* hn;
+  int64_t hn_stride;
+  int n;
+  hipStream_t stream;
+};
+hipError_t launch_block_norm(const BlockNormArgs& a);
+
 // Sets the calling thread's gdn_last_error() message and returns code.
 gdn_status set_error(gdn_status code, const char* msg);
 

@@ -65,6 +65,18 @@ SIGNATURES = {
     "gdn_qlinear_forward_sums": ([_VP, _VP, ctypes.c_int64, _VP, _I32, _VP, ctypes.c_int64, _VP],
                                  ctypes.c_int),
     "gdn_add_rms_norm": ([_VP, _VP, _I32, _I32, _VP, ctypes.c_float, _VP, _VP, _VP], ctypes.c_int),
+    "gdn_moe_route": ([_VP, _VP, ctypes.c_int64, _I32, _VP, _VP, _VP, _VP], ctypes.c_int),
+    "gdn_moe_create": ([_I32, _I32, _I32, _VP, _I32, _I32, _I32, _VP, ctypes.POINTER(_VP)],
+                       ctypes.c_int),
+    "gdn_moe_destroy": ([_VP], ctypes.c_int),
+    "gdn_moe_dims": ([_VP, ctypes.POINTER(_I32), ctypes.POINTER(_I32), ctypes.POINTER(_I32)],
+                     ctypes.c_int),
+    "gdn_moe_workspace_bytes": ([_VP, _I32, _I32, ctypes.POINTER(ctypes.c_size_t)], ctypes.c_int),
+    "gdn_moe_forward": ([_VP, _VP, ctypes.c_int64, _I32, _I32, _VP, _VP, _VP, ctypes.c_int64, _VP,
+                         ctypes.c_size_t, _VP], ctypes.c_int),
+    "gdn_block_norm": ([_VP, _I32, _VP, ctypes.c_int64, _VP, ctypes.c_int64, _VP, _VP,
+                        ctypes.c_int64, _VP, _VP, ctypes.c_int64, _VP, ctypes.c_int64, _VP],
+                       ctypes.c_int),
     "gdn_exec_create": ([_VP, _VP, ctypes.POINTER(_VP)], ctypes.c_int),
     "gdn_exec_destroy": ([_VP], ctypes.c_int),
     "gdn_exec_prefill": ([_VP, ctypes.c_uint64, _VP, _I32, ctypes.POINTER(ctypes.c_uint32)],
@@ -133,6 +145,24 @@ class ExecDesc(ctypes.Structure):
                 ("max_batch", _I32), ("max_prompt", _I32), ("device", _I32),
                 ("num_attn_layers", _I32), ("attn_layers", ctypes.POINTER(ExecAttnLayer)),
                 ("kv", _VP), ("rope_theta", ctypes.c_float), ("rotary_dim", _I32)]
+
+
+class MoeRouteDesc(ctypes.Structure):
+    _fields_ = [("num_experts", _I32), ("top_k", _I32), ("score", _I32), ("num_groups", _I32),
+                ("top_groups", _I32), ("group_top", _I32), ("renorm", _I32),
+                ("scale", ctypes.c_float), ("num_shared", _I32), ("shared_gate", _I32),
+                ("logits_f32", _I32)]
+
+
+class MoePart(ctypes.Structure):
+    _fields_ = [("experts", _I32)] + [(f"{m}_{t}", _VP) for m in ("gate", "up", "down")
+                                      for t in ("w", "scales", "biases")]
+
+
+class BlockNormDesc(ctypes.Structure):
+    _fields_ = [("hidden", _I32), ("h_f32", _I32), ("gate", _I32), ("gate_sigmoid", _I32),
+                ("unit_offset", _I32), ("scale", ctypes.c_float), ("post_eps", ctypes.c_float),
+                ("pre_eps", ctypes.c_float)]
 
 
 class PoolDesc(ctypes.Structure):
@@ -246,6 +276,86 @@ def add_rms_norm(h, d, w, eps, hn, group_sums=None, stream=None):
     n, hidden = h.shape
     _check(load().gdn_add_rms_norm(_ptr(h), _ptr(d), n, hidden, _ptr(w), float(eps), _ptr(hn),
                                    _ptr(group_sums), _stream(stream)))
+
+
+def _is_f32(t, what: str) -> bool:
+    """Whether t holds f32 rather than bf16 (torch.bfloat16 or 16-bit patterns)."""
+    import torch
+    if t.dtype == torch.float32:
+        return True
+    if t.element_size() != 2 or t.dtype == torch.float16:
+        raise ValueError(f"{what} must be float32 or bf16, not {t.dtype}")
+    return False
+
+
+def _typed(t, dtypes, what: str):
+    if t.dtype not in dtypes:
+        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
+    return t
+
+
+def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=None, num_groups=1,
+              top_groups=1, group_top=1, renorm=True, scale=1.0, num_shared=0, shared_gate=False,
+              stream=None):
+    """Experts of every token (gdn_moe_route): logits [T, >= num_experts (+ 1 with
+    shared_gate)] bf16 or f32 rows -> ids int32 and weights f32 [T, top_k + num_shared].
+    score: "softmax" or "sigmoid"; bias f32 [num_experts] moves the choice only."""
+    import torch
+    codes = {"softmax": 0, "sigmoid": 1}
+    if score not in codes:
+        raise ValueError(f"score must be softmax or sigmoid, not {score!r}")
+    lp, ls = _rows(logits)
+    T = logits.shape[0]
+    if logits.shape[1] < num_experts + (1 if shared_gate else 0):
+        raise ValueError("logits hold fewer columns than experts")
+    for t, d, what in ((ids, torch.int32, "ids"), (weights, torch.float32, "weights")):
+        if tuple(_typed(t, (d,), what).shape) != (T, top_k + num_shared):
+            raise ValueError(f"{what} must be [{T}, {top_k + num_shared}]")
+    if bias is not None and _typed(bias, (torch.float32,), "bias").numel() != num_experts:
+        raise ValueError("one bias per expert")
+    d = MoeRouteDesc(num_experts, top_k, codes[score], num_groups, top_groups, group_top,
+                     int(bool(renorm)), float(scale), num_shared, int(bool(shared_gate)),
+                     int(_is_f32(logits, "logits")))
+    _check(load().gdn_moe_route(ctypes.byref(d), lp, ls, T, _ptr(bias), _ptr(ids), _ptr(weights),
+                                _stream(stream)))
+
+
+def block_norm(h, x, h_out=None, hn=None, pre_w=None, pre_eps=1e-6, post_w=None, post_eps=1e-6,
+               gate=None, gate_sigmoid=False, scale=1.0, unit_offset=False, stream=None):
+    """The norms around a block (gdn_block_norm): b = rms_norm(x) * post_w (or x),
+    h_out = h + scale * gate * b, hn = rms_norm(h_out) * pre_w. h, h_out [n, hidden]
+    bf16 or f32 (h_out None: in place), the others bf16; gate [n, 1] or [n, hidden] rows,
+    or [hidden] for one row shared by all; pre_w and hn None: no second norm."""
+    n, hidden = h.shape
+    h_out = h if h_out is None else h_out
+    hp, hs = _rows(h)
+    xp, xs = _rows(x)
+    op, os_ = _rows(h_out)
+    f32 = _is_f32(h, "h")
+    if h_out.dtype != h.dtype or h_out.shape != h.shape or tuple(x.shape) != (n, hidden):
+        raise ValueError("h, x and h_out must have the same shape, h and h_out the same type")
+    np_, ns = (None, 0) if hn is None else _rows(hn)
+    for t, what in ((x, "x"), (hn, "hn"), (gate, "gate"), (post_w, "post_w"), (pre_w, "pre_w")):
+        if t is not None and _is_f32(t, what):
+            raise ValueError(f"{what} must be bf16")
+    if hn is not None and tuple(hn.shape) != (n, hidden):
+        raise ValueError("hn must have h's shape")
+    for w in (post_w, pre_w):
+        if w is not None and w.numel() != hidden:
+            raise ValueError("norm weights hold one value per column")
+    kind, gp, gs = 0, None, 0
+    if gate is not None:
+        if gate.dim() == 1 and gate.shape[0] == hidden:
+            kind, gp, gs = 2, _ptr(gate), 0
+        elif gate.dim() == 2 and tuple(gate.shape) in ((n, 1), (n, hidden)):
+            gp, gs = _rows(gate)
+            kind = 1 if gate.shape[1] == 1 else 2
+        else:
+            raise ValueError("gate must be [n, 1], [n, hidden] or [hidden]")
+    d = BlockNormDesc(hidden, int(f32), kind, int(bool(gate_sigmoid)), int(bool(unit_offset)),
+                      float(scale), float(post_eps), float(pre_eps))
+    _check(load().gdn_block_norm(ctypes.byref(d), n, hp, hs, xp, xs, _ptr(post_w), gp, gs,
+                                 _ptr(pre_w), op, os_, np_, ns, _stream(stream)))
 
 
 class Pool:
@@ -439,6 +549,80 @@ class QLinear:
     def close(self):
         if getattr(self, "handle", None):
             _check(self.lib.gdn_qlinear_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class MoE:
+    """The 4-bit experts of a sparse MLP (gdn_moe_*). parts: sets of experts in id order,
+    each ((gate w, scales, biases), (up ...), (down ...)) of MLX-format device tensors:
+    gate and up w int32 [n, inner, hidden/8] with scales and biases [n, inner, hidden/64],
+    down [n, hidden, inner/8] and [n, hidden, inner/64] (bf16 or their bit patterns)."""
+
+    def __init__(self, hidden: int, inner: int, parts, device: int = 0, stream=None,
+                 group_size: int = 64, bits: int = 4):
+        self.lib = load()
+        self.handle = None
+        arr = (MoePart * len(parts))()
+        for i, part in enumerate(parts):
+            n = int(part[0][0].shape[0])
+            ptrs = []
+            for (w, s, b), (rows, cols) in zip(part, ((inner, hidden), (inner, hidden),
+                                                      (hidden, inner))):
+                if (tuple(w.shape) != (n, rows, cols // 8) or w.element_size() != 4 or
+                        any(tuple(t.shape) != (n, rows, cols // 64) or _is_f32(t, "scales")
+                            for t in (s, b))):
+                    raise ValueError(f"part {i}: expected [{n}, {rows}, {cols}] in 4-bit groups "
+                                     "of 64")
+                ptrs += [_ptr(w), _ptr(s), _ptr(b)]
+            arr[i] = MoePart(n, *ptrs)
+        h = _VP()
+        _check(self.lib.gdn_moe_create(hidden, inner, len(parts), arr, group_size, bits, device,
+                                       _stream(stream), ctypes.byref(h)))
+        self.handle = h
+        self.hidden, self.inner, self.device = hidden, inner, device
+        self.experts = sum(int(p.experts) for p in arr)
+
+    def workspace_bytes(self, T: int, k: int) -> int:
+        n = ctypes.c_size_t()
+        _check(self.lib.gdn_moe_workspace_bytes(self.handle, T, k, ctypes.byref(n)))
+        return n.value
+
+    def workspace(self, T: int, k: int):
+        """A device tensor that serves calls of up to T tokens and k columns, of this
+        layer and every other one with its hidden, inner and expert count."""
+        import torch
+        return torch.empty(self.workspace_bytes(T, k), dtype=torch.uint8,
+                           device=f"cuda:{self.device}")
+
+    def forward(self, x, ids, weights, out, workspace, stream=None):
+        """out[t] = sum_j weights[t, j] * expert ids[t, j] of x[t]; x, out [T, hidden] bf16
+        rows, ids int32 and weights f32 [T, k]; ids outside [0, experts) add nothing."""
+        import torch
+        xp, xs = _rows(x)
+        op, os_ = _rows(out)
+        for t, what in ((x, "x"), (out, "out")):
+            if _is_f32(t, what):
+                raise ValueError(f"{what} must be bf16")
+        T, k = ids.shape
+        if (tuple(x.shape) != (T, self.hidden) or out.shape != x.shape or
+                weights.shape != ids.shape):
+            raise ValueError(f"need x, out [{T}, {self.hidden}] and weights [{T}, {k}]")
+        _typed(ids, (torch.int32,), "ids")
+        _typed(weights, (torch.float32,), "weights")
+        _check(self.lib.gdn_moe_forward(self.handle, xp, xs, T, k, _ptr(ids), _ptr(weights), op,
+                                        os_, _ptr(workspace),
+                                        workspace.numel() * workspace.element_size(),
+                                        _stream(stream)))
+
+    def close(self):
+        if getattr(self, "handle", None):
+            _check(self.lib.gdn_moe_destroy(self.handle))
             self.handle = None
 
     def __del__(self):
