@@ -407,8 +407,8 @@ hipError_t launch_moe_route(const MoeRouteArgs& a);
 
 // Packed matrices of all experts, rows in 16-row fragments, k in stages of 128
 // (two groups of 64): weights [expert][fragment][stage][64 lanes] u32x4 in
-// qlinear's nibble order, and {scales, biases} [expert][fragment][stage][16 rows]
-// as two dwords (a bf16 pair, one per group, each).
+// qlinear's nibble order, and [expert][fragment][stage] 16 rows' scales, then their
+// biases, a dword each (a bf16 pair, one per group).
 struct MoePackArgs {
   const uint32_t* w;       // [experts, n, k / 8]
   const uint16_t* s;       // [experts, n, k / 64]
@@ -416,7 +416,7 @@ struct MoePackArgs {
   int experts, n, k;
   int frags, fmul, fofs;   // fragment f of the part goes to fmul * f + fofs of frags
   void* wp;                // of the first expert of the part
-  uint2* sb;
+  uint32_t* sb;
   hipStream_t stream;
 };
 hipError_t launch_moe_pack(const MoePackArgs& a);
@@ -424,9 +424,9 @@ hipError_t launch_moe_pack(const MoePackArgs& a);
 struct MoeArgs {
   int hidden, inner, experts;
   const void* w1;          // gate and up fragments in turn
-  const uint2* sb1;
+  const uint32_t* sb1;
   const void* w2;          // down
-  const uint2* sb2;
+  const uint32_t* sb2;
   const uint16_t* x;       // [T, xs]
   int64_t xs;
   int T, k;

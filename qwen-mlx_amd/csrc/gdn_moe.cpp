@@ -52,9 +52,9 @@ struct gdn_moe {
   int hidden = 0, inner = 0, experts = 0, device = 0;
   void* base = nullptr;  // one allocation holds the packed arrays
   void* w1 = nullptr;
-  uint2* sb1 = nullptr;
+  uint32_t* sb1 = nullptr;
   void* w2 = nullptr;
-  uint2* sb2 = nullptr;
+  uint32_t* sb2 = nullptr;
 };
 
 namespace {
@@ -177,8 +177,8 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
   char* p = static_cast<char*>(m->base);
   m->w1 = p;
   m->w2 = p + 2 * w;
-  m->sb1 = reinterpret_cast<uint2*>(p + 3 * w);
-  m->sb2 = reinterpret_cast<uint2*>(p + 3 * w + 2 * s);
+  m->sb1 = reinterpret_cast<uint32_t*>(p + 3 * w);
+  m->sb2 = reinterpret_cast<uint32_t*>(p + 3 * w + 2 * s);
   const hipStream_t st = static_cast<hipStream_t>(stream);
   int64_t first = 0;
   for (int i = 0; i < nparts; ++i) {
@@ -187,7 +187,7 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
     a.experts = q.experts;
     a.stream = st;
     auto pack = [&](const uint32_t* wsrc, const uint16_t* ssrc, const uint16_t* bsrc, int n, int k,
-                    int fmul, int fofs, void* wp, uint2* sb) {
+                    int fmul, int fofs, void* wp, uint32_t* sb) {
       a.w = wsrc;
       a.s = ssrc;
       a.b = bsrc;
@@ -197,7 +197,7 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
       a.fofs = fofs;
       a.frags = fmul * (n / 16);
       a.wp = static_cast<char*>(wp) + first * fmul * (terms / 2);
-      a.sb = sb + first * fmul * (terms / 128);
+      a.sb = sb + first * fmul * (terms / 64);
       return gdn::launch_moe_pack(a);
     };
     hipError_t e = pack(q.gate_w, q.gate_scales, q.gate_biases, inner, hidden, 2, 0, m->w1, m->sb1);

@@ -1,8 +1,7 @@
-// gdn_moe.hip -- the sparse MLP half of a decoder layer: routing of tokens to
-// experts and the experts' products on 4-bit weights (SparseMoeBlock,
-// qwen3_5.rs:226-311; SwitchMlp, :102-160).
+// gdn_moe.hip -- the experts' products on 4-bit weights (SwitchMlp,
+// qwen3_5.rs:102-160; SharedExpert, :164-222).
 //
-// Experts. Entry (t, j) of ids [T, k] names expert e = ids[t, j]:
+// Entry (t, j) of ids [T, k] names expert e = ids[t, j]:
 //   h = silu(Wg_e x_t) * (Wu_e x_t),   out_t = sum_j weights[t, j] * Wd_e h.
 // The entries are sorted by expert, the rows of an expert cut into tiles, and
 // a work-group takes one tile through some columns of its expert's matrix.
@@ -15,6 +14,7 @@
 // from the same MFMA against ones. h is rounded once to bf16, the operand type
 // of its product; out is rounded once from the f32 sum over j.
 #include <climits>
+#include <type_traits>
 
 #include "gdn_common.h"
 
@@ -25,194 +25,6 @@ typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
-
-// ---------------------------------------------------------------- router --
-
-__device__ __forceinline__ float wave_max(float v) {
-#pragma unroll
-  for (int off = 32; off > 0; off >>= 1) v = fmaxf(v, __shfl_xor(v, off, 64));
-  return v;
-}
-
-// 1 / (1 + exp(-l)), small values with their relative accuracy
-__device__ __forceinline__ float sigmoid(float l) {
-  const float q = expf(-fabsf(l));
-  return (l < 0.f ? q : 1.f) / (1.f + q);
-}
-
-// its logarithm, also where it underflows
-__device__ __forceinline__ float log_sigmoid(float l) {
-  return fminf(l, 0.f) - log1pf(expf(-fabsf(l)));
-}
-
-// One wave per token, lane L holding experts L R .. L R + R - 1. The score that
-// orders the choice is the logit itself (Key = float) or, where a bias or a sum
-// of two scores enters, the score in f64: f32 would make ties of scores that
-// differ. The best of all lanes' scores is taken top_k times, equal ones by the
-// lower index.
-template <int R, typename Key>
-__global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a) {
-  extern __shared__ double lds[];  // f64 scores per wave when there are groups
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-  const int t = blockIdx.x * 4 + wave;
-  const int E = a.d.num_experts, k = a.d.top_k;
-  const bool here = t < a.T;
-  const int64_t row = (int64_t)min(t, a.T - 1) * a.stride;
-  const Key none = -(Key)INFINITY;
-  constexpr bool kF64 = sizeof(Key) == 8;
-  auto logit = [&](int e) {
-    float v = a.d.logits_f32 ? static_cast<const float*>(a.logits)[row + e]
-                             : bf2f(static_cast<const uint16_t*>(a.logits)[row + e]);
-    if (v != v) v = -INFINITY;
-    return fminf(v, 3.402823466e38f);
-  };
-  float l[R];
-  float m = -INFINITY;
-#pragma unroll
-  for (int r = 0; r < R; ++r) {
-    const int e = lane * R + r;
-    l[r] = e < E ? logit(e) : -INFINITY;
-    m = fmaxf(m, l[r]);
-  }
-  m = wave_max(m);
-  const bool softmax = a.d.score == GDN_MOE_SOFTMAX;
-  Key key[R];
-  if constexpr (kF64) {
-    double sum = 1.0;
-    if (softmax && m > -INFINITY) {
-      sum = 0.0;
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (l[r] > -INFINITY) sum += exp((double)l[r] - (double)m);
-#pragma unroll
-      for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int e = lane * R + r;
-      key[r] = none;
-      if (l[r] > -INFINITY) {
-        key[r] = softmax ? exp((double)l[r] - (double)m) / sum : 1.0 / (1.0 + exp(-(double)l[r]));
-        if (a.bias) key[r] += (double)a.bias[e];
-        if (key[r] != key[r]) key[r] = none;
-      }
-    }
-  } else {
-#pragma unroll
-    for (int r = 0; r < R; ++r) key[r] = l[r];
-  }
-  const int G = a.d.num_groups;
-  if (G > 1) {
-    Key* const sc = reinterpret_cast<Key*>(lds) + wave * (64 * R);
-#pragma unroll
-    for (int r = 0; r < R; ++r) sc[lane * R + r] = key[r];
-    __syncthreads();
-    // per lanes to a group, so that all of them take part
-    int per = 1;
-    while (2 * per * G <= 64) per *= 2;
-    const int size = E / G, g = lane / per;
-    Key b1 = none, b2 = none;
-    if (g < G)
-      for (int i = lane % per; i < size; i += per) {
-        const Key v = sc[g * size + i];
-        b2 = v > b1 ? b1 : v > b2 ? v : b2;
-        b1 = v > b1 ? v : b1;
-      }
-    for (int off = 1; off < per; off *= 2) {
-      const Key o1 = __shfl_xor(b1, off, 64), o2 = __shfl_xor(b2, off, 64);
-      b2 = o1 > b1 ? (b1 > o2 ? b1 : o2) : (o1 > b2 ? o1 : b2);
-      b1 = o1 > b1 ? o1 : b1;
-    }
-    const Key gs = a.d.group_top == 2 && b2 > none ? b1 + b2 : b1;
-    // a group stays if fewer than top_groups others go before it
-    int before = 0;
-    for (int o = 0; o < G; ++o) {
-      const Key v = __shfl(gs, o * per, 64);
-      before += v > gs || (v == gs && o < g);
-    }
-    const uint64_t stay = __ballot(before < a.d.top_groups);
-#pragma unroll
-    for (int r = 0; r < R; ++r) {
-      const int e = lane * R + r;
-      if (e < E && !(stay >> (e / size * per) & 1)) key[r] = none;
-    }
-  }
-  // the choice: lane j keeps the j-th
-  int id = -1;
-  float lw = -INFINITY;
-  for (int j = 0; j < k; ++j) {
-    Key best = none;
-    float bl = -INFINITY;
-    int be = INT_MAX;
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (key[r] > best) {
-        best = key[r];
-        bl = l[r];
-        be = lane * R + r;
-      }
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) {
-      const Key ob = __shfl_xor(best, off, 64);
-      const float ol = __shfl_xor(bl, off, 64);
-      const int oe = __shfl_xor(be, off, 64);
-      if (ob > best || (ob == best && oe < be)) {
-        best = ob;
-        bl = ol;
-        be = oe;
-      }
-    }
-    if (be == INT_MAX) break;  // nothing left in any lane
-    if (lane == j) {
-      id = be;
-      lw = bl;
-    }
-#pragma unroll
-    for (int r = 0; r < R; ++r)
-      if (lane * R + r == be) key[r] = none;
-  }
-  // weights, f32; renormalised ones through logarithms, so that scores too small
-  // for f32 keep their ratio
-  float w;
-  if (a.d.renorm) {
-    const float base = id < 0 ? -INFINITY : softmax ? lw : log_sigmoid(lw);
-    const float bm = wave_max(base);
-    const float ex = id < 0 ? 0.f : expf(base - bm);
-    w = ex / wave_sum(ex);
-  } else {
-    if (softmax) {
-      float ex = 0.f;
-#pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (l[r] > -INFINITY) ex += expf(l[r] - m);
-      w = expf(lw - m) / wave_sum(ex);
-    } else {
-      w = sigmoid(lw);
-    }
-  }
-  w = id < 0 ? 0.f : w * a.d.scale;
-  const int S = a.d.num_shared;
-  if (lane >= k && lane < k + S) {
-    id = E + lane - k;
-    w = 1.f;
-    if (a.d.shared_gate) {
-      const float g = logit(E);
-      w = sigmoid(g);
-    }
-  }
-  if (here && lane < k + S) {
-    a.ids[(int64_t)t * (k + S) + lane] = id;
-    a.weights[(int64_t)t * (k + S) + lane] = w;
-  }
-}
-
-template <int R>
-hipError_t launch_route(const MoeRouteArgs& a, bool by_logit) {
-  const size_t lds = a.d.num_groups > 1 ? 4 * 64 * R * (by_logit ? 4 : 8) : 0;
-  auto kern = by_logit ? moe_route_kernel<R, float> : moe_route_kernel<R, double>;
-  hipLaunchKernelGGL(kern, dim3((a.T + 3) / 4), dim3(256), lds, a.stream, a);
-  return hipGetLastError();
-}
 
 // --------------------------------------------------------------- packing --
 
@@ -239,10 +51,10 @@ __global__ void moe_pack_kernel(MoePackArgs a) {
     }
     const int64_t fp = ((int64_t)blockIdx.y * a.frags + a.fmul * f + a.fofs) * P + p;
     static_cast<u32x4*>(a.wp)[fp * 64 + lane] = o;
-    if (lane < 16) {
+    if (lane < 32) {  // lanes 0-15 the scales of rows r, 16-31 their biases
+      const uint16_t* const v = lane < 16 ? a.s : a.b;
       const int64_t g = n * G + 2 * p;
-      a.sb[fp * 16 + lane] = make_uint2(a.s[g] | (uint32_t)a.s[g + 1] << 16,
-                                        a.b[g] | (uint32_t)a.b[g + 1] << 16);
+      a.sb[fp * 32 + lane] = v[g] | (uint32_t)v[g + 1] << 16;
     }
   }
 }
@@ -261,27 +73,45 @@ __device__ __forceinline__ u32x4 unpack_w(uint32_t w, uint32_t m) {
   return (u32x4){(w & m) | e, ((w >> 4) & m) | e, ((w >> 8) & m) | e, ((w >> 12) & m) | e};
 }
 
-// silu(g) * u
-__device__ __forceinline__ float swiglu(float g, float u) { return g / (1.0f + expf(-g)) * u; }
+// silu(g) * u. exp2 and the reciprocal are the hardware's (1 ulp); the product
+// under exp2 adds |g| half steps of f32. h is rounded to bf16 right after.
+__device__ __forceinline__ float swiglu(float g, float u) {
+  const float q = __builtin_amdgcn_exp2f(-1.44269504089f * g);
+  return g * __builtin_amdgcn_rcpf(1.0f + q) * u;
+}
 
-constexpr int kTileRows = 16;  // rows of a tile
-constexpr int kPassEntries = 1 << 18;
+constexpr int kPassEntries = 1 << 18;  // of a pass over the experts
+constexpr int kStageK = 128;           // k of a stage: two groups
 
-// Work-space of a call: the plan, then the rows between the products.
+// Work-space of a pass: the plan, then what the products hand to each other.
 struct MoeSpace {
   int32_t* ntiles;
   int4* tiles;     // expert, first sorted row, rows, -
-  int32_t* perm;   // entry of a sorted row
+  int2* perm;      // token and entry of a sorted row
+  uint16_t* xs;    // [T][3][gpad(hidden)] split group sums of x
+  uint16_t* hs;    // [entries][3][gpad(inner)] and of h, by sorted row
   uint16_t* h;     // [entries, inner] by sorted row
-  float* rows;     // [entries, hidden] by entry
+  uint16_t* rows;  // [entries, hidden] weighted rows of down by entry
+  int32_t* counts; // [chunks of entries][experts] (moe_count_kernel)
   size_t bytes;
 };
 
-int64_t max_tiles(int64_t entries, int experts) {
-  return entries / kTileRows + (entries < experts ? entries : experts);
-}
+// The rows between down and the sum over a token's columns are bf16: half a step
+// of each summand, beside the half step of the result, for half of a prompt's
+// largest traffic.
 
-MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t entries) {
+// Entries of a chunk of the two-launch plan, and those up to which one launch
+// does it.
+constexpr int kChunk = 4096, kPlanEntries = 8192;
+
+// Groups of k columns, padded with zeros to whole 16-byte loads.
+__host__ __device__ __forceinline__ int gpad(int k) { return (k / 64 + 7) & ~7; }
+
+// Slots for tiles of `rows` rows (moe_plan_kernel).
+int64_t max_tiles(int64_t entries, int experts, int rows) { return entries / rows + experts; }
+
+MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t tokens,
+                   int64_t entries) {
   MoeSpace s{};
   char* const p = static_cast<char*>(base);
   size_t at = 0;
@@ -291,215 +121,1278 @@ MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t entri
     return r;
   };
   s.ntiles = reinterpret_cast<int32_t*>(take(4));
-  s.tiles = reinterpret_cast<int4*>(take(max_tiles(entries, experts) * sizeof(int4)));
-  s.perm = reinterpret_cast<int32_t*>(take(entries * 4));
+  s.tiles = reinterpret_cast<int4*>(take(max_tiles(entries, experts, 16) * sizeof(int4)));
+  s.perm = reinterpret_cast<int2*>(take(entries * 8));
+  s.xs = reinterpret_cast<uint16_t*>(take(tokens * 6 * gpad(hidden)));
+  s.hs = reinterpret_cast<uint16_t*>(take(entries * 6 * gpad(inner)));
   s.h = reinterpret_cast<uint16_t*>(take(entries * inner * 2));
-  s.rows = reinterpret_cast<float*>(take(entries * hidden * 4));
+  s.rows = reinterpret_cast<uint16_t*>(take(entries * hidden * 2));
+  s.counts = reinterpret_cast<int32_t*>(take((entries + kChunk - 1) / kChunk * experts * 4));
   s.bytes = at;
   return s;
 }
 
-// The plan: a work-group per expert e sorts that expert's entries, in entry
-// order, behind those of the experts before it, and lists its tiles. Every
-// work-group counts all entries by itself (LDS), so that one launch does it.
-constexpr int kPlanThreads = 1024;
-__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(const int32_t* __restrict__ ids,
-                                                                int entries, int experts,
-                                                                int32_t* __restrict__ ntiles,
-                                                                int4* __restrict__ tiles,
-                                                                int32_t* __restrict__ perm) {
-  extern __shared__ int cnt[];
-  __shared__ int own[kPlanThreads / 64], sums[2][kPlanThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, e = blockIdx.x;
-  for (int i = tid; i < experts; i += kPlanThreads) cnt[i] = 0;
-  __syncthreads();
-  // a wave takes a run of entries, so that its own ones keep their order
-  constexpr int W = kPlanThreads / 64;
-  const int run = ((entries + W - 1) / W + 63) & ~63;
-  const int i0 = wave * run, i1 = min(entries, i0 + run);
-  int mine = 0;
-  for (int i = i0; i < i1; i += 64) {
-    const int id = i + lane < i1 ? ids[i + lane] : -1;
-    if ((uint32_t)id < (uint32_t)experts) atomicAdd(&cnt[id], 1);
-    mine += __popcll(__ballot(id == e));
+// v as three bf16 parts, v = hi + mid + lo exactly, at dst, dst + step, ...
+__device__ __forceinline__ void store_split(float v, uint16_t* dst, int step) {
+  const uint16_t hi = f2bf(v);
+  const float q = v - bf2f(hi);
+  const uint16_t mid = f2bf(q);
+  dst[0] = hi;
+  dst[step] = mid;
+  dst[2 * step] = f2bf(q - bf2f(mid));
+}
+
+// Split group sums of x's rows, [T][3][gpad(hidden)]. A lane takes 8 of a
+// group's 64 columns, 8 lanes a group; a thread of a padded group stores zeros.
+// i: the thread's number.
+__device__ __forceinline__ void moe_row_sums(const uint16_t* __restrict__ x, int64_t xs, int T,
+                                             int hidden, uint16_t* __restrict__ sums, int64_t i) {
+  const int gp = gpad(hidden);
+  const int64_t t = i / (8 * gp);
+  const int c = (int)(i - t * 8 * gp);  // 8-column chunk of the row
+  if (t >= T) return;
+  float v = 0.f;
+  if (8 * c < hidden) {
+    const u32x4 q = *reinterpret_cast<const u32x4*>(x + t * xs + 8 * c);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v += bf_lo(q[e]) + bf_hi(q[e]);
   }
-  if (lane == 0) own[wave] = mine;
-  __syncthreads();
-  int before = 0, tbefore = 0;
-  for (int i = tid; i < experts; i += kPlanThreads) {
-    const int c = cnt[i], n = (c + kTileRows - 1) / kTileRows;
-    before += i < e ? c : 0;
-    tbefore += i < e ? n : 0;
+  v = sum8(v);
+  if ((c & 7) == 0) store_split(v, sums + t * 3 * gp + c / 8, gp);
+}
+
+// The plan: work-group e sorts expert e's entries, in entry order, behind those
+// of the experts before it, and lists its tiles. It counts the entries of lower
+// experts and its own by itself, so that one launch without atomics does it.
+// Expert e's tiles start at slot (entries before it) / rows + e: never fewer
+// slots than tiles, the ones left over marked empty (rows = 0).
+// Work-groups from `experts` on form the split group sums of x's rows
+// (moe_row_sums) beside it.
+constexpr int kPlanThreads = 1024;
+typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
+__global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(MoeArgs a, int rows, MoeSpace s) {
+  constexpr int W = kPlanThreads / 64;
+  __shared__ int lower[W], own[W];
+  const int32_t* const ids = a.ids;
+  const int entries = a.T * a.k, k = a.k, experts = a.experts;
+  if (blockIdx.x >= (uint32_t)experts) {
+    moe_row_sums(a.x, a.xs, a.T, a.hidden, s.xs,
+                 (int64_t)(blockIdx.x - experts) * kPlanThreads + threadIdx.x);
+    return;
+  }
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const uint32_t e = blockIdx.x;
+  // a wave takes a run of entries, 4 a lane at a time, so that they keep their order
+  const int run = ((entries + W - 1) / W + 255) & ~255;
+  const int i0 = wave * run, i1 = min(entries, i0 + run);
+  auto load = [&](int i, int (&v)[4]) {
+    if (i + 4 <= i1) {
+      const i32x4_a4 q = *reinterpret_cast<const i32x4_a4*>(ids + i);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = q[c];
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) v[c] = i + c < i1 ? ids[i + c] : -1;
+    }
+  };
+  int lo = 0, mine = 0;
+#pragma unroll 4
+  for (int i = i0 + 4 * lane; i < i1; i += 256) {
+    int v[4];
+    load(i, v);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      lo += (uint32_t)v[c] < e;
+      mine += (uint32_t)v[c] == e;
+    }
   }
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
-    before += __shfl_xor(before, off, 64);
-    tbefore += __shfl_xor(tbefore, off, 64);
+    lo += __shfl_xor(lo, off, 64);
+    mine += __shfl_xor(mine, off, 64);
   }
   if (lane == 0) {
-    sums[0][wave] = before;
-    sums[1][wave] = tbefore;
+    lower[wave] = lo;
+    own[wave] = mine;
   }
   __syncthreads();
-  before = tbefore = 0;
-  int at = 0;
+  int before = 0, n = 0, at = 0;
   for (int w = 0; w < W; ++w) {
-    before += sums[0][w];
-    tbefore += sums[1][w];
-    if (w < wave) at += own[w];
+    before += lower[w];
+    at += w < wave ? own[w] : 0;
+    n += own[w];
   }
-  const int n = cnt[e], nt = (n + kTileRows - 1) / kTileRows;
-  if (e == experts - 1 && tid == 0) *ntiles = tbefore + nt;
-  for (int i = tid; i < nt; i += kPlanThreads)
-    tiles[tbefore + i] = make_int4(e, before + kTileRows * i, min(kTileRows, n - kTileRows * i), 0);
+  const int t0 = before / rows + (int)e, t1 = (before + n) / rows + (int)e + 1;
+  if ((int)e == experts - 1 && tid == 0) *s.ntiles = t1;
+  for (int i = tid; i < t1 - t0; i += kPlanThreads)
+    s.tiles[t0 + i] = make_int4((int)e, before + rows * i, max(0, min(rows, n - rows * i)), 0);
   if (mine == 0) return;
   at += before;
-  for (int i = i0; i < i1; i += 64) {
-    const bool hit = i + lane < i1 && ids[i + lane] == e;
-    const uint64_t b = __ballot(hit);
-    if (hit) perm[at + __popcll(b & ((1ull << lane) - 1))] = i + lane;
-    at += __popcll(b);
+  for (int i = i0 + 4 * lane; i - 4 * lane < i1; i += 256) {
+    int v[4];
+    load(i, v);
+    int below = 0, all = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const uint64_t b = __ballot((uint32_t)v[c] == e);
+      below += __popcll(b & ((1ull << lane) - 1));
+      all += __popcll(b);
+    }
+    if (all == 0) continue;
+#pragma unroll
+    for (int c = 0; c < 4; ++c)
+      if ((uint32_t)v[c] == e) s.perm[at + below++] = make_int2((i + c) / k, i + c);
+    at += all;
   }
 }
 
-// One 16-row tile against NF 16-column fragments over the stages p0, p0 + 1,
-// ..., 4 at a time: every load of the four goes out before the first product.
-// x is the MFMA A operand, so lane (r16, c4) supplies row r16 (zeros past the
-// tile's rows) and ends with rows 4 c4 + i, column r16 of each fragment: one
-// scale and one offset per group for all of its sums.
-template <int NF>
-__device__ __forceinline__ void tile_product(const uint16_t* xrow, bool live,
-                                             const u32x4* wp, const uint2* sb, int P, int p0,
-                                             int step, f32x4 (&T)[NF]) {
-  const int lane = threadIdx.x & 63, r16 = lane & 15, c4 = lane >> 4;
-  const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  uint32_t nib = 0x000F000Fu;
-  asm volatile("" : "+v"(nib));
-#pragma unroll
-  for (int f = 0; f < NF; ++f) T[f] = zero;
-  for (; p0 < P; p0 += step) {
-    u32x4 w[4][NF], X[4][4];
-    uint2 s[4][NF];
-#pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int p = min(p0 + q, P - 1);
-#pragma unroll
-      for (int f = 0; f < NF; ++f) {
-        w[q][f] = __builtin_nontemporal_load(wp + ((int64_t)f * P + p) * 64 + lane);
-        s[q][f] = sb[((int64_t)f * P + p) * 16 + r16];
-      }
+// The plan of many entries in two launches. First a work-group per chunk of
+// entries counts them by expert; others form the rows' sums.
+__global__ __launch_bounds__(kPlanThreads) void moe_count_kernel(MoeArgs a, int chunks, MoeSpace s) {
+  extern __shared__ int cnt[];
+  if (blockIdx.x >= (uint32_t)chunks) {
+    moe_row_sums(a.x, a.xs, a.T, a.hidden, s.xs,
+                 (int64_t)(blockIdx.x - chunks) * kPlanThreads + threadIdx.x);
+    return;
+  }
+  for (int e = threadIdx.x; e < a.experts; e += kPlanThreads) cnt[e] = 0;
+  __syncthreads();
+  const int i1 = min(a.T * a.k, (int)(blockIdx.x + 1) * kChunk);
+  for (int i = blockIdx.x * kChunk + threadIdx.x; i < i1; i += kPlanThreads) {
+    const int id = a.ids[i];
+    if ((uint32_t)id < (uint32_t)a.experts) atomicAdd(&cnt[id], 1);
+  }
+  __syncthreads();
+  for (int e = threadIdx.x; e < a.experts; e += kPlanThreads)
+    s.counts[(int64_t)blockIdx.x * a.experts + e] = cnt[e];
+}
+
+// Then a work-group per chunk places its entries behind those of lower experts
+// and of its expert in the chunks before, and writes its share of the tile list.
+// Inside a chunk an expert's entries take their places in any order: a row's
+// sums do not depend on where it stands.
+__global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(MoeArgs a, int rows, MoeSpace s) {
+  extern __shared__ int lds[];
+  __shared__ int wsum[kPlanThreads / 64];
+  const int E = a.experts, chunks = gridDim.x, chunk = blockIdx.x;
+  int* const before = lds;   // entries of lower experts
+  int* const at = lds + E;   // the chunk's next place of an expert
+  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  const int epp = (E + kPlanThreads - 1) / kPlanThreads;  // experts of a thread, in a run
+  int mine = 0;
+  for (int e = tid * epp; e < min(E, (tid + 1) * epp); ++e) {
+    int n = 0, o = 0;
+#pragma unroll 8
+    for (int c = 0; c < chunks; ++c) {
+      const int v = s.counts[(int64_t)c * E + e];
+      n += v;
+      o += c < chunk ? v : 0;
     }
+    before[e] = n;
+    at[e] = o;
+    mine += n;
+  }
+  int run = mine;  // inclusive over the wave, then over the waves
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      const int p = min(p0 + q, P - 1);
+  for (int off = 1; off < 64; off *= 2) {
+    const int v = __shfl_up(run, off, 64);
+    run += lane >= off ? v : 0;
+  }
+  if (lane == 63) wsum[wave] = run;
+  __syncthreads();
+  run -= mine;
+  for (int w = 0; w < wave; ++w) run += wsum[w];
+  for (int e = tid * epp; e < min(E, (tid + 1) * epp); ++e) {
+    const int n = before[e];
+    before[e] = run;
+    at[e] += run;
+    run += n;
+  }
+  __syncthreads();
+  int total = 0;
+  for (int w = 0; w < kPlanThreads / 64; ++w) total += wsum[w];
+  // slots as in moe_plan_kernel: expert e's from before / rows + e on
+  const int slots = total / rows + E, share = (slots + chunks - 1) / chunks;
+  if (chunk == 0 && tid == 0) *s.ntiles = slots;
+  for (int t = chunk * share + tid; t < min(slots, (chunk + 1) * share); t += kPlanThreads) {
+    int lo = 0, hi = E - 1;  // the last expert whose slots start at t or before
+    while (lo < hi) {
+      const int m = (lo + hi + 1) >> 1;
+      if (before[m] / rows + m <= t)
+        lo = m;
+      else
+        hi = m - 1;
+    }
+    const int n = (lo + 1 < E ? before[lo + 1] : total) - before[lo];
+    const int i = t - before[lo] / rows - lo;
+    s.tiles[t] = make_int4(lo, before[lo] + rows * i, max(0, min(rows, n - rows * i)), 0);
+  }
+  const int i1 = min(a.T * a.k, (chunk + 1) * kChunk);
+  for (int i = chunk * kChunk + tid; i < i1; i += kPlanThreads) {
+    const int id = a.ids[i];
+    if ((uint32_t)id < (uint32_t)E) s.perm[atomicAdd(&at[id], 1)] = make_int2(i / a.k, i);
+  }
+}
+
+// ---- very few entries: no plan ----
+
+// Most entries of a call whose work-groups find their rows by themselves: a
+// wave holds every id.
+constexpr int kFewEntries = 64;
+// ... and the most tokens: down reads an expert's weights for each of them again.
+constexpr int kFewTokens = 8;
+
+// NS stages p0, p0 + step, ... of a 16-row fragment: its weights, scales and
+// biases (stages past P: the last one again; their x is zero).
+template <int NS>
+struct Frag {
+  u32x4 w[NS];
+  uint32_t s[NS], b[NS];
+  __device__ __forceinline__ void load(const u32x4* wp, const uint32_t* sb, int P, int p0,
+                                       int step) {
+    const int lane = threadIdx.x & 63, r16 = lane & 15;
+#pragma unroll
+    for (int q = 0; q < NS; ++q) {
+      const int p = min(p0 + step * q, P - 1);
+      w[q] = __builtin_nontemporal_load(wp + p * 64 + lane);
+      s[q] = __builtin_nontemporal_load(sb + p * 32 + r16);
+      b[q] = __builtin_nontemporal_load(sb + p * 32 + 16 + r16);
+    }
+  }
+};
+
+// The same stages of 16 rows of x; lane (r16, c4) holds row r16 (row null:
+// zeros). Sums of a group: xg rows 4 c4 + i.
+template <int NS>
+struct Rows {
+  u32x4 x[NS][4];
+  __device__ __forceinline__ void load(const uint16_t* row, int P, int p0, int step) {
+    const int c4 = (threadIdx.x & 63) >> 4;
+#pragma unroll
+    for (int q = 0; q < NS; ++q) {
+      const int p = p0 + step * q;
 #pragma unroll
       for (int h = 0; h < 4; ++h) {
-        X[q][h] = (u32x4){0u, 0u, 0u, 0u};
-        if (live) X[q][h] = *reinterpret_cast<const u32x4*>(xrow + 128 * p + 32 * h + 8 * c4);
+        x[q][h] = (u32x4){0u, 0u, 0u, 0u};
+        if (row && p < P) x[q][h] = *reinterpret_cast<const u32x4*>(row + 128 * p + 32 * h + 8 * c4);
       }
     }
+  }
+};
+
+// T[f] += x . w of NF fragments over NS stages. x is the MFMA A operand: a
+// lane ends with rows 4 c4 + i, column r16 of each fragment, so that one scale
+// and one offset per group serve all of its sums.
+template <int NF, int NS>
+__device__ __forceinline__ void product(const Rows<NS>& x, const Frag<NS> (&f)[NF], uint32_t nib,
+                                        f32x4 (&T)[NF]) {
+  const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int q = 0; q < 4; ++q) {
-      if (p0 + q >= P) break;
+  for (int q = 0; q < NS; ++q) {
+    __builtin_amdgcn_sched_barrier(0);  // one stage's operands at a time
 #pragma unroll
-      for (int gl = 0; gl < 2; ++gl) {
-        f32x4 xg = mfma(X[q][2 * gl], ones, zero);
-        xg = mfma(X[q][2 * gl + 1], ones, xg);
+    for (int gl = 0; gl < 2; ++gl) {
+      f32x4 xg = mfma(x.x[q][2 * gl], ones, zero);
+      xg = mfma(x.x[q][2 * gl + 1], ones, xg);
 #pragma unroll
-        for (int f = 0; f < NF; ++f) {
-          f32x4 d = mfma(X[q][2 * gl], unpack_w(w[q][f][2 * gl], nib), zero);
-          d = mfma(X[q][2 * gl + 1], unpack_w(w[q][f][2 * gl + 1], nib), d);
-          const float sc = gl ? bf_hi(s[q][f].x) : bf_lo(s[q][f].x);
-          const float of = fmaf(-128.0f, sc, gl ? bf_hi(s[q][f].y) : bf_lo(s[q][f].y));
+      for (int i = 0; i < NF; ++i) {
+        f32x4 d = mfma(x.x[q][2 * gl], unpack_w(f[i].w[q][2 * gl], nib), zero);
+        d = mfma(x.x[q][2 * gl + 1], unpack_w(f[i].w[q][2 * gl + 1], nib), d);
+        const float sc = gl ? bf_hi(f[i].s[q]) : bf_lo(f[i].s[q]);
+        const float of = fmaf(-128.0f, sc, gl ? bf_hi(f[i].b[q]) : bf_lo(f[i].b[q]));
 #pragma unroll
-          for (int i = 0; i < 4; ++i) T[f][i] = fmaf(sc, d[i], fmaf(of, xg[i], T[f][i]));
+        for (int r = 0; r < 4; ++r) T[i][r] = fmaf(sc, d[r], fmaf(of, xg[r], T[i][r]));
+      }
+    }
+  }
+}
+
+// h by entry: work-group (entry u, 16 inner columns), four waves, wave w over
+// the stages 4 w .. 4 w + 3 (and on from 16 stages ahead), added in wave order.
+// It takes every row of the expert that entry u names first; a later entry of
+// the same expert has nothing to do.
+__global__ __launch_bounds__(256) void moe_few_up_kernel(MoeArgs a, uint16_t* __restrict__ h) {
+  __shared__ f32x4 part[4][2][64];
+  const int blocks = a.inner / 16, entries = a.T * a.k;
+  const int u = blockIdx.x / blocks, j = blockIdx.x - u * blocks;
+  const int lane = threadIdx.x & 63, r16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int id = lane < entries ? a.ids[lane] : -1;
+  const int e = __builtin_amdgcn_readlane(id, u);
+  const uint64_t hits = __ballot(id == e);
+  if ((uint32_t)e >= (uint32_t)a.experts || (hits & ((1ull << u) - 1)) != 0) return;
+  const int n = __popcll(hits);
+  // lane r receives the r-th entry of the expert (the others push to lane 63, which
+  // is read only where it is itself the 64th)
+  const int rank = id == e ? __popcll(hits & ((1ull << lane) - 1)) : 63;
+  const int mine = __builtin_amdgcn_ds_permute(rank << 2, lane);
+  const int P = a.hidden >> 7;
+  const int64_t f0 = ((int64_t)e * blocks + j) * 2 * P;
+  const u32x4* const wp = static_cast<const u32x4*>(a.w1) + f0 * 64;
+  const uint32_t* const sb = a.sb1 + f0 * 32;
+  uint32_t nib = 0x000F000Fu;
+  asm volatile("" : "+v"(nib));
+  for (int m0 = 0; m0 < n; m0 += 16) {
+    const int en = __shfl(mine, m0 + r16, 64);
+    const uint16_t* const row = m0 + r16 < n ? a.x + (int64_t)(en / a.k) * a.xs : nullptr;
+    f32x4 T[2] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+    for (int p = 4 * wave; p < P; p += 16) {
+      Frag<4> f[2];
+      Rows<4> x;
+#pragma unroll
+      for (int i = 0; i < 2; ++i) f[i].load(wp + (int64_t)i * P * 64, sb + (int64_t)i * P * 32, P, p, 1);
+      x.load(row, P, p, 1);
+      product<2, 4>(x, f, nib, T);
+    }
+    part[wave][0][lane] = T[0];
+    part[wave][1][lane] = T[1];
+    __syncthreads();
+    // thread (element i of lane l): row 4 (l / 16) + i, column l % 16
+    const int l = threadIdx.x >> 2, i = threadIdx.x & 3, m = m0 + 4 * (l >> 4) + i;
+    const int em = __shfl(mine, m, 64);
+    float g = 0.f, up = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      g += part[w][0][l][i];
+      up += part[w][1][l][i];
+    }
+    if (m < n) h[(int64_t)em * a.inner + 16 * j + (l & 15)] = f2bf(swiglu(g, up));
+    __syncthreads();
+  }
+}
+
+// Down and the sum over a token's columns in one. Work-group
+// (token, 16 columns), a wave per column of ids (rounds of 16), added in order.
+__global__ __launch_bounds__(1024) void moe_few_down_kernel(MoeArgs a,
+                                                              const uint16_t* __restrict__ h) {
+  __shared__ float part[16][16];
+  const int blocks = a.hidden / 16, t = blockIdx.x / blocks, j = blockIdx.x - t * blocks;
+  const int lane = threadIdx.x & 63, r16 = lane & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int P = a.inner >> 7;
+  uint32_t nib = 0x000F000Fu;
+  asm volatile("" : "+v"(nib));
+  float y = 0.f;
+  for (int c0 = 0; c0 < a.k; c0 += waves) {
+    const int c = c0 + wave, en = t * a.k + c;
+    const int e = c < a.k ? __builtin_amdgcn_readfirstlane(a.ids[en]) : -1;
+    f32x4 T[1] = {{0.f, 0.f, 0.f, 0.f}};
+    if ((uint32_t)e < (uint32_t)a.experts) {
+      const int64_t f0 = ((int64_t)e * blocks + j) * P;
+      const uint16_t* const row = r16 == 0 ? h + (int64_t)en * a.inner : nullptr;
+      for (int p = 0; p < P; p += 4) {
+        Rows<4> x;
+        Frag<4> f[1];
+        f[0].load(static_cast<const u32x4*>(a.w2) + f0 * 64, a.sb2 + f0 * 32, P, p, 1);
+        x.load(row, P, p, 1);
+        product<1, 4>(x, f, nib, T);
+      }
+      T[0][0] *= a.weights[en];
+    }
+    if (lane < 16) part[wave][lane] = T[0][0];
+    __syncthreads();
+    if (threadIdx.x < 16)
+      for (int w = 0; w < min(waves, a.k - c0); ++w) y += part[w][threadIdx.x];
+    __syncthreads();
+  }
+  if (threadIdx.x < 16) a.out[(int64_t)t * a.os + 16 * j + threadIdx.x] = f2bf(y);
+}
+
+// s_waitcnt lgkmcnt(0), and vmcnt(N) below (gfx9 encodings, the other counters
+// at their maximum)
+__device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+// ---- tiles ----
+
+template <int N>
+__device__ __forceinline__ void wait_vm() {
+  static_assert(N >= 0 && N < 64, "vmcnt range");
+  __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (15 << 8));
+}
+
+// A tile of 16 MW rows against 128 columns (8 fragments); four waves in a row,
+// each with all rows and two fragments. The weights are the MFMA A operand, so a
+// lane ends with four consecutive columns of one row.
+// Per stage of 128 k the rows go to LDS by DMA, 16-byte chunk c of row r at
+// chunk c ^ (r % 16) (operand reads without conflicts), as do the fragments'
+// scales; the weights go to registers; all of them R - 1 stages ahead. The ring's
+// slots are arrays of their own, so that the compiler can tell copies into one
+// from reads of another.
+// The offsets' sum over the groups, sum_g (b_g - 128 s_g) X_g, is a short MFMA
+// product at the end: X_g as three bf16 parts (exact), b and s as stored.
+//   UP: rows are gathered tokens of x, the fragments gate and up in turn: a wave
+//     ends with gate and up of the same 16 columns and stores h; the work-group's
+//     64 columns are one group of down's input, whose split sums it stores.
+//   else: rows of h, and the weighted rows of down go to their entries.
+template <int MW, bool UP>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) void moe_tile_kernel(
+    MoeArgs a, MoeSpace s) {
+  constexpr int MT = 16 * MW, XROW = kStageK * 2, R = 3;
+  constexpr int LB = MW + 3;  // loads of a stage
+  __shared__ __align__(16) uint8_t xl0[MT * XROW], xl1[MT * XROW], xl2[MT * XROW];
+  __shared__ __align__(16) uint8_t sl0[4 * 256], sl1[4 * 256], sl2[4 * 256];
+  __shared__ float gsum[UP ? 4 : 1][MT];
+  const int K = UP ? a.hidden : a.inner, N = UP ? 2 * a.inner : a.hidden;
+  const int P = K >> 7, blocks = N >> 7;
+  // an XCD (work-groups L % 8) takes a run of the tiles, all columns of a tile
+  // side by side
+  const int n = *s.ntiles * blocks, per = (n + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || idx >= n) return;
+  const int tile = idx / blocks, cb = idx - tile * blocks;
+  int4 tl = s.tiles[tile];
+  tl.x = __builtin_amdgcn_readfirstlane(tl.x);
+  tl.y = __builtin_amdgcn_readfirstlane(tl.y);
+  tl.z = __builtin_amdgcn_readfirstlane(tl.z);
+  if (tl.z == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, c4 = lane >> 4;
+
+  const int64_t f0 = (int64_t)tl.x * (N >> 4) + 8 * cb;  // first fragment of the work-group
+  const u32x4* const wp = static_cast<const u32x4*>(UP ? a.w1 : a.w2) + f0 * P * 64;
+  const uint32_t* const sb = (UP ? a.sb1 : a.sb2) + f0 * P * 32;
+  const uint16_t* const xbase = UP ? a.x : s.h + (int64_t)tl.y * a.inner;
+  uint32_t xvo[MW];
+#pragma unroll
+  for (int j = 0; j < MW; ++j) {
+    const int r = 4 * (wave + 4 * j) + c4, src = min(r, tl.z - 1);
+    const int64_t at = UP ? (int64_t)s.perm[tl.y + src].x * a.xs : (int64_t)src * a.inner;
+    xvo[j] = (uint32_t)(at * 2) + 16 * (r16 ^ (r & 15));
+  }
+  const int wvo = (wave * 2 * P * 64 + lane) * 16;
+  // scale copy: lane L -> fragment (L / 16) % 2 of the wave, dword L % 16
+  const int svo = (wave * 2 + (c4 & 1)) * P * 128 + 4 * r16;
+
+  u32x4 wr[R][2];
+  auto xbuf = [&](auto slot) -> uint8_t* {
+    constexpr int S = decltype(slot)::value;
+    return S == 0 ? xl0 : S == 1 ? xl1 : xl2;
+  };
+  auto sbuf = [&](auto slot) -> uint8_t* {
+    constexpr int S = decltype(slot)::value;
+    return (S == 0 ? sl0 : S == 1 ? sl1 : sl2) + wave * 256;
+  };
+  // stage p's loads into ring slot S (none of a stage past the last)
+  auto batch = [&](int p, auto slot) {
+    constexpr int S = decltype(slot)::value;
+    const int in = __builtin_amdgcn_readfirstlane(p < P ? -1 : 0);
+    const __amdgpu_buffer_rsrc_t xrs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)xbase, (short)0, in, 0x00020000);
+    const __amdgpu_buffer_rsrc_t wrs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)wp, (short)0, in & (8 * P * 1024), 0x00020000);
+    const __amdgpu_buffer_rsrc_t srs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, in & (8 * P * 128), 0x00020000);
+#pragma unroll
+    for (int j = 0; j < MW; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          xrs, (void __attribute__((address_space(3)))*)(xbuf(slot) + 4 * (wave + 4 * j) * XROW),
+          16, (int)xvo[j], p * XROW, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      wr[S][i] = __builtin_amdgcn_raw_buffer_load_b128(wrs, wvo, (i * P + p) * 1024, 0);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        srs, (void __attribute__((address_space(3)))*)sbuf(slot), 4, svo, p * 128, 0, 0);
+  };
+  // all but the youngest B stages have landed, in every wave
+  auto landed = [&](auto behind) {
+    wait_vm<decltype(behind)::value * LB>();
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
+  };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  f32x4 T[2][MW];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int u = 0; u < MW; ++u) T[i][u] = zero;
+  uint32_t nib = 0x000F000Fu;
+  asm volatile("" : "+v"(nib));
+
+  auto compute = [&](auto slot) {
+    constexpr int S = decltype(slot)::value;
+    const uint8_t* const cur = xbuf(slot);
+    u32x4 sv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      sv[i] = *reinterpret_cast<const u32x4*>(sbuf(slot) + i * 64 + c4 * 16);
+#pragma unroll
+    for (int gl = 0; gl < 2; ++gl) {
+      u32x4 A[2][2];
+      float sc[2][4];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        A[i][0] = unpack_w(wr[S][i][2 * gl], nib);
+        A[i][1] = unpack_w(wr[S][i][2 * gl + 1], nib);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) sc[i][r] = gl ? bf_hi(sv[i][r]) : bf_lo(sv[i][r]);
+      }
+#pragma unroll
+      for (int u = 0; u < MW; ++u) {
+        u32x4 X[2];
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+          X[h] = *reinterpret_cast<const u32x4*>(
+              &cur[(u * 16 + r16) * XROW + (((8 * gl + 4 * h + c4) ^ r16) << 4)]);
+        f32x4 d[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) d[i] = mfma(A[i][0], X[0], zero);
+#pragma unroll
+        for (int i = 0; i < 2; ++i) d[i] = mfma(A[i][1], X[1], d[i]);
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int r = 0; r < 4; ++r) T[i][u][r] = fmaf(sc[i][r], d[i][r], T[i][u][r]);
+      }
+    }
+  };
+  // Whole turns of the ring, then up to R - 1 stages more. The turns' body has no
+  // branch: a stage past the last one is loaded through an empty resource.
+  auto step = [&](int p, auto slot) {
+    constexpr int S = decltype(slot)::value;
+    batch(p + R - 1, std::integral_constant<int, (S + R - 1) % R>{});
+    __builtin_amdgcn_sched_barrier(0);
+    compute(slot);
+    landed(std::integral_constant<int, R - 2>{});
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, 2>;
+  batch(0, S0{});
+  batch(1, S1{});
+  landed(std::integral_constant<int, R - 2>{});
+
+  // rows' sums, and where down's rows go
+  const int gp = gpad(K), go = gp >> 3;
+  const uint16_t* xg[MW];
+  int en[MW];
+#pragma unroll
+  for (int u = 0; u < MW; ++u) {
+    const int row = tl.y + min(u * 16 + r16, tl.z - 1);
+    const int2 pe = s.perm[row];
+    xg[u] = UP ? s.xs + (int64_t)pe.x * 3 * gp : s.hs + (int64_t)row * 3 * gp;
+    en[u] = pe.y;
+  }
+  int p = 0;
+#pragma nounroll
+  for (; p + R <= P; p += R) {
+    step(p, S0{});
+    step(p + 1, S1{});
+    step(p + 2, S2{});
+  }
+  if (p < P) {
+    compute(S0{});
+    landed(std::integral_constant<int, 0>{});
+    if (p + 1 < P) compute(S1{});
+  }
+  wait_vm<0>();  // no copy is left behind
+
+  // The offsets' sum. A row's sums are [hi | mid | lo][gp]: octet o of the row is
+  // part o / go of groups 8 (o % go) .., and a product takes four octets, one a
+  // lane group.
+  float wt[MW];
+  if constexpr (!UP)
+#pragma unroll
+    for (int u = 0; u < MW; ++u) wt[u] = a.weights[en[u]];
+#pragma nounroll
+  for (int jb = 0; 4 * jb < 3 * go; ++jb) {
+    const int o = 4 * jb + c4, oc = o < go ? o : o < 2 * go ? o - go : o - 2 * go;
+    u32x4 as[2], ab[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int ps = 4 * oc + q;
+        const bool in = o < 3 * go && ps < P;
+        const uint32_t* const sq = sb + ((wave * 2 + i) * P + (in ? ps : 0)) * 32 + r16;
+        as[i][q] = in ? sq[0] : 0u;
+        ab[i][q] = in ? sq[16] : 0u;
+      }
+#pragma unroll
+    for (int u = 0; u < MW; ++u) {
+      const u32x4 xp = *reinterpret_cast<const u32x4*>(xg[u] + 8 * (o < 3 * go ? o : 0));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        const f32x4 d = mfma(as[i], xp, zero);
+        T[i][u] = mfma(ab[i], xp, T[i][u]);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) T[i][u][r] = fmaf(-128.0f, d[r], T[i][u][r]);
+      }
+    }
+  }
+
+  if constexpr (UP) {
+    const int col = 64 * cb + 16 * wave + 4 * c4;
+#pragma unroll
+    for (int u = 0; u < MW; ++u) {
+      const int m = u * 16 + r16;
+      const uint32_t lo = f2bf2(swiglu(T[0][u][0], T[1][u][0]), swiglu(T[0][u][1], T[1][u][1]));
+      const uint32_t hi = f2bf2(swiglu(T[0][u][2], T[1][u][2]), swiglu(T[0][u][3], T[1][u][3]));
+      if (m < tl.z)
+        *reinterpret_cast<u32x2*>(s.h + (int64_t)(tl.y + m) * a.inner + col) = (u32x2){lo, hi};
+      float v = (bf_lo(lo) + bf_hi(lo)) + (bf_lo(hi) + bf_hi(hi));
+      v += __shfl_xor(v, 16, 64);
+      v += __shfl_xor(v, 32, 64);
+      if (c4 == 0) gsum[wave][m] = v;
+    }
+    lds_barrier();
+    if (tid < tl.z) {
+      const int gi = gpad(a.inner);
+      uint16_t* const dst = s.hs + (int64_t)(tl.y + tid) * 3 * gi;
+      store_split((gsum[0][tid] + gsum[1][tid]) + (gsum[2][tid] + gsum[3][tid]), dst + cb, gi);
+      if (cb == blocks - 1)  // the padded groups
+        for (int g = blocks; g < gi; ++g) store_split(0.f, dst + g, gi);
+    }
+  } else {
+#pragma unroll
+    for (int u = 0; u < MW; ++u) {
+      if (u * 16 + r16 >= tl.z) continue;
+      uint16_t* const o = s.rows + (int64_t)en[u] * a.hidden + 128 * cb +
+                          32 * wave + 4 * c4;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+        *reinterpret_cast<u32x2*>(o + 16 * i) =
+            (u32x2){f2bf2(wt[u] * T[i][u][0], wt[u] * T[i][u][1]),
+                    f2bf2(wt[u] * T[i][u][2], wt[u] * T[i][u][3])};
+    }
+  }
+}
+
+// ---- tiles of many rows ----
+
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
+  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+}
+
+// moe_tile_kernel for experts with many rows: a tile of 64 rows against 256
+// columns, four waves in a row, each with all rows and 64 columns (two fragments
+// of 32), on 32 x 32 x 16 products. x is the A operand: lane (r32, c2) supplies
+// row r32 and ends with column r32, rows 8 (e / 4) + 4 c2 + e % 4 of a product's
+// 16 sums. An unpacked weight serves two products and a row read from LDS two.
+// The k order inside a stage is the packing's: of a fragment's four dwords d and
+// the lane groups c = 2 sg + c2 of the two loads sg, product (d, sg) takes the
+// 8-column chunks 4 d + 2 sg + c2 of x.
+// The rows are copied one stage ahead (two slots), the weights go to registers
+// half a stage ahead, once the last of the stage before are unpacked.
+template <bool UP>
+__global__ __launch_bounds__(256)
+    __attribute__((amdgpu_waves_per_eu(2, 2))) void
+    moe_wide_kernel(MoeArgs a, MoeSpace s) {
+  constexpr int MT = 64, XROW = kStageK * 2, XJ = 4, RB = 2;
+  __shared__ __align__(16) uint8_t xl0[MT * XROW], xl1[MT * XROW];
+  __shared__ int2 row_of[MT];   // a row's token and entry
+  __shared__ float wt_of[MT];   // and its weight
+  const int K = UP ? a.hidden : a.inner, N = UP ? 2 * a.inner : a.hidden;
+  const int P = K >> 7, blocks = (N + 255) >> 8;
+  const int n = *s.ntiles * blocks, per = (n + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || idx >= n) return;
+  const int tile = idx / blocks, cb = idx - tile * blocks;
+  int4 tl = s.tiles[tile];
+  tl.x = __builtin_amdgcn_readfirstlane(tl.x);
+  tl.y = __builtin_amdgcn_readfirstlane(tl.y);
+  tl.z = __builtin_amdgcn_readfirstlane(tl.z);
+  if (tl.z == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, c2 = lane >> 5;
+  const bool live = 256 * cb + 64 * wave < N;  // an odd last half block leaves two waves idle
+
+  if (tid < MT) {
+    const int2 pe = s.perm[tl.y + min(tid, tl.z - 1)];
+    row_of[tid] = pe;
+    if constexpr (!UP) wt_of[tid] = a.weights[pe.y];
+  }
+  // the wave's first 16-row fragment, and the lane's of its 32-column fragment i
+  const int64_t f0 = (int64_t)tl.x * (N >> 4) + 16 * cb + (live ? 4 * wave : 0);
+  const u32x4* const wp = static_cast<const u32x4*>(UP ? a.w1 : a.w2) + f0 * P * 64;
+  const uint32_t* const sb = (UP ? a.sb1 : a.sb2) + f0 * P * 32;
+  int fr[2];
+#pragma unroll
+  for (int i = 0; i < 2; ++i) fr[i] = (UP ? i : 2 * i) + (r32 >> 4) * (UP ? 2 : 1);
+  const uint16_t* const xbase = UP ? a.x : s.h + (int64_t)tl.y * a.inner;
+  __syncthreads();
+  uint32_t xvo[XJ];
+#pragma unroll
+  for (int j = 0; j < XJ; ++j) {
+    const int r = 4 * (wave + 4 * j) + (lane >> 4);
+    const int64_t at = UP ? (int64_t)row_of[r].x * a.xs : (int64_t)min(r, tl.z - 1) * a.inner;
+    xvo[j] = (uint32_t)(at * 2) + 16 * ((lane & 15) ^ (r & 15));
+  }
+  const int wvo = (fr[0] * P * 64 + 16 * c2 + (r32 & 15)) * 16;
+  const int svo = fr[0] * P * 128 + (r32 & 15) * 4, fi = UP ? P : 2 * P;
+  auto batch_x = [&](int p, auto slot) {
+    constexpr int S = decltype(slot)::value;
+    const int in = __builtin_amdgcn_readfirstlane(p < P ? -1 : 0);
+    const __amdgpu_buffer_rsrc_t xrs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)xbase, (short)0, in, 0x00020000);
+#pragma unroll
+    for (int j = 0; j < XJ; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          xrs,
+          (void __attribute__((address_space(3)))*)((S ? xl1 : xl0) + 4 * (wave + 4 * j) * XROW), 16,
+          (int)xvo[j], p * XROW, 0, 0);
+  };
+  u32x4 wr[2][2];
+  uint32_t sr[2];
+  constexpr int LW = 6;  // loads of a stage's weights
+  auto batch_w = [&](int p) {
+    const int in = __builtin_amdgcn_readfirstlane(p < P ? -1 : 0);
+    const __amdgpu_buffer_rsrc_t wrs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)wp, (short)0, in & (4 * P * 1024), 0x00020000);
+    const __amdgpu_buffer_rsrc_t srs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, in & (4 * P * 128), 0x00020000);
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        wr[i][g] = __builtin_amdgcn_raw_buffer_load_b128(wrs, wvo + 512 * g, (p + i * fi) * 1024, 0);
+      sr[i] = __builtin_amdgcn_raw_buffer_load_b32(srs, svo, (p + i * fi) * 128, 0);
+    }
+  };
+  uint32_t nib = 0x000F000Fu;
+  asm volatile("" : "+v"(nib));
+  f32x16 T[2][RB];
+#pragma unroll
+  for (int i = 0; i < 2; ++i)
+#pragma unroll
+    for (int u = 0; u < RB; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) T[i][u][e] = 0.f;
+
+  batch_x(0, std::integral_constant<int, 0>{});
+  batch_w(0);
+  wait_vm<LW>();
+  wait_lgkm0();
+  __builtin_amdgcn_s_barrier();
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
+
+  // The loop over the stages with the tile's first NB row blocks. A task is a
+  // group of 64 k on a row block: 8 products into one of two sets of sums, beside
+  // which the task before's sums are scaled into T and the next task's rows are
+  // read.
+  auto stages = [&](auto nbc) {
+    constexpr int NB = decltype(nbc)::value;
+    f32x16 y[2][2];
+    float sp[2] = {0.f, 0.f};  // scales of the sums not yet in T
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) y[1][i][e] = 0.f;
+    u32x4 X[2][2][2], W[2][2][2];
+    // byte of chunk c2 of row r32 in a slot; chunk c2 + even number: its bits flipped
+    int xrd = r32 * XROW + ((c2 ^ (r32 & 15)) << 4);
+    auto rows = [&](const uint8_t* cur, auto tc) {
+      constexpr int t = decltype(tc)::value, gl = t / NB, u = t % NB;
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          X[t & 1][d][g] = *reinterpret_cast<const u32x4*>(
+              cur + u * 32 * XROW + (xrd ^ ((8 * gl + 4 * d + 2 * g) << 4)));
+    };
+    auto unpack = [&](int gl) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) W[i][d][g] = unpack_w(wr[i][g][2 * gl + d], nib);
+    };
+    auto task = [&](const uint8_t* cur, auto tc) {
+      constexpr int t = decltype(tc)::value, up = (t + NB - 1) % NB;
+      if constexpr (t + 1 < 2 * NB) rows(cur, std::integral_constant<int, t + 1>{});
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[t & 1][i][e] = 0.f;
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            y[t & 1][i] = mfma32(X[t & 1][d][g], W[i][d][g], y[t & 1][i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          T[i][up][e] = fmaf(sp[i], y[1 - (t & 1)][i][e], T[i][up][e]);
+      if constexpr (t + 1 < 2 * NB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    auto step = [&](int p, auto slot, auto lastc) {
+      constexpr int S = decltype(slot)::value;
+      constexpr bool last = decltype(lastc)::value;
+      const uint8_t* const cur = S ? xl1 : xl0;
+      asm volatile("" : "+v"(xrd));  // one address register, not one a chunk
+      rows(cur, std::integral_constant<int, 0>{});
+      if constexpr (!last) batch_x(p + 1, std::integral_constant<int, 1 - S>{});
+      unpack(0);
+      float s0[2], s1[2];
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        s0[i] = bf_lo(sr[i]);
+        s1[i] = bf_hi(sr[i]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+      task(cur, std::integral_constant<int, 0>{});
+      sp[0] = s0[0], sp[1] = s0[1];
+      if constexpr (NB > 1) task(cur, std::integral_constant<int, 1 % (2 * NB)>{});
+      unpack(1);
+      if constexpr (!last) batch_w(p + 1);
+      __builtin_amdgcn_sched_barrier(0);
+      task(cur, std::integral_constant<int, NB>{});
+      sp[0] = s1[0], sp[1] = s1[1];
+      if constexpr (NB > 1) task(cur, std::integral_constant<int, NB + 1 < 2 * NB ? NB + 1 : NB>{});
+      if constexpr (!last) {
+        wait_vm<LW>();  // the rows; the weights are waited for where they are unpacked
+        wait_lgkm0();
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
+      }
+    };
+    using S0 = std::integral_constant<int, 0>;
+    using S1 = std::integral_constant<int, 1>;
+    int p = 0;
+#pragma nounroll
+    for (; p + 2 <= P; p += 2) {
+      step(p, S0{}, std::false_type{});
+      step(p + 1, S1{}, std::false_type{});
+    }
+    if (p < P) step(p, S0{}, std::true_type{});
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) T[i][NB - 1][e] = fmaf(sp[i], y[1][i][e], T[i][NB - 1][e]);
+  };
+  const int nb = (tl.z + 31) >> 5;
+  if (nb == 2)
+    stages(std::integral_constant<int, 2>{});
+  else
+    stages(std::integral_constant<int, 1>{});
+
+  // the offsets' sum, as in moe_tile_kernel, two octets a product
+  const int gp = gpad(K), go = gp >> 3;
+#pragma nounroll
+  for (int jb = 0; 2 * jb < 3 * go; ++jb) {
+    const int o = 2 * jb + c2, oc = o < go ? o : o < 2 * go ? o - go : o - 2 * go;
+    u32x4 as[2], ab[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const int ps = 4 * oc + q;
+        const bool in = o < 3 * go && ps < P;
+        const uint32_t* const sq = sb + (fr[i] * P + (in ? ps : 0)) * 32 + (r32 & 15);
+        as[i][q] = in ? sq[0] : 0u;
+        ab[i][q] = in ? sq[16] : 0u;
+      }
+#pragma unroll
+    for (int u = 0; u < RB; ++u) {
+      if (32 * u >= tl.z) continue;
+      const int r = min(u * 32 + r32, tl.z - 1);
+      const uint16_t* const xg =
+          UP ? s.xs + (int64_t)row_of[r].x * 3 * gp : s.hs + (int64_t)(tl.y + r) * 3 * gp;
+      const u32x4 xp = *reinterpret_cast<const u32x4*>(xg + 8 * (o < 3 * go ? o : 0));
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x16 y;
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[e] = 0.f;
+        y = mfma32(xp, as[i], y);
+        T[i][u] = mfma32(xp, ab[i], T[i][u]);
+#pragma unroll
+        for (int e = 0; e < 16; ++e) T[i][u][e] = fmaf(-128.0f, y[e], T[i][u][e]);
+      }
+    }
+  }
+
+  // The results go through LDS, so that rows are written 16 bytes a lane; the
+  // slots are free once every wave is here.
+  lds_barrier();
+  if constexpr (UP) {
+    uint16_t* const hb = reinterpret_cast<uint16_t*>(xl0);  // [MT][128], chunks of 8 swizzled
+    const int c = 32 * wave + r32;
+#pragma unroll
+    for (int u = 0; u < RB; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = 32 * u + 8 * (e >> 2) + 4 * c2 + (e & 3);
+        if (live) hb[r * 128 + 8 * ((c >> 3) ^ (r & 15)) + (c & 7)] = f2bf(swiglu(T[0][u][e], T[1][u][e]));
+      }
+    lds_barrier();
+    const int gi = gpad(a.inner), ch = tid & 15, cols = min(128, a.inner - 128 * cb);
+#pragma unroll
+    for (int j = 0; j < MT / 16; ++j) {
+      const int r = 16 * j + (tid >> 4);
+      if (r >= tl.z || 8 * ch >= cols) continue;
+      const u32x4 v = *reinterpret_cast<const u32x4*>(hb + r * 128 + 8 * (ch ^ (r & 15)));
+      *reinterpret_cast<u32x4*>(s.h + (int64_t)(tl.y + r) * a.inner + 128 * cb + 8 * ch) = v;
+      float t = 0.f;
+#pragma unroll
+      for (int q = 0; q < 4; ++q) t += bf_lo(v[q]) + bf_hi(v[q]);
+      t = sum8(t);
+      if ((ch & 7) == 0) {
+        uint16_t* const dst = s.hs + (int64_t)(tl.y + r) * 3 * gi;
+        store_split(t, dst + 2 * cb + (ch >> 3), gi);
+        if (cb == blocks - 1 && ch == 0)  // the padded groups
+          for (int g = a.inner >> 6; g < gi; ++g) store_split(0.f, dst + g, gi);
+      }
+    }
+  } else {
+    if (!live) return;
+    // a wave's 32 rows at a time, [32][64] with 8-column chunks swizzled
+    uint16_t* const ob = reinterpret_cast<uint16_t*>(xl0) + wave * 32 * 64;
+#pragma unroll
+    for (int u = 0; u < RB; ++u) {
+      if (32 * u >= tl.z) break;
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = 8 * (e >> 2) + 4 * c2 + (e & 3);
+        const float wt = wt_of[32 * u + r];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+          const int c = 32 * i + r32;
+          ob[r * 64 + 8 * ((c >> 3) ^ (r & 7)) + (c & 7)] = f2bf(wt * T[i][u][e]);
         }
       }
+      wait_lgkm0();
+      __builtin_amdgcn_wave_barrier();
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const int r = 8 * j + (lane >> 3), ch = lane & 7;
+        const u32x4 v = *reinterpret_cast<const u32x4*>(ob + r * 64 + 8 * (ch ^ (r & 7)));
+        if (32 * u + r < tl.z)
+          *reinterpret_cast<u32x4*>(s.rows +
+                                    (int64_t)row_of[32 * u + r].y * a.hidden + 256 * cb + 64 * wave +
+                                    8 * ch) = v;
+      }
+      wait_lgkm0();
+      __builtin_amdgcn_wave_barrier();
     }
   }
 }
 
-// h of one tile's rows, 16 inner columns: work-group (tile, column block) of
-// four waves, each over a quarter of the stages, added in wave order.
-__global__ __launch_bounds__(256) void moe_up_kernel(MoeArgs a, MoeSpace s) {
-  const int blocks = a.inner / 16;
-  const int tile = blockIdx.x / blocks, j = blockIdx.x - tile * blocks;
-  if (tile >= *s.ntiles) return;
-  __shared__ f32x4 part[4][2][64];
-  const int4 tl = s.tiles[tile];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15;
-  const int P = a.hidden >> 7;
-  const int row = min(r16, tl.z - 1);
-  const uint16_t* const xrow = a.x + (int64_t)(s.perm[tl.y + row] / a.k) * a.xs;
-  const int64_t f = ((int64_t)tl.x * blocks + j) * 2 * P;
-  f32x4 T[2];
-  tile_product<2>(xrow, r16 < tl.z, static_cast<const u32x4*>(a.w1) + f * 64, a.sb1 + f * 16, P,
-                  4 * wave, 16, T);
-  part[wave][0][lane] = T[0];
-  part[wave][1][lane] = T[1];
-  __syncthreads();
-  // thread (element i of lane l): row 4 (l / 16) + i, column l % 16
-  const int l = threadIdx.x >> 2, i = threadIdx.x & 3, m = 4 * (l >> 4) + i;
-  float g = 0.f, u = 0.f;
+// Down for experts with many rows and inner up to 512: a tile of 64 rows stays in
+// LDS (four stages) while the work-group takes `run` blocks of 256 columns one
+// after the other, weights ahead across blocks; no wave waits for another.
+// Products, tasks and roles as in moe_wide_kernel.
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
+    moe_wide_down_kernel(MoeArgs a, MoeSpace s, int run) {
+  constexpr int MT = 64, XROW = kStageK * 2, SLOT = MT * XROW;
+  __shared__ __align__(16) uint8_t xl[4 * SLOT];
+  __shared__ __align__(16) uint16_t stage_out[4][16 * 64];
+  __shared__ u32x4 sums[MT][3];  // a row's split group sums: hi, mid, lo octet
+  __shared__ int en_of[MT];
+  __shared__ __align__(16) float wt_of[MT];
+  const int P = a.inner >> 7, N = a.hidden, blocks = (N + 255) >> 8;
+  const int chunks = (blocks + run - 1) / run;
+  const int n = *s.ntiles * chunks, per = (n + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || idx >= n) return;
+  const int tile = idx / chunks;
+  const int cb0 = (idx - tile * chunks) * run, cb1 = min(cb0 + run, blocks);
+  int4 tl = s.tiles[tile];
+  tl.x = __builtin_amdgcn_readfirstlane(tl.x);
+  tl.y = __builtin_amdgcn_readfirstlane(tl.y);
+  tl.z = __builtin_amdgcn_readfirstlane(tl.z);
+  if (tl.z == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r32 = lane & 31, c2 = lane >> 5;
+
+  // the rows of all stages, and what goes with a row
+  {
+    const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)(s.h + (int64_t)tl.y * a.inner), (short)0, -1, 0x00020000);
+    for (int p = 0; p < P; ++p)
 #pragma unroll
-  for (int w = 0; w < 4; ++w) {
-    g += part[w][0][l][i];
-    u += part[w][1][l][i];
+      for (int j = 0; j < 4; ++j) {
+        const int r = 4 * (wave + 4 * j) + (lane >> 4);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(
+            xrs,
+            (void __attribute__((address_space(3)))*)(xl + p * SLOT + 4 * (wave + 4 * j) * XROW), 16,
+            min(r, tl.z - 1) * a.inner * 2 + 16 * ((lane & 15) ^ (r & 15)), p * XROW, 0, 0);
+      }
+    if (tid < 3 * MT)
+      sums[tid / 3][tid % 3] = *reinterpret_cast<const u32x4*>(
+          s.hs + ((int64_t)tl.y + min(tid / 3, tl.z - 1)) * 24 + 8 * (tid % 3));
+    if (tid < MT) {
+      const int en = s.perm[tl.y + min(tid, tl.z - 1)].y;
+      en_of[tid] = en;
+      wt_of[tid] = a.weights[en];
+    }
+    wait_vm<0>();
+    __syncthreads();
   }
-  if (m < tl.z) s.h[(int64_t)(tl.y + m) * a.inner + 16 * j + (l & 15)] = f2bf(swiglu(g, u));
+  const int f16 = r32 >> 4;  // which of a column fragment's two 16-row fragments
+  const u32x4* const wp = static_cast<const u32x4*>(a.w2) + (int64_t)tl.x * (N >> 4) * P * 64;
+  const uint32_t* const sb = a.sb2 + (int64_t)tl.x * (N >> 4) * P * 32;
+  const int wvo = (f16 * P * 64 + 16 * c2 + (r32 & 15)) * 16;
+  const int svo = f16 * P * 128 + (r32 & 15) * 4;
+  // this wave's blocks: those whose 64 columns are there
+  const int cbw = min(cb1, (N - 64 * wave + 255) >> 8);
+  if (cb0 >= cbw) return;
+  u32x4 wr[2][2];
+  uint32_t sr[2], ob[2][4];
+  auto batch_w = [&](int cb, int p) {
+    const int in = __builtin_amdgcn_readfirstlane(cb < cbw ? -1 : 0);
+    const __amdgpu_buffer_rsrc_t wrs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)wp, (short)0, in & ((N >> 4) * P * 1024), 0x00020000);
+    const __amdgpu_buffer_rsrc_t srs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)sb, (short)0, in & ((N >> 4) * P * 128), 0x00020000);
+    const int f0 = 16 * cb + 4 * wave;
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+#pragma unroll
+      for (int g = 0; g < 2; ++g)
+        wr[i][g] = __builtin_amdgcn_raw_buffer_load_b128(wrs, wvo + 512 * g,
+                                                         ((f0 + 2 * i) * P + p) * 1024, 0);
+      sr[i] = __builtin_amdgcn_raw_buffer_load_b32(srs, svo, ((f0 + 2 * i) * P + p) * 128, 0);
+    }
+  };
+  uint32_t nib = 0x000F000Fu;
+  asm volatile("" : "+v"(nib));
+
+  auto body = [&](auto nbc) {
+    constexpr int NB = decltype(nbc)::value;
+    f32x16 T[2][NB], y[2][2];
+    float sp[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        y[1][i][e] = 0.f;
+#pragma unroll
+        for (int u = 0; u < NB; ++u) T[i][u][e] = 0.f;
+      }
+    u32x4 X[2][2][2], W[2][2][2];
+    const int xrd = r32 * XROW + ((c2 ^ (r32 & 15)) << 4);
+    auto rows = [&](int at, auto tc) {
+      constexpr int t = decltype(tc)::value, gl = t / NB, u = t % NB;
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+          X[t & 1][d][g] = *reinterpret_cast<const u32x4*>(
+              xl + u * 32 * XROW + (at ^ ((8 * gl + 4 * d + 2 * g) << 4)));
+    };
+    auto unpack = [&](int gl) {
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int d = 0; d < 2; ++d)
+#pragma unroll
+          for (int g = 0; g < 2; ++g) W[i][d][g] = unpack_w(wr[i][g][2 * gl + d], nib);
+    };
+    auto task = [&](int at, auto tc) {
+      constexpr int t = decltype(tc)::value, up = (t + NB - 1) % NB;
+      if constexpr (t + 1 < 2 * NB) rows(at, std::integral_constant<int, t + 1>{});
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e) y[t & 1][i][e] = 0.f;
+#pragma unroll
+      for (int d = 0; d < 2; ++d)
+#pragma unroll
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+            y[t & 1][i] = mfma32(X[t & 1][d][g], W[i][d][g], y[t & 1][i]);
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int e = 0; e < 16; ++e)
+          T[i][up][e] = fmaf(sp[i], y[1 - (t & 1)][i][e], T[i][up][e]);
+      if constexpr (t + 1 < 2 * NB) __builtin_amdgcn_sched_group_barrier(0x100, 4, 0);
+#pragma unroll
+      for (int q = 0; q < 8; ++q) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        __builtin_amdgcn_sched_group_barrier(0x002, 4, 0);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    };
+    batch_w(cb0, 0);
+    for (int cb = cb0; cb < cbw; ++cb) {
+#pragma nounroll
+      for (int p = 0; p < P; ++p) {
+        int at = xrd + p * SLOT;
+        asm volatile("" : "+v"(at));
+        rows(at, std::integral_constant<int, 0>{});
+        unpack(0);
+        const float s0[2] = {bf_lo(sr[0]), bf_lo(sr[1])}, s1[2] = {bf_hi(sr[0]), bf_hi(sr[1])};
+        __builtin_amdgcn_sched_barrier(0);
+        task(at, std::integral_constant<int, 0>{});
+        sp[0] = s0[0], sp[1] = s0[1];
+        if constexpr (NB > 1) task(at, std::integral_constant<int, 1 % (2 * NB)>{});
+        unpack(1);
+        // the sums so far are not moved behind the branch
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+          for (int u = 0; u < NB; ++u) asm volatile("" : "+v"(T[i][u]));
+        if (p + 1 < P) {
+          batch_w(cb, p + 1);
+        } else {
+          batch_w(cb + 1, 0);
+          // biases (lanes c2 = 0) or scales (c2 = 1) of the block's stages
+          const __amdgpu_buffer_rsrc_t srs = __builtin_amdgcn_make_buffer_rsrc(
+              (void*)sb, (short)0, (N >> 4) * P * 128, 0x00020000);
+#pragma unroll
+          for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+              ob[i][q] = __builtin_amdgcn_raw_buffer_load_b32(
+                  srs, svo + (c2 ? 0 : 64), ((16 * cb + 4 * wave + 2 * i) * P + min(q, P - 1)) * 128, 0);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        task(at, std::integral_constant<int, NB>{});
+        sp[0] = s1[0], sp[1] = s1[1];
+        if constexpr (NB > 1) task(at, std::integral_constant<int, NB + 1 < 2 * NB ? NB + 1 : NB>{});
+      }
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+#pragma unroll
+        for (int e = 0; e < 16; ++e) T[i][NB - 1][e] = fmaf(sp[i], y[1][i][e], T[i][NB - 1][e]);
+        sp[i] = 0.f;
+      }
+      // the offsets' sum: both lane groups hold the same octet of X, against b
+      // and against -128 s
+      u32x4 B[2];
+      const float f = c2 ? -128.0f : 1.0f;
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)
+          B[i][q] = q < P ? f2bf2(f * bf_lo(ob[i][q]), f * bf_hi(ob[i][q])) : 0u;
+#pragma unroll
+      for (int k = 0; k < 3; ++k)
+#pragma unroll
+        for (int u = 0; u < NB; ++u) {
+          const u32x4 xp = sums[32 * u + r32][k];
+#pragma unroll
+          for (int i = 0; i < 2; ++i) T[i][u] = mfma32(xp, B[i], T[i][u]);
+        }
+      // Through LDS, 16 rows at a time, so that rows are written 16 bytes a lane:
+      // 8-column chunk ch of row r at chunk ch ^ (r % 8). The lane's first byte is
+      // that of row 4 c2, column r32; other rows and columns flip or add bits.
+      char* const so = reinterpret_cast<char*>(stage_out[wave]);
+      int wat = 512 * c2 + (((r32 >> 3) | 4 * c2) << 4) + 2 * (r32 & 7);
+      int rat = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+      asm volatile("" : "+v"(wat), "+v"(rat));  // addresses formed here, not kept
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int r0 = 32 * u + 16 * hf;
+          if (r0 >= tl.z) break;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const v4f wt = *reinterpret_cast<const v4f*>(&wt_of[r0 + 8 * g + 4 * c2]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<uint16_t*>(so + (wat ^ ((e << 4) | (i << 6))) + 128 * e + 1024 * g) =
+                    f2bf(wt[e] * T[i][u][8 * hf + 4 * g + e]);
+          }
+          wait_lgkm0();
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = r0 + 8 * j + (lane >> 3);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(so + rat + 1024 * j);
+            if (r < tl.z)
+              *reinterpret_cast<u32x4*>(s.rows + (int64_t)en_of[r] * N +
+                                        256 * cb + 64 * wave + 8 * (lane & 7)) = v;
+          }
+          wait_lgkm0();
+          __builtin_amdgcn_wave_barrier();
+        }
+#pragma unroll
+      for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int u = 0; u < NB; ++u)
+#pragma unroll
+          for (int e = 0; e < 16; ++e) T[i][u][e] = 0.f;
+    }
+  };
+  if (tl.z > 32)
+    body(std::integral_constant<int, 2>{});
+  else
+    body(std::integral_constant<int, 1>{});
 }
 
-// The weighted rows of down: a wave per 32 columns of a tile.
-__global__ __launch_bounds__(256) void moe_down_kernel(MoeArgs a, MoeSpace s) {
-  const int blocks = a.hidden / 128;
-  const int tile = blockIdx.x / blocks, cb = blockIdx.x - tile * blocks;
-  if (tile >= *s.ntiles) return;
-  const int4 tl = s.tiles[tile];
-  const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, r16 = lane & 15, c4 = lane >> 4;
-  const int P = a.inner >> 7, f0 = cb * 8 + 2 * wave;
-  const uint16_t* const hrow = s.h + (int64_t)(tl.y + min(r16, tl.z - 1)) * a.inner;
-  const int64_t f = ((int64_t)tl.x * (a.hidden / 16) + f0) * P;
-  f32x4 T[2];
-  tile_product<2>(hrow, r16 < tl.z, static_cast<const u32x4*>(a.w2) + f * 64, a.sb2 + f * 16, P, 0,
-                  4, T);
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const int m = 4 * c4 + i;
-    if (m >= tl.z) continue;
-    const int en = s.perm[tl.y + m];
-    const float wt = a.weights[en];
-    float* const o = s.rows + (int64_t)en * a.hidden + 16 * f0 + r16;
-    o[0] = wt * T[0][i];
-    o[16] = wt * T[1][i];
-  }
-}
-
-// out[t] = the sum of its entries' rows in column order. A thread per 4 columns.
-__global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, MoeSpace s) {
-  const int q = a.hidden / 4;
+// out[t] = the sum of its entries' rows in column order. A thread per 8 columns,
+// eight rows' loads at a time. Bound by reading the rows.
+__global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const uint16_t* rows) {
+  const int q = a.hidden / 8;
   const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= (int64_t)a.T * q) return;
   const int64_t t = i / q;
-  const int c = (int)(i - t * q) * 4;
-  f32x4 y = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < a.k; ++j)
-    if ((uint32_t)a.ids[t * a.k + j] < (uint32_t)a.experts)
-      y += *reinterpret_cast<const f32x4*>(s.rows + (t * a.k + j) * a.hidden + c);
-  *reinterpret_cast<u32x2*>(a.out + t * a.os + c) = (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
+  const int c = (int)(i - t * q);
+  const u32x4* const r = reinterpret_cast<const u32x4*>(rows) + t * a.k * q + c;
+  float y[8] = {};
+  for (int j0 = 0; j0 < a.k; j0 += 8) {
+    u32x4 v[8];
+#pragma unroll
+    for (int j = 0; j < 8; ++j) {
+      v[j] = (u32x4){0u, 0u, 0u, 0u};
+      if (j0 + j < a.k && (uint32_t)a.ids[t * a.k + j0 + j] < (uint32_t)a.experts)
+        v[j] = __builtin_nontemporal_load(r + (int64_t)(j0 + j) * q);
+    }
+#pragma unroll
+    for (int j = 0; j < 8; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) {
+        y[2 * e] += bf_lo(v[j][e]);
+        y[2 * e + 1] += bf_hi(v[j][e]);
+      }
+  }
+  u32x2* const o = reinterpret_cast<u32x2*>(a.out + t * a.os + c * 8);
+  o[0] = (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
+  o[1] = (u32x2){f2bf2(y[4], y[5]), f2bf2(y[6], y[7])};
+}
+
+dim3 tile_grid(int64_t tiles, int blocks) {
+  return dim3((unsigned)(tiles * blocks + 7) & ~7u);  // the same number for every XCD
+}
+
+template <int MW>
+void launch_tiles(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
+  hipLaunchKernelGGL((moe_tile_kernel<MW, true>), tile_grid(slots, a.inner / 64), dim3(256), 0,
+                     a.stream, a, s);
+  hipLaunchKernelGGL((moe_tile_kernel<MW, false>), tile_grid(slots, a.hidden / 128), dim3(256), 0,
+                     a.stream, a, s);
+}
+
+void launch_wide(const MoeArgs& a, const MoeSpace& s, int64_t slots, int64_t tiles) {
+  hipLaunchKernelGGL(moe_wide_kernel<true>, tile_grid(slots, (a.inner + 127) / 128), dim3(256), 0,
+                     a.stream, a, s);
+  const int blocks = (a.hidden + 255) / 256;
+  if (a.inner > 4 * kStageK) {
+    hipLaunchKernelGGL(moe_wide_kernel<false>, tile_grid(slots, blocks), dim3(256), 0, a.stream, a,
+                       s);
+    return;
+  }
+  int run = blocks;  // long runs, as long as they leave two work-groups per slot of 512
+  while (run > 1 && tiles * ((blocks + run - 1) / run) < 1024) run = (run + 1) / 2;
+  hipLaunchKernelGGL(moe_wide_down_kernel, tile_grid(slots, (blocks + run - 1) / run), dim3(256), 0,
+                     a.stream, a, s, run);
 }
 
 }  // namespace
-
-hipError_t launch_moe_route(const MoeRouteArgs& a) {
-  const bool by_logit = !a.bias && (a.d.group_top == 1 || a.d.num_groups == 1);
-  const int R = (a.d.num_experts + 63) / 64;
-  return R <= 1   ? launch_route<1>(a, by_logit)
-         : R <= 2 ? launch_route<2>(a, by_logit)
-         : R <= 4 ? launch_route<4>(a, by_logit)
-         : R <= 8 ? launch_route<8>(a, by_logit)
-                  : launch_route<16>(a, by_logit);
-}
 
 hipError_t launch_moe_pack(const MoePackArgs& a) {
   const int blocks = (a.n * (a.k / 128) * 4 + 255) / 256;
@@ -508,28 +1401,61 @@ hipError_t launch_moe_pack(const MoePackArgs& a) {
   return hipGetLastError();
 }
 
+// A pass's rows of x are reached by 32-bit byte offsets.
 int moe_pass_tokens(int k, int64_t x_stride) {
-  (void)x_stride;
-  return kPassEntries / k;
+  const int64_t n = kPassEntries / k, reach = INT32_MAX / x_stride;
+  return (int)(n < reach ? n : reach > 1 ? reach : 1);
 }
 
 size_t moe_workspace_bytes(int hidden, int inner, int experts, int T, int k) {
-  const int64_t entries = (int64_t)T * k;
-  return moe_space(nullptr, hidden, inner, experts, entries < kPassEntries ? entries : kPassEntries)
-      .bytes;
+  int64_t entries = (int64_t)T * k, tokens = T;
+  if (entries > kPassEntries) entries = kPassEntries;
+  if (tokens > kPassEntries) tokens = kPassEntries;
+  return moe_space(nullptr, hidden, inner, experts, tokens, entries).bytes;
 }
 
 hipError_t launch_moe(const MoeArgs& a) {
   const int entries = a.T * a.k;
-  const MoeSpace s = moe_space(a.workspace, a.hidden, a.inner, a.experts, entries);
-  const unsigned tiles = (unsigned)max_tiles(entries, a.experts);
-  hipLaunchKernelGGL(moe_plan_kernel, dim3(a.experts), dim3(kPlanThreads), a.experts * 4, a.stream,
-                     a.ids, entries, a.experts, s.ntiles, s.tiles, s.perm);
-  hipLaunchKernelGGL(moe_up_kernel, dim3(tiles * (a.inner / 16)), dim3(256), 0, a.stream, a, s);
-  hipLaunchKernelGGL(moe_down_kernel, dim3(tiles * (a.hidden / 128)), dim3(256), 0, a.stream, a, s);
-  const int64_t n = (int64_t)a.T * (a.hidden / 4);
-  hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, a.stream,
-                     a, s);
+  const MoeSpace s = moe_space(a.workspace, a.hidden, a.inner, a.experts, a.T, entries);
+  if (entries <= kFewEntries && a.T <= kFewTokens) {
+    hipLaunchKernelGGL(moe_few_up_kernel, dim3(entries * (a.inner / 16)), dim3(256), 0, a.stream, a,
+                       s.h);
+    hipLaunchKernelGGL(moe_few_down_kernel, dim3(a.T * (a.hidden / 16)),
+                       dim3(64 * (a.k < 16 ? a.k : 16)), 0, a.stream, a, s.h);
+    return hipGetLastError();
+  }
+  // Rows of a tile by the rows that an expert has on average. At hidden 2048,
+  // inner 512, 257 experts, 9 columns, 16 / 32 / 64 rows: 64 tokens 91 / 94 / 115
+  // us, 317 tokens 114 / 117 / 143, 600 tokens 145 / 135 / 153, 2000 tokens 315 /
+  // 259 / 233. Tiles of 64 rows also want a work-group for most of the 512 that
+  // run side by side (hidden 1024, inner 1408, 32 experts, 4 columns: 1000 tokens,
+  // 312 work-groups, 78 us by 32 rows and 79 by 64; 1500 tokens, 436, 101 / 93).
+  const int mean = entries / a.experts;
+  const int64_t wide_tiles = max_tiles(entries, a.experts, 64) - a.experts / 2;
+  const bool wide = mean >= 64 && wide_tiles * ((a.hidden + 255) / 256) >= 384;
+  const int rows = wide ? 64 : mean <= 16 ? 16 : 32;
+  const int64_t slots = max_tiles(entries, a.experts, rows);
+  const int64_t sums = (int64_t)a.T * 8 * gpad(a.hidden);
+  const unsigned sum_groups = (unsigned)((sums + kPlanThreads - 1) / kPlanThreads);
+  if (entries <= kPlanEntries) {
+    hipLaunchKernelGGL(moe_plan_kernel, dim3(a.experts + sum_groups), dim3(kPlanThreads), 0,
+                       a.stream, a, rows, s);
+  } else {
+    const unsigned chunks = (unsigned)((entries + kChunk - 1) / kChunk);
+    hipLaunchKernelGGL(moe_count_kernel, dim3(chunks + sum_groups), dim3(kPlanThreads),
+                       a.experts * 4, a.stream, a, chunks, s);
+    hipLaunchKernelGGL(moe_place_kernel, dim3(chunks), dim3(kPlanThreads), a.experts * 8, a.stream,
+                       a, rows, s);
+  }
+  if (wide)
+    launch_wide(a, s, slots, wide_tiles);
+  else if (rows == 16)
+    launch_tiles<1>(a, s, slots);
+  else
+    launch_tiles<2>(a, s, slots);
+  const int64_t n = (int64_t)a.T * (a.hidden / 8);
+  hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, a.stream, a,
+                     s.rows);
   return hipGetLastError();
 }
 

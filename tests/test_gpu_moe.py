@@ -293,6 +293,11 @@ def draw_x(seed, T, hidden):
     (4096, 128, [2], 5, 1),
     (128, 2048, [2], 5, 2),
     (2176, 256, [3], 130, 2),
+    (128, 128, [300], 3000, 4),   # more than 8192 entries
+    (128, 128, [1030], 2100, 4),  # and more experts than threads that place them
+    (2048, 128, [2], 1700, 2),    # tiles of 64 rows, down's input in LDS
+    (1792, 384, [3, 1], 2100, 3),
+    (1152, 640, [2, 1], 1700, 3), # and in stages, half a block of columns over
 ])
 def test_experts(gpu, hidden, inner, parts, T, k):
     ex = Experts(hidden, inner, parts, seed=hidden + inner)
@@ -300,7 +305,7 @@ def test_experts(gpu, hidden, inner, parts, T, k):
     ex.check(draw_x(T, T, hidden), ids, w)
 
 
-@pytest.mark.parametrize("T", [1, 4, 19, 300, 1100])
+@pytest.mark.parametrize("T", [1, 4, 19, 300, 1100, 2500])
 def test_experts_uneven_absent_and_repeated_ids(gpu, T):
     """All rows on one expert, experts without rows, ids outside the layer, tokens
     without any, an expert twice in a token, weights that are zero or negative."""
