@@ -439,8 +439,9 @@ gdn_status gdn_layer_prefill(gdn_layer* layer, const int32_t* slot_ids,
  * :723-743 without the MLP half). A mixer is a GatedDeltaNet layer or, at the
  * positions attn_layers name, an attention layer (qwen3_5.rs:377-455: merged
  * q|k|v projection, gdn_attn_forward on the executor's gdn_kv, o_proj). The
- * KV cache uses the pool's slot ids. MoE MLPs and temperature sampling are
- * outside this library; the greedy pick keeps runs reproducible.
+ * KV cache uses the pool's slot ids. The layers' sparse MLP halves are added
+ * by gdn_exec_set_moe. Temperature sampling is outside this library; the
+ * greedy pick keeps runs reproducible.
  *
  * One thread owns an executor (qwen_mlx_serve.rs:96-99). All its device work
  * runs on the stream given at creation, in call order. Sequence ids are the
@@ -742,6 +743,28 @@ gdn_status gdn_moe_forward(const gdn_moe* moe, const uint16_t* x, int64_t x_stri
                            int32_t k, const int32_t* ids, const float* weights, uint16_t* out,
                            int64_t out_stride, void* workspace, size_t workspace_bytes,
                            void* stream);
+
+/* The MLP half of one decoder layer for an executor: behind its mixer
+ *   h = h + mixer output
+ *   h = h + gdn_moe_forward(rms_norm(h, norm_w), gdn_moe_route(gate(..)))
+ * (DecoderLayer::forward_with_cache, qwen3_5.rs:735-739). */
+typedef struct gdn_exec_moe {
+  int32_t position;                /* index in the decoder stack                  */
+  const uint16_t* norm_w;          /* post_attention_layernorm [hidden] bf16, 16-byte aligned */
+  const gdn_qlinear* gate;         /* hidden -> the router's logits: num_experts (and one
+                                      more with shared_gate) columns or more      */
+  const gdn_moe_route_desc* route; /* copied; logits_f32 0, num_experts + num_shared the
+                                      experts of moe                              */
+  const float* bias;               /* [num_experts] or NULL                       */
+  const gdn_moe* moe;              /* hidden sizes equal                          */
+} gdn_exec_moe;
+
+/* Give n layers of the executor's stack their MLP halves (positions distinct;
+ * n = 0 takes all away). While the executor holds no sequences. Allocates the
+ * halves' logits, ids, weights and workspace for the executor's largest step
+ * once, shared by all layers: steps and prefills allocate nothing for them.
+ * The layers keep pointers to the weights. */
+gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layers);
 
 /* The seam behind and before a block in general form (gdn_add_rms_norm is the
  * decoder's own): over n rows

@@ -4,6 +4,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <memory>
+#include <vector>
+
 #include "gdn.h"
 
 namespace gdn {
@@ -461,6 +464,24 @@ hipError_t launch_block_norm(const BlockNormArgs& a);
 
 // Sets the calling thread's gdn_last_error() message and returns code.
 gdn_status set_error(gdn_status code, const char* msg);
+
+// The MLP half that an executor runs behind decoder layer `position`'s mixer:
+//   h += mixer output; hn = rms_norm(h, norm_w); h += run(hn)   (qwen3_5.rs:735-739)
+// run writes n rows of out [n, hidden] on the stream by kernel launches alone
+// (a decode step's are captured). ctx lives as long as the executor needs it.
+struct ExecMlp {
+  int position = 0;
+  const uint16_t* norm_w = nullptr;
+  gdn_status (*run)(void* ctx, const uint16_t* hn, int n, uint16_t* out, hipStream_t s) = nullptr;
+  std::shared_ptr<void> ctx;
+};
+struct ExecShape {
+  int hidden, rows, depth, device;  // rows: the most a step or prefill runs
+};
+ExecShape exec_shape(const gdn_exec* x);
+// Replaces the executor's MLP halves (at most one a position). Refused while the
+// executor holds sequences.
+gdn_status exec_set_mlp(gdn_exec* x, std::vector<ExecMlp> halves);
 
 // Executor model-body kernels (gdn_exec.hip).
 hipError_t launch_embed(const uint16_t* table, const int32_t* tok, int n, int vocab, int hidden,

@@ -78,6 +78,7 @@ struct gdn_exec {
   // decoder stack: entry >= 0 is GDN layer entry, < 0 attention layer -entry - 1
   std::vector<int> stack;
   std::vector<const uint16_t*> norm_w;  // per stack position
+  std::vector<gdn::ExecMlp> mlp;        // per stack position; run null: none
   gdn_kv* kv = nullptr;
   float rope_theta = 0.f;
   int rotary_dim = 0, Hq = 0, Hkv = 0, nqkv = 0;
@@ -191,6 +192,18 @@ gdn_status seam(gdn_exec* x, size_t p, int n, const int32_t* toks, uint16_t* xsp
   return GDN_OK;
 }
 
+// The MLP half behind position p's mixer, if there is one: its output takes the
+// mixer's place in mix, for the next seam to add.
+gdn_status mlp_half(gdn_exec* x, size_t p, int n) {
+  if (p >= x->mlp.size() || !x->mlp[p].run) return GDN_OK;
+  const gdn::ExecMlp& m = x->mlp[p];
+  HIP_TRY(gdn::launch_add_norm(x->h, x->mix, &x->pend, n, x->hidden, m.norm_w, x->eps, x->hn,
+                               x->stream),
+          "residual add + norm before the MLP");
+  x->pend = gdn::QPartial{};
+  return m.run(m.ctx.get(), x->hn, n, x->mix, x->stream);
+}
+
 // The model body over n rows of the tokens toks: every decoder layer with its
 // residual seam (an empty stack only embeds). Prefill rows are nseq packed
 // sequences. The KV step for these rows is planned before this runs.
@@ -219,6 +232,7 @@ gdn_status run_layers(gdn_exec* x, int n, bool prefill, const int32_t* toks, int
       GDN_TRY(gdn::layer_decode(x->layers[e], slots, n, x->hn, x->hidden, x->mix, x->hidden,
                                 x->stream, &x->pend));
     }
+    GDN_TRY(mlp_half(x, p, n));
   }
   return GDN_OK;
 }
@@ -254,6 +268,7 @@ gdn_status decode_seg(gdn_exec* x, int B, int k, int ps) {
       if (e >= 0) {
         GDN_TRY(gdn::layer_decode(x->layers[e], x->d_dec, B, x->hn, x->hidden, x->mix, x->hidden,
                                   x->stream, &x->pend, xsp));
+        GDN_TRY(mlp_half(x, p, B));
       } else {
         GDN_TRY(gdn_qlinear_forward(x->attn[-e - 1].qkv, x->hn, x->hidden, B, x->qkv, x->nqkv,
                                     x->stream));
@@ -261,9 +276,11 @@ gdn_status decode_seg(gdn_exec* x, int B, int k, int ps) {
     }
     if (e < 0) {
       ++seg;
-      if (seg == k)
+      if (seg == k) {
         GDN_TRY(gdn::qlinear_forward(x->attn[-e - 1].o, x->att, x->Hq * 256, B, x->mix, x->hidden,
                                      x->stream, &x->pend));
+        GDN_TRY(mlp_half(x, p, B));
+      }
     }
   }
   if (seg != k) return GDN_OK;
@@ -370,6 +387,24 @@ gdn_status queue_step(gdn_exec* x, int32_t B) {
 }
 
 }  // namespace
+
+gdn::ExecShape gdn::exec_shape(const gdn_exec* x) {
+  return {x->hidden, x->rows, (int)x->stack.size(), x->device};
+}
+
+gdn_status gdn::exec_set_mlp(gdn_exec* x, std::vector<gdn::ExecMlp> halves) {
+  if (!x->slot_of.empty() || x->pend_n > 0)
+    return efail(GDN_ERR_INVALID, "gdn_exec_set_moe: the executor holds %zu sequences",
+                 x->slot_of.size());
+  DevScope dev(x->device);
+  // nothing queued or captured holds the halves replaced here
+  HIP_TRY(hipStreamSynchronize(x->stream), "gdn_exec_set_moe");
+  drop_graphs(x);
+  x->chain_B = 0;
+  x->mlp.assign(x->stack.size(), gdn::ExecMlp{});
+  for (gdn::ExecMlp& m : halves) x->mlp[m.position] = std::move(m);
+  return GDN_OK;
+}
 
 extern "C" {
 

@@ -67,6 +67,43 @@ void moe_release(gdn_moe* m) {
 
 }  // namespace
 
+namespace {
+
+// What an executor's MLP halves share: the rows between their steps.
+struct ExecMoeBuffers {
+  uint16_t* logits = nullptr;
+  int32_t* ids = nullptr;
+  float* weights = nullptr;
+  void* workspace = nullptr;
+  size_t workspace_bytes = 0;
+  ~ExecMoeBuffers() {
+    for (void* p : {(void*)logits, (void*)ids, (void*)weights, workspace})
+      if (p) (void)hipFree(p);
+  }
+};
+
+struct ExecMoe {
+  const gdn_qlinear* gate = nullptr;
+  int64_t gate_cols = 0;
+  gdn_moe_route_desc route{};
+  const float* bias = nullptr;
+  const gdn_moe* moe = nullptr;
+  std::shared_ptr<ExecMoeBuffers> buf;
+};
+
+gdn_status run_exec_moe(void* ctx, const uint16_t* hn, int n, uint16_t* out, hipStream_t s) {
+  const ExecMoe& m = *static_cast<const ExecMoe*>(ctx);
+  const int k = m.route.top_k + m.route.num_shared;
+  gdn_status st = gdn_qlinear_forward(m.gate, hn, m.moe->hidden, n, m.buf->logits, m.gate_cols, s);
+  if (st != GDN_OK) return st;
+  st = gdn_moe_route(&m.route, m.buf->logits, m.gate_cols, n, m.bias, m.buf->ids, m.buf->weights, s);
+  if (st != GDN_OK) return st;
+  return gdn_moe_forward(m.moe, hn, m.moe->hidden, n, k, m.buf->ids, m.buf->weights, out,
+                         m.moe->hidden, m.buf->workspace, m.buf->workspace_bytes, s);
+}
+
+}  // namespace
+
 extern "C" {
 
 gdn_status gdn_moe_route(const gdn_moe_route_desc* desc, const void* logits,
@@ -295,6 +332,72 @@ gdn_status gdn_moe_forward(const gdn_moe* m, const uint16_t* x, int64_t x_stride
     if (e != hipSuccess) return hip_fail(e, "gdn_moe_forward launch");
   }
   return GDN_OK;
+}
+
+gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layers) {
+  if (!exec) return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: NULL executor");
+  if (n < 0 || (n > 0 && !layers))
+    return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: n = %d / NULL layers", n);
+  const gdn::ExecShape x = gdn::exec_shape(exec);
+  std::vector<char> taken(x.depth, 0);
+  std::vector<gdn::ExecMlp> halves(n);
+  std::vector<std::shared_ptr<ExecMoe>> moes(n);
+  int64_t cols = 0;
+  int entries = 0;
+  size_t workspace = 0;
+  for (int i = 0; i < n; ++i) {
+    const gdn_exec_moe& l = layers[i];
+    if (l.position < 0 || l.position >= x.depth || taken[l.position])
+      return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: half %d at position %d (distinct, < %d)", i,
+                   l.position, x.depth);
+    taken[l.position] = 1;
+    if (!l.norm_w || !l.gate || !l.route || !l.moe || !aligned(l.norm_w, 16))
+      return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: half %d has a NULL or misaligned weight", i);
+    const gdn_moe_route_desc& r = *l.route;
+    int32_t gk = 0, gn = 0;
+    gdn_status st = gdn_qlinear_dims(l.gate, &gk, &gn);
+    if (st != GDN_OK) return st;
+    if (gk != x.hidden || l.moe->hidden != x.hidden || l.moe->device != x.device ||
+        gn < r.num_experts + (r.shared_gate ? 1 : 0) || r.logits_f32 ||
+        (int64_t)r.num_experts + r.num_shared != l.moe->experts)
+      return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: half %d: gate %d -> %d, %d + %d experts "
+                   "routed, layer of %d experts, hidden %d, device %d; executor hidden %d, device %d",
+                   i, gk, gn, r.num_experts, r.num_shared, l.moe->experts, l.moe->hidden,
+                   l.moe->device, x.hidden, x.device);
+    st = gdn_moe_route(&r, nullptr, 0, 0, nullptr, nullptr, nullptr, nullptr);  // its descriptor
+    if (st != GDN_OK) return st;
+    auto m = std::make_shared<ExecMoe>();
+    m->gate = l.gate;
+    m->gate_cols = gn;
+    m->route = r;
+    m->bias = l.bias;
+    m->moe = l.moe;
+    moes[i] = m;
+    const int k = r.top_k + r.num_shared;
+    if (gn > cols) cols = gn;
+    if (k > entries) entries = k;
+    const size_t w = gdn::moe_workspace_bytes(x.hidden, l.moe->inner, l.moe->experts, x.rows, k);
+    if (w > workspace) workspace = w;
+    halves[i].position = l.position;
+    halves[i].norm_w = l.norm_w;
+    halves[i].run = run_exec_moe;
+    halves[i].ctx = m;
+  }
+  if (n > 0) {
+    DeviceScope scope(x.device);
+    auto buf = std::make_shared<ExecMoeBuffers>();
+    buf->workspace_bytes = workspace;
+    if (hipMalloc(&buf->logits, (size_t)x.rows * cols * 2) != hipSuccess ||
+        hipMalloc(&buf->ids, (size_t)x.rows * entries * 4) != hipSuccess ||
+        hipMalloc(&buf->weights, (size_t)x.rows * entries * 4) != hipSuccess ||
+        hipMalloc(&buf->workspace, workspace) != hipSuccess) {
+      (void)hipGetLastError();
+      return mfail(GDN_ERR_OOM, "gdn_exec_set_moe: buffers for %d rows (%zu bytes of workspace)",
+                   x.rows, workspace);
+    }
+    for (auto& m : moes) m->buf = buf;
+  }
+  return gdn::exec_set_mlp(exec, std::move(halves));
 }
 
 gdn_status gdn_block_norm(const gdn_block_norm_desc* desc, int32_t n, const void* h,

@@ -92,6 +92,7 @@ SIGNATURES = {
     "gdn_exec_seq_slot": ([_VP, ctypes.c_uint64, ctypes.POINTER(_I32)], ctypes.c_int),
     "gdn_exec_logits": ([_VP, ctypes.POINTER(_VP), ctypes.POINTER(_I32), ctypes.POINTER(_I32)],
                         ctypes.c_int),
+    "gdn_exec_set_moe": ([_VP, _I32, _VP], ctypes.c_int),
     "gdn_kv_create": ([_VP, ctypes.POINTER(_VP)], ctypes.c_int),
     "gdn_kv_describe": ([_VP, _VP], ctypes.c_int),
     "gdn_pool_describe": ([_VP, _VP], ctypes.c_int),
@@ -152,6 +153,11 @@ class MoeRouteDesc(ctypes.Structure):
                 ("top_groups", _I32), ("group_top", _I32), ("renorm", _I32),
                 ("scale", ctypes.c_float), ("num_shared", _I32), ("shared_gate", _I32),
                 ("logits_f32", _I32)]
+
+
+class ExecMoe(ctypes.Structure):
+    _fields_ = [("position", _I32), ("norm_w", _VP), ("gate", _VP),
+                ("route", ctypes.POINTER(MoeRouteDesc)), ("bias", _VP), ("moe", _VP)]
 
 
 class MoePart(ctypes.Structure):
@@ -294,6 +300,17 @@ def _typed(t, dtypes, what: str):
     return t
 
 
+def route_desc(num_experts, top_k, score="softmax", num_groups=1, top_groups=1, group_top=1,
+               renorm=True, scale=1.0, num_shared=0, shared_gate=False, logits_f32=False):
+    """A router's descriptor (gdn_moe_route_desc)."""
+    codes = {"softmax": 0, "sigmoid": 1}
+    if score not in codes:
+        raise ValueError(f"score must be softmax or sigmoid, not {score!r}")
+    return MoeRouteDesc(num_experts, top_k, codes[score], num_groups, top_groups, group_top,
+                        int(bool(renorm)), float(scale), num_shared, int(bool(shared_gate)),
+                        int(bool(logits_f32)))
+
+
 def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=None, num_groups=1,
               top_groups=1, group_top=1, renorm=True, scale=1.0, num_shared=0, shared_gate=False,
               stream=None):
@@ -301,9 +318,6 @@ def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=No
     shared_gate)] bf16 or f32 rows -> ids int32 and weights f32 [T, top_k + num_shared].
     score: "softmax" or "sigmoid"; bias f32 [num_experts] moves the choice only."""
     import torch
-    codes = {"softmax": 0, "sigmoid": 1}
-    if score not in codes:
-        raise ValueError(f"score must be softmax or sigmoid, not {score!r}")
     lp, ls = _rows(logits)
     T = logits.shape[0]
     if logits.shape[1] < num_experts + (1 if shared_gate else 0):
@@ -313,9 +327,8 @@ def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=No
             raise ValueError(f"{what} must be [{T}, {top_k + num_shared}]")
     if bias is not None and _typed(bias, (torch.float32,), "bias").numel() != num_experts:
         raise ValueError("one bias per expert")
-    d = MoeRouteDesc(num_experts, top_k, codes[score], num_groups, top_groups, group_top,
-                     int(bool(renorm)), float(scale), num_shared, int(bool(shared_gate)),
-                     int(_is_f32(logits, "logits")))
+    d = route_desc(num_experts, top_k, score, num_groups, top_groups, group_top, renorm, scale,
+                   num_shared, shared_gate, _is_f32(logits, "logits"))
     _check(load().gdn_moe_route(ctypes.byref(d), lp, ls, T, _ptr(bias), _ptr(ids), _ptr(weights),
                                 _stream(stream)))
 
@@ -756,12 +769,13 @@ class Executor:
     `pool`, in order; attn_layers: (position, qkv QLinear, o_proj QLinear,
     q_norm_w, k_norm_w) per attention layer, on the KVCache `kv`; input_norm_w:
     one per decoder layer in stack order; embed [vocab, hidden] bf16 device
-    tensor; head: QLinear hidden -> vocab. Sequence ids are caller-chosen
-    integers."""
+    tensor; head: QLinear hidden -> vocab; moe_layers: (position, norm_w, gate
+    QLinear, route_desc(...), bias or None, MoE) per layer with a sparse MLP half
+    (set_moe). Sequence ids are caller-chosen integers."""
 
     def __init__(self, pool, layers, input_norm_w, final_norm_w, embed, head, rms_eps=1e-6,
                  max_batch=64, max_prompt=4096, device=0, stream=None, attn_layers=(), kv=None,
-                 rope_theta=1.0e7, rotary_dim=64):
+                 rope_theta=1.0e7, rotary_dim=64, moe_layers=()):
         self.lib = load()
         attn_layers = list(attn_layers)
         self._keep = (pool, list(layers), list(input_norm_w), final_norm_w, embed, head,
@@ -788,6 +802,19 @@ class Executor:
                     owner._deps = _Dependents()
                 owner._deps.add(self)
                 self._owners.append(owner._deps)
+        if moe_layers:
+            self.set_moe(moe_layers)
+
+    def set_moe(self, moe_layers):
+        """Give layers their sparse MLP halves (gdn_exec_set_moe), while no sequence is
+        held; an empty list takes them away."""
+        moe_layers = list(moe_layers)
+        n = len(moe_layers)
+        arr = (ExecMoe * max(n, 1))(
+            *[ExecMoe(int(p), _ptr(w), gate.handle, ctypes.pointer(route), _ptr(bias), moe.handle)
+              for p, w, gate, route, bias, moe in moe_layers])
+        _check(self.lib.gdn_exec_set_moe(self.handle, n, arr))
+        self._keep_moe = moe_layers
 
     def prefill(self, seq_id: int, prompt) -> int:
         p = (_I32 * len(prompt))(*[int(t) for t in prompt])
