@@ -82,6 +82,8 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 
 constexpr int kPassEntries = 1 << 18;  // of a pass over the experts
 constexpr int kStageK = 128;           // k of a stage: two groups
+// The bytes of x that a pass's 32-bit offsets reach, and an offset past them.
+constexpr uint32_t kReach = 0xFFFF0000u, kNowhere = 0xFFFF8000u;
 
 // Work-space of a pass: the plan, then what the products hand to each other.
 struct MoeSpace {
@@ -340,7 +342,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(MoeArgs a, int 
 // wave holds every id.
 constexpr int kFewEntries = 64;
 // ... and the most tokens: down reads an expert's weights for each of them again.
-constexpr int kFewTokens = 8;
+constexpr int kFewTokens = 6;
 
 // NS stages p0, p0 + step, ... of a 16-row fragment: its weights, scales and
 // biases (stages past P: the last one again; their x is zero).
@@ -760,6 +762,181 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
   }
 }
 
+// moe_tile_kernel for up to 16 rows, where the weights' stream is the work:
+// 64 columns a work-group (small ones fill the chip evenly), KS pairs of waves each
+// over a part of the stages (a wave's stages run one after the other, at about
+// STAGE_US us each, also where nothing is left to wait for), the groups' sums of x
+// from products against ones instead of beforehand, and the offsets applied with
+// the scales. Rows past the tile's are not read: their copies are out of the
+// buffer's range, which gives zeros.
+template <int KS, bool UP>
+__global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))) void
+    moe_stream_kernel(MoeArgs a, MoeSpace s) {
+  constexpr int XROW = kStageK * 2, R = 3, LB = 2 + 2 + 1;
+  __shared__ __align__(16) uint8_t xl0[KS][16 * XROW], xl1[KS][16 * XROW], xl2[KS][16 * XROW];
+  __shared__ __align__(16) uint8_t sl0[512 * KS], sl1[512 * KS], sl2[512 * KS];
+  const int K = UP ? a.hidden : a.inner, N = UP ? 2 * a.inner : a.hidden;
+  const int P = K >> 7, blocks = N >> 6;
+  const int n = *s.ntiles * blocks, per = (n + 7) >> 3;
+  const int idx = (blockIdx.x & 7) * per + (blockIdx.x >> 3);
+  if ((int)(blockIdx.x >> 3) >= per || idx >= n) return;
+  const int tile = idx / blocks, cb = idx - tile * blocks;
+  int4 tl = s.tiles[tile];
+  tl.x = __builtin_amdgcn_readfirstlane(tl.x);
+  tl.y = __builtin_amdgcn_readfirstlane(tl.y);
+  tl.z = __builtin_amdgcn_readfirstlane(tl.z);
+  if (tl.z == 0) return;
+  const int tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r16 = lane & 15, c4 = lane >> 4;
+  const int cw = wave & 1, kw = wave >> 1;  // column pair, part of the stages
+  // the part's stages: p0 + (0 .. mine - 1), mine or one less for every part
+  const int least = P / KS, more = P - least * KS;
+  const int p0 = kw * least + min(kw, more), mine = least + (kw < more);
+
+  const int64_t f0 = (int64_t)tl.x * (N >> 4) + 4 * cb + 2 * cw;  // the wave's first fragment
+  const u32x4* const wp = static_cast<const u32x4*>(UP ? a.w1 : a.w2) + f0 * P * 64;
+  const uint32_t* const sb = (UP ? a.sb1 : a.sb2) + f0 * P * 32;
+  const uint16_t* const xbase = UP ? a.x : s.h + (int64_t)tl.y * a.inner;
+  uint32_t xvo[2];
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {
+    const int r = 4 * (cw + 2 * j) + c4;
+    xvo[j] = kNowhere;
+    if (r < tl.z) {
+      const int64_t at = UP ? (int64_t)s.perm[tl.y + r].x * a.xs : (int64_t)r * a.inner;
+      xvo[j] = (uint32_t)(at * 2) + 16 * (r16 ^ (r & 15));
+    }
+  }
+  // a row's place for the results: the tile's sorted row (up) or its entry
+  const int m = min(r16, tl.z - 1), en = UP ? 0 : s.perm[tl.y + m].y;
+  const float wt = UP ? 0.f : a.weights[en];
+  const int svo = (lane >> 5) * P * 128 + 4 * (lane & 31);  // fragment, dword
+  u32x4 wr[R][2];
+  auto xbuf = [&](auto slot) -> uint8_t* {
+    constexpr int S = decltype(slot)::value;
+    return (S == 0 ? xl0 : S == 1 ? xl1 : xl2)[kw];
+  };
+  auto sbuf = [&](auto slot) -> uint8_t* {
+    constexpr int S = decltype(slot)::value;
+    return (S == 0 ? sl0 : S == 1 ? sl1 : sl2) + wave * 256;
+  };
+  auto batch = [&](int p, auto slot) {
+    constexpr int S = decltype(slot)::value;
+    const int in = __builtin_amdgcn_readfirstlane(p < mine ? -1 : 0);
+    const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc(
+        (void*)xbase, (short)0, in & (int)kReach, 0x00020000);
+    const __amdgpu_buffer_rsrc_t wrs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)wp, (short)0, in & (2 * P * 1024), 0x00020000);
+    const __amdgpu_buffer_rsrc_t srs =
+        __builtin_amdgcn_make_buffer_rsrc((void*)sb, (short)0, in & (2 * P * 128), 0x00020000);
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+      __builtin_amdgcn_raw_ptr_buffer_load_lds(
+          xrs, (void __attribute__((address_space(3)))*)(xbuf(slot) + 4 * (cw + 2 * j) * XROW),
+          16, (int)xvo[j], (p0 + p) * XROW, 0, 0);
+#pragma unroll
+    for (int i = 0; i < 2; ++i)  // read once: nontemporal
+      wr[S][i] = __builtin_amdgcn_raw_buffer_load_b128(wrs, lane * 16, (i * P + p0 + p) * 1024, 2);
+    __builtin_amdgcn_raw_ptr_buffer_load_lds(
+        srs, (void __attribute__((address_space(3)))*)sbuf(slot), 4, svo, (p0 + p) * 128, 0, 0);
+  };
+  auto landed = [&](auto behind) {
+    wait_vm<decltype(behind)::value * LB>();
+    wait_lgkm0();
+    __builtin_amdgcn_s_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
+  };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  f32x4 T[2] = {zero, zero};
+  uint32_t nib = 0x000F000Fu;
+  asm volatile("" : "+v"(nib));
+  auto compute = [&](auto slot) {
+    constexpr int S = decltype(slot)::value;
+    const uint8_t* const cur = xbuf(slot);
+    u32x4 sv[2], bv[2];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      sv[i] = *reinterpret_cast<const u32x4*>(sbuf(slot) + i * 128 + c4 * 16);
+      bv[i] = *reinterpret_cast<const u32x4*>(sbuf(slot) + i * 128 + 64 + c4 * 16);
+    }
+#pragma unroll
+    for (int gl = 0; gl < 2; ++gl) {
+      u32x4 X[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        X[h] = *reinterpret_cast<const u32x4*>(
+            &cur[r16 * XROW + (((8 * gl + 4 * h + c4) ^ r16) << 4)]);
+      f32x4 xg = mfma(ones, X[0], zero);
+      xg = mfma(ones, X[1], xg);
+#pragma unroll
+      for (int i = 0; i < 2; ++i) {
+        f32x4 d = mfma(unpack_w(wr[S][i][2 * gl], nib), X[0], zero);
+        d = mfma(unpack_w(wr[S][i][2 * gl + 1], nib), X[1], d);
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+          const float sc = gl ? bf_hi(sv[i][r]) : bf_lo(sv[i][r]);
+          const float of = fmaf(-128.0f, sc, gl ? bf_hi(bv[i][r]) : bf_lo(bv[i][r]));
+          T[i][r] = fmaf(sc, d[r], fmaf(of, xg[0], T[i][r]));
+        }
+      }
+    }
+  };
+  auto step = [&](int p, auto slot) {
+    constexpr int S = decltype(slot)::value;
+    batch(p + R - 1, std::integral_constant<int, (S + R - 1) % R>{});
+    __builtin_amdgcn_sched_barrier(0);
+    compute(slot);
+    landed(std::integral_constant<int, R - 2>{});
+  };
+  using S0 = std::integral_constant<int, 0>;
+  using S1 = std::integral_constant<int, 1>;
+  using S2 = std::integral_constant<int, 2>;
+  batch(0, S0{});
+  batch(1, S1{});
+  landed(std::integral_constant<int, R - 2>{});
+  int p = 0;
+#pragma nounroll
+  for (; p + R <= least; p += R) {
+    step(p, S0{});
+    step(p + 1, S1{});
+    step(p + 2, S2{});
+  }
+  batch(p + 2, S2{});
+  if (p < mine) compute(S0{});
+  landed(std::integral_constant<int, 0>{});
+  if (p + 1 < mine) compute(S1{});
+  if (p + 2 < mine) compute(S2{});
+
+  if constexpr (KS > 1) {  // the parts' sums, added in order
+    lds_barrier();         // the slots are free once every wave is here
+    f32x4* const part = reinterpret_cast<f32x4*>(xl0);
+    if (kw > 0)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) part[((kw - 1) * 4 + 2 * cw + i) * 64 + lane] = T[i];
+    lds_barrier();
+    if (kw > 0) return;
+#pragma unroll
+    for (int v = 0; v < KS - 1; ++v)
+#pragma unroll
+      for (int i = 0; i < 2; ++i) T[i] += part[(v * 4 + 2 * cw + i) * 64 + lane];
+  }
+  if (r16 >= tl.z) return;
+  if constexpr (UP) {
+    const uint32_t lo = f2bf2(swiglu(T[0][0], T[1][0]), swiglu(T[0][1], T[1][1]));
+    const uint32_t hi = f2bf2(swiglu(T[0][2], T[1][2]), swiglu(T[0][3], T[1][3]));
+    *reinterpret_cast<u32x2*>(s.h + (int64_t)(tl.y + r16) * a.inner + 32 * cb + 16 * cw + 4 * c4) =
+        (u32x2){lo, hi};
+  } else {
+    uint16_t* const o = s.rows + (int64_t)en * a.hidden + 64 * cb + 32 * cw + 4 * c4;
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+      *reinterpret_cast<u32x2*>(o + 16 * i) =
+          (u32x2){f2bf2(wt * T[i][0], wt * T[i][1]), f2bf2(wt * T[i][2], wt * T[i][3])};
+  }
+}
+
 // ---- tiles of many rows ----
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
@@ -982,21 +1159,20 @@ __global__ __launch_bounds__(256)
   else
     stages(std::integral_constant<int, 1>{});
 
-  // the offsets' sum, as in moe_tile_kernel, two octets a product
+  // The offsets' sum: both lane groups hold the same octet of X, one against b and
+  // the other against -128 s.
   const int gp = gpad(K), go = gp >> 3;
+  const float f = c2 ? -128.0f : 1.0f;
 #pragma nounroll
-  for (int jb = 0; 2 * jb < 3 * go; ++jb) {
-    const int o = 2 * jb + c2, oc = o < go ? o : o < 2 * go ? o - go : o - 2 * go;
-    u32x4 as[2], ab[2];
+  for (int o = 0; o < go; ++o) {
+    u32x4 B[2];
 #pragma unroll
     for (int i = 0; i < 2; ++i)
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        const int ps = 4 * oc + q;
-        const bool in = o < 3 * go && ps < P;
-        const uint32_t* const sq = sb + (fr[i] * P + (in ? ps : 0)) * 32 + (r32 & 15);
-        as[i][q] = in ? sq[0] : 0u;
-        ab[i][q] = in ? sq[16] : 0u;
+        const int ps = 4 * o + q;
+        const uint32_t v = ps < P ? sb[(fr[i] * P + ps) * 32 + (c2 ? 0 : 16) + (r32 & 15)] : 0u;
+        B[i][q] = f2bf2(f * bf_lo(v), f * bf_hi(v));
       }
 #pragma unroll
     for (int u = 0; u < RB; ++u) {
@@ -1004,16 +1180,11 @@ __global__ __launch_bounds__(256)
       const int r = min(u * 32 + r32, tl.z - 1);
       const uint16_t* const xg =
           UP ? s.xs + (int64_t)row_of[r].x * 3 * gp : s.hs + (int64_t)(tl.y + r) * 3 * gp;
-      const u32x4 xp = *reinterpret_cast<const u32x4*>(xg + 8 * (o < 3 * go ? o : 0));
 #pragma unroll
-      for (int i = 0; i < 2; ++i) {
-        f32x16 y;
+      for (int k = 0; k < 3; ++k) {
+        const u32x4 xp = *reinterpret_cast<const u32x4*>(xg + k * gp + 8 * o);
 #pragma unroll
-        for (int e = 0; e < 16; ++e) y[e] = 0.f;
-        y = mfma32(xp, as[i], y);
-        T[i][u] = mfma32(xp, ab[i], T[i][u]);
-#pragma unroll
-        for (int e = 0; e < 16; ++e) T[i][u][e] = fmaf(-128.0f, y[e], T[i][u][e]);
+        for (int i = 0; i < 2; ++i) T[i][u] = mfma32(xp, B[i], T[i][u]);
       }
     }
   }
@@ -1334,31 +1505,36 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     body(std::integral_constant<int, 1>{});
 }
 
-// out[t] = the sum of its entries' rows in column order. A thread per 8 columns,
-// eight rows' loads at a time. Bound by reading the rows.
+// out[t] = the sum of its entries' rows in column order. A thread per 8 columns, B
+// rows' loads at a time; rows of ids outside the layer are read as they are in the
+// work-space and left out. Bound by reading the rows, in small calls by latency:
+// those take all of a token's rows at once, in small work-groups over more CUs.
+template <int B>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const uint16_t* rows) {
   const int q = a.hidden / 8;
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (int64_t)a.T * q) return;
   const int64_t t = i / q;
   const int c = (int)(i - t * q);
   const u32x4* const r = reinterpret_cast<const u32x4*>(rows) + t * a.k * q + c;
   float y[8] = {};
-  for (int j0 = 0; j0 < a.k; j0 += 8) {
-    u32x4 v[8];
+  for (int j0 = 0; j0 < a.k; j0 += B) {
+    u32x4 v[B];
+    bool in[B];
 #pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      v[j] = (u32x4){0u, 0u, 0u, 0u};
-      if (j0 + j < a.k && (uint32_t)a.ids[t * a.k + j0 + j] < (uint32_t)a.experts)
+    for (int j = 0; j < B; ++j)
+      if (j0 + j < a.k) {
         v[j] = __builtin_nontemporal_load(r + (int64_t)(j0 + j) * q);
-    }
-#pragma unroll
-    for (int j = 0; j < 8; ++j)
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        y[2 * e] += bf_lo(v[j][e]);
-        y[2 * e + 1] += bf_hi(v[j][e]);
+        in[j] = (uint32_t)a.ids[t * a.k + j0 + j] < (uint32_t)a.experts;
       }
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      if (j0 + j < a.k && in[j])
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          y[2 * e] += bf_lo(v[j][e]);
+          y[2 * e + 1] += bf_hi(v[j][e]);
+        }
   }
   u32x2* const o = reinterpret_cast<u32x2*>(a.out + t * a.os + c * 8);
   o[0] = (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
@@ -1367,6 +1543,20 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const uint1
 
 dim3 tile_grid(int64_t tiles, int blocks) {
   return dim3((unsigned)(tiles * blocks + 7) & ~7u);  // the same number for every XCD
+}
+
+// Two parts of the stages where a wave would have 8 or more: 8 tokens at hidden
+// 2048, inner 512, 257 experts, 9 columns, up 16.4 us against 22.9 and 20.4 in four
+// parts, 64 tokens 44.1 / 44.9 / 53.5; down, of 4 stages, 10.6 in one part and 12.7 in
+// two at 8 tokens, 27.8 / 32.5 at 64.
+template <bool UP>
+void launch_stream(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
+  const int stages = (UP ? a.hidden : a.inner) / kStageK;
+  const dim3 grid = tile_grid(slots, UP ? a.inner / 32 : a.hidden / 64);
+  if (stages >= 8)
+    hipLaunchKernelGGL((moe_stream_kernel<2, UP>), grid, dim3(256), 0, a.stream, a, s);
+  else
+    hipLaunchKernelGGL((moe_stream_kernel<1, UP>), grid, dim3(128), 0, a.stream, a, s);
 }
 
 template <int MW>
@@ -1403,7 +1593,7 @@ hipError_t launch_moe_pack(const MoePackArgs& a) {
 
 // A pass's rows of x are reached by 32-bit byte offsets.
 int moe_pass_tokens(int k, int64_t x_stride) {
-  const int64_t n = kPassEntries / k, reach = INT32_MAX / x_stride;
+  const int64_t n = kPassEntries / k, reach = kReach / 2 / x_stride;
   return (int)(n < reach ? n : reach > 1 ? reach : 1);
 }
 
@@ -1433,6 +1623,7 @@ hipError_t launch_moe(const MoeArgs& a) {
   const int mean = entries / a.experts;
   const int64_t wide_tiles = max_tiles(entries, a.experts, 64) - a.experts / 2;
   const bool wide = mean >= 64 && wide_tiles * ((a.hidden + 255) / 256) >= 384;
+  const bool stream = mean < 8;
   const int rows = wide ? 64 : mean <= 16 ? 16 : 32;
   const int64_t slots = max_tiles(entries, a.experts, rows);
   const int64_t sums = (int64_t)a.T * 8 * gpad(a.hidden);
@@ -1449,13 +1640,20 @@ hipError_t launch_moe(const MoeArgs& a) {
   }
   if (wide)
     launch_wide(a, s, slots, wide_tiles);
-  else if (rows == 16)
+  else if (stream) {
+    launch_stream<true>(a, s, slots);
+    launch_stream<false>(a, s, slots);
+  } else if (rows == 16)
     launch_tiles<1>(a, s, slots);
   else
     launch_tiles<2>(a, s, slots);
   const int64_t n = (int64_t)a.T * (a.hidden / 8);
-  hipLaunchKernelGGL(moe_combine_kernel, dim3((unsigned)((n + 255) / 256)), dim3(256), 0, a.stream, a,
-                     s.rows);
+  if (n < 1 << 16)
+    hipLaunchKernelGGL(moe_combine_kernel<16>, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, a.stream,
+                       a, s.rows);
+  else
+    hipLaunchKernelGGL(moe_combine_kernel<4>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
+                       a.stream, a, s.rows);
   return hipGetLastError();
 }
 

@@ -7,6 +7,7 @@ lib/libgdn.so is missing or the GPU is absent, calls raise.
 from __future__ import annotations
 
 import ctypes
+import functools
 import os
 import subprocess
 
@@ -229,9 +230,10 @@ def _rows(t) -> tuple[int, int]:
     contiguous (a column slice of a wider matrix is fine)."""
     if not t.is_cuda:
         raise ValueError("libgdn takes device tensors")
-    if t.dim() != 2 or (t.shape[1] > 1 and t.stride(1) != 1):
+    strides = t.stride()
+    if len(strides) != 2 or (strides[1] != 1 and t.shape[1] > 1):
         raise ValueError("expected a 2-D tensor with contiguous rows")
-    return t.data_ptr(), t.stride(0)
+    return t.data_ptr(), strides[0]
 
 
 def _stream(stream) -> int | None:
@@ -284,22 +286,39 @@ def add_rms_norm(h, d, w, eps, hn, group_sums=None, stream=None):
                                    _ptr(group_sums), _stream(stream)))
 
 
+_BF16_DTYPES = ()  # torch types taken as bf16 bit patterns, once torch is imported
+
+
 def _is_f32(t, what: str) -> bool:
     """Whether t holds f32 rather than bf16 (torch.bfloat16 or 16-bit patterns)."""
+    global _BF16_DTYPES
+    dt = t.dtype
+    if dt in _BF16_DTYPES:
+        return False
     import torch
-    if t.dtype == torch.float32:
+    if not _BF16_DTYPES:
+        _BF16_DTYPES = (torch.bfloat16, torch.int16, torch.uint16)
+    if dt == torch.float32:
         return True
-    if t.element_size() != 2 or t.dtype == torch.float16:
-        raise ValueError(f"{what} must be float32 or bf16, not {t.dtype}")
+    if dt not in _BF16_DTYPES:
+        raise ValueError(f"{what} must be float32 or bf16, not {dt}")
     return False
 
 
-def _typed(t, dtypes, what: str):
-    if t.dtype not in dtypes:
-        raise ValueError(f"{what} must be {' or '.join(str(d) for d in dtypes)}, not {t.dtype}")
+def _bf16(t, what: str):
+    if _is_f32(t, what):
+        raise ValueError(f"{what} must be bf16")
     return t
 
 
+def _typed(t, name: str, what: str):
+    import torch
+    if t.dtype != getattr(torch, name):
+        raise ValueError(f"{what} must be torch.{name}, not {t.dtype}")
+    return t
+
+
+@functools.lru_cache(maxsize=256)
 def route_desc(num_experts, top_k, score="softmax", num_groups=1, top_groups=1, group_top=1,
                renorm=True, scale=1.0, num_shared=0, shared_gate=False, logits_f32=False):
     """A router's descriptor (gdn_moe_route_desc)."""
@@ -317,20 +336,27 @@ def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=No
     """Experts of every token (gdn_moe_route): logits [T, >= num_experts (+ 1 with
     shared_gate)] bf16 or f32 rows -> ids int32 and weights f32 [T, top_k + num_shared].
     score: "softmax" or "sigmoid"; bias f32 [num_experts] moves the choice only."""
-    import torch
     lp, ls = _rows(logits)
-    T = logits.shape[0]
-    if logits.shape[1] < num_experts + (1 if shared_gate else 0):
+    T, cols = logits.shape
+    if cols < num_experts + (1 if shared_gate else 0):
         raise ValueError("logits hold fewer columns than experts")
-    for t, d, what in ((ids, torch.int32, "ids"), (weights, torch.float32, "weights")):
-        if tuple(_typed(t, (d,), what).shape) != (T, top_k + num_shared):
-            raise ValueError(f"{what} must be [{T}, {top_k + num_shared}]")
-    if bias is not None and _typed(bias, (torch.float32,), "bias").numel() != num_experts:
+    want = (T, top_k + num_shared)
+    if _typed(ids, "int32", "ids").shape != want:
+        raise ValueError(f"ids must be {want}")
+    if _typed(weights, "float32", "weights").shape != want:
+        raise ValueError(f"weights must be {want}")
+    if bias is not None and _typed(bias, "float32", "bias").numel() != num_experts:
         raise ValueError("one bias per expert")
     d = route_desc(num_experts, top_k, score, num_groups, top_groups, group_top, renorm, scale,
                    num_shared, shared_gate, _is_f32(logits, "logits"))
     _check(load().gdn_moe_route(ctypes.byref(d), lp, ls, T, _ptr(bias), _ptr(ids), _ptr(weights),
                                 _stream(stream)))
+
+
+@functools.lru_cache(maxsize=256)
+def _block_norm_desc(hidden, f32, kind, sigmoid, offset, scale, post_eps, pre_eps):
+    return BlockNormDesc(hidden, int(f32), kind, int(bool(sigmoid)), int(bool(offset)),
+                         float(scale), float(post_eps), float(pre_eps))
 
 
 def block_norm(h, x, h_out=None, hn=None, pre_w=None, pre_eps=1e-6, post_w=None, post_eps=1e-6,
@@ -339,34 +365,37 @@ def block_norm(h, x, h_out=None, hn=None, pre_w=None, pre_eps=1e-6, post_w=None,
     h_out = h + scale * gate * b, hn = rms_norm(h_out) * pre_w. h, h_out [n, hidden]
     bf16 or f32 (h_out None: in place), the others bf16; gate [n, 1] or [n, hidden] rows,
     or [hidden] for one row shared by all; pre_w and hn None: no second norm."""
-    n, hidden = h.shape
-    h_out = h if h_out is None else h_out
+    shape = h.shape
+    n, hidden = shape
     hp, hs = _rows(h)
-    xp, xs = _rows(x)
-    op, os_ = _rows(h_out)
+    xp, xs = _rows(_bf16(x, "x"))
     f32 = _is_f32(h, "h")
-    if h_out.dtype != h.dtype or h_out.shape != h.shape or tuple(x.shape) != (n, hidden):
-        raise ValueError("h, x and h_out must have the same shape, h and h_out the same type")
-    np_, ns = (None, 0) if hn is None else _rows(hn)
-    for t, what in ((x, "x"), (hn, "hn"), (gate, "gate"), (post_w, "post_w"), (pre_w, "pre_w")):
-        if t is not None and _is_f32(t, what):
-            raise ValueError(f"{what} must be bf16")
-    if hn is not None and tuple(hn.shape) != (n, hidden):
-        raise ValueError("hn must have h's shape")
+    if x.shape != shape:
+        raise ValueError("x must have h's shape")
+    op, os_ = hp, hs
+    if h_out is not None:
+        op, os_ = _rows(h_out)
+        if h_out.dtype != h.dtype or h_out.shape != shape:
+            raise ValueError("h_out must have h's shape and type")
+    np_, ns = None, 0
+    if hn is not None:
+        np_, ns = _rows(_bf16(hn, "hn"))
+        if hn.shape != shape:
+            raise ValueError("hn must have h's shape")
     for w in (post_w, pre_w):
-        if w is not None and w.numel() != hidden:
+        if w is not None and _bf16(w, "norm weights").numel() != hidden:
             raise ValueError("norm weights hold one value per column")
     kind, gp, gs = 0, None, 0
     if gate is not None:
-        if gate.dim() == 1 and gate.shape[0] == hidden:
+        gshape = _bf16(gate, "gate").shape
+        if gshape == (hidden,):
             kind, gp, gs = 2, _ptr(gate), 0
-        elif gate.dim() == 2 and tuple(gate.shape) in ((n, 1), (n, hidden)):
+        elif gshape == (n, 1) or gshape == shape:
             gp, gs = _rows(gate)
-            kind = 1 if gate.shape[1] == 1 else 2
+            kind = 1 if gshape[1] == 1 else 2
         else:
             raise ValueError("gate must be [n, 1], [n, hidden] or [hidden]")
-    d = BlockNormDesc(hidden, int(f32), kind, int(bool(gate_sigmoid)), int(bool(unit_offset)),
-                      float(scale), float(post_eps), float(pre_eps))
+    d = _block_norm_desc(hidden, f32, kind, gate_sigmoid, unit_offset, scale, post_eps, pre_eps)
     _check(load().gdn_block_norm(ctypes.byref(d), n, hp, hs, xp, xs, _ptr(post_w), gp, gs,
                                  _ptr(pre_w), op, os_, np_, ns, _stream(stream)))
 
@@ -616,22 +645,15 @@ class MoE:
     def forward(self, x, ids, weights, out, workspace, stream=None):
         """out[t] = sum_j weights[t, j] * expert ids[t, j] of x[t]; x, out [T, hidden] bf16
         rows, ids int32 and weights f32 [T, k]; ids outside [0, experts) add nothing."""
-        import torch
-        xp, xs = _rows(x)
-        op, os_ = _rows(out)
-        for t, what in ((x, "x"), (out, "out")):
-            if _is_f32(t, what):
-                raise ValueError(f"{what} must be bf16")
-        T, k = ids.shape
-        if (tuple(x.shape) != (T, self.hidden) or out.shape != x.shape or
-                weights.shape != ids.shape):
+        xp, xs = _rows(_bf16(x, "x"))
+        op, os_ = _rows(_bf16(out, "out"))
+        shape = _typed(ids, "int32", "ids").shape
+        T, k = shape
+        if x.shape != (T, self.hidden) or out.shape != x.shape or weights.shape != shape:
             raise ValueError(f"need x, out [{T}, {self.hidden}] and weights [{T}, {k}]")
-        _typed(ids, (torch.int32,), "ids")
-        _typed(weights, (torch.float32,), "weights")
+        _typed(weights, "float32", "weights")
         _check(self.lib.gdn_moe_forward(self.handle, xp, xs, T, k, _ptr(ids), _ptr(weights), op,
-                                        os_, _ptr(workspace),
-                                        workspace.numel() * workspace.element_size(),
-                                        _stream(stream)))
+                                        os_, _ptr(workspace), workspace.nbytes, _stream(stream)))
 
     def close(self):
         if getattr(self, "handle", None):
