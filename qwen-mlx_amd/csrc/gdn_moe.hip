@@ -764,10 +764,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
 
 // moe_tile_kernel for up to 16 rows, where the weights' stream is the work:
 // 64 columns a work-group (small ones fill the chip evenly), KS pairs of waves each
-// over a part of the stages (a wave's stages run one after the other, at about
-// STAGE_US us each, also where nothing is left to wait for), the groups' sums of x
-// from products against ones instead of beforehand, and the offsets applied with
-// the scales. Rows past the tile's are not read: their copies are out of the
+// over a part of the stages (a wave's stages run one after the other, so that a
+// small call takes as long as one wave's), the groups' sums of x from products
+// against ones instead of beforehand, and the offsets applied with the scales. Rows past the tile's are not read: their copies are out of the
 // buffer's range, which gives zeros.
 template <int KS, bool UP>
 __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))) void
@@ -1510,7 +1509,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // work-space and left out. Bound by reading the rows, in small calls by latency:
 // those take all of a token's rows at once, in small work-groups over more CUs.
 template <int B>
-__global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const uint16_t* rows) {
+__global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, uint16_t* rows) {
   const int q = a.hidden / 8;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (int64_t)a.T * q) return;
@@ -1541,45 +1540,54 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const uint1
   o[1] = (u32x2){f2bf2(y[4], y[5]), f2bf2(y[6], y[7])};
 }
 
-dim3 tile_grid(int64_t tiles, int blocks) {
-  return dim3((unsigned)(tiles * blocks + 7) & ~7u);  // the same number for every XCD
+// ---- launches ----
+
+template <typename... Par, typename... Arg>
+hipError_t launch(void (*kernel)(Par...), int64_t groups, int threads, size_t lds, hipStream_t stream,
+                  Arg... args) {
+  hipLaunchKernelGGL(kernel, dim3((unsigned)groups), dim3(threads), lds, stream, args...);
+  return hipGetLastError();
 }
+
+#define MOE_TRY(x)                        \
+  do {                                    \
+    const hipError_t e_ = (x);            \
+    if (e_ != hipSuccess) return e_;      \
+  } while (0)
+
+// Work-groups of `blocks` per tile slot, the same number for every XCD.
+int64_t tile_groups(int64_t slots, int blocks) { return (slots * blocks + 7) & ~(int64_t)7; }
 
 // Two parts of the stages where a wave would have 8 or more: 8 tokens at hidden
 // 2048, inner 512, 257 experts, 9 columns, up 16.4 us against 22.9 and 20.4 in four
 // parts, 64 tokens 44.1 / 44.9 / 53.5; down, of 4 stages, 10.6 in one part and 12.7 in
 // two at 8 tokens, 27.8 / 32.5 at 64.
 template <bool UP>
-void launch_stream(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
-  const int stages = (UP ? a.hidden : a.inner) / kStageK;
-  const dim3 grid = tile_grid(slots, UP ? a.inner / 32 : a.hidden / 64);
-  if (stages >= 8)
-    hipLaunchKernelGGL((moe_stream_kernel<2, UP>), grid, dim3(256), 0, a.stream, a, s);
-  else
-    hipLaunchKernelGGL((moe_stream_kernel<1, UP>), grid, dim3(128), 0, a.stream, a, s);
+hipError_t launch_stream(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
+  const int64_t groups = tile_groups(slots, UP ? a.inner / 32 : a.hidden / 64);
+  if ((UP ? a.hidden : a.inner) >= 8 * kStageK)
+    return launch(moe_stream_kernel<2, UP>, groups, 256, 0, a.stream, a, s);
+  return launch(moe_stream_kernel<1, UP>, groups, 128, 0, a.stream, a, s);
 }
 
 template <int MW>
-void launch_tiles(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
-  hipLaunchKernelGGL((moe_tile_kernel<MW, true>), tile_grid(slots, a.inner / 64), dim3(256), 0,
-                     a.stream, a, s);
-  hipLaunchKernelGGL((moe_tile_kernel<MW, false>), tile_grid(slots, a.hidden / 128), dim3(256), 0,
-                     a.stream, a, s);
+hipError_t launch_tiles(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
+  MOE_TRY(launch(moe_tile_kernel<MW, true>, tile_groups(slots, a.inner / 64), 256, 0, a.stream, a, s));
+  return launch(moe_tile_kernel<MW, false>, tile_groups(slots, a.hidden / 128), 256, 0, a.stream, a,
+                s);
 }
 
-void launch_wide(const MoeArgs& a, const MoeSpace& s, int64_t slots, int64_t tiles) {
-  hipLaunchKernelGGL(moe_wide_kernel<true>, tile_grid(slots, (a.inner + 127) / 128), dim3(256), 0,
-                     a.stream, a, s);
+hipError_t launch_wide(const MoeArgs& a, const MoeSpace& s, int64_t slots, int64_t tiles) {
+  MOE_TRY(launch(moe_wide_kernel<true>, tile_groups(slots, a.inner / 128), 256, 0, a.stream, a, s));
   const int blocks = (a.hidden + 255) / 256;
-  if (a.inner > 4 * kStageK) {
-    hipLaunchKernelGGL(moe_wide_kernel<false>, tile_grid(slots, blocks), dim3(256), 0, a.stream, a,
-                       s);
-    return;
-  }
-  int run = blocks;  // long runs, as long as they leave two work-groups per slot of 512
+  if (a.inner > 4 * kStageK)
+    return launch(moe_wide_kernel<false>, tile_groups(slots, blocks), 256, 0, a.stream, a, s);
+  // Long runs, as long as they leave two work-groups for each of the 512 that run
+  // side by side: 16,384 tokens (2,400 tiles) 401 us in runs of 8 blocks, 420 of 2.
+  int run = blocks;
   while (run > 1 && tiles * ((blocks + run - 1) / run) < 1024) run = (run + 1) / 2;
-  hipLaunchKernelGGL(moe_wide_down_kernel, tile_grid(slots, (blocks + run - 1) / run), dim3(256), 0,
-                     a.stream, a, s, run);
+  return launch(moe_wide_down_kernel, tile_groups(slots, (blocks + run - 1) / run), 256, 0, a.stream,
+                a, s, run);
 }
 
 }  // namespace
@@ -1608,15 +1616,14 @@ hipError_t launch_moe(const MoeArgs& a) {
   const int entries = a.T * a.k;
   const MoeSpace s = moe_space(a.workspace, a.hidden, a.inner, a.experts, a.T, entries);
   if (entries <= kFewEntries && a.T <= kFewTokens) {
-    hipLaunchKernelGGL(moe_few_up_kernel, dim3(entries * (a.inner / 16)), dim3(256), 0, a.stream, a,
-                       s.h);
-    hipLaunchKernelGGL(moe_few_down_kernel, dim3(a.T * (a.hidden / 16)),
-                       dim3(64 * (a.k < 16 ? a.k : 16)), 0, a.stream, a, s.h);
-    return hipGetLastError();
+    MOE_TRY(launch(moe_few_up_kernel, entries * (a.inner / 16), 256, 0, a.stream, a, s.h));
+    return launch(moe_few_down_kernel, a.T * (a.hidden / 16), 64 * (a.k < 16 ? a.k : 16), 0, a.stream,
+                  a, s.h);
   }
-  // Rows of a tile by the rows that an expert has on average. At hidden 2048,
-  // inner 512, 257 experts, 9 columns, 16 / 32 / 64 rows: 64 tokens 91 / 94 / 115
-  // us, 317 tokens 114 / 117 / 143, 600 tokens 145 / 135 / 153, 2000 tokens 315 /
+  // The kernel by the rows that an expert has on average. At hidden 2048, inner
+  // 512, 257 experts, 9 columns, tiles of 16 rows by the stream kernel / 16 / 32 /
+  // 64 rows: 64 tokens (mean 2) 77 / 86 / 94 / 115 us, 200 (7) 101 / 105 / 110 / 135,
+  // 317 (11) 120 / 114 / 117 / 143, 600 (21) - / 145 / 135 / 153, 2000 (70) - / 315 /
   // 259 / 233. Tiles of 64 rows also want a work-group for most of the 512 that
   // run side by side (hidden 1024, inner 1408, 32 experts, 4 columns: 1000 tokens,
   // 312 work-groups, 78 us by 32 rows and 79 by 64; 1500 tokens, 436, 101 / 93).
@@ -1626,35 +1633,27 @@ hipError_t launch_moe(const MoeArgs& a) {
   const bool stream = mean < 8;
   const int rows = wide ? 64 : mean <= 16 ? 16 : 32;
   const int64_t slots = max_tiles(entries, a.experts, rows);
-  const int64_t sums = (int64_t)a.T * 8 * gpad(a.hidden);
-  const unsigned sum_groups = (unsigned)((sums + kPlanThreads - 1) / kPlanThreads);
+  const int64_t sums = stream ? 0 : (int64_t)a.T * 8 * gpad(a.hidden);
+  const int64_t sum_groups = (sums + kPlanThreads - 1) / kPlanThreads;
   if (entries <= kPlanEntries) {
-    hipLaunchKernelGGL(moe_plan_kernel, dim3(a.experts + sum_groups), dim3(kPlanThreads), 0,
-                       a.stream, a, rows, s);
+    MOE_TRY(launch(moe_plan_kernel, a.experts + sum_groups, kPlanThreads, 0, a.stream, a, rows, s));
   } else {
-    const unsigned chunks = (unsigned)((entries + kChunk - 1) / kChunk);
-    hipLaunchKernelGGL(moe_count_kernel, dim3(chunks + sum_groups), dim3(kPlanThreads),
-                       a.experts * 4, a.stream, a, chunks, s);
-    hipLaunchKernelGGL(moe_place_kernel, dim3(chunks), dim3(kPlanThreads), a.experts * 8, a.stream,
-                       a, rows, s);
+    const int chunks = (entries + kChunk - 1) / kChunk;
+    MOE_TRY(launch(moe_count_kernel, chunks + sum_groups, kPlanThreads, a.experts * 4, a.stream, a,
+                   chunks, s));
+    MOE_TRY(launch(moe_place_kernel, chunks, kPlanThreads, a.experts * 8, a.stream, a, rows, s));
   }
-  if (wide)
-    launch_wide(a, s, slots, wide_tiles);
-  else if (stream) {
-    launch_stream<true>(a, s, slots);
-    launch_stream<false>(a, s, slots);
-  } else if (rows == 16)
-    launch_tiles<1>(a, s, slots);
-  else
-    launch_tiles<2>(a, s, slots);
+  if (wide) {
+    MOE_TRY(launch_wide(a, s, slots, wide_tiles));
+  } else if (stream) {
+    MOE_TRY(launch_stream<true>(a, s, slots));
+    MOE_TRY(launch_stream<false>(a, s, slots));
+  } else {
+    MOE_TRY(rows == 16 ? launch_tiles<1>(a, s, slots) : launch_tiles<2>(a, s, slots));
+  }
   const int64_t n = (int64_t)a.T * (a.hidden / 8);
-  if (n < 1 << 16)
-    hipLaunchKernelGGL(moe_combine_kernel<16>, dim3((unsigned)((n + 63) / 64)), dim3(64), 0, a.stream,
-                       a, s.rows);
-  else
-    hipLaunchKernelGGL(moe_combine_kernel<4>, dim3((unsigned)((n + 255) / 256)), dim3(256), 0,
-                       a.stream, a, s.rows);
-  return hipGetLastError();
+  if (n < 1 << 16) return launch(moe_combine_kernel<16>, (n + 63) / 64, 64, 0, a.stream, a, s.rows);
+  return launch(moe_combine_kernel<4>, (n + 255) / 256, 256, 0, a.stream, a, s.rows);
 }
 
 }  // namespace gdn

@@ -298,6 +298,10 @@ def draw_x(seed, T, hidden):
     (2048, 128, [2], 1700, 2),    # tiles of 64 rows, down's input in LDS
     (1792, 384, [3, 1], 2100, 3),
     (1152, 640, [2, 1], 1700, 3), # and in stages, half a block of columns over
+    (128, 128, [24], 3, 20),      # more columns than waves of a work-group
+    (256, 128, [50], 10, 40),
+    (1408, 1152, [40], 20, 3),    # stages in two parts of unequal length
+    (128, 128, [1500], 6, 64),
 ])
 def test_experts(gpu, hidden, inner, parts, T, k):
     ex = Experts(hidden, inner, parts, seed=hidden + inner)
@@ -305,12 +309,14 @@ def test_experts(gpu, hidden, inner, parts, T, k):
     ex.check(draw_x(T, T, hidden), ids, w)
 
 
-@pytest.mark.parametrize("T", [1, 4, 19, 300, 1100, 2500])
-def test_experts_uneven_absent_and_repeated_ids(gpu, T):
+@pytest.mark.parametrize("T,hidden,inner", [(1, 256, 256), (4, 256, 256), (12, 256, 256),
+                                            (19, 256, 256), (300, 256, 256), (1100, 256, 256),
+                                            (2500, 256, 256), (900, 2048, 128), (800, 1536, 640)])
+def test_experts_uneven_absent_and_repeated_ids(gpu, T, hidden, inner):
     """All rows on one expert, experts without rows, ids outside the layer, tokens
     without any, an expert twice in a token, weights that are zero or negative."""
-    ex = Experts(256, 256, [6, 1], seed=5)
-    x = draw_x(1, T, 256)
+    ex = Experts(hidden, inner, [6, 1], seed=5)
+    x = draw_x(1, T, hidden)
     _, w = draw_ids(2, T, 7, 4)
     one = torch.full((T, 4), 3, dtype=torch.int32)
     one[:, 1:] = -1
@@ -380,6 +386,36 @@ def test_experts_no_rows_and_workspace_of_a_larger_call(gpu):
         n = [ex.moe.workspace_bytes(T, k) for k in (1, 2, 3, 8, 64)]
         assert n == sorted(n) and n[0] >= last
         last = n[0]
+
+
+def test_experts_rows_far_apart(gpu):
+    """Rows of x whose byte offsets pass 32 bits: the call goes in pieces."""
+    ex = Experts(128, 128, [3], seed=11)
+    T, stride = 2500, 1 << 20
+    x, (ids, w) = draw_x(1, T, 128), draw_ids(2, T, 3, 2)
+    far = torch.empty(T * stride, device=DEV, dtype=BF).view(T, stride)[:, :128]
+    far.copy_(x)
+    out = torch.empty(T, 128, device=DEV, dtype=BF)
+    ex.moe.forward(far, ids.to(DEV), w.to(DEV), out, ex.moe.workspace(T, 2))
+    ref, tol = ex.ref(x, ids, w)
+    assert ((out.cpu().double() - ref).abs() <= tol).all()
+
+
+def test_experts_two_streams_at_once(gpu):
+    """Calls with work-spaces of their own may overlap."""
+    ex = Experts(512, 256, [9], seed=6)
+    calls = []
+    for T in (700, 40, 5):
+        x, (ids, w) = draw_x(T, T, 512), draw_ids(T + 1, T, 9, 2)
+        calls.append((x.to(DEV), ids.to(DEV), w.to(DEV), torch.empty(T, 512, device=DEV, dtype=BF),
+                      ex.moe.workspace(T, 2), torch.cuda.Stream(), ex.run(x, ids, w)))
+    torch.cuda.synchronize()
+    for _ in range(10):
+        for x, ids, w, out, ws, s, _ in calls:
+            ex.moe.forward(x, ids, w, out, ws, stream=s)
+    torch.cuda.synchronize()
+    for *_, out, ws, s, want in calls:
+        assert torch.equal(out.cpu().view(torch.int16), want.view(torch.int16))
 
 
 def test_experts_call_of_more_than_one_pass(gpu):
