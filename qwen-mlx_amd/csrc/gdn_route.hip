@@ -11,8 +11,10 @@
 //   else it is the score in f64, 64 bits: f32 would make ties of scores that
 //     differ. A round then finds the upper halves' maximum and, where several
 //     experts have it, the lower halves'.
-// Bound by the rounds' VALU work for prompts (16,384 tokens, 256 experts, 8 chosen:
-// 12.7 us) and by their latency for decode batches (64 tokens: 4.6 us).
+// Bound by the rounds' VALU work for prompts (16,384 tokens, 256 experts, 8 chosen,
+// f32 logits: 11.5 us) and by their latency for decode batches (64 tokens: 4.3 us).
+// Where a logit and its expert fit one 32-bit key, moe_route_rows_kernel does four
+// tokens a wave.
 #include <type_traits>
 
 #include "gdn_common.h"
@@ -240,6 +242,133 @@ __global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a) {
   }
 }
 
+// ---- four tokens a wave ----
+
+// Routing on bf16 logits in their own order, without groups, for up to 512 experts
+// and 16 columns: 16 lanes (a DPP row) a token, lane L with the R experts from R L on.
+// A key is the logit in 16 bits over the expert's number counted down, so that no
+// two of a token are equal, the larger one goes first and a tie to the lower
+// expert. A round then needs nothing removed: among the keys the next is the one
+// with the largest key - last (mod 2^32), since those chosen before, being no
+// smaller than the last, come out below all the others. 8 columns of 256 experts:
+// 64 tokens 3.2 us (4.3 by a wave a token), 16,384 in 5.2 (11.5), where the logits'
+// bytes alone take 1.7; 10 of 512: 3.9 (5.8) and 8.0 (16.6).
+typedef short i16x2 __attribute__((ext_vector_type(2)));
+
+// Two logits as 16 bits in order: sign and magnitude to two's complement, turned so
+// that the numbers from the lowest finite one to +infinity are 0x0100 .. 0xFFFF and
+// -infinity and NaN, which are never chosen, come below; -0 equals +0.
+__device__ __forceinline__ uint32_t ordered2(uint32_t v) {
+  const i16x2 neg = __builtin_bit_cast(i16x2, v) >> 15;
+  const i16x2 mag = __builtin_bit_cast(i16x2, v & 0x7FFF7FFFu);
+  const i16x2 base = {(short)0x807F, (short)0x807F};
+  return __builtin_bit_cast(uint32_t, (mag ^ neg) - neg + base);
+}
+constexpr uint32_t kValid = 0x01000000u;  // the lowest key of a number
+
+// The logit of a key, +infinity as the largest float.
+__device__ __forceinline__ float key_logit(uint32_t key) {
+  const int v = (int)(key >> 16) - 0x807F;
+  const float f = __uint_as_float((uint32_t)(v < 0 ? -v : v) << 16);
+  return v < 0 ? -f : fminf(f, 3.402823466e38f);
+}
+
+// Largest value, or sum, of the row's 16 lanes, in all of them (row_ror:8, 4, 2, 1).
+template <int CTRL>
+__device__ __forceinline__ uint32_t ror(uint32_t v) {
+  return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true);
+}
+__device__ __forceinline__ uint32_t row16_max(uint32_t v) {
+  v = max(v, ror<0x128>(v));
+  v = max(v, ror<0x124>(v));
+  v = max(v, ror<0x122>(v));
+  return max(v, ror<0x121>(v));
+}
+__device__ __forceinline__ float row16_sum(float v) {
+  v += __uint_as_float(ror<0x128>(__float_as_uint(v)));
+  v += __uint_as_float(ror<0x124>(__float_as_uint(v)));
+  v += __uint_as_float(ror<0x122>(__float_as_uint(v)));
+  return v + __uint_as_float(ror<0x121>(__float_as_uint(v)));
+}
+
+template <int R>
+__global__ __launch_bounds__(256) void moe_route_rows_kernel(MoeRouteArgs a) {
+  typedef uint32_t Raw __attribute__((ext_vector_type(R / 2), aligned(2)));
+  const int L = threadIdx.x & 15, t = blockIdx.x * (blockDim.x >> 4) + (threadIdx.x >> 4);
+  const int E = a.d.num_experts, k = a.d.top_k;
+  const uint16_t* const logits =
+      static_cast<const uint16_t*>(a.logits) + (int64_t)min(t, a.T - 1) * a.stride;
+  const uint16_t gate = logits[a.d.shared_gate ? E : 0];
+  uint32_t raw[R / 2];
+  if (R * (L + 1) <= E) {
+    const Raw v = *reinterpret_cast<const Raw*>(logits + R * L);
+#pragma unroll
+    for (int r = 0; r < R / 2; ++r) raw[r] = v[r];
+  } else {  // -infinity past the last expert
+#pragma unroll
+    for (int r = 0; r < R / 2; ++r) {
+      const int e = R * L + 2 * r;
+      const uint32_t lo = logits[min(e, E - 1)], hi = logits[min(e + 1, E - 1)];
+      raw[r] = (e < E ? lo : 0xFF80u) | (e + 1 < E ? hi : 0xFF80u) << 16;
+    }
+  }
+  uint32_t key[R];
+  const uint32_t down = (0xFFFFu - R * L) * 0x10001u - 0x10000u;  // of experts R L and R L + 1
+#pragma unroll
+  for (int r = 0; r < R / 2; ++r) {
+    const uint32_t v = ordered2(raw[r]), e = down - 2 * r * 0x10001u;
+    key[2 * r] = v << 16 | (e & 0xFFFFu);
+    key[2 * r + 1] = (v & 0xFFFF0000u) | e >> 16;
+  }
+  // the choice: lane j keeps the j-th key; no number is left once a key is below them
+  uint32_t last = 0, mine = 0;
+  for (int j = 0; j < k; ++j) {
+    uint32_t best = key[0] - last;
+#pragma unroll
+    for (int r = 1; r < R; ++r) best = max(best, key[r] - last);
+    const uint32_t next = last + row16_max(best);
+    last = j == 0 || last >= kValid ? next : 0;
+    if (L == j) mine = last;
+  }
+  const bool chosen = mine >= kValid;
+  int id = chosen ? (int)(0xFFFFu - (mine & 0xFFFFu)) : -1;
+  const bool softmax = a.d.score == GDN_MOE_SOFTMAX;
+  const float lw = chosen ? key_logit(mine) : -INFINITY;
+  // lane 0 holds the row's largest
+  const float top = __shfl(lw, (threadIdx.x & 63) & 48, 64);
+  float w;
+  if (a.d.renorm) {
+    const float ex =
+        !chosen ? 0.f : softmax ? expf(lw - top) : expf(log_sigmoid(lw) - log_sigmoid(top));
+    w = ex / row16_sum(ex);
+  } else if (softmax) {
+    float ex = 0.f;
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+      if (key[r] >= kValid) ex += expf(key_logit(key[r]) - top);
+    w = expf(lw - top) / row16_sum(ex);
+  } else {
+    w = sigmoid(lw);
+  }
+  w = chosen ? w * a.d.scale : 0.f;
+  const int S = a.d.num_shared;
+  if (L >= k && L < k + S) {
+    const float g = bf2f(gate);
+    id = E + L - k;
+    w = a.d.shared_gate ? sigmoid(g != g ? -INFINITY : fminf(g, 3.402823466e38f)) : 1.f;
+  }
+  if (t < a.T && L < k + S) {
+    a.ids[(int64_t)t * (k + S) + L] = id;
+    a.weights[(int64_t)t * (k + S) + L] = w;
+  }
+}
+
+template <int R>
+hipError_t launch_rows(const MoeRouteArgs& a) {
+  hipLaunchKernelGGL((moe_route_rows_kernel<R>), dim3((a.T + 15) / 16), dim3(256), 0, a.stream, a);
+  return hipGetLastError();
+}
+
 template <int R>
 hipError_t launch(const MoeRouteArgs& a, bool f64) {
   const size_t bytes = a.d.num_groups > 1 ? 4 * 64 * R * (f64 ? 8 : 4) : 0;
@@ -254,7 +383,13 @@ hipError_t launch(const MoeRouteArgs& a, bool f64) {
 
 hipError_t launch_moe_route(const MoeRouteArgs& a) {
   const bool f64 = a.bias || (a.d.group_top == 2 && a.d.num_groups > 1);
-  const int R = (a.d.num_experts + 63) / 64;
+  const int E = a.d.num_experts;
+  if (!f64 && !a.d.logits_f32 && a.d.num_groups == 1 && E <= 512 && a.d.top_k + a.d.num_shared <= 16)
+    return E <= 64    ? launch_rows<4>(a)
+           : E <= 128 ? launch_rows<8>(a)
+           : E <= 256 ? launch_rows<16>(a)
+                      : launch_rows<32>(a);
+  const int R = (E + 63) / 64;
   return R <= 1   ? launch<1>(a, f64)
          : R <= 2 ? launch<2>(a, f64)
          : R <= 4 ? launch<4>(a, f64)

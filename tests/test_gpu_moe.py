@@ -173,6 +173,35 @@ def test_route_masks_infinities_and_nan(gpu, kw):
     check_route(l, E, k, **kw)
 
 
+@pytest.mark.parametrize("E,k", [(1, 1), (3, 3), (16, 7), (63, 4), (64, 15), (65, 15), (100, 15),
+                                 (128, 8), (200, 3), (255, 8), (256, 15), (257, 8), (400, 11),
+                                 (512, 15), (512, 16), (513, 4), (60, 17)])
+@pytest.mark.parametrize("kw", [dict(), dict(renorm=False, scale=2.5), dict(score="sigmoid"),
+                                dict(score="sigmoid", renorm=False)])
+def test_route_bf16_rows(gpu, E, k, kw):
+    """bf16 logits in their own order: every size of a lane's share, rows with few or no
+    numbers, both zeros, subnormals, the type's lowest value, infinities and NaN."""
+    T = 37
+    g = torch.Generator().manual_seed(E + k)
+    l = torch.randn(T, E + 1, generator=g).mul(2).to(BF)
+    fin = torch.finfo(BF)
+    l[1, :E] = -INF
+    l[2, :E] = math.nan
+    l[3, :E] = torch.where(torch.rand(E, generator=g) < 0.5, 0.0, -0.0).to(BF)
+    l[4, :E] = torch.randint(-3, 4, (E,), generator=g).to(torch.int16).abs().view(BF)  # subnormals
+    l[5, :E] = fin.min
+    l[6, :E] = torch.where(torch.rand(E, generator=g) < 0.3, -INF, fin.min).to(BF)
+    l[7, :E:2] = math.nan
+    l[8, :E:3] = -INF
+    l[9, E - 1] = INF
+    l[10, :E] = INF
+    l[11, : E - 1] = -INF
+    l[12, 1:E] = math.nan
+    l[13, :E] = torch.randint(-2, 3, (E,), generator=g).to(BF)
+    shared = dict(shared=1, shared_gate=True) if k < 16 else {}
+    check_route(l, E, k, **kw, **shared)
+
+
 def test_route_bias_takes_experts_out(gpu):
     b = torch.zeros(16)
     b[3], b[5] = -INF, math.nan
