@@ -3,6 +3,7 @@
 // experts' packed weights. See include/gdn.h for the contract.
 #include <hip/hip_runtime.h>
 
+#include <algorithm>
 #include <cstdarg>
 #include <cstdio>
 #include <new>
@@ -43,6 +44,10 @@ class DeviceScope {
   int prev_ = -1;
   bool ok_ = true;
 };
+
+// Rows of one launch of the kernels with a work-group or a wave a row: a grid
+// holds less than 2^32 threads, of which a row takes up to 512.
+constexpr int64_t kRowsOfLaunch = 1 << 22;
 
 bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; }
 
@@ -146,15 +151,18 @@ gdn_status gdn_moe_route(const gdn_moe_route_desc* desc, const void* logits,
     return mfail(GDN_ERR_INVALID, "gdn_moe_route: tensors need their element's alignment");
   gdn::MoeRouteArgs a{};
   a.d = d;
-  a.logits = logits;
   a.stride = logits_stride;
-  a.T = T;
   a.bias = bias;
-  a.ids = ids;
-  a.weights = weights;
   a.stream = static_cast<hipStream_t>(stream);
-  const hipError_t e = gdn::launch_moe_route(a);
-  return e == hipSuccess ? GDN_OK : hip_fail(e, "gdn_moe_route launch");
+  for (int64_t t = 0; t < T; t += kRowsOfLaunch) {
+    a.T = (int)std::min<int64_t>(T - t, kRowsOfLaunch);
+    a.logits = static_cast<const char*>(logits) + t * logits_stride * (d.logits_f32 ? 4 : 2);
+    a.ids = ids + t * (d.top_k + d.num_shared);
+    a.weights = weights + t * (d.top_k + d.num_shared);
+    const hipError_t e = gdn::launch_moe_route(a);
+    if (e != hipSuccess) return hip_fail(e, "gdn_moe_route launch");
+  }
+  return GDN_OK;
 }
 
 gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const gdn_moe_part* parts,
@@ -334,11 +342,12 @@ gdn_status gdn_moe_forward(const gdn_moe* m, const uint16_t* x, int64_t x_stride
   return GDN_OK;
 }
 
-gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layers) {
+gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layers) try {
   if (!exec) return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: NULL executor");
-  if (n < 0 || (n > 0 && !layers))
-    return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: n = %d / NULL layers", n);
   const gdn::ExecShape x = gdn::exec_shape(exec);
+  if (n < 0 || n > x.depth || (n > 0 && !layers))
+    return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: n = %d (a stack of %d layers) / NULL layers", n,
+                 x.depth);
   std::vector<char> taken(x.depth, 0);
   std::vector<gdn::ExecMlp> halves(n);
   std::vector<std::shared_ptr<ExecMoe>> moes(n);
@@ -398,6 +407,8 @@ gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layer
     for (auto& m : moes) m->buf = buf;
   }
   return gdn::exec_set_mlp(exec, std::move(halves));
+} catch (const std::bad_alloc&) {
+  return mfail(GDN_ERR_OOM, "gdn_exec_set_moe: out of host memory");
 }
 
 gdn_status gdn_block_norm(const gdn_block_norm_desc* desc, int32_t n, const void* h,
@@ -447,22 +458,26 @@ gdn_status gdn_block_norm(const gdn_block_norm_desc* desc, int32_t n, const void
     return mfail(GDN_ERR_INVALID, "gdn_block_norm: a tensor updated in place keeps its stride");
   gdn::BlockNormArgs a{};
   a.d = d;
-  a.h = h;
-  a.h_out = h_out;
-  a.x = x;
   a.h_stride = h_stride;
   a.h_out_stride = h_out_stride;
   a.x_stride = x_stride;
   a.post_w = post_w;
-  a.gate = gate;
   a.gate_stride = gate_stride;
   a.pre_w = pre_w;
-  a.hn = hn;
   a.hn_stride = hn_stride;
-  a.n = n;
   a.stream = static_cast<hipStream_t>(stream);
-  const hipError_t e = gdn::launch_block_norm(a);
-  return e == hipSuccess ? GDN_OK : hip_fail(e, "gdn_block_norm launch");
+  const int64_t hb = d.h_f32 ? 4 : 2;
+  for (int64_t i = 0; i < n; i += kRowsOfLaunch) {
+    a.n = (int)std::min<int64_t>(n - i, kRowsOfLaunch);
+    a.h = static_cast<const char*>(h) + i * h_stride * hb;
+    a.h_out = static_cast<char*>(h_out) + i * h_out_stride * hb;
+    a.x = x + i * x_stride;
+    a.gate = gate ? gate + i * gate_stride : nullptr;
+    a.hn = hn ? hn + i * hn_stride : nullptr;
+    const hipError_t e = gdn::launch_block_norm(a);
+    if (e != hipSuccess) return hip_fail(e, "gdn_block_norm launch");
+  }
+  return GDN_OK;
 }
 
 }  // extern "C"

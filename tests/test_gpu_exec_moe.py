@@ -197,5 +197,10 @@ def test_set_moe_refusals(model):
                 [(0, w, gate, gdn_amd.route_desc(E + 40, TOPK, num_shared=1), None, moe)]):
         with pytest.raises(gdn_amd.GdnError):
             ex.set_moe(bad)
+    # more halves than layers are refused before any of them is read
+    one = (gdn_amd.ExecMoe * 1)()
+    for n in (4, 2 ** 31 - 1, -1):
+        assert ex.lib.gdn_exec_set_moe(ex.handle, n, one) != 0
+        assert b"3 layers" in ex.lib.gdn_last_error()
     assert ex.prefill(1, [1, 2, 3]) >= 0  # nothing changed
     ex.close()

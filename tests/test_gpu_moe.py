@@ -217,6 +217,23 @@ def test_route_column_slices_and_no_rows(gpu):
     run_route(dev[:0, :256], 256, 8)
 
 
+@pytest.mark.parametrize("dtype", [BF, F32])
+def test_route_of_more_rows_than_a_launch(gpu, dtype):
+    """2^22 rows go in a launch; the rows on both sides of the cut and the last ones."""
+    T, E, k = (1 << 22) + 5, 8, 2
+    g = torch.Generator(DEV).manual_seed(6)
+    l = torch.randn(T, E + 1, generator=g, device=DEV).to(dtype)
+    ids = torch.full((T, k + 1), -7, device=DEV, dtype=torch.int32)
+    w = torch.full((T, k + 1), -7.0, device=DEV)
+    gdn_amd.moe_route(l, ids, w, E, k, num_shared=1, shared_gate=True)
+    torch.cuda.synchronize()
+    for lo, hi in ((0, 4), ((1 << 22) - 4, T)):
+        rids, rw = ref_route(l[lo:hi].cpu(), E, k, shared=1, shared_gate=True)
+        assert torch.equal(ids[lo:hi].cpu(), rids)
+        assert ((w[lo:hi].cpu().double() - rw).abs() <= 2.0 ** -17 * rw).all()
+    assert int(ids.min()) == 0 and int(ids.max()) == E
+
+
 # ----------------------------------------------------------------- experts --
 
 def w4(g, e, n, k):
@@ -532,6 +549,23 @@ def test_block_norm_in_place_strided_and_no_rows(gpu):
     assert torch.equal(gate, wide[:, -1:])
     gdn_amd.block_norm(h[:0], x[:0], hn=x[:0], pre_w=w)
     assert torch.equal(h, h1)
+
+
+def test_block_norm_of_more_rows_than_a_launch(gpu):
+    """2^22 rows go in a launch: the rows around the cut as a small call gives them."""
+    n, hidden = (1 << 22) + 3, 8
+    g = torch.Generator(DEV).manual_seed(8)
+    h = torch.randn(n, hidden, generator=g, device=DEV)
+    x = torch.randn(n, 2 * hidden, generator=g, device=DEV).to(BF)[:, hidden:]
+    gate = torch.rand(n, 1, generator=g, device=DEV).to(BF)
+    w = torch.rand(hidden, generator=g, device=DEV).to(BF)
+    out, hn = torch.empty_like(h), torch.empty(n, hidden, device=DEV, dtype=BF)
+    kw = dict(pre_w=w, post_w=w, gate_sigmoid=True)
+    gdn_amd.block_norm(h, x, h_out=out, hn=hn, gate=gate, **kw)
+    for lo, hi in ((0, 3), ((1 << 22) - 3, n)):
+        o1, hn1 = torch.empty_like(out[lo:hi]), torch.empty_like(hn[lo:hi])
+        gdn_amd.block_norm(h[lo:hi], x[lo:hi], h_out=o1, hn=hn1, gate=gate[lo:hi], **kw)
+        assert torch.equal(out[lo:hi], o1) and torch.equal(hn[lo:hi], hn1)
 
 
 def test_block_norm_agrees_with_add_rms_norm(gpu):
