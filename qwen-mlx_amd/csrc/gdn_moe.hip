@@ -93,14 +93,10 @@ struct MoeSpace {
   uint16_t* xs;    // [T][3][gpad(hidden)] split group sums of x
   uint16_t* hs;    // [entries][3][gpad(inner)] and of h, by sorted row
   uint16_t* h;     // [entries, inner] by sorted row
-  uint16_t* rows;  // [entries, hidden] weighted rows of down by entry
+  float* rows;     // [entries, hidden] weighted rows of down by entry
   int32_t* counts; // [chunks of entries][experts] (moe_count_kernel)
   size_t bytes;
 };
-
-// The rows between down and the sum over a token's columns are bf16: half a step
-// of each summand, beside the half step of the result, for half of a prompt's
-// largest traffic.
 
 // Entries of a chunk of the two-launch plan, and those up to which one launch
 // does it.
@@ -128,7 +124,7 @@ MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t token
   s.xs = reinterpret_cast<uint16_t*>(take(tokens * 6 * gpad(hidden)));
   s.hs = reinterpret_cast<uint16_t*>(take(entries * 6 * gpad(inner)));
   s.h = reinterpret_cast<uint16_t*>(take(entries * inner * 2));
-  s.rows = reinterpret_cast<uint16_t*>(take(entries * hidden * 2));
+  s.rows = reinterpret_cast<float*>(take(entries * hidden * 4));
   s.counts = reinterpret_cast<int32_t*>(take((entries + kChunk - 1) / kChunk * experts * 4));
   s.bytes = at;
   return s;
@@ -169,7 +165,8 @@ __device__ __forceinline__ void moe_row_sums(const uint16_t* __restrict__ x, int
 // Expert e's tiles start at slot (entries before it) / rows + e: never fewer
 // slots than tiles, the ones left over marked empty (rows = 0).
 // Work-groups from `experts` on form the split group sums of x's rows
-// (moe_row_sums) beside it.
+// (moe_row_sums) beside it. 4 to 5 us up to 8192 entries: a launch and two rounds of
+// loads.
 constexpr int kPlanThreads = 1024;
 typedef int i32x4_a4 __attribute__((ext_vector_type(4), aligned(4)));
 __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(MoeArgs a, int rows, MoeSpace s) {
@@ -272,7 +269,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_count_kernel(MoeArgs a, int 
 // Then a work-group per chunk places its entries behind those of lower experts
 // and of its expert in the chunks before, and writes its share of the tile list.
 // Inside a chunk an expert's entries take their places in any order: a row's
-// sums do not depend on where it stands.
+// sums do not depend on where it stands. 147,456 entries of 16,384 rows: 17 us, most
+// of it reading x for the sums, and 9.5; in one launch as above 58.
 __global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(MoeArgs a, int rows, MoeSpace s) {
   extern __shared__ int lds[];
   __shared__ int wsum[kPlanThreads / 64];
@@ -340,6 +338,9 @@ __global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(MoeArgs a, int 
 
 // Most entries of a call whose work-groups find their rows by themselves: a
 // wave holds every id.
+// They and the rows' product with the sum are two launches: one token of 9 columns,
+// hidden 2048, inner 512, takes 6.4 + 5.7 us, the latency of a launch and a chain of
+// loads each (16 MB of weights); by a plan, tiles and a sum the call took 21.7.
 constexpr int kFewEntries = 64;
 // ... and the most tokens: down reads an expert's weights for each of them again.
 constexpr int kFewTokens = 6;
@@ -527,6 +528,8 @@ __device__ __forceinline__ void wait_vm() {
 //     ends with gate and up of the same 16 columns and stores h; the work-group's
 //     64 columns are one group of down's input, whose split sums it stores.
 //   else: rows of h, and the weighted rows of down go to their entries.
+// Bound by the weights' bytes and the loads' latency: 317 tokens of 9 columns, hidden
+// 2048, inner 512, 257 experts (11 rows each): up 66 us (269 MB), down 42.
 template <int MW, bool UP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) void moe_tile_kernel(
     MoeArgs a, MoeSpace s) {
@@ -751,13 +754,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
 #pragma unroll
     for (int u = 0; u < MW; ++u) {
       if (u * 16 + r16 >= tl.z) continue;
-      uint16_t* const o = s.rows + (int64_t)en[u] * a.hidden + 128 * cb +
-                          32 * wave + 4 * c4;
+      float* const o = s.rows + (int64_t)en[u] * a.hidden + 128 * cb + 32 * wave + 4 * c4;
 #pragma unroll
-      for (int i = 0; i < 2; ++i)
-        *reinterpret_cast<u32x2*>(o + 16 * i) =
-            (u32x2){f2bf2(wt[u] * T[i][u][0], wt[u] * T[i][u][1]),
-                    f2bf2(wt[u] * T[i][u][2], wt[u] * T[i][u][3])};
+      for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(o + 16 * i) = wt[u] * T[i][u];
     }
   }
 }
@@ -766,8 +765,10 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
 // 64 columns a work-group (small ones fill the chip evenly), KS pairs of waves each
 // over a part of the stages (a wave's stages run one after the other, so that a
 // small call takes as long as one wave's), the groups' sums of x from products
-// against ones instead of beforehand, and the offsets applied with the scales. Rows past the tile's are not read: their copies are out of the
-// buffer's range, which gives zeros.
+// against ones instead of beforehand, and the offsets applied with the scales. Rows
+// past the tile's are not read: their copies are out of the buffer's range, which
+// gives zeros. Bound by the weights' bytes: 64 tokens of 9 columns, hidden 2048, inner
+// 512, 257 experts: up 45 us at 5.9 TB/s, down 28 at 4.7.
 template <int KS, bool UP>
 __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))) void
     moe_stream_kernel(MoeArgs a, MoeSpace s) {
@@ -928,11 +929,9 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
     *reinterpret_cast<u32x2*>(s.h + (int64_t)(tl.y + r16) * a.inner + 32 * cb + 16 * cw + 4 * c4) =
         (u32x2){lo, hi};
   } else {
-    uint16_t* const o = s.rows + (int64_t)en * a.hidden + 64 * cb + 32 * cw + 4 * c4;
+    float* const o = s.rows + (int64_t)en * a.hidden + 64 * cb + 32 * cw + 4 * c4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i)
-      *reinterpret_cast<u32x2*>(o + 16 * i) =
-          (u32x2){f2bf2(wt * T[i][0], wt * T[i][1]), f2bf2(wt * T[i][2], wt * T[i][3])};
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(o + 16 * i) = wt * T[i];
   }
 }
 
@@ -945,6 +944,26 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
+// Down's sums T of two 32-column fragments and NB row blocks, times their rows'
+// weights, to the rows of their entries: of(r) gives row r's entry and weight. A
+// store writes 32 columns, 128 bytes, of two rows.
+template <int NB, typename Of>
+__device__ __forceinline__ void store_rows(float* __restrict__ rows, int N, int col, int c2, int n,
+                                           const f32x16 (&T)[2][NB], Of of) {
+#pragma unroll
+  for (int u = 0; u < NB; ++u)
+#pragma unroll
+    for (int e = 0; e < 16; ++e) {
+      const int r = 32 * u + 8 * (e >> 2) + 4 * c2 + (e & 3);
+      if (r < n) {
+        const int2 ew = of(r);
+        float* const o = rows + (int64_t)ew.x * N + col;
+        o[0] = __int_as_float(ew.y) * T[0][u][e];
+        o[32] = __int_as_float(ew.y) * T[1][u][e];
+      }
+    }
+}
+
 // moe_tile_kernel for experts with many rows: a tile of 64 rows against 256
 // columns, four waves in a row, each with all rows and 64 columns (two fragments
 // of 32), on 32 x 32 x 16 products. x is the A operand: lane (r32, c2) supplies
@@ -955,6 +974,14 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // 8-column chunks 4 d + 2 sg + c2 of x.
 // The rows are copied one stage ahead (two slots), the weights go to registers
 // half a stage ahead, once the last of the stage before are unpacked.
+// Bound by the vector instructions beside the products: a product of 32 cycles comes
+// with 9 of 4 cycles, 4 of them the scaling and 3.5 the unpacking, whose issue it
+// blocks for 12, and the card takes its clock back to 2.0 GHz. 16,384 tokens of 9
+// columns, hidden 2048, inner 512, 257 experts: up 713 us, 870 TFLOP/s. In copies
+// without a part: without the row copies 565 us, the weights 607, the offsets 635,
+// the unpacking 663; without any of them 350. Half the unpacking with 128 rows a wave
+// and half the columns (twice the row copies) took 760; three slots of rows and
+// weights more than two stages ahead, 690 to 700 in 256 registers, was not kept.
 template <bool UP>
 __global__ __launch_bounds__(256)
     __attribute__((amdgpu_waves_per_eu(2, 2))) void
@@ -1188,10 +1215,10 @@ __global__ __launch_bounds__(256)
     }
   }
 
-  // The results go through LDS, so that rows are written 16 bytes a lane; the
-  // slots are free once every wave is here.
-  lds_barrier();
   if constexpr (UP) {
+    // h goes through LDS, so that rows are written 16 bytes a lane; the slots are
+    // free once every wave is here.
+    lds_barrier();
     uint16_t* const hb = reinterpret_cast<uint16_t*>(xl0);  // [MT][128], chunks of 8 swizzled
     const int c = 32 * wave + r32;
 #pragma unroll
@@ -1222,47 +1249,21 @@ __global__ __launch_bounds__(256)
     }
   } else {
     if (!live) return;
-    // a wave's 32 rows at a time, [32][64] with 8-column chunks swizzled
-    uint16_t* const ob = reinterpret_cast<uint16_t*>(xl0) + wave * 32 * 64;
-#pragma unroll
-    for (int u = 0; u < RB; ++u) {
-      if (32 * u >= tl.z) break;
-#pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = 8 * (e >> 2) + 4 * c2 + (e & 3);
-        const float wt = wt_of[32 * u + r];
-#pragma unroll
-        for (int i = 0; i < 2; ++i) {
-          const int c = 32 * i + r32;
-          ob[r * 64 + 8 * ((c >> 3) ^ (r & 7)) + (c & 7)] = f2bf(wt * T[i][u][e]);
-        }
-      }
-      wait_lgkm0();
-      __builtin_amdgcn_wave_barrier();
-#pragma unroll
-      for (int j = 0; j < 4; ++j) {
-        const int r = 8 * j + (lane >> 3), ch = lane & 7;
-        const u32x4 v = *reinterpret_cast<const u32x4*>(ob + r * 64 + 8 * (ch ^ (r & 7)));
-        if (32 * u + r < tl.z)
-          *reinterpret_cast<u32x4*>(s.rows +
-                                    (int64_t)row_of[32 * u + r].y * a.hidden + 256 * cb + 64 * wave +
-                                    8 * ch) = v;
-      }
-      wait_lgkm0();
-      __builtin_amdgcn_wave_barrier();
-    }
+    store_rows<2>(s.rows, a.hidden, 256 * cb + 64 * wave + r32, c2, tl.z, T, [&](int r) {
+      return make_int2(row_of[r].y, __float_as_int(wt_of[r]));
+    });
   }
 }
 
 // Down for experts with many rows and inner up to 512: a tile of 64 rows stays in
 // LDS (four stages) while the work-group takes `run` blocks of 256 columns one
 // after the other, weights ahead across blocks; no wave waits for another.
-// Products, tasks and roles as in moe_wide_kernel.
+// Products, tasks and roles as in moe_wide_kernel, and so is its bound; the same
+// 16,384 tokens take 460 us, 670 TFLOP/s, and 1.2 GB of rows written.
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
     moe_wide_down_kernel(MoeArgs a, MoeSpace s, int run) {
   constexpr int MT = 64, XROW = kStageK * 2, SLOT = MT * XROW;
   __shared__ __align__(16) uint8_t xl[4 * SLOT];
-  __shared__ __align__(16) uint16_t stage_out[4][16 * 64];
   __shared__ u32x4 sums[MT][3];  // a row's split group sums: hi, mid, lo octet
   __shared__ int en_of[MT];
   __shared__ __align__(16) float wt_of[MT];
@@ -1454,42 +1455,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
           for (int i = 0; i < 2; ++i) T[i][u] = mfma32(xp, B[i], T[i][u]);
         }
-      // Through LDS, 16 rows at a time, so that rows are written 16 bytes a lane:
-      // 8-column chunk ch of row r at chunk ch ^ (r % 8). The lane's first byte is
-      // that of row 4 c2, column r32; other rows and columns flip or add bits.
-      char* const so = reinterpret_cast<char*>(stage_out[wave]);
-      int wat = 512 * c2 + (((r32 >> 3) | 4 * c2) << 4) + 2 * (r32 & 7);
-      int rat = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
-      asm volatile("" : "+v"(wat), "+v"(rat));  // addresses formed here, not kept
-#pragma unroll
-      for (int u = 0; u < NB; ++u)
-#pragma unroll
-        for (int hf = 0; hf < 2; ++hf) {
-          const int r0 = 32 * u + 16 * hf;
-          if (r0 >= tl.z) break;
-#pragma unroll
-          for (int g = 0; g < 2; ++g) {
-            const v4f wt = *reinterpret_cast<const v4f*>(&wt_of[r0 + 8 * g + 4 * c2]);
-#pragma unroll
-            for (int e = 0; e < 4; ++e)
-#pragma unroll
-              for (int i = 0; i < 2; ++i)
-                *reinterpret_cast<uint16_t*>(so + (wat ^ ((e << 4) | (i << 6))) + 128 * e + 1024 * g) =
-                    f2bf(wt[e] * T[i][u][8 * hf + 4 * g + e]);
-          }
-          wait_lgkm0();
-          __builtin_amdgcn_wave_barrier();
-#pragma unroll
-          for (int j = 0; j < 2; ++j) {
-            const int r = r0 + 8 * j + (lane >> 3);
-            const u32x4 v = *reinterpret_cast<const u32x4*>(so + rat + 1024 * j);
-            if (r < tl.z)
-              *reinterpret_cast<u32x4*>(s.rows + (int64_t)en_of[r] * N +
-                                        256 * cb + 64 * wave + 8 * (lane & 7)) = v;
-          }
-          wait_lgkm0();
-          __builtin_amdgcn_wave_barrier();
-        }
+      store_rows<NB>(s.rows, N, 256 * cb + 64 * wave + r32, c2, tl.z, T, [&](int r) {
+        return make_int2(en_of[r], __float_as_int(wt_of[r]));
+      });
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1504,21 +1472,24 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
     body(std::integral_constant<int, 1>{});
 }
 
-// out[t] = the sum of its entries' rows in column order. A thread per 8 columns, B
+// out[t] = the sum of its entries' rows in column order. A thread per 4 columns, B
 // rows' loads at a time; rows of ids outside the layer are read as they are in the
 // work-space and left out. Bound by reading the rows, in small calls by latency:
 // those take all of a token's rows at once, in small work-groups over more CUs.
+// The rows are f32: as bf16 they would take half of a prompt's largest traffic
+// (16,384 tokens: the sum 101 us against 215, down 410 against 460) and put the
+// result off by 0.0029 of its norm instead of 0.0024; rounding it alone is 0.0017.
 template <int B>
-__global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, uint16_t* rows) {
-  const int q = a.hidden / 8;
+__global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const float* rows) {
+  const int q = a.hidden / 4;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (int64_t)a.T * q) return;
   const int64_t t = i / q;
   const int c = (int)(i - t * q);
-  const u32x4* const r = reinterpret_cast<const u32x4*>(rows) + t * a.k * q + c;
-  float y[8] = {};
+  const f32x4* const r = reinterpret_cast<const f32x4*>(rows) + t * a.k * q + c;
+  f32x4 y = {0.f, 0.f, 0.f, 0.f};
   for (int j0 = 0; j0 < a.k; j0 += B) {
-    u32x4 v[B];
+    f32x4 v[B];
     bool in[B];
 #pragma unroll
     for (int j = 0; j < B; ++j)
@@ -1528,16 +1499,10 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, uint16_t* r
       }
 #pragma unroll
     for (int j = 0; j < B; ++j)
-      if (j0 + j < a.k && in[j])
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          y[2 * e] += bf_lo(v[j][e]);
-          y[2 * e + 1] += bf_hi(v[j][e]);
-        }
+      if (j0 + j < a.k && in[j]) y += v[j];
   }
-  u32x2* const o = reinterpret_cast<u32x2*>(a.out + t * a.os + c * 8);
-  o[0] = (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
-  o[1] = (u32x2){f2bf2(y[4], y[5]), f2bf2(y[6], y[7])};
+  *reinterpret_cast<u32x2*>(a.out + t * a.os + c * 4) =
+      (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
 }
 
 // ---- launches ----
@@ -1582,10 +1547,11 @@ hipError_t launch_wide(const MoeArgs& a, const MoeSpace& s, int64_t slots, int64
   const int blocks = (a.hidden + 255) / 256;
   if (a.inner > 4 * kStageK)
     return launch(moe_wide_kernel<false>, tile_groups(slots, blocks), 256, 0, a.stream, a, s);
-  // Long runs, as long as they leave two work-groups for each of the 512 that run
-  // side by side: 16,384 tokens (2,400 tiles) 401 us in runs of 8 blocks, 420 of 2.
+  // Long runs, as long as they leave three work-groups for each of the 512 that run
+  // side by side. The whole call in runs of 8 / 4 / 2 / 1 blocks: 16,384 tokens (2,400
+  // tiles) 1380 / 1365 / 1386 / 1432 us, 4,000 (690) 412 / 400 / 396 / 409.
   int run = blocks;
-  while (run > 1 && tiles * ((blocks + run - 1) / run) < 1024) run = (run + 1) / 2;
+  while (run > 1 && tiles * ((blocks + run - 1) / run) < 1536) run = (run + 1) / 2;
   return launch(moe_wide_down_kernel, tile_groups(slots, (blocks + run - 1) / run), 256, 0, a.stream,
                 a, s, run);
 }
@@ -1622,11 +1588,11 @@ hipError_t launch_moe(const MoeArgs& a) {
   }
   // The kernel by the rows that an expert has on average. At hidden 2048, inner
   // 512, 257 experts, 9 columns, tiles of 16 rows by the stream kernel / 16 / 32 /
-  // 64 rows: 64 tokens (mean 2) 77 / 86 / 94 / 115 us, 200 (7) 101 / 105 / 110 / 135,
-  // 317 (11) 120 / 114 / 117 / 143, 600 (21) - / 145 / 135 / 153, 2000 (70) - / 315 /
-  // 259 / 233. Tiles of 64 rows also want a work-group for most of the 512 that
+  // 64 rows: 64 tokens (mean 2) 81 / 85 / 88 / 108 us, 200 (7) 103 / 104 / 109 / 135,
+  // 317 (11) 123 / 114 / 118 / 141, 600 (21) - / 150 / 137 / 153, 2000 (70) - / 334 /
+  // 276 / 253. Tiles of 64 rows also want a work-group for most of the 512 that
   // run side by side (hidden 1024, inner 1408, 32 experts, 4 columns: 1000 tokens,
-  // 312 work-groups, 78 us by 32 rows and 79 by 64; 1500 tokens, 436, 101 / 93).
+  // 312 work-groups, 78 us by 32 rows and 78 by 64; 1500 tokens, 436, 102 / 91).
   const int mean = entries / a.experts;
   const int64_t wide_tiles = max_tiles(entries, a.experts, 64) - a.experts / 2;
   const bool wide = mean >= 64 && wide_tiles * ((a.hidden + 255) / 256) >= 384;
@@ -1651,8 +1617,8 @@ hipError_t launch_moe(const MoeArgs& a) {
   } else {
     MOE_TRY(rows == 16 ? launch_tiles<1>(a, s, slots) : launch_tiles<2>(a, s, slots));
   }
-  const int64_t n = (int64_t)a.T * (a.hidden / 8);
-  if (n < 1 << 16) return launch(moe_combine_kernel<16>, (n + 63) / 64, 64, 0, a.stream, a, s.rows);
+  const int64_t n = (int64_t)a.T * (a.hidden / 4);
+  if (n < 1 << 17) return launch(moe_combine_kernel<16>, (n + 63) / 64, 64, 0, a.stream, a, s.rows);
   return launch(moe_combine_kernel<4>, (n + 255) / 256, 256, 0, a.stream, a, s.rows);
 }
 

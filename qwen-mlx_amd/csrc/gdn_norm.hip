@@ -5,6 +5,8 @@
 // Both means are sums over a row, so a work-group holds one row in registers
 // (f32) from its only read to its only write. h' enters the second norm before
 // its rounding to the residual stream's type.
+// Bound by HBM: 16,384 rows of 2048 in bf16 take 40 us, 268 MB at 6.6 TB/s; 64 rows by
+// the latency of a launch, the loads and two sums, 3.5 us.
 #include "gdn_common.h"
 
 namespace gdn {
