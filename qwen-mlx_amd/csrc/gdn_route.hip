@@ -68,6 +68,15 @@ __device__ __forceinline__ float max_f32(float v) {
   return unordered(wave_max(ordered(v)));
 }
 
+// v of lane i (uniform)
+__device__ __forceinline__ float of_lane(float v, int i) {
+  return __int_as_float(__builtin_amdgcn_readlane(__float_as_int(v), i));
+}
+__device__ __forceinline__ double of_lane(double v, int i) {
+  return __hiloint2double(__builtin_amdgcn_readlane(__double2hiint(v), i),
+                          __builtin_amdgcn_readlane(__double2loint(v), i));
+}
+
 template <int R, bool F64, typename In>
 __global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a) {
   typedef std::conditional_t<F64, double, float> Key;
@@ -91,6 +100,10 @@ __global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a) {
 #pragma unroll
   for (int r = 0; r < R; ++r) raw[r] = logits[min(lane + 64 * r, E - 1)];
   const In gate = logits[a.d.shared_gate ? E : 0];
+  float bias[F64 ? R : 1];
+  if constexpr (F64)
+#pragma unroll
+    for (int r = 0; r < R; ++r) bias[r] = a.bias ? a.bias[min(lane + 64 * r, E - 1)] : 0.f;
   float l[R];
   float m = -INFINITY;
 #pragma unroll
@@ -103,23 +116,27 @@ __global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a) {
   if (exps) m = max_f32(m);
   Key key[R];
   if constexpr (F64) {
-    double sum = 1.0;
-    if (softmax && m > -INFINITY) {
-      sum = 0.0;
+    // for every expert and without branches, so that the R chains run side by side
+    const double top = m > -INFINITY ? (double)m : 0.0;
+    double ex[R];
+    if (softmax) {
+      double sum = 0.0;
 #pragma unroll
-      for (int r = 0; r < R; ++r)
-        if (l[r] > -INFINITY) sum += exp((double)l[r] - (double)m);
+      for (int r = 0; r < R; ++r) sum += ex[r] = exp((double)l[r] - top);
 #pragma unroll
       for (int off = 32; off > 0; off >>= 1) sum += __shfl_xor(sum, off, 64);
+#pragma unroll
+      for (int r = 0; r < R; ++r) key[r] = ex[r] / sum;
+    } else {
+#pragma unroll
+      for (int r = 0; r < R; ++r) ex[r] = exp(-(double)l[r]);
+#pragma unroll
+      for (int r = 0; r < R; ++r) key[r] = 1.0 / (1.0 + ex[r]);
     }
 #pragma unroll
     for (int r = 0; r < R; ++r) {
-      key[r] = none;
-      if (l[r] > -INFINITY) {
-        key[r] = softmax ? exp((double)l[r] - (double)m) / sum : 1.0 / (1.0 + exp(-(double)l[r]));
-        if (a.bias) key[r] += (double)a.bias[lane + 64 * r];
-        if (key[r] != key[r]) key[r] = none;
-      }
+      if (a.bias) key[r] += (double)bias[r];
+      key[r] = l[r] > -INFINITY && key[r] == key[r] ? key[r] : none;
     }
   } else {
 #pragma unroll
@@ -151,7 +168,7 @@ __global__ __launch_bounds__(256) void moe_route_kernel(MoeRouteArgs a) {
     // a group stays if fewer than top_groups others go before it
     int before = 0;
     for (int o = 0; o < G; ++o) {
-      const Key v = __shfl(gs, o * per, 64);
+      const Key v = of_lane(gs, o * per);
       before += v > gs || (v == gs && o < g);
     }
     const uint64_t stay = __ballot(before < a.d.top_groups);
