@@ -697,7 +697,11 @@ gdn_status gdn_moe_route(const gdn_moe_route_desc* desc, const void* logits,
  *   out[t] = sum_j weights[t, j] * down_e(silu(gate_e(x[t])) * up_e(x[t])),
  * each product on MLX 4-bit weights (group 64: scales * q + biases). A column
  * whose id is outside [0, E) adds nothing; a token without any gets zeros. An
- * id may appear in several columns of a token. */
+ * id may appear in several columns of a token. h = silu(gate) * up is rounded to
+ * bf16 and out once from f32; a call's results are the same bits every time. A
+ * token's do not depend on what the other tokens hold, but the kernel is chosen
+ * by T, k and E, so that calls of other sizes may differ by rounding. A token
+ * of x with infinities or NaN gets infinities or NaN, and it alone. */
 typedef struct gdn_moe gdn_moe;
 
 /* One set of experts, appended to the layer's in order: MLX-format arrays of
