@@ -423,6 +423,9 @@ struct MoePackArgs {
   hipStream_t stream;
 };
 hipError_t launch_moe_pack(const MoePackArgs& a);
+// bound (zeros before): of every expert the largest sum of |w| over a row of w that is
+// finite; wp, sb and the fragments are not used.
+hipError_t launch_moe_bound(const MoePackArgs& a, float* bound);
 
 struct MoeArgs {
   int hidden, inner, experts;
@@ -430,6 +433,7 @@ struct MoeArgs {
   const uint32_t* sb1;
   const void* w2;          // down
   const uint32_t* sb2;
+  const float* bound;      // [experts] of down (launch_moe_bound)
   const uint16_t* x;       // [T, xs]
   int64_t xs;
   int T, k;

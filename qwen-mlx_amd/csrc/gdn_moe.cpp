@@ -60,6 +60,7 @@ struct gdn_moe {
   uint32_t* sb1 = nullptr;
   void* w2 = nullptr;
   uint32_t* sb2 = nullptr;
+  float* bound = nullptr;
 };
 
 namespace {
@@ -212,7 +213,7 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
   // one expert's matrix product terms: words of 8 weights, {scale, bias} per 64
   const size_t terms = (size_t)hidden * inner;
   const size_t w = terms / 2 * experts, s = terms / 16 * experts;
-  const size_t bytes = 3 * (w + s);  // every part of it a multiple of 1024 bytes
+  const size_t bytes = 3 * (w + s) + 4 * (size_t)experts;  // w, s multiples of 1024 bytes
   if (hipMalloc(&m->base, bytes) != hipSuccess) {
     (void)hipGetLastError();
     m->base = nullptr;
@@ -224,7 +225,9 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
   m->w2 = p + 2 * w;
   m->sb1 = reinterpret_cast<uint32_t*>(p + 3 * w);
   m->sb2 = reinterpret_cast<uint32_t*>(p + 3 * w + 2 * s);
+  m->bound = reinterpret_cast<float*>(p + 3 * (w + s));
   const hipStream_t st = static_cast<hipStream_t>(stream);
+  hipError_t e = hipMemsetAsync(m->bound, 0, 4 * (size_t)experts, st);
   int64_t first = 0;
   for (int i = 0; i < nparts; ++i) {
     const gdn_moe_part& q = parts[i];
@@ -245,11 +248,13 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
       a.sb = sb + first * fmul * (terms / 64);
       return gdn::launch_moe_pack(a);
     };
-    hipError_t e = pack(q.gate_w, q.gate_scales, q.gate_biases, inner, hidden, 2, 0, m->w1, m->sb1);
+    if (e == hipSuccess)
+      e = pack(q.gate_w, q.gate_scales, q.gate_biases, inner, hidden, 2, 0, m->w1, m->sb1);
     if (e == hipSuccess)
       e = pack(q.up_w, q.up_scales, q.up_biases, inner, hidden, 2, 1, m->w1, m->sb1);
     if (e == hipSuccess)
       e = pack(q.down_w, q.down_scales, q.down_biases, hidden, inner, 1, 0, m->w2, m->sb2);
+    if (e == hipSuccess) e = gdn::launch_moe_bound(a, m->bound + first);  // down's matrices
     if (e != hipSuccess) {
       (void)hipStreamSynchronize(st);
       moe_release(m);
@@ -257,7 +262,7 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
     }
     first += q.experts;
   }
-  const hipError_t e = hipStreamSynchronize(st);
+  e = hipStreamSynchronize(st);
   if (e != hipSuccess) {
     moe_release(m);
     return hip_fail(e, "gdn_moe_create: synchronize");
@@ -324,6 +329,7 @@ gdn_status gdn_moe_forward(const gdn_moe* m, const uint16_t* x, int64_t x_stride
   a.sb1 = m->sb1;
   a.w2 = m->w2;
   a.sb2 = m->sb2;
+  a.bound = m->bound;
   a.xs = x_stride;
   a.k = k;
   a.os = out_stride;

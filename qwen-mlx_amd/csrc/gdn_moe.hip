@@ -59,6 +59,35 @@ __global__ void moe_pack_kernel(MoePackArgs a) {
   }
 }
 
+// bound[e] = the largest sum of |w| over a row of expert e's matrix [n, k] whose sum is
+// finite; bound starts at zeros. grid (n / 64 rounded up, experts), a wave 16 rows,
+// four lanes a row. Positive floats are in the order of their bits, and a maximum has
+// no order.
+__global__ __launch_bounds__(256) void moe_bound_kernel(MoePackArgs a, float* bound) {
+  const int lane = threadIdx.x & 63, c = lane & 3;
+  const int n = blockIdx.x * 64 + (threadIdx.x >> 6) * 16 + (lane >> 2);
+  const int words = a.k >> 3, G = a.k >> 6;
+  float sum = 0.f;
+  if (n < a.n) {
+    const int64_t row = (int64_t)blockIdx.y * a.n + n;
+    for (int j = 4 * c; j < words; j += 16) {
+      const float sc = bf2f(a.s[row * G + (j >> 3)]), of = bf2f(a.b[row * G + (j >> 3)]);
+#pragma unroll
+      for (int q = 0; q < 4; ++q) {
+        const uint32_t v = a.w[row * words + j + q];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) sum += fabsf(fmaf(sc, (float)(v >> (4 * i) & 15), of));
+      }
+    }
+  }
+  sum += __shfl_xor(sum, 1, 64);
+  sum += __shfl_xor(sum, 2, 64);
+  if (!(sum < INFINITY)) sum = 0.f;
+#pragma unroll
+  for (int off = 4; off < 64; off *= 2) sum = fmaxf(sum, __shfl_xor(sum, off, 64));
+  if (lane == 0) atomicMax(reinterpret_cast<int*>(bound) + blockIdx.y, __float_as_int(sum));
+}
+
 // --------------------------------------------------------------- experts --
 
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
@@ -82,6 +111,7 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 
 constexpr int kPassEntries = 1 << 18;  // of a pass over the experts
 constexpr int kStageK = 128;           // k of a stage: two groups
+constexpr int kWideInner = 512;        // inner up to which wide down keeps its rows in LDS
 // The bytes of x that a pass's 32-bit offsets reach, and an offset past them.
 constexpr uint32_t kReach = 0xFFFF0000u, kNowhere = 0xFFFF8000u;
 
@@ -93,7 +123,10 @@ struct MoeSpace {
   uint16_t* xs;    // [T][3][gpad(hidden)] split group sums of x
   uint16_t* hs;    // [entries][3][gpad(inner)] and of h, by sorted row
   uint16_t* h;     // [entries, inner] by sorted row
-  float* rows;     // [entries, hidden] weighted rows of down by entry
+  float* rows;     // [entries, hidden] weighted rows of down by entry, or
+                   // f16 of 2^-exps (moe_wide_down_kernel)
+  int32_t* exps;   // [entries]
+  uint16_t* hmax;  // [entries][8] largest |h| of a row's groups by sorted row, inner <= 512
   int32_t* counts; // [chunks of entries][experts] (moe_count_kernel)
   size_t bytes;
 };
@@ -125,9 +158,20 @@ MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t token
   s.hs = reinterpret_cast<uint16_t*>(take(entries * 6 * gpad(inner)));
   s.h = reinterpret_cast<uint16_t*>(take(entries * inner * 2));
   s.rows = reinterpret_cast<float*>(take(entries * hidden * 4));
+  s.exps = reinterpret_cast<int32_t*>(take(entries * 4));
+  s.hmax = reinterpret_cast<uint16_t*>(take(inner <= kWideInner ? entries * 16 : 0));
   s.counts = reinterpret_cast<int32_t*>(take((entries + kChunk - 1) / kChunk * experts * 4));
   s.bytes = at;
   return s;
+}
+
+// Largest value of 8 neighbouring lanes, in all of them.
+template <int CTRL>
+__device__ __forceinline__ uint32_t max_dpp(uint32_t v) {
+  return max(v, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, 0xF, 0xF, true));
+}
+__device__ __forceinline__ uint32_t max8(uint32_t v) {
+  return max_dpp<0x141>(max_dpp<0x4E>(max_dpp<0xB1>(v)));  // lane ^ 1, ^ 2, half mirror
 }
 
 // v as three bf16 parts, v = hi + mid + lo exactly, at dst, dst + step, ...
@@ -944,26 +988,6 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
                                                  __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// Down's sums T of two 32-column fragments and NB row blocks, times their rows'
-// weights, to the rows of their entries: of(r) gives row r's entry and weight. A
-// store writes 32 columns, 128 bytes, of two rows.
-template <int NB, typename Of>
-__device__ __forceinline__ void store_rows(float* __restrict__ rows, int N, int col, int c2, int n,
-                                           const f32x16 (&T)[2][NB], Of of) {
-#pragma unroll
-  for (int u = 0; u < NB; ++u)
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int r = 32 * u + 8 * (e >> 2) + 4 * c2 + (e & 3);
-      if (r < n) {
-        const int2 ew = of(r);
-        float* const o = rows + (int64_t)ew.x * N + col;
-        o[0] = __int_as_float(ew.y) * T[0][u][e];
-        o[32] = __int_as_float(ew.y) * T[1][u][e];
-      }
-    }
-}
-
 // moe_tile_kernel for experts with many rows: a tile of 64 rows against 256
 // columns, four waves in a row, each with all rows and 64 columns (two fragments
 // of 32), on 32 x 32 x 16 products. x is the A operand: lane (r32, c2) supplies
@@ -1237,36 +1261,59 @@ __global__ __launch_bounds__(256)
       const u32x4 v = *reinterpret_cast<const u32x4*>(hb + r * 128 + 8 * (ch ^ (r & 15)));
       *reinterpret_cast<u32x4*>(s.h + (int64_t)(tl.y + r) * a.inner + 128 * cb + 8 * ch) = v;
       float t = 0.f;
+      uint32_t m = 0;  // |h| as the order of its bits
 #pragma unroll
-      for (int q = 0; q < 4; ++q) t += bf_lo(v[q]) + bf_hi(v[q]);
+      for (int q = 0; q < 4; ++q) {
+        t += bf_lo(v[q]) + bf_hi(v[q]);
+        m = max(m, max(v[q] & 0x7FFFu, v[q] >> 16 & 0x7FFFu));
+      }
       t = sum8(t);
+      m = max8(m);
       if ((ch & 7) == 0) {
         uint16_t* const dst = s.hs + (int64_t)(tl.y + r) * 3 * gi;
         store_split(t, dst + 2 * cb + (ch >> 3), gi);
+        if (a.inner <= kWideInner) s.hmax[(tl.y + r) * 8 + 2 * cb + (ch >> 3)] = (uint16_t)m;
         if (cb == blocks - 1 && ch == 0)  // the padded groups
           for (int g = a.inner >> 6; g < gi; ++g) store_split(0.f, dst + g, gi);
       }
     }
   } else {
     if (!live) return;
-    store_rows<2>(s.rows, a.hidden, 256 * cb + 64 * wave + r32, c2, tl.z, T, [&](int r) {
-      return make_int2(row_of[r].y, __float_as_int(wt_of[r]));
-    });
+    // a store writes 32 columns, 128 bytes, of two rows
+    float* const rows = s.rows + 256 * cb + 64 * wave + r32;
+#pragma unroll
+    for (int u = 0; u < RB; ++u)
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int r = 32 * u + 8 * (e >> 2) + 4 * c2 + (e & 3);
+        if (r < tl.z) {
+          float* const o = rows + (int64_t)row_of[r].y * a.hidden;
+          o[0] = wt_of[r] * T[0][u][e];
+          o[32] = wt_of[r] * T[1][u][e];
+        }
+      }
   }
 }
 
 // Down for experts with many rows and inner up to 512: a tile of 64 rows stays in
 // LDS (four stages) while the work-group takes `run` blocks of 256 columns one
 // after the other, weights ahead across blocks; no wave waits for another.
-// Products, tasks and roles as in moe_wide_kernel, and so is its bound; the same
-// 16,384 tokens take 460 us, 670 TFLOP/s, and 1.2 GB of rows written.
+// Products, tasks and roles as in moe_wide_kernel, and so is its bound.
+// A row goes out in f16 under an exponent of its own: |down h| is at most the largest
+// sum of |w| over a column's inputs times the largest |h|, and the power of two above
+// that and the weight is brought to 2^15. A value keeps 11 bits down to 2^-29 of the
+// bound and 2^-40 of it absolutely; only the result's own 8 bits follow. The same
+// 16,384 tokens: 410 us, 750 TFLOP/s, and 102 for their sum. In f32 it was 460 and 215,
+// and in bf16, at 410 and 101, the result was off by 0.0029 of its norm instead of
+// 0.0024 (0.0017 is its own rounding).
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
     moe_wide_down_kernel(MoeArgs a, MoeSpace s, int run) {
   constexpr int MT = 64, XROW = kStageK * 2, SLOT = MT * XROW;
   __shared__ __align__(16) uint8_t xl[4 * SLOT];
+  __shared__ __align__(16) uint16_t stage_out[4][16 * 64];
   __shared__ u32x4 sums[MT][3];  // a row's split group sums: hi, mid, lo octet
   __shared__ int en_of[MT];
-  __shared__ __align__(16) float wt_of[MT];
+  __shared__ __align__(16) float wt_of[MT];  // weights times 2^-exponent
   const int P = a.inner >> 7, N = a.hidden, blocks = (N + 255) >> 8;
   const int chunks = (blocks + run - 1) / run;
   const int n = *s.ntiles * chunks, per = (n + 7) >> 3;
@@ -1283,6 +1330,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, c2 = lane >> 5;
 
+  const int bound = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(a.bound[tl.x]));
   // the rows of all stages, and what goes with a row
   {
     const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc(
@@ -1301,8 +1349,19 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
           s.hs + ((int64_t)tl.y + min(tid / 3, tl.z - 1)) * 24 + 8 * (tid % 3));
     if (tid < MT) {
       const int en = s.perm[tl.y + min(tid, tl.z - 1)].y;
+      const float w = a.weights[en];
+      const u32x4 hm =
+          *reinterpret_cast<const u32x4*>(s.hmax + (tl.y + min(tid, tl.z - 1)) * 8);
+      uint32_t m = 0;
+#pragma unroll
+      for (int q = 0; q < 4; ++q)  // stages: two groups each
+        if (q < P) m = max(m, max(hm[q] & 0xFFFFu, hm[q] >> 16));
+      // 2^b is above the row's values before the weight, 2^(b + exponent of w) after
+      const int b = __builtin_amdgcn_frexp_expf(__uint_as_float(m << 16)) + bound;
+      const int e = max(-100, min(b, 128)) + __builtin_amdgcn_frexp_expf(w) - 15;
       en_of[tid] = en;
-      wt_of[tid] = a.weights[en];
+      wt_of[tid] = ldexpf(w, -e);
+      if (cb0 == 0 && tid < tl.z) s.exps[en] = e;
     }
     wait_vm<0>();
     __syncthreads();
@@ -1455,9 +1514,42 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
           for (int i = 0; i < 2; ++i) T[i][u] = mfma32(xp, B[i], T[i][u]);
         }
-      store_rows<NB>(s.rows, N, 256 * cb + 64 * wave + r32, c2, tl.z, T, [&](int r) {
-        return make_int2(en_of[r], __float_as_int(wt_of[r]));
-      });
+      // Through LDS, 16 rows at a time, so that rows are written 16 bytes a lane:
+      // 8-column chunk ch of row r at chunk ch ^ (r % 8). The lane's first byte is
+      // that of row 4 c2, column r32; other rows and columns flip or add bits.
+      char* const so = reinterpret_cast<char*>(stage_out[wave]);
+      int wat = 512 * c2 + (((r32 >> 3) | 4 * c2) << 4) + 2 * (r32 & 7);
+      int rat = (lane >> 3) * 128 + (((lane & 7) ^ (lane >> 3)) << 4);
+      asm volatile("" : "+v"(wat), "+v"(rat));  // addresses formed here, not kept
+#pragma unroll
+      for (int u = 0; u < NB; ++u)
+#pragma unroll
+        for (int hf = 0; hf < 2; ++hf) {
+          const int r0 = 32 * u + 16 * hf;
+          if (r0 >= tl.z) break;
+#pragma unroll
+          for (int g = 0; g < 2; ++g) {
+            const v4f wt = *reinterpret_cast<const v4f*>(&wt_of[r0 + 8 * g + 4 * c2]);
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+#pragma unroll
+              for (int i = 0; i < 2; ++i)
+                *reinterpret_cast<_Float16*>(so + (wat ^ ((e << 4) | (i << 6))) + 128 * e + 1024 * g) =
+                    (_Float16)(wt[e] * T[i][u][8 * hf + 4 * g + e]);
+          }
+          wait_lgkm0();
+          __builtin_amdgcn_wave_barrier();
+#pragma unroll
+          for (int j = 0; j < 2; ++j) {
+            const int r = r0 + 8 * j + (lane >> 3);
+            const u32x4 v = *reinterpret_cast<const u32x4*>(so + rat + 1024 * j);
+            if (r < tl.z)
+              *reinterpret_cast<u32x4*>(reinterpret_cast<_Float16*>(s.rows) + (int64_t)en_of[r] * N +
+                                        256 * cb + 64 * wave + 8 * (lane & 7)) = v;
+          }
+          wait_lgkm0();
+          __builtin_amdgcn_wave_barrier();
+        }
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1476,9 +1568,6 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 // rows' loads at a time; rows of ids outside the layer are read as they are in the
 // work-space and left out. Bound by reading the rows, in small calls by latency:
 // those take all of a token's rows at once, in small work-groups over more CUs.
-// The rows are f32: as bf16 they would take half of a prompt's largest traffic
-// (16,384 tokens: the sum 101 us against 215, down 410 against 460) and put the
-// result off by 0.0029 of its norm instead of 0.0024; rounding it alone is 0.0017.
 template <int B>
 __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const float* rows) {
   const int q = a.hidden / 4;
@@ -1503,6 +1592,39 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const float
   }
   *reinterpret_cast<u32x2*>(a.out + t * a.os + c * 4) =
       (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
+}
+
+// The same of f16 rows: a thread per 8 columns.
+__global__ __launch_bounds__(256) void moe_combine_half_kernel(MoeArgs a, MoeSpace s) {
+  constexpr int B = 4;
+  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+  const int q = a.hidden / 8;
+  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+  if (i >= (int64_t)a.T * q) return;
+  const int64_t t = i / q;
+  const int c = (int)(i - t * q);
+  const f16x8* const r = reinterpret_cast<const f16x8*>(s.rows) + t * a.k * q + c;
+  float y[8] = {};
+  for (int j0 = 0; j0 < a.k; j0 += B) {
+    f16x8 v[B];
+    int e[B];
+    bool in[B];
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      if (j0 + j < a.k) {
+        v[j] = __builtin_nontemporal_load(r + (int64_t)(j0 + j) * q);
+        e[j] = s.exps[t * a.k + j0 + j];
+        in[j] = (uint32_t)a.ids[t * a.k + j0 + j] < (uint32_t)a.experts;
+      }
+#pragma unroll
+    for (int j = 0; j < B; ++j)
+      if (j0 + j < a.k && in[j])
+#pragma unroll
+        for (int n = 0; n < 8; ++n) y[n] += ldexpf((float)v[j][n], e[j]);
+  }
+  u32x2* const o = reinterpret_cast<u32x2*>(a.out + t * a.os + c * 8);
+  o[0] = (u32x2){f2bf2(y[0], y[1]), f2bf2(y[2], y[3])};
+  o[1] = (u32x2){f2bf2(y[4], y[5]), f2bf2(y[6], y[7])};
 }
 
 // ---- launches ----
@@ -1545,11 +1667,11 @@ hipError_t launch_tiles(const MoeArgs& a, const MoeSpace& s, int64_t slots) {
 hipError_t launch_wide(const MoeArgs& a, const MoeSpace& s, int64_t slots, int64_t tiles) {
   MOE_TRY(launch(moe_wide_kernel<true>, tile_groups(slots, a.inner / 128), 256, 0, a.stream, a, s));
   const int blocks = (a.hidden + 255) / 256;
-  if (a.inner > 4 * kStageK)
+  if (a.inner > kWideInner)
     return launch(moe_wide_kernel<false>, tile_groups(slots, blocks), 256, 0, a.stream, a, s);
   // Long runs, as long as they leave three work-groups for each of the 512 that run
   // side by side. The whole call in runs of 8 / 4 / 2 / 1 blocks: 16,384 tokens (2,400
-  // tiles) 1380 / 1365 / 1386 / 1432 us, 4,000 (690) 412 / 400 / 396 / 409.
+  // tiles) 1210 / 1214 / 1226 / 1251 us, 4,000 (690) 398 / 385 / 385 / 396.
   int run = blocks;
   while (run > 1 && tiles * ((blocks + run - 1) / run) < 1536) run = (run + 1) / 2;
   return launch(moe_wide_down_kernel, tile_groups(slots, (blocks + run - 1) / run), 256, 0, a.stream,
@@ -1562,6 +1684,12 @@ hipError_t launch_moe_pack(const MoePackArgs& a) {
   const int blocks = (a.n * (a.k / 128) * 4 + 255) / 256;
   hipLaunchKernelGGL(moe_pack_kernel, dim3(blocks < 64 ? blocks : 64, a.experts), dim3(256), 0,
                      a.stream, a);
+  return hipGetLastError();
+}
+
+hipError_t launch_moe_bound(const MoePackArgs& a, float* bound) {
+  hipLaunchKernelGGL(moe_bound_kernel, dim3((a.n + 63) / 64, a.experts), dim3(256), 0, a.stream, a,
+                     bound);
   return hipGetLastError();
 }
 
@@ -1589,13 +1717,14 @@ hipError_t launch_moe(const MoeArgs& a) {
   // The kernel by the rows that an expert has on average. At hidden 2048, inner
   // 512, 257 experts, 9 columns, tiles of 16 rows by the stream kernel / 16 / 32 /
   // 64 rows: 64 tokens (mean 2) 81 / 85 / 88 / 108 us, 200 (7) 103 / 104 / 109 / 135,
-  // 317 (11) 123 / 114 / 118 / 141, 600 (21) - / 150 / 137 / 153, 2000 (70) - / 334 /
-  // 276 / 253. Tiles of 64 rows also want a work-group for most of the 512 that
-  // run side by side (hidden 1024, inner 1408, 32 experts, 4 columns: 1000 tokens,
-  // 312 work-groups, 78 us by 32 rows and 78 by 64; 1500 tokens, 436, 102 / 91).
+  // 317 (11) 123 / 114 / 118 / 141, 600 (21) - / 150 / 137 / 153, 1000 (35) - / - / 190 /
+  // 181, 2000 (70) - / 327 / 275 / 248. Tiles of 64 rows also want a work-group for
+  // most of the 512 that run side by side (hidden 1024, inner 1408, 32 experts, 4
+  // columns: 1000 tokens, 312 work-groups, 78 us by 32 rows and 78 by 64; 1500 tokens,
+  // 436, 102 / 91).
   const int mean = entries / a.experts;
   const int64_t wide_tiles = max_tiles(entries, a.experts, 64) - a.experts / 2;
-  const bool wide = mean >= 64 && wide_tiles * ((a.hidden + 255) / 256) >= 384;
+  const bool wide = mean >= 32 && wide_tiles * ((a.hidden + 255) / 256) >= 384;
   const bool stream = mean < 8;
   const int rows = wide ? 64 : mean <= 16 ? 16 : 32;
   const int64_t slots = max_tiles(entries, a.experts, rows);
@@ -1618,6 +1747,8 @@ hipError_t launch_moe(const MoeArgs& a) {
     MOE_TRY(rows == 16 ? launch_tiles<1>(a, s, slots) : launch_tiles<2>(a, s, slots));
   }
   const int64_t n = (int64_t)a.T * (a.hidden / 4);
+  if (wide && a.inner <= kWideInner)
+    return launch(moe_combine_half_kernel, (n / 2 + 255) / 256, 256, 0, a.stream, a, s);
   if (n < 1 << 17) return launch(moe_combine_kernel<16>, (n + 63) / 64, 64, 0, a.stream, a, s.rows);
   return launch(moe_combine_kernel<4>, (n + 255) / 256, 256, 0, a.stream, a, s.rows);
 }

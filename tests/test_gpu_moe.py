@@ -261,7 +261,9 @@ class Experts:
 
     def ref(self, x, ids, weights):
         """(out, bound) in 64 bits: the result and how far f32 sums, the bf16
-        rounding of h and of the rows, and the last rounding may move it."""
+        rounding of h, the rows' of long prompts to 11 bits and the last rounding may
+        move it. A row's f16 has its power of two within 2^3 of 2^15 times the bound
+        max |h| * max sum |w|: half a step of its smallest numbers is 2^-37 of that."""
         x = x.double()
         out, tol = torch.zeros_like(x), torch.zeros_like(x)
         e = 0
@@ -288,7 +290,8 @@ class Experts:
                 # |silu'| <= 1.1, |silu(a)| <= |a|; 8 half steps for the exponential
                 eh = 1.1 * ea * u.abs() + a.abs() * eu + ea * eu + (HALF_BF + 8 * HALF_F32) * h.abs()
                 y = h @ wd.t()
-                ey = eh @ wd.abs().t() + err(part[2], i, h) + HALF_BF * y.abs()
+                ey = eh @ wd.abs().t() + err(part[2], i, h) + 2.0 ** -11 * y.abs()
+                ey += 2.0 ** -37 * (h.abs() + eh).amax(1, True) * wd.abs().sum(1).max()
                 out[rows] += w[rows].sum(1, keepdim=True) * y
                 tol[rows] += w[rows].abs().sum(1, keepdim=True) * ey
         return out, tol + HALF_BF * (out.abs() + tol)
@@ -377,6 +380,35 @@ def test_experts_uneven_absent_and_repeated_ids(gpu, T, hidden, inner):
     same = torch.full((T, 4), 6, dtype=torch.int32)
     ex.check(x, same, w)
     assert (ex.run(x, torch.full((T, 4), -1, dtype=torch.int32), w) == 0).all()
+
+
+@pytest.mark.parametrize("T,hidden,inner", [(2, 256, 256), (20, 256, 256), (300, 256, 256),
+                                            (1700, 2048, 128), (1750, 2048, 384)])
+def test_experts_of_all_magnitudes(gpu, T, hidden, inner):
+    """Tokens from 2^-30 to 2^30 (h to 2^60 either way), weights of 2^-40 to 2^40 in one
+    token, zeros among both, an expert whose down has no finite columns but one."""
+    ex = Experts(hidden, inner, [2], seed=11)
+    g = torch.Generator().manual_seed(T)
+    ids, w = draw_ids(T, T, 2, 2)
+    x = draw_x(T, T, hidden).double() * 2.0 ** torch.randint(-30, 31, (T, 1), generator=g)
+    x[:: 7] = 0
+    w = (w * 2.0 ** torch.randint(-40, 41, (T, 2), generator=g)).float()
+    w[::5, 0] = 0
+    ex.check(x.to(BF), ids, w)
+    wide = Experts(hidden, inner, [2], seed=12)
+    (_, _, (dw, ds, db)), = wide.parts
+    db[1, 1:] = INF
+    dev = [tuple(tuple(t.to(DEV) for t in m) for m in p) for p in wide.parts]
+    wide.moe = gdn_amd.MoE(hidden, inner, dev)
+    x = draw_x(T + 1, T, hidden)
+    only = torch.stack([torch.full((T,), 1), torch.full((T,), -1)], 1).to(torch.int32)
+    only[:, 1] = torch.where(torch.arange(T) % 2 == 0, 0, -1)
+    w = torch.ones(T, 2)
+    out = wide.run(x, only, w)
+    db[1, 1:] = 0
+    ref, tol = wide.ref(x, only, w)
+    assert ((out.double() - ref).abs() <= tol)[:, 0].all()
+    assert not out[:, 1:].isfinite().any()
 
 
 def test_experts_rows_keep_to_themselves(gpu):
