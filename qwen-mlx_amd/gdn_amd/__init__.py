@@ -198,7 +198,8 @@ def load(path: str = LIB_PATH):
     # same runtime instance, so device pointers from torch's allocator and its
     # streams are valid inside the library.
     try:
-        import torch  # noqa: F401
+        import torch
+        _torch_names(torch)
     except ImportError:
         pass
     lib = ctypes.CDLL(path)
@@ -249,6 +250,50 @@ def _stream(stream) -> int | None:
     return raw(torch.cuda.current_device())
 
 
+# torch's names for the calls below, which take some microseconds in all: looked up
+# once, when the library is loaded
+_IS_BF16 = _IS_F32 = _IS_I32 = _IS_U8 = ()  # types, bf16 also as bit patterns
+_current_device = _raw_stream = None
+
+
+def _torch_names(torch):
+    global _IS_BF16, _IS_F32, _IS_I32, _IS_U8, _current_device, _raw_stream
+    _IS_BF16, _IS_F32 = (torch.bfloat16, torch.int16, torch.uint16), (torch.float32,)
+    _IS_I32, _IS_U8 = (torch.int32,), (torch.uint8,)
+    _current_device = torch.cuda.current_device
+    _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
+        lambda dev: torch.cuda.current_stream(dev).cuda_stream)
+
+
+def _refuse(t, dev, size, types, what: str):
+    if t.get_device() != dev:
+        raise ValueError(f"{what} must be on cuda:{dev}, not {t.device}")
+    if t.dtype not in types:
+        raise ValueError(f"{what} must be {types[0]}, not {t.dtype}")
+    if t.size() != size:
+        raise ValueError(f"{what} must be {list(size)}, not {list(t.size())}")
+    raise ValueError(f"{what} must be contiguous (a matrix: its rows)")
+
+
+def _mat(t, dev: int, size, types, what: str):
+    """(pointer, row stride in elements) of a matrix of that size and type on device
+    dev whose rows are contiguous."""
+    if t.size() != size or t.get_device() != dev or t.dtype not in types:
+        _refuse(t, dev, size, types, what)
+    rows, cols = t.stride()
+    if cols != 1 and size[1] > 1:
+        _refuse(t, dev, size, types, what)
+    return t.data_ptr(), rows
+
+
+def _dense(t, dev: int, size, types, what: str) -> int:
+    """Pointer of a contiguous tensor of that size and type on device dev."""
+    if (t.size() != size or t.get_device() != dev or t.dtype not in types or
+            not t.is_contiguous()):
+        _refuse(t, dev, size, types, what)
+    return t.data_ptr()
+
+
 class _Dependents:
     """Destroy order of library objects whose C destroy touches another object.
 
@@ -286,38 +331,6 @@ def add_rms_norm(h, d, w, eps, hn, group_sums=None, stream=None):
                                    _ptr(group_sums), _stream(stream)))
 
 
-_BF16_DTYPES = ()  # torch types taken as bf16 bit patterns, once torch is imported
-
-
-def _is_f32(t, what: str) -> bool:
-    """Whether t holds f32 rather than bf16 (torch.bfloat16 or 16-bit patterns)."""
-    global _BF16_DTYPES
-    dt = t.dtype
-    if dt in _BF16_DTYPES:
-        return False
-    import torch
-    if not _BF16_DTYPES:
-        _BF16_DTYPES = (torch.bfloat16, torch.int16, torch.uint16)
-    if dt == torch.float32:
-        return True
-    if dt not in _BF16_DTYPES:
-        raise ValueError(f"{what} must be float32 or bf16, not {dt}")
-    return False
-
-
-def _bf16(t, what: str):
-    if _is_f32(t, what):
-        raise ValueError(f"{what} must be bf16")
-    return t
-
-
-def _typed(t, name: str, what: str):
-    import torch
-    if t.dtype != getattr(torch, name):
-        raise ValueError(f"{what} must be torch.{name}, not {t.dtype}")
-    return t
-
-
 @functools.lru_cache(maxsize=256)
 def route_desc(num_experts, top_k, score="softmax", num_groups=1, top_groups=1, group_top=1,
                renorm=True, scale=1.0, num_shared=0, shared_gate=False, logits_f32=False):
@@ -336,21 +349,20 @@ def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=No
     """Experts of every token (gdn_moe_route): logits [T, >= num_experts (+ 1 with
     shared_gate)] bf16 or f32 rows -> ids int32 and weights f32 [T, top_k + num_shared].
     score: "softmax" or "sigmoid"; bias f32 [num_experts] moves the choice only."""
-    lp, ls = _rows(logits)
-    T, cols = logits.shape
+    lib, dev = load(), _current_device()
+    size = logits.size()
+    T, cols = size
+    f32 = logits.dtype in _IS_F32
+    lp, ls = _mat(logits, dev, size, _IS_F32 if f32 else _IS_BF16, "logits")
     if cols < num_experts + (1 if shared_gate else 0):
         raise ValueError("logits hold fewer columns than experts")
     want = (T, top_k + num_shared)
-    if _typed(ids, "int32", "ids").shape != want:
-        raise ValueError(f"ids must be {want}")
-    if _typed(weights, "float32", "weights").shape != want:
-        raise ValueError(f"weights must be {want}")
-    if bias is not None and _typed(bias, "float32", "bias").numel() != num_experts:
-        raise ValueError("one bias per expert")
+    ip, wp = _dense(ids, dev, want, _IS_I32, "ids"), _dense(weights, dev, want, _IS_F32, "weights")
+    bp = None if bias is None else _dense(bias, dev, (num_experts,), _IS_F32, "bias")
     d = route_desc(num_experts, top_k, score, num_groups, top_groups, group_top, renorm, scale,
-                   num_shared, shared_gate, _is_f32(logits, "logits"))
-    _check(load().gdn_moe_route(ctypes.byref(d), lp, ls, T, _ptr(bias), _ptr(ids), _ptr(weights),
-                                _stream(stream)))
+                   num_shared, shared_gate, f32)
+    _check(lib.gdn_moe_route(ctypes.byref(d), lp, ls, T, bp, ip, wp,
+                             _raw_stream(dev) if stream is None else stream.cuda_stream))
 
 
 @functools.lru_cache(maxsize=256)
@@ -365,39 +377,31 @@ def block_norm(h, x, h_out=None, hn=None, pre_w=None, pre_eps=1e-6, post_w=None,
     h_out = h + scale * gate * b, hn = rms_norm(h_out) * pre_w. h, h_out [n, hidden]
     bf16 or f32 (h_out None: in place), the others bf16; gate [n, 1] or [n, hidden] rows,
     or [hidden] for one row shared by all; pre_w and hn None: no second norm."""
-    shape = h.shape
-    n, hidden = shape
-    hp, hs = _rows(h)
-    xp, xs = _rows(_bf16(x, "x"))
-    f32 = _is_f32(h, "h")
-    if x.shape != shape:
-        raise ValueError("x must have h's shape")
-    op, os_ = hp, hs
+    lib, dev = load(), _current_device()
+    size = h.size()
+    n, hidden = size
+    f32 = h.dtype in _IS_F32
+    types = _IS_F32 if f32 else _IS_BF16
+    hp, hs = op, os_ = _mat(h, dev, size, types, "h")
     if h_out is not None:
-        op, os_ = _rows(h_out)
-        if h_out.dtype != h.dtype or h_out.shape != shape:
-            raise ValueError("h_out must have h's shape and type")
-    np_, ns = None, 0
-    if hn is not None:
-        np_, ns = _rows(_bf16(hn, "hn"))
-        if hn.shape != shape:
-            raise ValueError("hn must have h's shape")
-    for w in (post_w, pre_w):
-        if w is not None and _bf16(w, "norm weights").numel() != hidden:
-            raise ValueError("norm weights hold one value per column")
+        op, os_ = _mat(h_out, dev, size, types, "h_out")
+    xp, xs = _mat(x, dev, size, _IS_BF16, "x")
+    np_, ns = (None, 0) if hn is None else _mat(hn, dev, size, _IS_BF16, "hn")
+    post = None if post_w is None else _dense(post_w, dev, (hidden,), _IS_BF16, "post_w")
+    pre = None if pre_w is None else _dense(pre_w, dev, (hidden,), _IS_BF16, "pre_w")
     kind, gp, gs = 0, None, 0
     if gate is not None:
-        gshape = _bf16(gate, "gate").shape
-        if gshape == (hidden,):
-            kind, gp, gs = 2, _ptr(gate), 0
-        elif gshape == (n, 1) or gshape == shape:
-            gp, gs = _rows(gate)
-            kind = 1 if gshape[1] == 1 else 2
+        gsize = gate.size()
+        if gsize == (hidden,):
+            kind, gp = 2, _dense(gate, dev, gsize, _IS_BF16, "gate")
+        elif gsize == (n, 1) or gsize == size:
+            kind = 1 if gsize[1] == 1 else 2
+            gp, gs = _mat(gate, dev, gsize, _IS_BF16, "gate")
         else:
             raise ValueError("gate must be [n, 1], [n, hidden] or [hidden]")
     d = _block_norm_desc(hidden, f32, kind, gate_sigmoid, unit_offset, scale, post_eps, pre_eps)
-    _check(load().gdn_block_norm(ctypes.byref(d), n, hp, hs, xp, xs, _ptr(post_w), gp, gs,
-                                 _ptr(pre_w), op, os_, np_, ns, _stream(stream)))
+    _check(lib.gdn_block_norm(ctypes.byref(d), n, hp, hs, xp, xs, post, gp, gs, pre, op, os_, np_,
+                              ns, _raw_stream(dev) if stream is None else stream.cuda_stream))
 
 
 class Pool:
@@ -617,7 +621,7 @@ class MoE:
             for (w, s, b), (rows, cols) in zip(part, ((inner, hidden), (inner, hidden),
                                                       (hidden, inner))):
                 if (tuple(w.shape) != (n, rows, cols // 8) or w.element_size() != 4 or
-                        any(tuple(t.shape) != (n, rows, cols // 64) or _is_f32(t, "scales")
+                        any(tuple(t.shape) != (n, rows, cols // 64) or t.dtype not in _IS_BF16
                             for t in (s, b))):
                     raise ValueError(f"part {i}: expected [{n}, {rows}, {cols}] in 4-bit groups "
                                      "of 64")
@@ -645,15 +649,17 @@ class MoE:
     def forward(self, x, ids, weights, out, workspace, stream=None):
         """out[t] = sum_j weights[t, j] * expert ids[t, j] of x[t]; x, out [T, hidden] bf16
         rows, ids int32 and weights f32 [T, k]; ids outside [0, experts) add nothing."""
-        xp, xs = _rows(_bf16(x, "x"))
-        op, os_ = _rows(_bf16(out, "out"))
-        shape = _typed(ids, "int32", "ids").shape
-        T, k = shape
-        if x.shape != (T, self.hidden) or out.shape != x.shape or weights.shape != shape:
-            raise ValueError(f"need x, out [{T}, {self.hidden}] and weights [{T}, {k}]")
-        _typed(weights, "float32", "weights")
-        _check(self.lib.gdn_moe_forward(self.handle, xp, xs, T, k, _ptr(ids), _ptr(weights), op,
-                                        os_, _ptr(workspace), workspace.nbytes, _stream(stream)))
+        dev = self.device
+        want = ids.size()
+        T, k = want
+        size = (T, self.hidden)
+        xp, xs = _mat(x, dev, size, _IS_BF16, "x")
+        op, os_ = _mat(out, dev, size, _IS_BF16, "out")
+        ip, wp = _dense(ids, dev, want, _IS_I32, "ids"), _dense(weights, dev, want, _IS_F32, "weights")
+        sp = _dense(workspace, dev, workspace.size(), _IS_U8, "workspace")
+        _check(self.lib.gdn_moe_forward(self.handle, xp, xs, T, k, ip, wp, op, os_, sp,
+                                        workspace.nbytes,
+                                        _raw_stream(dev) if stream is None else stream.cuda_stream))
 
     def close(self):
         if getattr(self, "handle", None):

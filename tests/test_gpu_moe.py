@@ -702,3 +702,44 @@ def test_the_half_captured_and_replayed(gpu, T):
         eager = ins[3 - i][0].clone()
         m.run(eager, ins[3 - i][1])
         assert torch.equal(eager, want[3 - i][0])
+
+
+def test_binding_refuses_what_the_kernels_cannot_take(gpu):
+    """Tensors of another device, type, size or layout are refused before a launch."""
+    def z(*shape, dtype=BF, device=DEV):
+        return torch.zeros(shape, dtype=dtype, device=device)
+
+    ids, w = z(4, 2, dtype=torch.int32), z(4, 2, dtype=F32)
+    gdn_amd.moe_route(z(4, 8), ids, w, 8, 2)
+    for l, i, v, kw in ((z(4, 8, device="cpu"), ids, w, {}), (z(4, 8, dtype=F64), ids, w, {}),
+                        (z(8, 4).t(), ids, w, {}), (z(4, 7), ids, w, {}),
+                        (z(4, 8), ids.long(), w, {}), (z(4, 8), ids[:3], w, {}),
+                        (z(4, 8), ids, w.to(BF), {}), (z(4, 8), z(2, 4, dtype=torch.int32).t(), w, {}),
+                        (z(4, 8), ids, w.cpu(), {}), (z(4, 8), ids, w, dict(bias=z(7, dtype=F32))),
+                        (z(4, 8), ids, w, dict(bias=z(8)))):
+        with pytest.raises(ValueError):
+            gdn_amd.moe_route(l, i, v, 8, 2, **kw)
+
+    h, x, n = z(4, 64), z(4, 64), z(64)
+    gdn_amd.block_norm(h, x, hn=z(4, 64), pre_w=n)
+    for a, b, kw in ((h.cpu(), x, {}), (h, x.cpu(), {}), (h, x.float(), {}), (h, z(3, 64), {}),
+                     (h.to(F64), x, {}), (z(64, 4).t(), x, {}), (h, x, dict(h_out=h.float())),
+                     (h, x, dict(hn=z(4, 32), pre_w=n)), (h, x, dict(hn=z(4, 64), pre_w=n.float())),
+                     (h, x, dict(post_w=z(32))), (h, x, dict(post_w=z(128)[::2])),
+                     (h, x, dict(gate=z(4, 2))), (h, x, dict(gate=z(4, 1, dtype=F32)))):
+        with pytest.raises(ValueError):
+            gdn_amd.block_norm(a, b, **kw)
+
+    ex = Experts(128, 128, [2])
+    ws, x = ex.moe.workspace(4, 2), z(4, 128)
+    ex.moe.forward(x, ids, w, z(4, 128), ws)
+    for a, i, v, o, s in ((x.cpu(), ids, w, z(4, 128), ws), (z(4, 64), ids, w, z(4, 128), ws),
+                          (x.float(), ids, w, z(4, 128), ws), (x, ids.long(), w, z(4, 128), ws),
+                          (x, ids, w.double(), z(4, 128), ws), (x, ids, w[:2], z(4, 128), ws),
+                          (x, ids, w, z(3, 128), ws), (x, ids, w, z(4, 128, dtype=F32), ws),
+                          (x, ids, w, z(4, 128), ws.cpu()), (x, ids, w, z(4, 128), ws.float())):
+        with pytest.raises(ValueError):
+            ex.moe.forward(a, i, v, o, s)
+    with pytest.raises(gdn_amd.GdnError):
+        ex.moe.forward(x, ids, w, z(4, 128), ws[:256])
+    torch.cuda.synchronize()
