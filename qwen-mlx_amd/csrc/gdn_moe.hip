@@ -12,7 +12,8 @@
 // the nibbles enter the MFMA as the bf16 numbers 128 + q (one v_and_or_b32 per
 // two of them), its sums are exact products accumulated in f32, and X comes
 // from the same MFMA against ones. h is rounded once to bf16, the operand type
-// of its product; out is rounded once from the f32 sum over j.
+// of its product; out is rounded once from the f32 sum over j, whose rows are f32
+// or, of long prompts, f16 under an exponent per row (moe_wide_down_kernel).
 #include <climits>
 #include <type_traits>
 

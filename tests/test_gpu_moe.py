@@ -428,6 +428,36 @@ def test_experts_rows_keep_to_themselves(gpu):
     assert torch.equal(back.view(torch.int16), clean.view(torch.int16))
 
 
+@pytest.mark.parametrize("T,hidden,inner,E", [
+    (5, 256, 256, 4),         # very few entries
+    (60, 1024, 1152, 40),     # tiles of 16 rows by the weights' stream
+    (100, 256, 256, 12),      # tiles of 16
+    (200, 256, 128, 12),      # and of 32
+    (1700, 2048, 384, 4),     # of 64, down's input in LDS
+    (1700, 1792, 640, 4),     # and in stages
+    (4500, 256, 128, 40),     # sorted in two launches
+    (7000, 1024, 256, 4),
+])
+def test_experts_rows_keep_to_themselves_in_every_kernel(gpu, T, hidden, inner, E):
+    ex = Experts(hidden, inner, [E], seed=T)
+    x, (ids, w) = draw_x(3, T, hidden), draw_ids(4, T, E, 2)
+    clean = ex.run(x, ids, w)
+    assert clean.isfinite().all()
+    g = torch.Generator().manual_seed(T)
+    at = torch.randperm(T, generator=g)[:max(1, T // 20)]
+    bad = x.clone()
+    bad[at, torch.randint(0, hidden, (len(at),), generator=g)] = math.nan
+    bad[at[::2]] = INF
+    out = ex.run(bad, ids, w)
+    keep = torch.ones(T, dtype=torch.bool)
+    keep[at] = False
+    assert torch.equal(out[keep].view(torch.int16), clean[keep].view(torch.int16))
+    assert not out[at].isfinite().any()
+    for order in (torch.arange(T).flip(0), torch.randperm(T, generator=g)):
+        there = ex.run(x[order], ids[order], w[order])
+        assert torch.equal(there.view(torch.int16), clean[order].view(torch.int16))
+
+
 @pytest.mark.parametrize("T", [2, 60, 900])
 def test_experts_strided_rows_other_stream_and_repeat(gpu, T):
     ex = Experts(256, 128, [6], seed=9)
