@@ -710,8 +710,11 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
   using S0 = std::integral_constant<int, 0>;
   using S1 = std::integral_constant<int, 1>;
   using S2 = std::integral_constant<int, 2>;
+  // `landed` counts loads: all of stage 0 go out before stage 1's first
   batch(0, S0{});
+  __builtin_amdgcn_sched_barrier(0);
   batch(1, S1{});
+  __builtin_amdgcn_sched_barrier(0);
   landed(std::integral_constant<int, R - 2>{});
 
   // rows' sums, and where down's rows go
@@ -938,8 +941,11 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
   using S0 = std::integral_constant<int, 0>;
   using S1 = std::integral_constant<int, 1>;
   using S2 = std::integral_constant<int, 2>;
+  // `landed` counts loads: all of stage 0 go out before stage 1's first
   batch(0, S0{});
+  __builtin_amdgcn_sched_barrier(0);
   batch(1, S1{});
+  __builtin_amdgcn_sched_barrier(0);
   landed(std::integral_constant<int, R - 2>{});
   int p = 0;
 #pragma nounroll
@@ -1093,8 +1099,11 @@ __global__ __launch_bounds__(256)
 #pragma unroll
       for (int e = 0; e < 16; ++e) T[i][u][e] = 0.f;
 
+  // the wait counts loads: every copy of rows goes out before the first of the weights
   batch_x(0, std::integral_constant<int, 0>{});
+  __builtin_amdgcn_sched_barrier(0);
   batch_w(0);
+  __builtin_amdgcn_sched_barrier(0);
   wait_vm<LW>();
   wait_lgkm0();
   __builtin_amdgcn_s_barrier();
