@@ -698,11 +698,14 @@ gdn_status gdn_moe_route(const gdn_moe_route_desc* desc, const void* logits,
  * each product on MLX 4-bit weights (group 64: scales * q + biases). A column
  * whose id is outside [0, E) adds nothing; a token without any gets zeros. An
  * id may appear in several columns of a token. h = silu(gate) * up is rounded to
- * bf16 and out once from the f32 sum (in long prompts the rows summed pass
- * between kernels in 11 bits of a scale per row); the same bits every time. A
- * token's do not depend on what the other tokens hold, but the kernel is chosen
- * by T, k and E, so that calls of other sizes may differ by rounding. A token
- * of x with infinities or NaN gets infinities or NaN, and it alone. */
+ * 11 bits or more under a power of two of its row (numbers below 2^-29 of the
+ * bound that sets the power, the largest sums of |w| over a row of the expert's
+ * gate and up times the largest |x| squared, lose bits), and out once from the
+ * f32 sum (in long prompts the rows summed pass between kernels in 11 bits of a
+ * scale per row); the same bits every time. A token's do not depend on what the
+ * other tokens hold, but the kernel is chosen by T, k and E, so that calls of
+ * other sizes may differ by rounding. A token of x with infinities or NaN gets
+ * infinities or NaN, and it alone. */
 typedef struct gdn_moe gdn_moe;
 
 /* One set of experts, appended to the layer's in order: MLX-format arrays of

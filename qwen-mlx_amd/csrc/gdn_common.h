@@ -424,8 +424,9 @@ struct MoePackArgs {
 };
 hipError_t launch_moe_pack(const MoePackArgs& a);
 // bound (zeros before): of every expert the largest sum of |w| over a row of w that is
-// finite; wp, sb and the fragments are not used.
-hipError_t launch_moe_bound(const MoePackArgs& a, float* bound);
+// finite, with the products' f32 error (of down or of gate and up); wp, sb and the
+// fragments are not used.
+hipError_t launch_moe_bound(const MoePackArgs& a, bool down, float* bound);
 
 struct MoeArgs {
   int hidden, inner, experts;
@@ -433,7 +434,7 @@ struct MoeArgs {
   const uint32_t* sb1;
   const void* w2;          // down
   const uint32_t* sb2;
-  const float* bound;      // [experts] of down (launch_moe_bound)
+  const float* bound;      // [3][experts] of gate, up and down (launch_moe_bound)
   const uint16_t* x;       // [T, xs]
   int64_t xs;
   int T, k;

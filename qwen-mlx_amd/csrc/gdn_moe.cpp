@@ -213,7 +213,7 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
   // one expert's matrix product terms: words of 8 weights, {scale, bias} per 64
   const size_t terms = (size_t)hidden * inner;
   const size_t w = terms / 2 * experts, s = terms / 16 * experts;
-  const size_t bytes = 3 * (w + s) + 4 * (size_t)experts;  // w, s multiples of 1024 bytes
+  const size_t bytes = 3 * (w + s) + 12 * (size_t)experts;  // w, s multiples of 1024 bytes
   if (hipMalloc(&m->base, bytes) != hipSuccess) {
     (void)hipGetLastError();
     m->base = nullptr;
@@ -227,7 +227,7 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
   m->sb2 = reinterpret_cast<uint32_t*>(p + 3 * w + 2 * s);
   m->bound = reinterpret_cast<float*>(p + 3 * (w + s));
   const hipStream_t st = static_cast<hipStream_t>(stream);
-  hipError_t e = hipMemsetAsync(m->bound, 0, 4 * (size_t)experts, st);
+  hipError_t e = hipMemsetAsync(m->bound, 0, 12 * (size_t)experts, st);
   int64_t first = 0;
   for (int i = 0; i < nparts; ++i) {
     const gdn_moe_part& q = parts[i];
@@ -248,13 +248,19 @@ gdn_status gdn_moe_create(int32_t hidden, int32_t inner, int32_t nparts, const g
       a.sb = sb + first * fmul * (terms / 64);
       return gdn::launch_moe_pack(a);
     };
+    // of the matrices packed last
+    auto bound = [&](int which) {
+      return gdn::launch_moe_bound(a, which == 2, m->bound + which * experts + first);
+    };
     if (e == hipSuccess)
       e = pack(q.gate_w, q.gate_scales, q.gate_biases, inner, hidden, 2, 0, m->w1, m->sb1);
+    if (e == hipSuccess) e = bound(0);
     if (e == hipSuccess)
       e = pack(q.up_w, q.up_scales, q.up_biases, inner, hidden, 2, 1, m->w1, m->sb1);
+    if (e == hipSuccess) e = bound(1);
     if (e == hipSuccess)
       e = pack(q.down_w, q.down_scales, q.down_biases, hidden, inner, 1, 0, m->w2, m->sb2);
-    if (e == hipSuccess) e = gdn::launch_moe_bound(a, m->bound + first);  // down's matrices
+    if (e == hipSuccess) e = bound(2);
     if (e != hipSuccess) {
       (void)hipStreamSynchronize(st);
       moe_release(m);

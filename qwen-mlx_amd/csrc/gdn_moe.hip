@@ -11,9 +11,17 @@
 //   s (sum x (128 + q)) + (b - 128 s) X:
 // the nibbles enter the MFMA as the bf16 numbers 128 + q (one v_and_or_b32 per
 // two of them), its sums are exact products accumulated in f32, and X comes
-// from the same MFMA against ones. h is rounded once to bf16, the operand type
-// of its product; out is rounded once from the f32 sum over j, whose rows are f32
-// or, of long prompts, f16 under an exponent per row (moe_wide_down_kernel).
+// from the same MFMA against ones.
+// h enters down's product, at the same rate, as f16 times a power of two of its row
+// (11 bits; as bf16 the result's error was 0.0025 of its norm, 0.0017 of which is its
+// own rounding), and the nibbles as the f16 numbers 1024 + q. The power is known
+// before h is: with S_g and S_u the largest sums of |w| over a row of the expert's
+// gate and up, |h| <= |g| |u| <= S_g S_u max|x|^2, and this is brought to 2^15 at
+// most (row_exponent). A value has its 11 bits down to 2^-29 of that. Calls of very
+// few entries have h in two bf16 parts instead. out is rounded once from the f32 sum
+// over j, whose rows are f32 or, of long prompts, f16 under an exponent per row
+// (moe_wide_down_kernel).
+#include <algorithm>
 #include <climits>
 #include <type_traits>
 
@@ -23,6 +31,8 @@ namespace gdn {
 namespace {
 
 typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -61,10 +71,12 @@ __global__ void moe_pack_kernel(MoePackArgs a) {
 }
 
 // bound[e] = the largest sum of |w| over a row of expert e's matrix [n, k] whose sum is
-// finite; bound starts at zeros. grid (n / 64 rounded up, experts), a wave 16 rows,
-// four lanes a row. Positive floats are in the order of their bits, and a maximum has
-// no order.
-__global__ __launch_bounds__(256) void moe_bound_kernel(MoePackArgs a, float* bound) {
+// finite; bound starts at zeros. Every term counts 2^-16 of the magnitudes that its
+// products with the numbers offset + q pass through as well: weights that cancel to
+// less than the f32 sums' error leave that. grid (n / 64 rounded up, experts), a wave
+// 16 rows, four lanes a row. Positive floats are in the order of their bits, and a
+// maximum has no order.
+__global__ __launch_bounds__(256) void moe_bound_kernel(MoePackArgs a, float offset, float* bound) {
   const int lane = threadIdx.x & 63, c = lane & 3;
   const int n = blockIdx.x * 64 + (threadIdx.x >> 6) * 16 + (lane >> 2);
   const int words = a.k >> 3, G = a.k >> 6;
@@ -73,6 +85,8 @@ __global__ __launch_bounds__(256) void moe_bound_kernel(MoePackArgs a, float* bo
     const int64_t row = (int64_t)blockIdx.y * a.n + n;
     for (int j = 4 * c; j < words; j += 16) {
       const float sc = bf2f(a.s[row * G + (j >> 3)]), of = bf2f(a.b[row * G + (j >> 3)]);
+      const float err = 0x1p-16f * fmaf(2.0f * offset + 15.0f, fabsf(sc), fabsf(of));
+      sum = fmaf(32.0f, err, sum);  // the lane's 32 terms
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
         const uint32_t v = a.w[row * words + j + q];
@@ -91,20 +105,37 @@ __global__ __launch_bounds__(256) void moe_bound_kernel(MoePackArgs a, float* bo
 
 // --------------------------------------------------------------- experts --
 
+// The products' operands: bf16, or f16 for H (rows of h).
+template <bool H = false>
 __device__ __forceinline__ f32x4 mfma(u32x4 a, u32x4 b, f32x4 c) {
-  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  if constexpr (H)
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
-// One packed dword -> the operand dwords (128 + q_k0, 128 + q_k1), ... of eight
+// What a nibble's number is above it: the type's first power of two with steps of one.
+constexpr float kOffsetX = 128.0f, kOffsetH = 1024.0f;
+
+// One packed dword -> the operand dwords (offset + q_k0, offset + q_k1), ... of eight
 // consecutive k (m = 0x000F000F held in a VGPR: v_and_or_b32 takes one literal)
+template <bool H = false>
 __device__ __forceinline__ u32x4 unpack_w(uint32_t w, uint32_t m) {
-  const uint32_t e = 0x43004300u;
+  const uint32_t e = H ? 0x64006400u : 0x43004300u;
   return (u32x4){(w & m) | e, ((w >> 4) & m) | e, ((w >> 8) & m) | e, ((w >> 12) & m) | e};
 }
 
+// Two numbers as f16, and back.
+__device__ __forceinline__ uint32_t f2h2(float a, float b) {
+  return __builtin_bit_cast(uint32_t, (f16x2){(_Float16)a, (_Float16)b});
+}
+__device__ __forceinline__ float h_lo(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[0]; }
+__device__ __forceinline__ float h_hi(uint32_t v) { return (float)__builtin_bit_cast(f16x2, v)[1]; }
+
 // silu(g) * u. exp2 and the reciprocal are the hardware's (1 ulp); the product
-// under exp2 adds |g| half steps of f32. h is rounded to bf16 right after.
+// under exp2 adds |g| half steps of f32. h is rounded to 11 or more bits right after.
 __device__ __forceinline__ float swiglu(float g, float u) {
   const float q = __builtin_amdgcn_exp2f(-1.44269504089f * g);
   return g * __builtin_amdgcn_rcpf(1.0f + q) * u;
@@ -122,8 +153,11 @@ struct MoeSpace {
   int4* tiles;     // expert, first sorted row, rows, -
   int2* perm;      // token and entry of a sorted row
   uint16_t* xs;    // [T][3][gpad(hidden)] split group sums of x
-  uint16_t* hs;    // [entries][3][gpad(inner)] and of h, by sorted row
-  uint16_t* h;     // [entries, inner] by sorted row
+  uint16_t* xmax;  // [T][16] largest |x| of runs of 512 columns
+  uint16_t* hs;    // [entries][3][gpad(inner)] split group sums of h, by sorted row
+  uint16_t* h;     // [entries, inner] f16 of 2^-hexp by sorted row, or
+                   // [entries][2][inner] two bf16 parts by entry (moe_few_up_kernel)
+  int32_t* hexp;   // [entries] by sorted row
   float* rows;     // [entries, hidden] weighted rows of down by entry, or
                    // f16 of 2^-exps (moe_wide_down_kernel)
   int32_t* exps;   // [entries]
@@ -135,6 +169,15 @@ struct MoeSpace {
 // Entries of a chunk of the two-launch plan, and those up to which one launch
 // does it.
 constexpr int kChunk = 4096, kPlanEntries = 8192;
+
+// Most entries of a call whose work-groups find their rows by themselves: a
+// wave holds every id.
+// They and the rows' product with the sum are two launches: one token of 9 columns,
+// hidden 2048, inner 512, takes 6.4 + 5.7 us, the latency of a launch and a chain of
+// loads each (16 MB of weights); by a plan, tiles and a sum the call took 21.7.
+constexpr int kFewEntries = 64;
+// ... and the most tokens: down reads an expert's weights for each of them again.
+constexpr int kFewTokens = 6;
 
 // Groups of k columns, padded with zeros to whole 16-byte loads.
 __host__ __device__ __forceinline__ int gpad(int k) { return (k / 64 + 7) & ~7; }
@@ -156,8 +199,11 @@ MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t token
   s.tiles = reinterpret_cast<int4*>(take(max_tiles(entries, experts, 16) * sizeof(int4)));
   s.perm = reinterpret_cast<int2*>(take(entries * 8));
   s.xs = reinterpret_cast<uint16_t*>(take(tokens * 6 * gpad(hidden)));
+  s.xmax = reinterpret_cast<uint16_t*>(take(tokens * 32));
   s.hs = reinterpret_cast<uint16_t*>(take(entries * 6 * gpad(inner)));
-  s.h = reinterpret_cast<uint16_t*>(take(entries * inner * 2));
+  s.h = reinterpret_cast<uint16_t*>(
+      take(std::max(entries, 2 * std::min<int64_t>(entries, kFewEntries)) * inner * 2));
+  s.hexp = reinterpret_cast<int32_t*>(take(entries * 4));
   s.rows = reinterpret_cast<float*>(take(entries * hidden * 4));
   s.exps = reinterpret_cast<int32_t*>(take(entries * 4));
   s.hmax = reinterpret_cast<uint16_t*>(take(inner <= kWideInner ? entries * 16 : 0));
@@ -185,23 +231,63 @@ __device__ __forceinline__ void store_split(float v, uint16_t* dst, int step) {
   dst[2 * step] = f2bf(q - bf2f(mid));
 }
 
-// Split group sums of x's rows, [T][3][gpad(hidden)]. A lane takes 8 of a
-// group's 64 columns, 8 lanes a group; a thread of a padded group stores zeros.
-// i: the thread's number.
+// Largest |v| of two numbers in 16 bits, in the order of their bits (infinity above
+// every number, NaN above it).
+__device__ __forceinline__ uint32_t max_abs2(uint32_t v) {
+  return max(v & 0x7FFFu, v >> 16 & 0x7FFFu);
+}
+
+// Split group sums of x's rows, [T][3][gpad(hidden)] (not if sums is null), and the
+// largest |x| of every 512 columns, [T][16]. A lane takes 8 of a group's 64 columns, 8
+// lanes a group, a wave 8 groups; a thread of a padded group stores zeros. i: the
+// thread's number.
 __device__ __forceinline__ void moe_row_sums(const uint16_t* __restrict__ x, int64_t xs, int T,
-                                             int hidden, uint16_t* __restrict__ sums, int64_t i) {
+                                             int hidden, uint16_t* __restrict__ sums,
+                                             uint16_t* __restrict__ xmax, int64_t i) {
   const int gp = gpad(hidden);
   const int64_t t = i / (8 * gp);
   const int c = (int)(i - t * 8 * gp);  // 8-column chunk of the row
   if (t >= T) return;
   float v = 0.f;
+  uint32_t m = 0;
   if (8 * c < hidden) {
     const u32x4 q = *reinterpret_cast<const u32x4*>(x + t * xs + 8 * c);
 #pragma unroll
-    for (int e = 0; e < 4; ++e) v += bf_lo(q[e]) + bf_hi(q[e]);
+    for (int e = 0; e < 4; ++e) {
+      v += bf_lo(q[e]) + bf_hi(q[e]);
+      m = max(m, max_abs2(q[e]));
+    }
   }
+  // 8 lanes, a row of 16, then rows 0 -> 1, 2 -> 3 and 1 -> 2, 3: lane 63 has all
+  m = max_dpp<0x143>(max_dpp<0x142>(max_dpp<0x128>(max8(m))));
+  if ((c & 63) == 63) xmax[t * 16 + c / 64] = (uint16_t)m;
+  if (!sums) return;
   v = sum8(v);
   if ((c & 7) == 0) store_split(v, sums + t * 3 * gp + c / 8, gp);
+}
+
+struct RowMax {
+  u32x4 v[2];  // 16 maxima
+};
+__device__ __forceinline__ RowMax load_row_max(const uint16_t* xmax, int64_t token) {
+  const u32x4* const p = reinterpret_cast<const u32x4*>(xmax + token * 16);
+  return {{p[0], p[1]}};
+}
+// The exponent of h's power of two for a row of x and the expert's bounds of gate and
+// up: |h| 2^-exponent < 2^15. It stays where 2^exponent and 2^-exponent are f32 numbers:
+// h, an f32 number itself, is below 2^(113 + 15), and where the bound lets it be raised
+// by 2^126 only, it is below 2^(15 - 126).
+__device__ __forceinline__ int row_exponent(const RowMax& xm, int hidden, const float (&bound)[2]) {
+  const int n = gpad(hidden) >> 3;
+  uint32_t m = 0;
+#pragma unroll
+  for (int q = 0; q < 8; ++q) {
+    if (2 * q < n) m = max(m, xm.v[q >> 2][q & 3] & 0xFFFFu);
+    if (2 * q + 1 < n) m = max(m, xm.v[q >> 2][q & 3] >> 16);
+  }
+  const int e = __builtin_amdgcn_frexp_expf(bound[0]) + __builtin_amdgcn_frexp_expf(bound[1]) +
+                2 * __builtin_amdgcn_frexp_expf(__uint_as_float(m << 16)) - 15;
+  return max(-126, min(e, 113));
 }
 
 // The plan: work-group e sorts expert e's entries, in entry order, behind those
@@ -209,7 +295,7 @@ __device__ __forceinline__ void moe_row_sums(const uint16_t* __restrict__ x, int
 // experts and its own by itself, so that one launch without atomics does it.
 // Expert e's tiles start at slot (entries before it) / rows + e: never fewer
 // slots than tiles, the ones left over marked empty (rows = 0).
-// Work-groups from `experts` on form the split group sums of x's rows
+// Work-groups from `experts` on form the split group sums and maxima of x's rows
 // (moe_row_sums) beside it. 4 to 5 us up to 8192 entries: a launch and two rounds of
 // loads.
 constexpr int kPlanThreads = 1024;
@@ -220,7 +306,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(MoeArgs a, int r
   const int32_t* const ids = a.ids;
   const int entries = a.T * a.k, k = a.k, experts = a.experts;
   if (blockIdx.x >= (uint32_t)experts) {
-    moe_row_sums(a.x, a.xs, a.T, a.hidden, s.xs,
+    moe_row_sums(a.x, a.xs, a.T, a.hidden, s.xs, s.xmax,
                  (int64_t)(blockIdx.x - experts) * kPlanThreads + threadIdx.x);
     return;
   }
@@ -295,7 +381,7 @@ __global__ __launch_bounds__(kPlanThreads) void moe_plan_kernel(MoeArgs a, int r
 __global__ __launch_bounds__(kPlanThreads) void moe_count_kernel(MoeArgs a, int chunks, MoeSpace s) {
   extern __shared__ int cnt[];
   if (blockIdx.x >= (uint32_t)chunks) {
-    moe_row_sums(a.x, a.xs, a.T, a.hidden, s.xs,
+    moe_row_sums(a.x, a.xs, a.T, a.hidden, s.xs, s.xmax,
                  (int64_t)(blockIdx.x - chunks) * kPlanThreads + threadIdx.x);
     return;
   }
@@ -314,8 +400,8 @@ __global__ __launch_bounds__(kPlanThreads) void moe_count_kernel(MoeArgs a, int 
 // Then a work-group per chunk places its entries behind those of lower experts
 // and of its expert in the chunks before, and writes its share of the tile list.
 // Inside a chunk an expert's entries take their places in any order: a row's
-// sums do not depend on where it stands. 147,456 entries of 16,384 rows: 17 us, most
-// of it reading x for the sums, and 9.5; in one launch as above 58.
+// sums do not depend on where it stands. 147,456 entries of 16,384 rows: 18.5 us, most
+// of it reading x for the sums and maxima, and 9.6; in one launch as above 58.
 __global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(MoeArgs a, int rows, MoeSpace s) {
   extern __shared__ int lds[];
   __shared__ int wsum[kPlanThreads / 64];
@@ -380,15 +466,6 @@ __global__ __launch_bounds__(kPlanThreads) void moe_place_kernel(MoeArgs a, int 
 }
 
 // ---- very few entries: no plan ----
-
-// Most entries of a call whose work-groups find their rows by themselves: a
-// wave holds every id.
-// They and the rows' product with the sum are two launches: one token of 9 columns,
-// hidden 2048, inner 512, takes 6.4 + 5.7 us, the latency of a launch and a chain of
-// loads each (16 MB of weights); by a plan, tiles and a sum the call took 21.7.
-constexpr int kFewEntries = 64;
-// ... and the most tokens: down reads an expert's weights for each of them again.
-constexpr int kFewTokens = 6;
 
 // NS stages p0, p0 + step, ... of a 16-row fragment: its weights, scales and
 // biases (stages past P: the last one again; their x is zero).
@@ -456,8 +533,10 @@ __device__ __forceinline__ void product(const Rows<NS>& x, const Frag<NS> (&f)[N
   }
 }
 
-// h by entry: work-group (entry u, 16 inner columns), four waves, wave w over
-// the stages 4 w .. 4 w + 3 (and on from 16 stages ahead), added in wave order.
+// h by entry, as two bf16 parts (16 bits): the second is one more row of down's
+// product, which has 16 of them for one. Work-group (entry u, 16 inner columns), four
+// waves, wave w over the stages 4 w .. 4 w + 3 (and on from 16 stages ahead), added in
+// wave order.
 // It takes every row of the expert that entry u names first; a later entry of
 // the same expert has nothing to do.
 __global__ __launch_bounds__(256) void moe_few_up_kernel(MoeArgs a, uint16_t* __restrict__ h) {
@@ -505,7 +584,13 @@ __global__ __launch_bounds__(256) void moe_few_up_kernel(MoeArgs a, uint16_t* __
       g += part[w][0][l][i];
       up += part[w][1][l][i];
     }
-    if (m < n) h[(int64_t)em * a.inner + 16 * j + (l & 15)] = f2bf(swiglu(g, up));
+    if (m < n) {
+      const float v = swiglu(g, up);
+      const uint16_t hi = f2bf(v);
+      uint16_t* const o = h + 2 * (int64_t)em * a.inner + 16 * j + (l & 15);
+      o[0] = hi;
+      o[a.inner] = f2bf(v - bf2f(hi));
+    }
     __syncthreads();
   }
 }
@@ -528,7 +613,7 @@ __global__ __launch_bounds__(1024) void moe_few_down_kernel(MoeArgs a,
     f32x4 T[1] = {{0.f, 0.f, 0.f, 0.f}};
     if ((uint32_t)e < (uint32_t)a.experts) {
       const int64_t f0 = ((int64_t)e * blocks + j) * P;
-      const uint16_t* const row = r16 == 0 ? h + (int64_t)en * a.inner : nullptr;
+      const uint16_t* const row = r16 < 2 ? h + (2 * (int64_t)en + r16) * a.inner : nullptr;
       for (int p = 0; p < P; p += 4) {
         Rows<4> x;
         Frag<4> f[1];
@@ -536,7 +621,7 @@ __global__ __launch_bounds__(1024) void moe_few_down_kernel(MoeArgs a,
         x.load(row, P, p, 1);
         product<1, 4>(x, f, nib, T);
       }
-      T[0][0] *= a.weights[en];
+      T[0][0] = (T[0][0] + T[0][1]) * a.weights[en];
     }
     if (lane < 16) part[wave][lane] = T[0][0];
     __syncthreads();
@@ -550,6 +635,13 @@ __global__ __launch_bounds__(1024) void moe_few_down_kernel(MoeArgs a,
 // s_waitcnt lgkmcnt(0), and vmcnt(N) below (gfx9 encodings, the other counters
 // at their maximum)
 __device__ __forceinline__ void wait_lgkm0() { __builtin_amdgcn_s_waitcnt(0xC07F); }
+
+// v 2^e
+__device__ __forceinline__ f32x4 scaled(f32x4 v, int e) {
+#pragma unroll
+  for (int r = 0; r < 4; ++r) v[r] = ldexpf(v[r], e);
+  return v;
+}
 
 // ---- tiles ----
 
@@ -674,8 +766,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
       float sc[2][4];
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        A[i][0] = unpack_w(wr[S][i][2 * gl], nib);
-        A[i][1] = unpack_w(wr[S][i][2 * gl + 1], nib);
+        A[i][0] = unpack_w<!UP>(wr[S][i][2 * gl], nib);
+        A[i][1] = unpack_w<!UP>(wr[S][i][2 * gl + 1], nib);
 #pragma unroll
         for (int r = 0; r < 4; ++r) sc[i][r] = gl ? bf_hi(sv[i][r]) : bf_lo(sv[i][r]);
       }
@@ -688,9 +780,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
               &cur[(u * 16 + r16) * XROW + (((8 * gl + 4 * h + c4) ^ r16) << 4)]);
         f32x4 d[2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i) d[i] = mfma(A[i][0], X[0], zero);
+        for (int i = 0; i < 2; ++i) d[i] = mfma<!UP>(A[i][0], X[0], zero);
 #pragma unroll
-        for (int i = 0; i < 2; ++i) d[i] = mfma(A[i][1], X[1], d[i]);
+        for (int i = 0; i < 2; ++i) d[i] = mfma<!UP>(A[i][1], X[1], d[i]);
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -721,13 +813,18 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
   const int gp = gpad(K), go = gp >> 3;
   const uint16_t* xg[MW];
   int en[MW];
+  RowMax xm[UP ? MW : 1];
+  float bound[2];
 #pragma unroll
   for (int u = 0; u < MW; ++u) {
     const int row = tl.y + min(u * 16 + r16, tl.z - 1);
     const int2 pe = s.perm[row];
     xg[u] = UP ? s.xs + (int64_t)pe.x * 3 * gp : s.hs + (int64_t)row * 3 * gp;
     en[u] = pe.y;
+    if constexpr (UP) xm[u] = load_row_max(s.xmax, pe.x);
   }
+  if constexpr (UP)
+    for (int i = 0; i < 2; ++i) bound[i] = a.bound[i * a.experts + tl.x];
   int p = 0;
 #pragma nounroll
   for (; p + R <= P; p += R) {
@@ -746,9 +843,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
   // part o / go of groups 8 (o % go) .., and a product takes four octets, one a
   // lane group.
   float wt[MW];
-  if constexpr (!UP)
+  int he[MW];  // exponents of h's rows
 #pragma unroll
-    for (int u = 0; u < MW; ++u) wt[u] = a.weights[en[u]];
+  for (int u = 0; u < MW; ++u) {
+    if constexpr (UP) {
+      he[u] = row_exponent(xm[u], a.hidden, bound);
+    } else {
+      wt[u] = a.weights[en[u]];
+      he[u] = s.hexp[tl.y + min(u * 16 + r16, tl.z - 1)];
+    }
+  }
 #pragma nounroll
   for (int jb = 0; 4 * jb < 3 * go; ++jb) {
     const int o = 4 * jb + c4, oc = o < go ? o : o < 2 * go ? o - go : o - 2 * go;
@@ -771,7 +875,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
         const f32x4 d = mfma(as[i], xp, zero);
         T[i][u] = mfma(ab[i], xp, T[i][u]);
 #pragma unroll
-        for (int r = 0; r < 4; ++r) T[i][u][r] = fmaf(-128.0f, d[r], T[i][u][r]);
+        for (int r = 0; r < 4; ++r)
+          T[i][u][r] = fmaf(UP ? -kOffsetX : -kOffsetH, d[r], T[i][u][r]);
       }
     }
   }
@@ -781,11 +886,16 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
 #pragma unroll
     for (int u = 0; u < MW; ++u) {
       const int m = u * 16 + r16;
-      const uint32_t lo = f2bf2(swiglu(T[0][u][0], T[1][u][0]), swiglu(T[0][u][1], T[1][u][1]));
-      const uint32_t hi = f2bf2(swiglu(T[0][u][2], T[1][u][2]), swiglu(T[0][u][3], T[1][u][3]));
-      if (m < tl.z)
+      const float sc = ldexpf(1.0f, -he[u]);
+      const uint32_t lo =
+          f2h2(sc * swiglu(T[0][u][0], T[1][u][0]), sc * swiglu(T[0][u][1], T[1][u][1]));
+      const uint32_t hi =
+          f2h2(sc * swiglu(T[0][u][2], T[1][u][2]), sc * swiglu(T[0][u][3], T[1][u][3]));
+      if (m < tl.z) {
         *reinterpret_cast<u32x2*>(s.h + (int64_t)(tl.y + m) * a.inner + col) = (u32x2){lo, hi};
-      float v = (bf_lo(lo) + bf_hi(lo)) + (bf_lo(hi) + bf_hi(hi));
+        if (cb == 0 && wave == 0 && c4 == 0) s.hexp[tl.y + m] = he[u];
+      }
+      float v = (h_lo(lo) + h_hi(lo)) + (h_lo(hi) + h_hi(hi));
       v += __shfl_xor(v, 16, 64);
       v += __shfl_xor(v, 32, 64);
       if (c4 == 0) gsum[wave][m] = v;
@@ -804,7 +914,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
       if (u * 16 + r16 >= tl.z) continue;
       float* const o = s.rows + (int64_t)en[u] * a.hidden + 128 * cb + 32 * wave + 4 * c4;
 #pragma unroll
-      for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(o + 16 * i) = wt[u] * T[i][u];
+      for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(o + 16 * i) = scaled(wt[u] * T[i][u], he[u]);
     }
   }
 }
@@ -857,8 +967,11 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
     }
   }
   // a row's place for the results: the tile's sorted row (up) or its entry
-  const int m = min(r16, tl.z - 1), en = UP ? 0 : s.perm[tl.y + m].y;
+  const int m = min(r16, tl.z - 1);
+  const int2 pe = s.perm[tl.y + m];
+  const int en = pe.y;
   const float wt = UP ? 0.f : a.weights[en];
+  const int hexp = UP ? 0 : s.hexp[tl.y + m];
   const int svo = (lane >> 5) * P * 128 + 4 * (lane & 31);  // fragment, dword
   u32x4 wr[R][2];
   auto xbuf = [&](auto slot) -> uint8_t* {
@@ -896,7 +1009,8 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
   };
   const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const u32x4 ones = {0x3F803F80u, 0x3F803F80u, 0x3F803F80u, 0x3F803F80u};
+  const uint32_t one2 = UP ? 0x3F803F80u : 0x3C003C00u;
+  const u32x4 ones = {one2, one2, one2, one2};
   f32x4 T[2] = {zero, zero};
   uint32_t nib = 0x000F000Fu;
   asm volatile("" : "+v"(nib));
@@ -916,16 +1030,17 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
       for (int h = 0; h < 2; ++h)
         X[h] = *reinterpret_cast<const u32x4*>(
             &cur[r16 * XROW + (((8 * gl + 4 * h + c4) ^ r16) << 4)]);
-      f32x4 xg = mfma(ones, X[0], zero);
-      xg = mfma(ones, X[1], xg);
+      f32x4 xg = mfma<!UP>(ones, X[0], zero);
+      xg = mfma<!UP>(ones, X[1], xg);
 #pragma unroll
       for (int i = 0; i < 2; ++i) {
-        f32x4 d = mfma(unpack_w(wr[S][i][2 * gl], nib), X[0], zero);
-        d = mfma(unpack_w(wr[S][i][2 * gl + 1], nib), X[1], d);
+        f32x4 d = mfma<!UP>(unpack_w<!UP>(wr[S][i][2 * gl], nib), X[0], zero);
+        d = mfma<!UP>(unpack_w<!UP>(wr[S][i][2 * gl + 1], nib), X[1], d);
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
           const float sc = gl ? bf_hi(sv[i][r]) : bf_lo(sv[i][r]);
-          const float of = fmaf(-128.0f, sc, gl ? bf_hi(bv[i][r]) : bf_lo(bv[i][r]));
+          const float of =
+              fmaf(UP ? -kOffsetX : -kOffsetH, sc, gl ? bf_hi(bv[i][r]) : bf_lo(bv[i][r]));
           T[i][r] = fmaf(sc, d[r], fmaf(of, xg[0], T[i][r]));
         }
       }
@@ -947,6 +1062,12 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
   batch(1, S1{});
   __builtin_amdgcn_sched_barrier(0);
   landed(std::integral_constant<int, R - 2>{});
+  RowMax xm;  // used behind the stages
+  float bound[2];
+  if constexpr (UP) {
+    xm = load_row_max(s.xmax, pe.x);
+    for (int i = 0; i < 2; ++i) bound[i] = a.bound[i * a.experts + tl.x];
+  }
   int p = 0;
 #pragma nounroll
   for (; p + R <= least; p += R) {
@@ -975,14 +1096,17 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
   }
   if (r16 >= tl.z) return;
   if constexpr (UP) {
-    const uint32_t lo = f2bf2(swiglu(T[0][0], T[1][0]), swiglu(T[0][1], T[1][1]));
-    const uint32_t hi = f2bf2(swiglu(T[0][2], T[1][2]), swiglu(T[0][3], T[1][3]));
+    const int he = row_exponent(xm, a.hidden, bound);
+    const float sc = ldexpf(1.0f, -he);
+    const uint32_t lo = f2h2(sc * swiglu(T[0][0], T[1][0]), sc * swiglu(T[0][1], T[1][1]));
+    const uint32_t hi = f2h2(sc * swiglu(T[0][2], T[1][2]), sc * swiglu(T[0][3], T[1][3]));
+    if (cb == 0 && cw == 0 && c4 == 0) s.hexp[tl.y + r16] = he;
     *reinterpret_cast<u32x2*>(s.h + (int64_t)(tl.y + r16) * a.inner + 32 * cb + 16 * cw + 4 * c4) =
         (u32x2){lo, hi};
   } else {
     float* const o = s.rows + (int64_t)en * a.hidden + 64 * cb + 32 * cw + 4 * c4;
 #pragma unroll
-    for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(o + 16 * i) = wt * T[i];
+    for (int i = 0; i < 2; ++i) *reinterpret_cast<f32x4*>(o + 16 * i) = scaled(wt * T[i], hexp);
   }
 }
 
@@ -990,9 +1114,14 @@ __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))
 
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+template <bool H = false>
 __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
-  return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
-                                                 __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+  if constexpr (H)
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(__builtin_bit_cast(f16x8, a),
+                                                  __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+  else
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(__builtin_bit_cast(bf16x8, a),
+                                                   __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
 }
 
 // moe_tile_kernel for experts with many rows: a tile of 64 rows against 256
@@ -1020,7 +1149,9 @@ __global__ __launch_bounds__(256)
   constexpr int MT = 64, XROW = kStageK * 2, XJ = 4, RB = 2;
   __shared__ __align__(16) uint8_t xl0[MT * XROW], xl1[MT * XROW];
   __shared__ int2 row_of[MT];   // a row's token and entry
-  __shared__ float wt_of[MT];   // and its weight
+  __shared__ __align__(16) float wt_of[MT];  // !UP: its weight
+  // 2^-exponent of its row of h (UP), or 2^exponent
+  __shared__ __align__(16) float hs_of[MT];
   const int K = UP ? a.hidden : a.inner, N = UP ? 2 * a.inner : a.hidden;
   const int P = K >> 7, blocks = (N + 255) >> 8;
   const int n = *s.ntiles * blocks, per = (n + 7) >> 3;
@@ -1037,10 +1168,19 @@ __global__ __launch_bounds__(256)
   const int r32 = lane & 31, c2 = lane >> 5;
   const bool live = 256 * cb + 64 * wave < N;  // an odd last half block leaves two waves idle
 
+  float bound[2];
+  if constexpr (UP)
+    for (int i = 0; i < 2; ++i) bound[i] = a.bound[i * a.experts + tl.x];
+  RowMax xm;
   if (tid < MT) {
     const int2 pe = s.perm[tl.y + min(tid, tl.z - 1)];
     row_of[tid] = pe;
-    if constexpr (!UP) wt_of[tid] = a.weights[pe.y];
+    if constexpr (UP) {
+      xm = load_row_max(s.xmax, pe.x);
+    } else {
+      wt_of[tid] = a.weights[pe.y];
+      hs_of[tid] = ldexpf(1.0f, s.hexp[tl.y + min(tid, tl.z - 1)]);
+    }
   }
   // the wave's first 16-row fragment, and the lane's of its 32-column fragment i
   const int64_t f0 = (int64_t)tl.x * (N >> 4) + 16 * cb + (live ? 4 * wave : 0);
@@ -1104,6 +1244,12 @@ __global__ __launch_bounds__(256)
   __builtin_amdgcn_sched_barrier(0);
   batch_w(0);
   __builtin_amdgcn_sched_barrier(0);
+  if constexpr (UP)  // beside the first stage's loads
+    if (tid < MT) {
+      const int he = row_exponent(xm, a.hidden, bound);
+      hs_of[tid] = ldexpf(1.0f, -he);
+      if (cb == 0 && tid < tl.z) s.hexp[tl.y + tid] = he;
+    }
   wait_vm<LW>();
   wait_lgkm0();
   __builtin_amdgcn_s_barrier();
@@ -1139,7 +1285,7 @@ __global__ __launch_bounds__(256)
 #pragma unroll
         for (int d = 0; d < 2; ++d)
 #pragma unroll
-          for (int g = 0; g < 2; ++g) W[i][d][g] = unpack_w(wr[i][g][2 * gl + d], nib);
+          for (int g = 0; g < 2; ++g) W[i][d][g] = unpack_w<!UP>(wr[i][g][2 * gl + d], nib);
     };
     auto task = [&](const uint8_t* cur, auto tc) {
       constexpr int t = decltype(tc)::value, up = (t + NB - 1) % NB;
@@ -1154,7 +1300,7 @@ __global__ __launch_bounds__(256)
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            y[t & 1][i] = mfma32(X[t & 1][d][g], W[i][d][g], y[t & 1][i]);
+            y[t & 1][i] = mfma32<!UP>(X[t & 1][d][g], W[i][d][g], y[t & 1][i]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1220,9 +1366,9 @@ __global__ __launch_bounds__(256)
     stages(std::integral_constant<int, 1>{});
 
   // The offsets' sum: both lane groups hold the same octet of X, one against b and
-  // the other against -128 s.
+  // the other against -offset s.
   const int gp = gpad(K), go = gp >> 3;
-  const float f = c2 ? -128.0f : 1.0f;
+  const float f = c2 ? UP ? -kOffsetX : -kOffsetH : 1.0f;
 #pragma nounroll
   for (int o = 0; o < go; ++o) {
     u32x4 B[2];
@@ -1258,9 +1404,16 @@ __global__ __launch_bounds__(256)
 #pragma unroll
     for (int u = 0; u < RB; ++u)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = 32 * u + 8 * (e >> 2) + 4 * c2 + (e & 3);
-        if (live) hb[r * 128 + 8 * ((c >> 3) ^ (r & 15)) + (c & 7)] = f2bf(swiglu(T[0][u][e], T[1][u][e]));
+      for (int q = 0; q < 4; ++q) {
+        const int r0 = 32 * u + 8 * q + 4 * c2;
+        const f32x4 sc = *reinterpret_cast<const f32x4*>(&hs_of[r0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int r = r0 + e;
+          if (live)
+            hb[r * 128 + 8 * ((c >> 3) ^ (r & 15)) + (c & 7)] = __builtin_bit_cast(
+                uint16_t, (_Float16)(sc[e] * swiglu(T[0][u][4 * q + e], T[1][u][4 * q + e])));
+        }
       }
     lds_barrier();
     const int gi = gpad(a.inner), ch = tid & 15, cols = min(128, a.inner - 128 * cb);
@@ -1274,8 +1427,8 @@ __global__ __launch_bounds__(256)
       uint32_t m = 0;  // |h| as the order of its bits
 #pragma unroll
       for (int q = 0; q < 4; ++q) {
-        t += bf_lo(v[q]) + bf_hi(v[q]);
-        m = max(m, max(v[q] & 0x7FFFu, v[q] >> 16 & 0x7FFFu));
+        t += h_lo(v[q]) + h_hi(v[q]);
+        m = max(m, max_abs2(v[q]));
       }
       t = sum8(t);
       m = max8(m);
@@ -1294,13 +1447,17 @@ __global__ __launch_bounds__(256)
 #pragma unroll
     for (int u = 0; u < RB; ++u)
 #pragma unroll
-      for (int e = 0; e < 16; ++e) {
-        const int r = 32 * u + 8 * (e >> 2) + 4 * c2 + (e & 3);
-        if (r < tl.z) {
-          float* const o = rows + (int64_t)row_of[r].y * a.hidden;
-          o[0] = wt_of[r] * T[0][u][e];
-          o[32] = wt_of[r] * T[1][u][e];
-        }
+      for (int q = 0; q < 4; ++q) {
+        const int r0 = 32 * u + 8 * q + 4 * c2;
+        const f32x4 wt = *reinterpret_cast<const f32x4*>(&wt_of[r0]);
+        const f32x4 hs = *reinterpret_cast<const f32x4*>(&hs_of[r0]);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (r0 + e < tl.z) {
+            float* const o = rows + (int64_t)row_of[r0 + e].y * a.hidden;
+            o[0] = wt[e] * T[0][u][4 * q + e] * hs[e];
+            o[32] = wt[e] * T[1][u][4 * q + e] * hs[e];
+          }
       }
   }
 }
@@ -1313,9 +1470,9 @@ __global__ __launch_bounds__(256)
 // sum of |w| over a column's inputs times the largest |h|, and the power of two above
 // that and the weight is brought to 2^15. A value keeps 11 bits down to 2^-29 of the
 // bound and 2^-40 of it absolutely; only the result's own 8 bits follow. The same
-// 16,384 tokens: 410 us, 750 TFLOP/s, and 102 for their sum. In f32 it was 460 and 215,
-// and in bf16, at 410 and 101, the result was off by 0.0029 of its norm instead of
-// 0.0024 (0.0017 is its own rounding).
+// 16,384 tokens: 415 us, 745 TFLOP/s, and 102 for their sum. In f32 it was 460 and 215.
+// In bf16, at 410 and 101, the rows' rounding moved the result by as much as its own
+// does, 0.0017 of its norm; so it stays at the 0.0017.
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void
     moe_wide_down_kernel(MoeArgs a, MoeSpace s, int run) {
   constexpr int MT = 64, XROW = kStageK * 2, SLOT = MT * XROW;
@@ -1340,7 +1497,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r32 = lane & 31, c2 = lane >> 5;
 
-  const int bound = __builtin_amdgcn_readfirstlane(__builtin_amdgcn_frexp_expf(a.bound[tl.x]));
+  const int bound = __builtin_amdgcn_readfirstlane(
+      __builtin_amdgcn_frexp_expf(a.bound[2 * a.experts + tl.x]));
   // the rows of all stages, and what goes with a row
   {
     const __amdgpu_buffer_rsrc_t xrs = __builtin_amdgcn_make_buffer_rsrc(
@@ -1366,12 +1524,13 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
       for (int q = 0; q < 4; ++q)  // stages: two groups each
         if (q < P) m = max(m, max(hm[q] & 0xFFFFu, hm[q] >> 16));
-      // 2^b is above the row's values before the weight, 2^(b + exponent of w) after
-      const int b = __builtin_amdgcn_frexp_expf(__uint_as_float(m << 16)) + bound;
+      // 2^b is above the row's values before the weight and h's own power of two, 2^(b +
+      // exponent of w) after the weight
+      const int b = __builtin_amdgcn_frexp_expf(h_lo(m)) + bound;
       const int e = max(-100, min(b, 128)) + __builtin_amdgcn_frexp_expf(w) - 15;
       en_of[tid] = en;
       wt_of[tid] = ldexpf(w, -e);
-      if (cb0 == 0 && tid < tl.z) s.exps[en] = e;
+      if (cb0 == 0 && tid < tl.z) s.exps[en] = e + s.hexp[tl.y + tid];
     }
     wait_vm<0>();
     __syncthreads();
@@ -1434,7 +1593,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 #pragma unroll
         for (int d = 0; d < 2; ++d)
 #pragma unroll
-          for (int g = 0; g < 2; ++g) W[i][d][g] = unpack_w(wr[i][g][2 * gl + d], nib);
+          for (int g = 0; g < 2; ++g) W[i][d][g] = unpack_w<true>(wr[i][g][2 * gl + d], nib);
     };
     auto task = [&](int at, auto tc) {
       constexpr int t = decltype(tc)::value, up = (t + NB - 1) % NB;
@@ -1449,7 +1608,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         for (int g = 0; g < 2; ++g)
 #pragma unroll
           for (int i = 0; i < 2; ++i)
-            y[t & 1][i] = mfma32(X[t & 1][d][g], W[i][d][g], y[t & 1][i]);
+            y[t & 1][i] = mfma32<true>(X[t & 1][d][g], W[i][d][g], y[t & 1][i]);
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1508,9 +1667,9 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
         sp[i] = 0.f;
       }
       // the offsets' sum: both lane groups hold the same octet of X, against b
-      // and against -128 s
+      // and against -offset s
       u32x4 B[2];
-      const float f = c2 ? -128.0f : 1.0f;
+      const float f = c2 ? -kOffsetH : 1.0f;
 #pragma unroll
       for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1697,9 +1856,9 @@ hipError_t launch_moe_pack(const MoePackArgs& a) {
   return hipGetLastError();
 }
 
-hipError_t launch_moe_bound(const MoePackArgs& a, float* bound) {
+hipError_t launch_moe_bound(const MoePackArgs& a, bool down, float* bound) {
   hipLaunchKernelGGL(moe_bound_kernel, dim3((a.n + 63) / 64, a.experts), dim3(256), 0, a.stream, a,
-                     bound);
+                     down ? kOffsetH : kOffsetX, bound);
   return hipGetLastError();
 }
 
@@ -1718,7 +1877,7 @@ size_t moe_workspace_bytes(int hidden, int inner, int experts, int T, int k) {
 
 hipError_t launch_moe(const MoeArgs& a) {
   const int entries = a.T * a.k;
-  const MoeSpace s = moe_space(a.workspace, a.hidden, a.inner, a.experts, a.T, entries);
+  MoeSpace s = moe_space(a.workspace, a.hidden, a.inner, a.experts, a.T, entries);
   if (entries <= kFewEntries && a.T <= kFewTokens) {
     MOE_TRY(launch(moe_few_up_kernel, entries * (a.inner / 16), 256, 0, a.stream, a, s.h));
     return launch(moe_few_down_kernel, a.T * (a.hidden / 16), 64 * (a.k < 16 ? a.k : 16), 0, a.stream,
@@ -1738,8 +1897,8 @@ hipError_t launch_moe(const MoeArgs& a) {
   const bool stream = mean < 8;
   const int rows = wide ? 64 : mean <= 16 ? 16 : 32;
   const int64_t slots = max_tiles(entries, a.experts, rows);
-  const int64_t sums = stream ? 0 : (int64_t)a.T * 8 * gpad(a.hidden);
-  const int64_t sum_groups = (sums + kPlanThreads - 1) / kPlanThreads;
+  const int64_t sum_groups = ((int64_t)a.T * 8 * gpad(a.hidden) + kPlanThreads - 1) / kPlanThreads;
+  if (stream) s.xs = nullptr;  // the maxima only
   if (entries <= kPlanEntries) {
     MOE_TRY(launch(moe_plan_kernel, a.experts + sum_groups, kPlanThreads, 0, a.stream, a, rows, s));
   } else {
