@@ -120,3 +120,45 @@ def test_h_keeps_eleven_bits(gpu, T, hidden, inner, pairs, spread):
     d = (out - ref).abs()
     assert (d <= tol).all(), float((d / tol.clamp_min(1e-30)).max())
     assert (ref != 0).any(1).float().mean() > 0.9
+
+
+@pytest.mark.parametrize("T,hidden,inner,E", [(6, 256, 256, 2), (40, 256, 256, 40), (60, 256, 256, 4),
+                                              (1700, 2048, 384, 2), (1700, 2048, 640, 2)])
+@pytest.mark.parametrize("which", ["gate", "down"])
+def test_weights_that_cancel(gpu, T, hidden, inner, E, which):
+    """All weights of a matrix are 8 s - 8 s = 0, but for a group of about 2^-40: what the
+    sums leave of the zeros is far above those, and stays within the sums' error."""
+    g = torch.Generator().manual_seed(T + inner)
+
+    def mat(n, k, zeros):
+        w = torch.randint(-2 ** 31, 2 ** 31, (E, n, k // 8), dtype=torch.int32, generator=g)
+        s = ((torch.rand(E, n, k // 64, generator=g) + 0.5) * k ** -0.5 / 4.8).to(BF)
+        b = (-7.5 * s.float()).to(BF)
+        if zeros:
+            w[:, :, 8:] = -0x77777778  # every nibble 8
+            s[:, :, 1:], b[:, :, 1:] = 1.0, -8.0
+            s[:, :, 0] *= 2.0 ** -40
+            b[:, :, 0] *= 2.0 ** -40
+        return w, s, b
+
+    part = (mat(inner, hidden, which == "gate"), mat(inner, hidden, False),
+            mat(hidden, inner, which == "down"))
+    moe = gdn_amd.MoE(hidden, inner, [tuple(tuple(t.to(DEV) for t in m) for m in part)])
+    x = torch.randn(T, hidden, generator=g).to(BF)
+    ids = torch.rand(T, E, generator=g).argsort(1)[:, :2].to(torch.int32)
+    out = torch.empty(T, hidden, device=DEV, dtype=BF)
+    moe.forward(x.to(DEV), ids.to(DEV), torch.ones(T, 2, device=DEV), out, moe.workspace(T, 2))
+    out = out.cpu().double()
+    tol = torch.zeros(T, hidden, dtype=torch.float64)
+    for e in range(E):
+        rows = (ids == e).any(1)
+        xr = x[rows].double()
+        (wg, wu, wd) = (full(*(t[e] for t in m)) for m in part)
+        # as in test_h_keeps_eleven_bits; the magnitudes of a group add up to 271 s + |b|,
+        # of down's f16 numbers 2063 s + |b|
+        ea = (hidden // 64 + 8) * HALF_F32 * xr.abs().sum(1, True) * (271 + 8)
+        a, u = (xr @ wg.t()).abs() + (ea if which == "gate" else 0), (xr @ wu.t()).abs()
+        h = 1.001 * a * (u + ea)
+        ey = (inner // 64 + 8) * HALF_F32 * h.sum(1, True) * (2063 + 8) if which == "down" else 0
+        tol[rows] += 1.01 * (h @ wd.abs().t() + ey)
+    assert (out.abs() <= tol).all()
