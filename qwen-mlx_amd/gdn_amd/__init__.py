@@ -331,16 +331,20 @@ def add_rms_norm(h, d, w, eps, hn, group_sums=None, stream=None):
                                    _ptr(group_sums), _stream(stream)))
 
 
-@functools.lru_cache(maxsize=256)
 def route_desc(num_experts, top_k, score="softmax", num_groups=1, top_groups=1, group_top=1,
                renorm=True, scale=1.0, num_shared=0, shared_gate=False, logits_f32=False):
-    """A router's descriptor (gdn_moe_route_desc)."""
+    """A router's descriptor (gdn_moe_route_desc), the caller's own."""
     codes = {"softmax": 0, "sigmoid": 1}
     if score not in codes:
         raise ValueError(f"score must be softmax or sigmoid, not {score!r}")
     return MoeRouteDesc(num_experts, top_k, codes[score], num_groups, top_groups, group_top,
                         int(bool(renorm)), float(scale), num_shared, int(bool(shared_gate)),
                         int(bool(logits_f32)))
+
+
+# The descriptors of the calls below, by plain numbers (an argument's value at the call,
+# whatever holds it); none leaves this module. Built anew a call takes 0.4 us longer.
+_route_desc = functools.lru_cache(maxsize=256)(route_desc)
 
 
 def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=None, num_groups=1,
@@ -359,16 +363,16 @@ def moe_route(logits, ids, weights, num_experts, top_k, score="softmax", bias=No
     want = (T, top_k + num_shared)
     ip, wp = _dense(ids, dev, want, _IS_I32, "ids"), _dense(weights, dev, want, _IS_F32, "weights")
     bp = None if bias is None else _dense(bias, dev, (num_experts,), _IS_F32, "bias")
-    d = route_desc(num_experts, top_k, score, num_groups, top_groups, group_top, renorm, scale,
-                   num_shared, shared_gate, f32)
+    d = _route_desc(int(num_experts), int(top_k), score, int(num_groups), int(top_groups),
+                    int(group_top), bool(renorm), float(scale), int(num_shared), bool(shared_gate),
+                    f32)
     _check(lib.gdn_moe_route(ctypes.byref(d), lp, ls, T, bp, ip, wp,
                              _raw_stream(dev) if stream is None else stream.cuda_stream))
 
 
 @functools.lru_cache(maxsize=256)
 def _block_norm_desc(hidden, f32, kind, sigmoid, offset, scale, post_eps, pre_eps):
-    return BlockNormDesc(hidden, int(f32), kind, int(bool(sigmoid)), int(bool(offset)),
-                         float(scale), float(post_eps), float(pre_eps))
+    return BlockNormDesc(hidden, f32, kind, sigmoid, offset, scale, post_eps, pre_eps)
 
 
 def block_norm(h, x, h_out=None, hn=None, pre_w=None, pre_eps=1e-6, post_w=None, post_eps=1e-6,
@@ -399,7 +403,8 @@ def block_norm(h, x, h_out=None, hn=None, pre_w=None, pre_eps=1e-6, post_w=None,
             gp, gs = _mat(gate, dev, gsize, _IS_BF16, "gate")
         else:
             raise ValueError("gate must be [n, 1], [n, hidden] or [hidden]")
-    d = _block_norm_desc(hidden, f32, kind, gate_sigmoid, unit_offset, scale, post_eps, pre_eps)
+    d = _block_norm_desc(hidden, f32, kind, bool(gate_sigmoid), bool(unit_offset), float(scale),
+                         float(post_eps), float(pre_eps))
     _check(lib.gdn_block_norm(ctypes.byref(d), n, hp, hs, xp, xs, post, gp, gs, pre, op, os_, np_,
                               ns, _raw_stream(dev) if stream is None else stream.cuda_stream))
 
