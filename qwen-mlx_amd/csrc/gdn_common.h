@@ -482,10 +482,12 @@ struct ExecMlp {
 };
 struct ExecShape {
   int hidden, rows, depth, device;  // rows: the most a step or prefill runs
+  size_t held;                      // sequences
+  bool pending;                     // a step is not collected yet
 };
 ExecShape exec_shape(const gdn_exec* x);
-// Replaces the executor's MLP halves (at most one a position). Refused while the
-// executor holds sequences.
+// Replaces the executor's MLP halves (at most one a position). For an executor that
+// holds no sequences and no step.
 gdn_status exec_set_mlp(gdn_exec* x, std::vector<ExecMlp> halves);
 
 // Executor model-body kernels (gdn_exec.hip).

@@ -389,13 +389,10 @@ gdn_status queue_step(gdn_exec* x, int32_t B) {
 }  // namespace
 
 gdn::ExecShape gdn::exec_shape(const gdn_exec* x) {
-  return {x->hidden, x->rows, (int)x->stack.size(), x->device};
+  return {x->hidden, x->rows, (int)x->stack.size(), x->device, x->slot_of.size(), x->pend_n > 0};
 }
 
 gdn_status gdn::exec_set_mlp(gdn_exec* x, std::vector<gdn::ExecMlp> halves) {
-  if (!x->slot_of.empty() || x->pend_n > 0)
-    return efail(GDN_ERR_INVALID, "gdn_exec_set_moe: the executor holds %zu sequences",
-                 x->slot_of.size());
   DevScope dev(x->device);
   // nothing queued or captured holds the halves replaced here
   HIP_TRY(hipStreamSynchronize(x->stream), "gdn_exec_set_moe");

@@ -357,6 +357,8 @@ gdn_status gdn_moe_forward(const gdn_moe* m, const uint16_t* x, int64_t x_stride
 gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layers) try {
   if (!exec) return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: NULL executor");
   const gdn::ExecShape x = gdn::exec_shape(exec);
+  if (x.held > 0 || x.pending)
+    return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: the executor holds %zu sequences", x.held);
   if (n < 0 || n > x.depth || (n > 0 && !layers))
     return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: n = %d (a stack of %d layers) / NULL layers", n,
                  x.depth);

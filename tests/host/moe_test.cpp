@@ -252,8 +252,10 @@ static int test_exec_halves(bool graphs) {
     const int made = gdn_fake::graphs_made;
     CHECK(gdn_exec_decode_batch(s.ex, ids, toks, 2, next) == GDN_OK);
     CHECK(gdn_fake::graphs_made == made && (made > 0) == graphs);
+    gdn_fake::malloc_bytes = 0;
     CHECK(gdn_exec_set_moe(s.ex, n, n ? halves : nullptr) == GDN_ERR_INVALID);
     CHECK(std::strstr(gdn_last_error(), "holds 2 sequences"));
+    CHECK(gdn_fake::malloc_bytes == 0);  // refused before anything is allocated
     for (uint64_t id : ids) CHECK(gdn_exec_release(s.ex, id) == GDN_OK);
   }
   // no memory for the buffers: the halves stay as they were
