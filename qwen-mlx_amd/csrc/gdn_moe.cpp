@@ -374,7 +374,7 @@ gdn_status gdn_exec_set_moe(gdn_exec* exec, int32_t n, const gdn_exec_moe* layer
       return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: half %d at position %d (distinct, < %d)", i,
                    l.position, x.depth);
     taken[l.position] = 1;
-    if (!l.norm_w || !l.gate || !l.route || !l.moe || !aligned(l.norm_w, 16))
+    if (!l.norm_w || !l.gate || !l.route || !l.moe || !aligned(l.norm_w, 16) || !aligned(l.bias, 4))
       return mfail(GDN_ERR_INVALID, "gdn_exec_set_moe: half %d has a NULL or misaligned weight", i);
     const gdn_moe_route_desc& r = *l.route;
     int32_t gk = 0, gn = 0;

@@ -258,7 +258,11 @@ static int test_exec_halves(bool graphs) {
     CHECK(gdn_fake::malloc_bytes == 0);  // refused before anything is allocated
     for (uint64_t id : ids) CHECK(gdn_exec_release(s.ex, id) == GDN_OK);
   }
-  // no memory for the buffers: the halves stay as they were
+  // what every later step would fail at is refused here; the halves stay as they were
+  gdn_exec_moe odd = halves[1];
+  odd.bias = reinterpret_cast<const float*>(reinterpret_cast<const char*>(bias) + 2);
+  CHECK(gdn_exec_set_moe(s.ex, 1, &odd) == GDN_ERR_INVALID);
+  // no memory for the buffers: the same
   gdn_fake::malloc_limit = 1000;
   CHECK(gdn_exec_set_moe(s.ex, 3, halves) == GDN_ERR_OOM);
   gdn_fake::malloc_limit = ~(size_t)0;
