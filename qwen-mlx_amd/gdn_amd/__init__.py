@@ -252,14 +252,14 @@ def _stream(stream) -> int | None:
 
 # torch's names for the calls below, which take some microseconds in all: looked up
 # once, when the library is loaded
-_IS_BF16 = _IS_F32 = _IS_I32 = _IS_U8 = ()  # types, bf16 also as bit patterns
+_IS_BF16 = _IS_F32 = _IS_I32 = _IS_U8 = _IS_W4 = ()  # types, bf16 also as bit patterns
 _current_device = _raw_stream = None
 
 
 def _torch_names(torch):
-    global _IS_BF16, _IS_F32, _IS_I32, _IS_U8, _current_device, _raw_stream
+    global _IS_BF16, _IS_F32, _IS_I32, _IS_U8, _IS_W4, _current_device, _raw_stream
     _IS_BF16, _IS_F32 = (torch.bfloat16, torch.int16, torch.uint16), (torch.float32,)
-    _IS_I32, _IS_U8 = (torch.int32,), (torch.uint8,)
+    _IS_I32, _IS_U8, _IS_W4 = (torch.int32,), (torch.uint8,), (torch.int32, torch.uint32)
     _current_device = torch.cuda.current_device
     _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (
         lambda dev: torch.cuda.current_stream(dev).cuda_stream)
@@ -613,7 +613,8 @@ class MoE:
     """The 4-bit experts of a sparse MLP (gdn_moe_*). parts: sets of experts in id order,
     each ((gate w, scales, biases), (up ...), (down ...)) of MLX-format device tensors:
     gate and up w int32 [n, inner, hidden/8] with scales and biases [n, inner, hidden/64],
-    down [n, hidden, inner/8] and [n, hidden, inner/64] (bf16 or their bit patterns)."""
+    down [n, hidden, inner/8] and [n, hidden, inner/64] (bf16 or their bit patterns),
+    contiguous, on `device`."""
 
     def __init__(self, hidden: int, inner: int, parts, device: int = 0, stream=None,
                  group_size: int = 64, bits: int = 4):
@@ -625,16 +626,14 @@ class MoE:
             ptrs = []
             for (w, s, b), (rows, cols) in zip(part, ((inner, hidden), (inner, hidden),
                                                       (hidden, inner))):
-                if (tuple(w.shape) != (n, rows, cols // 8) or w.element_size() != 4 or
-                        any(tuple(t.shape) != (n, rows, cols // 64) or t.dtype not in _IS_BF16
-                            for t in (s, b))):
-                    raise ValueError(f"part {i}: expected [{n}, {rows}, {cols}] in 4-bit groups "
-                                     "of 64")
-                ptrs += [_ptr(w), _ptr(s), _ptr(b)]
+                ptrs += [_dense(w, device, (n, rows, cols // 8), _IS_W4, f"part {i}: weights")]
+                ptrs += [_dense(t, device, (n, rows, cols // 64), _IS_BF16, f"part {i}: {what}")
+                         for t, what in ((s, "scales"), (b, "biases"))]
             arr[i] = MoePart(n, *ptrs)
         h = _VP()
         _check(self.lib.gdn_moe_create(hidden, inner, len(parts), arr, group_size, bits, device,
-                                       _stream(stream), ctypes.byref(h)))
+                                       _raw_stream(device) if stream is None else stream.cuda_stream,
+                                       ctypes.byref(h)))
         self.handle = h
         self.hidden, self.inner, self.device = hidden, inner, device
         self.experts = sum(int(p.experts) for p in arr)
@@ -813,6 +812,7 @@ class Executor:
         attn_layers = list(attn_layers)
         self._keep = (pool, list(layers), list(input_norm_w), final_norm_w, embed, head,
                       attn_layers, kv)
+        self.device, self.hidden = device, head.K
         n = len(layers)
         na = len(attn_layers)
         self._layers = (_VP * max(n, 1))(*[l.handle.value for l in layers])
@@ -840,12 +840,19 @@ class Executor:
 
     def set_moe(self, moe_layers):
         """Give layers their sparse MLP halves (gdn_exec_set_moe), while no sequence is
-        held; an empty list takes them away."""
+        held; an empty list takes them away. norm_w: bf16 [hidden], bias: f32
+        [num_experts], on the executor's device."""
         moe_layers = list(moe_layers)
-        n = len(moe_layers)
-        arr = (ExecMoe * max(n, 1))(
-            *[ExecMoe(int(p), _ptr(w), gate.handle, ctypes.pointer(route), _ptr(bias), moe.handle)
-              for p, w, gate, route, bias, moe in moe_layers])
+        n, dev = len(moe_layers), self.device
+        arr = (ExecMoe * max(n, 1))()
+        for i, (p, w, gate, route, bias, moe) in enumerate(moe_layers):
+            if gate.device != dev:
+                raise ValueError(f"half {i}: gate must be on cuda:{dev}, not cuda:{gate.device}")
+            np_ = None if w is None else _dense(w, dev, (self.hidden,), _IS_BF16,
+                                                f"half {i}: norm_w")
+            bp = None if bias is None else _dense(bias, dev, (route.num_experts,), _IS_F32,
+                                                  f"half {i}: bias")
+            arr[i] = ExecMoe(int(p), np_, gate.handle, ctypes.pointer(route), bp, moe.handle)
         _check(self.lib.gdn_exec_set_moe(self.handle, n, arr))
         self._keep_moe = moe_layers
 

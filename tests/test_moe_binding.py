@@ -79,3 +79,74 @@ def test_flags_of_any_type(lib):
         t.fill_(v)
         _route(renorm=t)
         assert _desc(lib, gdn_amd.MoeRouteDesc).renorm == int(v)
+
+
+def _part(n=2, hidden=128, inner=128):
+    def mat(r, c):
+        return (torch.zeros(n, r, c // 8, dtype=I32), torch.zeros(n, r, c // 64, dtype=BF),
+                torch.zeros(n, r, c // 64, dtype=BF))
+    return [mat(inner, hidden), mat(inner, hidden), mat(hidden, inner)]
+
+
+def _swap(part, m, t, tensor):
+    part = [list(x) for x in part]
+    part[m][t] = tensor
+    return part
+
+
+def test_experts_refuse_parts_of_another_type_size_layout_or_device(lib, monkeypatch):
+    """What the kernels would read as something else, or past its end."""
+    asked = []
+    monkeypatch.setattr(gdn_amd, "_raw_stream", lambda dev: asked.append(dev))
+    ok = _part()
+    bits = [[w.view(torch.uint32), s.view(torch.int16), b.view(torch.uint16)] for w, s, b in ok]
+    for part in (ok, bits):
+        assert gdn_amd.MoE(128, 128, [part], device=-1).experts == 2
+        assert lib.calls[-1][0] == "gdn_moe_create"
+    assert asked == [-1, -1]  # the stream of the layer's device
+    made = len(lib.calls)
+    for bad in (_swap(ok, 0, 0, torch.zeros(2, 128, 16)),                     # floats as packed weights
+                _swap(ok, 1, 0, torch.zeros(2, 128, 16, dtype=torch.int64)),
+                _swap(ok, 2, 0, torch.zeros(2, 128, 8, dtype=I32)),           # too short
+                _swap(ok, 0, 1, torch.zeros(2, 128, 2)),                      # f32 scales
+                _swap(ok, 1, 2, torch.zeros(2, 128, 2, dtype=torch.float16)),
+                _swap(ok, 2, 1, torch.zeros(1, 128, 2, dtype=BF)),            # fewer experts
+                _swap(ok, 0, 0, torch.zeros(2, 16, 128, dtype=I32).transpose(1, 2))):
+        with pytest.raises(ValueError):
+            gdn_amd.MoE(128, 128, [bad], device=-1)
+    with pytest.raises(ValueError, match="cuda:0"):  # parts of another device than the layer's
+        gdn_amd.MoE(128, 128, [ok], device=0)
+    assert len([c for c in lib.calls[made:] if c[0] == "gdn_moe_create"]) == 0
+
+
+class _Handle:
+    handle = ctypes.c_void_p(1)
+    device = -1
+
+
+def test_set_moe_refuses_weights_of_another_type_size_layout_or_device(lib):
+    """A half's norm weights and bias are read by every later step."""
+    ex = gdn_amd.Executor.__new__(gdn_amd.Executor)
+    ex.lib, ex.handle, ex.device, ex.hidden = lib, ctypes.c_void_p(1), -1, 128
+    norm, bias = torch.ones(128, dtype=BF), torch.zeros(24)
+    route = gdn_amd.route_desc(24, 4)
+    half = lambda w=norm, b=bias, g=_Handle: (0, w, g, route, b, _Handle)  # noqa: E731
+    for b in (bias, None):
+        ex.set_moe([half(b=b)])
+        assert lib.calls[-1][0] == "gdn_exec_set_moe"
+    ex.set_moe([half(w=norm.view(torch.int16))])
+    made = len(lib.calls)
+
+    class Elsewhere(_Handle):
+        device = 0
+
+    for bad in (half(w=torch.ones(128)), half(w=torch.ones(64, dtype=BF)),
+                half(w=torch.ones(256, dtype=BF)[::2]), half(w=torch.ones(1, 128, dtype=BF)),
+                half(b=bias.to(BF)), half(b=torch.zeros(23)), half(b=torch.zeros(48)[::2]),
+                half(b=torch.zeros(24, dtype=torch.float64)), half(g=Elsewhere)):
+        with pytest.raises(ValueError):
+            ex.set_moe([bad])
+    ex.device = 0
+    with pytest.raises(ValueError, match="cuda:0"):
+        ex.set_moe([half()])
+    assert len(lib.calls) == made
