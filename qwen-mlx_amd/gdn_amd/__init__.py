@@ -277,13 +277,14 @@ def _refuse(t, dev, size, types, what: str):
 
 def _mat(t, dev: int, size, types, what: str):
     """(pointer, row stride in elements) of a matrix of that size and type on device
-    dev whose rows are contiguous."""
+    dev whose rows are contiguous. A single row's stride is its length: torch's own
+    for it can be any number."""
     if t.size() != size or t.get_device() != dev or t.dtype not in types:
         _refuse(t, dev, size, types, what)
     rows, cols = t.stride()
     if cols != 1 and size[1] > 1:
         _refuse(t, dev, size, types, what)
-    return t.data_ptr(), rows
+    return t.data_ptr(), rows if size[0] != 1 else size[1]
 
 
 def _dense(t, dev: int, size, types, what: str) -> int:

@@ -150,3 +150,29 @@ def test_set_moe_refuses_weights_of_another_type_size_layout_or_device(lib):
     with pytest.raises(ValueError, match="cuda:0"):
         ex.set_moe([half()])
     assert len(lib.calls) == made
+
+
+def test_one_row_of_any_stride(lib):
+    """The stride of a single row does not matter: torch gives it none in particular."""
+    def one(n, dtype):  # [1, n], contiguous, with a row stride of 1
+        t = torch.zeros(n, 1, dtype=dtype).t()
+        assert t.is_contiguous() and t.stride(0) == 1
+        return t
+
+    def odd(n, dtype):  # a row of a matrix whose rows are n + 3 apart
+        return torch.zeros(2, n + 3, dtype=dtype)[:1, :n]
+
+    for row in (one, odd):
+        gdn_amd.moe_route(row(257, BF), torch.zeros(1, 9, dtype=I32), torch.zeros(1, 9), 256, 8,
+                          num_shared=1, shared_gate=True)
+        assert lib.calls[-1][1][2] >= 257
+        gdn_amd.block_norm(row(64, F32), row(64, BF), h_out=row(64, F32), hn=row(64, BF),
+                           pre_w=torch.ones(64, dtype=BF), gate=row(64, BF))
+        a = lib.calls[-1][1]
+        for stride in (a[3], a[5], a[8], a[11], a[13]):
+            assert stride >= 64 and stride % 8 == 0
+        moe = gdn_amd.MoE(128, 128, [_part()], device=-1)
+        ws = torch.zeros(256, dtype=torch.uint8)
+        moe.forward(row(128, BF), torch.zeros(1, 2, dtype=I32), torch.zeros(1, 2), row(128, BF), ws)
+        a = lib.calls[-1][1]
+        assert a[2] >= 128 and a[2] % 8 == 0 and a[8] >= 128 and a[8] % 4 == 0
