@@ -185,6 +185,14 @@ __host__ __device__ __forceinline__ int gpad(int k) { return (k / 64 + 7) & ~7; 
 // Slots for tiles of `rows` rows (moe_plan_kernel).
 int64_t max_tiles(int64_t entries, int experts, int rows) { return entries / rows + experts; }
 
+// Entries from which a call goes in tiles of 64 rows (launch_moe says why): 32 an expert
+// and, of its blocks of 256 columns, a work-group for most of the 512 that run side by
+// side, where the tiles are the whole ones and half an expert's last.
+int64_t wide_entries(int hidden, int experts) {
+  const int64_t blocks = (hidden + 255) / 256, tiles = (384 + blocks - 1) / blocks;
+  return std::max<int64_t>(32 * (int64_t)experts, 64 * (tiles - experts + experts / 2));
+}
+
 MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t tokens,
                    int64_t entries) {
   MoeSpace s{};
@@ -204,7 +212,10 @@ MoeSpace moe_space(void* base, int hidden, int inner, int experts, int64_t token
   s.h = reinterpret_cast<uint16_t*>(
       take(std::max(entries, 2 * std::min<int64_t>(entries, kFewEntries)) * inner * 2));
   s.hexp = reinterpret_cast<int32_t*>(take(entries * 4));
-  s.rows = reinterpret_cast<float*>(take(entries * hidden * 4));
+  // rows of long prompts are f16 (moe_wide_down_kernel), those of smaller calls f32
+  const int64_t f32 =
+      inner <= kWideInner ? std::min(entries, wide_entries(hidden, experts)) : entries;
+  s.rows = reinterpret_cast<float*>(take(std::max(4 * f32, 2 * entries) * hidden));
   s.exps = reinterpret_cast<int32_t*>(take(entries * 4));
   s.hmax = reinterpret_cast<uint16_t*>(take(inner <= kWideInner ? entries * 16 : 0));
   s.counts = reinterpret_cast<int32_t*>(take((entries + kChunk - 1) / kChunk * experts * 4));
@@ -1893,7 +1904,7 @@ hipError_t launch_moe(const MoeArgs& a) {
   // 436, 102 / 91).
   const int mean = entries / a.experts;
   const int64_t wide_tiles = max_tiles(entries, a.experts, 64) - a.experts / 2;
-  const bool wide = mean >= 32 && wide_tiles * ((a.hidden + 255) / 256) >= 384;
+  const bool wide = entries >= wide_entries(a.hidden, a.experts);
   const bool stream = mean < 8;
   const int rows = wide ? 64 : mean <= 16 ? 16 : 32;
   const int64_t slots = max_tiles(entries, a.experts, rows);
