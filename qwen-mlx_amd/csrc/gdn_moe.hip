@@ -173,7 +173,7 @@ constexpr int kChunk = 4096, kPlanEntries = 8192;
 // Most entries of a call whose work-groups find their rows by themselves: a
 // wave holds every id.
 // They and the rows' product with the sum are two launches: one token of 9 columns,
-// hidden 2048, inner 512, takes 6.4 + 5.7 us, the latency of a launch and a chain of
+// hidden 2048, inner 512, takes 7.1 + 6.1 us, the latency of a launch and a chain of
 // loads each (16 MB of weights); by a plan, tiles and a sum the call took 21.7.
 constexpr int kFewEntries = 64;
 // ... and the most tokens: down reads an expert's weights for each of them again.
@@ -677,7 +677,8 @@ __device__ __forceinline__ void wait_vm() {
 //     64 columns are one group of down's input, whose split sums it stores.
 //   else: rows of h, and the weighted rows of down go to their entries.
 // Bound by the weights' bytes and the loads' latency: 317 tokens of 9 columns, hidden
-// 2048, inner 512, 257 experts (11 rows each): up 66 us (269 MB), down 42.
+// 2048, inner 512, 257 experts (11 rows each): up 67 us (303 MB, 4.5 TB/s), down 43
+// (152 MB, 3.5 TB/s).
 template <int MW, bool UP>
 __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) void moe_tile_kernel(
     MoeArgs a, MoeSpace s) {
@@ -937,7 +938,7 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(4, 8))) voi
 // against ones instead of beforehand, and the offsets applied with the scales. Rows
 // past the tile's are not read: their copies are out of the buffer's range, which
 // gives zeros. Bound by the weights' bytes: 64 tokens of 9 columns, hidden 2048, inner
-// 512, 257 experts: up 45 us at 5.9 TB/s, down 28 at 4.7.
+// 512, 257 experts: up 45.5 us at 5.8 TB/s, down 26.6 at 4.9.
 template <int KS, bool UP>
 __global__ __launch_bounds__(128 * KS) __attribute__((amdgpu_waves_per_eu(4, 8))) void
     moe_stream_kernel(MoeArgs a, MoeSpace s) {
@@ -1148,11 +1149,12 @@ __device__ __forceinline__ f32x16 mfma32(u32x4 a, u32x4 b, f32x16 c) {
 // Bound by the vector instructions beside the products: a product of 32 cycles comes
 // with 9 of 4 cycles, 4 of them the scaling and 3.5 the unpacking, whose issue it
 // blocks for 12, and the card takes its clock back to 2.0 GHz. 16,384 tokens of 9
-// columns, hidden 2048, inner 512, 257 experts: up 713 us, 870 TFLOP/s. In copies
-// without a part: without the row copies 565 us, the weights 607, the offsets 635,
-// the unpacking 663; without any of them 350. Half the unpacking with 128 rows a wave
-// and half the columns (twice the row copies) took 760; three slots of rows and
-// weights more than two stages ahead, 690 to 700 in 256 registers, was not kept.
+// columns, hidden 2048, inner 512, 257 experts: up 734 to 747 us, 828 to 843 TFLOP/s.
+// In copies without a part, where it took 713: without the row copies 565, the weights
+// 607, the offsets 635, the unpacking 663; without any of them 350. Half the unpacking
+// with 128 rows a wave and half the columns (twice the row copies) took 760; three
+// slots of rows and weights more than two stages ahead, 690 to 700 in 256 registers,
+// was not kept.
 template <bool UP>
 __global__ __launch_bounds__(256)
     __attribute__((amdgpu_waves_per_eu(2, 2))) void
@@ -1851,7 +1853,7 @@ hipError_t launch_wide(const MoeArgs& a, const MoeSpace& s, int64_t slots, int64
     return launch(moe_wide_kernel<false>, tile_groups(slots, blocks), 256, 0, a.stream, a, s);
   // Long runs, as long as they leave three work-groups for each of the 512 that run
   // side by side. The whole call in runs of 8 / 4 / 2 / 1 blocks: 16,384 tokens (2,400
-  // tiles) 1210 / 1214 / 1226 / 1251 us, 4,000 (690) 398 / 385 / 385 / 396.
+  // tiles) 1197 / 1208 / 1221 / 1259 us, 4,000 (690) 379 / 368 / 364 / 374.
   int run = blocks;
   while (run > 1 && tiles * ((blocks + run - 1) / run) < 1536) run = (run + 1) / 2;
   return launch(moe_wide_down_kernel, tile_groups(slots, (blocks + run - 1) / run), 256, 0, a.stream,
@@ -1896,12 +1898,12 @@ hipError_t launch_moe(const MoeArgs& a) {
   }
   // The kernel by the rows that an expert has on average. At hidden 2048, inner
   // 512, 257 experts, 9 columns, tiles of 16 rows by the stream kernel / 16 / 32 /
-  // 64 rows: 64 tokens (mean 2) 81 / 85 / 88 / 108 us, 200 (7) 103 / 104 / 109 / 135,
-  // 317 (11) 123 / 114 / 118 / 141, 600 (21) - / 150 / 137 / 153, 1000 (35) - / - / 190 /
-  // 181, 2000 (70) - / 327 / 275 / 248. Tiles of 64 rows also want a work-group for
-  // most of the 512 that run side by side (hidden 1024, inner 1408, 32 experts, 4
-  // columns: 1000 tokens, 312 work-groups, 78 us by 32 rows and 78 by 64; 1500 tokens,
-  // 436, 102 / 91).
+  // 64 rows: 64 tokens (mean 2) 77 / 85 / 89 / 108 us, 200 (7) 101 / 104 / 110 / 132,
+  // 317 (11) 121 / 113 / 119 / 137, 600 (21) 169 / 145 / 138 / 147, 1000 (35) 244 / 194 /
+  // 178 / 167, 2000 (70) 428 / 329 / 281 / 226. Tiles of 64 rows also want a work-group
+  // for most of the 512 that run side by side (hidden 1024, inner 1408, 32 experts, 4
+  // columns: 1000 tokens, 312 work-groups, 78 us by 32 rows and 77 by 64; 1500 tokens,
+  // 436, 104 / 91).
   const int mean = entries / a.experts;
   const int64_t wide_tiles = max_tiles(entries, a.experts, 64) - a.experts / 2;
   const bool wide = entries >= wide_entries(a.hidden, a.experts);
