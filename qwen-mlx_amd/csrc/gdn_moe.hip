@@ -143,7 +143,9 @@ __device__ __forceinline__ float swiglu(float g, float u) {
 
 constexpr int kPassEntries = 1 << 18;  // of a pass over the experts
 constexpr int kStageK = 128;           // k of a stage: two groups
-constexpr int kWideInner = 512;        // inner up to which wide down keeps its rows in LDS
+// Inner up to which wide down keeps its rows in LDS: 64 rows of 512 and what goes with
+// them take 77 KB, so that two work-groups share a CU's 160; 640 would leave one.
+constexpr int kWideInner = 512;
 // The bytes of x that a pass's 32-bit offsets reach, and an offset past them.
 constexpr uint32_t kReach = 0xFFFF0000u, kNowhere = 0xFFFF8000u;
 
