@@ -1781,7 +1781,6 @@ __global__ __launch_bounds__(256) void moe_combine_kernel(MoeArgs a, const float
 // The same of f16 rows: a thread per 8 columns.
 __global__ __launch_bounds__(256) void moe_combine_half_kernel(MoeArgs a, MoeSpace s) {
   constexpr int B = 4;
-  typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
   const int q = a.hidden / 8;
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= (int64_t)a.T * q) return;
