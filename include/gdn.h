@@ -100,6 +100,7 @@ typedef int gdn_status;
 #define GDN_FLAG_BAD_SLOT 0x1u      /* a slot id was outside [0, num_slots)      */
 #define GDN_FLAG_DUP_SLOT 0x2u      /* gdn_slots_validate found a repeated id    */
 #define GDN_FLAG_BAD_SEQLENS 0x4u   /* cu_seqlens not non-decreasing / too long  */
+#define GDN_FLAG_NO_PAGES 0x8u      /* gdn_kv8_step: too few free pages for a row */
 
 #define GDN_ALL_LAYERS (-1)
 
@@ -806,6 +807,184 @@ gdn_status gdn_block_norm(const gdn_block_norm_desc* desc, int32_t n, const void
                           const uint16_t* post_w, const uint16_t* gate, int64_t gate_stride,
                           const uint16_t* pre_w, void* h_out, int64_t h_out_stride, uint16_t* hn,
                           int64_t hn_stride, void* stream);
+
+/* ------------------------------------------------------------------------
+ * An 8-bit paged KV cache planned on the GPU, and the operators around it
+ * (Qwen35Attention::forward_with_cache, qwen3_5.rs:377-455, with its cache of
+ * growing arrays, :419-424, in half the bytes of gdn_kv). Request lengths live
+ * in device memory: gdn_kv8_step builds block tables, positions and slot maps
+ * from them, and every launch shape follows the host's bounds alone, so a step
+ * (gdn_kv8_step, then per layer gdn_rope_forward, gdn_kv8_append and
+ * gdn_kv8_attention) may be captured in a HIP graph and replayed while the
+ * lengths change. No call after gdn_kv8_create allocates. All calls on one
+ * cache are ordered on one stream, replays of its graphs among them.
+ *
+ * A page holds 64 tokens of one layer: for keys and for values of each kv head
+ * 64 x head_dim e4m3 numbers (1 sign, 4 exponent, 3 fraction bits, largest 448)
+ * under one exponent e: number * 2^e, e the least integer in [-40, 56] with
+ * |x| <= 448 * 2^e for every finite x of the page's tokens. Values round to the
+ * nearest, ties to even; infinities and NaN are held as NaN, numbers past
+ * 448 * 2^56 as that.
+ * ------------------------------------------------------------------------ */
+typedef struct gdn_kv8 gdn_kv8;
+
+typedef struct gdn_kv8_desc {
+  int32_t num_layers;
+  int32_t num_slots;           /* sequences the cache can hold, at most 4096     */
+  int32_t num_pages;           /* 64-token pages shared by all slots             */
+  int32_t max_pages_per_slot;  /* longest context / 64                           */
+  int32_t num_q_heads;         /* 1 .. 16 query heads for each kv head           */
+  int32_t num_kv_heads;        /* at most 256                                    */
+  int32_t head_dim;            /* 64, 128 or 256                                 */
+  int32_t max_step_tokens;     /* most tokens of one step, at most 262144        */
+  int32_t device;
+} gdn_kv8_desc;
+
+/* Per layer num_pages * num_kv_heads * 128 * head_dim bytes of keys and values,
+ * the tables, and an attention workspace. */
+gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out);
+gdn_status gdn_kv8_destroy(gdn_kv8* kv);
+gdn_status gdn_kv8_describe(const gdn_kv8* kv, gdn_kv8_desc* desc);
+
+/* Plan a step on the GPU. Row i < n <= 4096: sequence slots[i] holds lens[i]
+ * tokens and appends ntok[i] >= 0 (DEVICE arrays). Its pages are made to fit
+ * lens[i] + ntok[i]: rows with more than that give the surplus back (in row order,
+ * each row's last page first, to the top of the free stack), then rows with less take
+ * pages from the top of the stack, in row order and order of position. So lens
+ * below what a slot held drops tokens, lens = ntok = 0 releases a sequence, and the
+ * same call twice changes nothing the second time. Positions below lens[i] hold
+ * what was appended there; where nothing was, whatever their page held before.
+ *
+ * The new tokens lie packed in row order in every tensor of the step's calls:
+ * row i's from cu[i] = the sum of the ntok before it. max_tokens (host; at most
+ * max_step_tokens) is those tensors' row count, max_row_tokens (0: max_tokens) a
+ * bound on ntok: 1 makes a decode step. A slot < 0 marks a row of padding, which
+ * takes no tokens. Rows are refused, and flagged for gdn_kv8_check, where the
+ * slot is >= num_slots (BAD_SLOT) or an earlier row's too (DUP_SLOT), where
+ * lens, ntok, their sum or cu break a bound (BAD_SEQLENS; a negative ntok takes
+ * no tokens, one above max_tokens counts as max_tokens + 1), and where the row
+ * needs pages but the rows up to it need more than are free (NO_PAGES; a row
+ * refused for it counts). A refused row keeps its pages; its tokens are skipped:
+ * they have no place, and attention gives them zeros.
+ *
+ * lens_out (or NULL; may be lens) receives lens[i] + ntok[i], a refused or
+ * padding row's lens[i]. */
+gdn_status gdn_kv8_step(gdn_kv8* kv, int32_t n, const int32_t* slots, const int32_t* lens,
+                        const int32_t* ntok, int32_t* lens_out, int32_t max_tokens,
+                        int32_t max_row_tokens, void* stream);
+
+/* The cache's tables in device memory, for reading on the cache's stream. */
+typedef struct gdn_kv8_view {
+  const int32_t* table;  /* [num_slots][max_pages_per_slot] page ids, -1 past the owned */
+  const int32_t* owned;  /* [num_slots] pages of a slot                                */
+  const int32_t* free_pages; /* [num_pages] the stack, -1 from free_count on           */
+  const int32_t* free_count; /* [1]                                                    */
+  /* of the last step: */
+  const int32_t* cu;     /* [n + 1] first token of each row                            */
+  const int32_t* pos;    /* [max_tokens] a token's position in its sequence, or -1     */
+  const int32_t* map;    /* [max_tokens] its place in the cache, page * 64 + position % 64, or -1 */
+} gdn_kv8_view;
+gdn_status gdn_kv8_views(const gdn_kv8* kv, gdn_kv8_view* view);
+
+/* Read (and clear) the flags latched by gdn_kv8_step. Synchronises the stream. */
+gdn_status gdn_kv8_check(gdn_kv8* kv, void* stream, uint32_t* flags);
+
+/* Put the step's new keys and values [max_tokens, stride] (num_kv_heads x
+ * head_dim bf16 each, 16-byte aligned, strides multiples of 8) into layer's
+ * pages. A page's exponent follows the tokens that it holds with them; where it
+ * changes, the older numbers are rounded anew from what was held. The same
+ * call twice leaves the same bits. */
+gdn_status gdn_kv8_append(gdn_kv8* kv, int32_t layer, const uint16_t* k, int64_t k_stride,
+                          const uint16_t* v, int64_t v_stride, void* stream);
+
+/* The values held at m places map[i] (page * 64 + position % 64, DEVICE array) of a
+ * layer -> k_out, v_out [m, stride] bf16 (exact; either may be NULL; 16-byte aligned,
+ * strides multiples of 8). A place outside the cache gives zeros. */
+gdn_status gdn_kv8_gather(gdn_kv8* kv, int32_t layer, int32_t m, const int32_t* map,
+                          uint16_t* k_out, int64_t k_stride, uint16_t* v_out, int64_t v_stride,
+                          void* stream);
+
+typedef struct gdn_kv8_attn_desc {
+  float scale;     /* factor on q . k; 0: 1 / sqrt(head_dim)                       */
+  float softcap;   /* > 0: scores become softcap * tanh(score / softcap)           */
+  int32_t window;  /* > 0: a token sees the last `window` positions, its own included */
+} gdn_kv8_attn_desc;
+
+/* Attention of the step's tokens over their sequences' cached keys (the new ones
+ * appended before). For the query of head h at position i and the key at position j
+ *   s = softcap(scale * q . k) - slopes[h] * (i - j)
+ * where i - window < j <= i, or j < prefix[row] (prefix NULL: 0; at most the row's
+ * length), else none; out = sum_j softmax(s)_j v_j, times sigmoid(gate) where there
+ * is a gate. Query head h reads kv head h / (num_q_heads / num_kv_heads). q, gate,
+ * out [max_tokens] rows of num_q_heads x head_dim bf16, token and head strides in
+ * elements; q and gate 16-byte aligned with strides that are multiples of 8, out
+ * 8-byte aligned with multiples of 4. slopes [num_q_heads] f32 and prefix [n] are
+ * DEVICE arrays (or NULL). Tokens of refused rows get zeros; rows behind the last
+ * token are left as they are.
+ *
+ * Products and sums are f32; the softmax's weights enter the product with the values in f16
+ * (11 bits), and out is rounded once. The bits are the same every time and do not
+ * depend on the step's other rows; they may differ between steps that cut a
+ * sequence differently. A NaN among the keys that a token sees makes its head NaN,
+ * one among the values their dimension; tokens that do not see it are not touched. */
+gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc* desc,
+                             const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
+                             const float* slopes, const int32_t* prefix, const uint16_t* gate,
+                             int64_t gate_stride, int64_t gate_head_stride, uint16_t* out,
+                             int64_t out_stride, int64_t out_head_stride, void* stream);
+
+/* Rotary positions (qwen3_5.rs:411-417 with its norm :399-407, in general form).
+ * Pair i < rotary_dim / 2 of a head turns by pos * f_i, f_i = base^(-2 i / rotary_dim)
+ * changed by the scaling, angles formed in 64 bits:
+ *   LINEAR  f_i / factor
+ *   YARN    f_i / factor * r_i + f_i * (1 - r_i), r_i = clamp((i - lo) / max(hi - lo, 0.001), 0, 1),
+ *           lo = max(floor(d(fast)), 0), hi = min(ceil(d(slow)), rotary_dim - 1),
+ *           d(b) = rotary_dim * ln(original / (2 pi b)) / (2 ln base); cos and sin times
+ *           magnitude (0: 0.1 ln(factor) + 1)
+ *   BANDS   f_i / factor * (1 - m_i) + f_i * m_i, m_i = clamp((t_i - slow) / (fast - slow), 0, 1),
+ *           t_i = original * f_i / (2 pi): pairs of fewer than `slow` turns in `original`
+ *           positions are slowed, of more than `fast` kept
+ * A pair is (i, i + rotary_dim / 2), or (2 i, 2 i + 1) with interleaved. */
+#define GDN_ROPE_NONE 0
+#define GDN_ROPE_LINEAR 1
+#define GDN_ROPE_YARN 2
+#define GDN_ROPE_BANDS 3
+typedef struct gdn_rope gdn_rope;
+
+typedef struct gdn_rope_desc {
+  int32_t head_dim;     /* multiple of 8, 8 .. 512                              */
+  int32_t rotary_dim;   /* even, 0 .. head_dim: the first dimensions of a head  */
+  int32_t interleaved;
+  int32_t scaling;      /* GDN_ROPE_*                                           */
+  float base;           /* > 1                                                  */
+  float factor;         /* > 0                                                  */
+  float original;       /* YARN, BANDS: context length of the training, > 0     */
+  float fast;           /* > slow > 0                                           */
+  float slow;
+  float magnitude;      /* factor on cos and sin; 0: 1, with YARN as above      */
+} gdn_rope_desc;
+
+gdn_status gdn_rope_create(const gdn_rope_desc* desc, int32_t device, gdn_rope** out);
+gdn_status gdn_rope_destroy(gdn_rope* rope);
+
+/* T tokens at positions pos [T] (DEVICE): q [T, q_heads, head_dim] -> q_out, k -> k_out
+ * (k_heads 0 and k NULL: no k), rows of one element type. Where norm weights q_norm_w,
+ * k_norm_w ([head_dim] bf16 or NULL) are given, a head is first multiplied by
+ * w / sqrt(mean(x^2) + eps). All in f32, rounded once. Dimensions from rotary_dim on
+ * are normalised and copied; a token at a negative position is copied as it is.
+ * inverse: turns back (the gradient of the turn). Pointers 16-byte aligned, token
+ * and head strides multiples of 8 elements; an output may be its input with the
+ * same strides, other overlaps are not allowed. Allocates nothing, may be captured. */
+typedef struct gdn_rope_rows {
+  const void* in;
+  void* out;
+  int32_t heads;
+  int64_t in_stride, in_head_stride, out_stride, out_head_stride;
+  const uint16_t* norm_w;
+} gdn_rope_rows;
+gdn_status gdn_rope_forward(const gdn_rope* rope, int32_t T, const int32_t* pos,
+                            const gdn_rope_rows* q, const gdn_rope_rows* k, int32_t f32, float eps,
+                            int32_t inverse, void* stream);
 
 #ifdef __cplusplus
 }

@@ -467,6 +467,88 @@ struct BlockNormArgs {
 };
 hipError_t launch_block_norm(const BlockNormArgs& a);
 
+// The 8-bit paged cache (gdn_kv8.hip, gdn_attn8.hip). Device state and the last step's plan.
+struct Kv8Plan {
+  int num_slots, num_pages, max_pages, Hq, Hkv, D;
+  int n, T, max_row;            // of the step: rows, tokens, most tokens of a row
+  int32_t* table;               // [num_slots][max_pages]
+  int32_t* owned;               // [num_slots]
+  int32_t* free_pages;          // [num_pages]
+  int32_t* free_count;          // [1]
+  int32_t* mark;                // [num_slots] INT_MAX between steps
+  uint32_t* status;
+  int32_t* cu;                  // [n + 1]
+  int32_t* pos;                 // [T]
+  int32_t* map;                 // [T]
+  int32_t* row_slot;            // [n] -1: no tokens
+  int32_t* row_pos;             // [n] tokens before the step
+  int32_t* row_new;             // [n] tokens of the step, 0 where refused
+  int32_t* blocks;              // [n + 1] pages that the rows before touch
+};
+constexpr int kKv8Rows = 4096;  // rows of a step
+struct Kv8StepArgs {
+  Kv8Plan p;
+  const int32_t *slots, *lens, *ntok;
+  int32_t* lens_out;
+  hipStream_t stream;
+};
+hipError_t launch_kv8_step(const Kv8StepArgs& a);
+
+struct Kv8AppendArgs {
+  Kv8Plan p;
+  uint8_t* pages;               // [num_pages][2][Hkv][64 * D]
+  int32_t* exps;                // [num_pages][2][Hkv]
+  const uint16_t *k, *v;
+  int64_t ks, vs;
+  hipStream_t stream;
+};
+hipError_t launch_kv8_append(const Kv8AppendArgs& a);
+
+struct Kv8GatherArgs {
+  Kv8Plan p;
+  const uint8_t* pages;
+  const int32_t* exps;
+  int m;
+  const int32_t* map;
+  uint16_t *k_out, *v_out;
+  int64_t ks, vs;
+  hipStream_t stream;
+};
+hipError_t launch_kv8_gather(const Kv8GatherArgs& a);
+
+struct Kv8AttnArgs {
+  Kv8Plan p;
+  const uint8_t* pages;
+  const int32_t* exps;
+  float scale, softcap;
+  int window;
+  const uint16_t* q;
+  int64_t qs, qhs;
+  const float* slopes;
+  const int32_t* prefix;
+  const uint16_t* gate;
+  int64_t gs, ghs;
+  uint16_t* out;
+  int64_t os, ohs;
+  void* workspace;
+  hipStream_t stream;
+};
+size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d);
+hipError_t launch_kv8_attn(const Kv8AttnArgs& a);
+
+// Rotary positions (gdn_rope.hip).
+struct RopeArgs {
+  int D, rot;
+  bool interleaved, f32, inverse;
+  float mag, eps;
+  const double* turns;          // [rot / 2] turns per position
+  int T;
+  const int32_t* pos;
+  gdn_rope_rows q, k;
+  hipStream_t stream;
+};
+hipError_t launch_rope(const RopeArgs& a);
+
 // Sets the calling thread's gdn_last_error() message and returns code.
 gdn_status set_error(gdn_status code, const char* msg);
 

@@ -24,6 +24,7 @@ GDN_ERR_SLOTS = 5
 GDN_FLAG_BAD_SLOT = 0x1
 GDN_FLAG_DUP_SLOT = 0x2
 GDN_FLAG_BAD_SEQLENS = 0x4
+GDN_FLAG_NO_PAGES = 0x8
 GDN_ALL_LAYERS = -1
 
 # Exported symbols and their signatures (restype is int status unless noted).
@@ -106,6 +107,22 @@ SIGNATURES = {
                           ctypes.c_int64, _VP, _VP, ctypes.c_float, ctypes.c_float, _I32, _VP,
                           ctypes.c_int64, _VP], ctypes.c_int),
     "gdn_kv_read": ([_VP, _I32, _I32, _VP, _VP, _VP], ctypes.c_int),
+    "gdn_kv8_create": ([_VP, ctypes.POINTER(_VP)], ctypes.c_int),
+    "gdn_kv8_destroy": ([_VP], ctypes.c_int),
+    "gdn_kv8_describe": ([_VP, _VP], ctypes.c_int),
+    "gdn_kv8_step": ([_VP, _I32, _VP, _VP, _VP, _VP, _I32, _I32, _VP], ctypes.c_int),
+    "gdn_kv8_views": ([_VP, _VP], ctypes.c_int),
+    "gdn_kv8_check": ([_VP, _VP, ctypes.POINTER(ctypes.c_uint32)], ctypes.c_int),
+    "gdn_kv8_append": ([_VP, _I32, _VP, ctypes.c_int64, _VP, ctypes.c_int64, _VP], ctypes.c_int),
+    "gdn_kv8_gather": ([_VP, _I32, _I32, _VP, _VP, ctypes.c_int64, _VP, ctypes.c_int64, _VP],
+                       ctypes.c_int),
+    "gdn_kv8_attention": ([_VP, _I32, _VP, _VP, ctypes.c_int64, ctypes.c_int64, _VP, _VP, _VP,
+                           ctypes.c_int64, ctypes.c_int64, _VP, ctypes.c_int64, ctypes.c_int64,
+                           _VP], ctypes.c_int),
+    "gdn_rope_create": ([_VP, _I32, ctypes.POINTER(_VP)], ctypes.c_int),
+    "gdn_rope_destroy": ([_VP], ctypes.c_int),
+    "gdn_rope_forward": ([_VP, _I32, _VP, _VP, _VP, _I32, ctypes.c_float, _I32, _VP],
+                         ctypes.c_int),
     "gdn_layer_create": ([_VP, ctypes.POINTER(_VP)], ctypes.c_int),
     "gdn_layer_destroy": ([_VP], ctypes.c_int),
     "gdn_pool_reserve": ([_VP, _I32, _VP], ctypes.c_int),
@@ -170,6 +187,32 @@ class BlockNormDesc(ctypes.Structure):
     _fields_ = [("hidden", _I32), ("h_f32", _I32), ("gate", _I32), ("gate_sigmoid", _I32),
                 ("unit_offset", _I32), ("scale", ctypes.c_float), ("post_eps", ctypes.c_float),
                 ("pre_eps", ctypes.c_float)]
+
+
+class KV8Desc(ctypes.Structure):
+    _fields_ = [("num_layers", _I32), ("num_slots", _I32), ("num_pages", _I32),
+                ("max_pages_per_slot", _I32), ("num_q_heads", _I32), ("num_kv_heads", _I32),
+                ("head_dim", _I32), ("max_step_tokens", _I32), ("device", _I32)]
+
+
+class KV8View(ctypes.Structure):
+    _fields_ = [(x, _VP) for x in ("table", "owned", "free", "count", "cu", "pos", "map")]
+
+
+class KV8AttnDesc(ctypes.Structure):
+    _fields_ = [("scale", ctypes.c_float), ("softcap", ctypes.c_float), ("window", _I32)]
+
+
+class RopeDesc(ctypes.Structure):
+    _fields_ = [("head_dim", _I32), ("rotary_dim", _I32), ("interleaved", _I32),
+                ("scaling", _I32)] + [(x, ctypes.c_float) for x in
+                                      ("base", "factor", "original", "fast", "slow", "magnitude")]
+
+
+class RopeRows(ctypes.Structure):
+    _fields_ = [("src", _VP), ("out", _VP), ("heads", _I32), ("in_stride", ctypes.c_int64),
+                ("in_head_stride", ctypes.c_int64), ("out_stride", ctypes.c_int64),
+                ("out_head_stride", ctypes.c_int64), ("norm_w", _VP)]
 
 
 class PoolDesc(ctypes.Structure):
@@ -285,6 +328,22 @@ def _mat(t, dev: int, size, types, what: str):
     if cols != 1 and size[1] > 1:
         _refuse(t, dev, size, types, what)
     return t.data_ptr(), rows if size[0] != 1 else size[1]
+
+
+def _heads(t, dev: int, size, types, what: str):
+    """(pointer, token stride, head stride in elements) of a tensor [tokens, heads, dim] of
+    that size and type on device dev whose heads are contiguous. A single token's or head's
+    stride does not matter."""
+    if t.size() != size or t.get_device() != dev or t.dtype not in types:
+        _refuse(t, dev, size, types, what)
+    a, b, c = t.stride()
+    if c != 1 and size[2] > 1:
+        raise ValueError(f"{what} must have contiguous heads")
+    if size[1] == 1:
+        b = size[2]
+    if size[0] == 1:
+        a = size[1] * b
+    return t.data_ptr(), a, b
 
 
 def _dense(t, dev: int, size, types, what: str) -> int:
@@ -795,6 +854,180 @@ class KVCache:
             pass
 
 
+class KV8Cache:
+    """Paged KV cache in 8 bits (e4m3, an exponent per 64-token page and head), planned on
+    the GPU (gdn_kv8_*): step(...) fits the slots' pages to the request lengths, append(...)
+    puts a layer's new keys and values into them, attention(...) reads them. The lengths are
+    device tensors and nothing waits for the GPU, so a step can be captured in a graph."""
+
+    def __init__(self, num_layers: int, num_slots: int, num_pages: int, max_pages_per_slot: int,
+                 num_q_heads: int = 16, num_kv_heads: int = 2, head_dim: int = 256,
+                 max_step_tokens: int = 4096, device: int = 0):
+        self.lib = load()
+        self.handle = None
+        self.desc = KV8Desc(num_layers, num_slots, num_pages, max_pages_per_slot, num_q_heads,
+                            num_kv_heads, head_dim, max_step_tokens, device)
+        h = _VP()
+        _check(self.lib.gdn_kv8_create(ctypes.byref(self.desc), ctypes.byref(h)))
+        self.handle = h
+        self.Hq, self.Hkv, self.D, self.device = num_q_heads, num_kv_heads, head_dim, device
+        self.rows = self.tokens = 0
+
+    def step(self, slots, lens, ntok, max_tokens: int, max_row_tokens: int = 0, lens_out=None,
+             stream=None):
+        """Plan a step (gdn_kv8_step): row i's sequence slots[i] holds lens[i] tokens and
+        appends ntok[i] (int32 device tensors); max_tokens rows in the step's tensors, at most
+        max_row_tokens (0: max_tokens) for a sequence. lens_out receives the new lengths."""
+        dev = self.device
+        size = slots.size()
+        (n,) = size
+        sp, lp, np_ = (_dense(t, dev, size, _IS_I32, what) for t, what in
+                       ((slots, "slots"), (lens, "lens"), (ntok, "ntok")))
+        op = None if lens_out is None else _dense(lens_out, dev, size, _IS_I32, "lens_out")
+        tokens = int(max_tokens)
+        _check(self.lib.gdn_kv8_step(self.handle, n, sp, lp, np_, op, tokens, int(max_row_tokens),
+                                     _raw_stream(dev) if stream is None else stream.cuda_stream))
+        self.rows, self.tokens = n, tokens
+
+    def views(self) -> dict:
+        """Views of the tables: table [slots, pages], owned [slots], free [pages], count [1], and
+        of the last step's cu (rows + 1 entries hold), pos and map (its tokens' entries hold)."""
+        import torch
+        v, d = KV8View(), self.desc
+        _check(self.lib.gdn_kv8_views(self.handle, ctypes.byref(v)))
+        sizes = dict(table=d.num_slots * d.max_pages_per_slot, owned=d.num_slots, free=d.num_pages,
+                     count=1, cu=4097, pos=d.max_step_tokens, map=d.max_step_tokens)
+        out = {k: _wrap_device(getattr(v, k), n, torch.int32, self.device) for k, n in sizes.items()}
+        out["table"] = out["table"].view(d.num_slots, d.max_pages_per_slot)
+        return out
+
+    def check(self, stream=None) -> int:
+        """Flags (GDN_FLAG_*) of the steps since the last call; waits for the stream."""
+        f = ctypes.c_uint32()
+        _check(self.lib.gdn_kv8_check(self.handle, _raw_stream(self.device) if stream is None
+                                      else stream.cuda_stream, ctypes.byref(f)))
+        return f.value
+
+    def _kv_rows(self, t, rows, what):
+        if t.dim() == 2:  # heads side by side in a row
+            return _mat(t, self.device, (rows, self.Hkv * self.D), _IS_BF16, what)
+        p, a, b = _heads(t, self.device, (rows, self.Hkv, self.D), _IS_BF16, what)
+        if b != self.D:
+            raise ValueError(f"{what} must have its heads side by side")
+        return p, a
+
+    def append(self, layer: int, k, v, stream=None):
+        """The step's new keys and values [tokens, kv heads, dim] (or [tokens, heads * dim])
+        bf16 into the layer's pages (gdn_kv8_append)."""
+        kp, ks = self._kv_rows(k, self.tokens, "k")
+        vp, vs = self._kv_rows(v, self.tokens, "v")
+        _check(self.lib.gdn_kv8_append(self.handle, layer, kp, ks, vp, vs,
+                                       _raw_stream(self.device) if stream is None
+                                       else stream.cuda_stream))
+
+    def gather(self, layer: int, places, k_out=None, v_out=None, stream=None):
+        """The values held at places [m] int32 (page * 64 + position % 64) -> [m, kv heads, dim]
+        bf16 (gdn_kv8_gather); zeros for a place outside the cache."""
+        (m,) = places.size()
+        pp = _dense(places, self.device, (m,), _IS_I32, "places")
+        kp, ks = (None, 0) if k_out is None else self._kv_rows(k_out, m, "k_out")
+        vp, vs = (None, 0) if v_out is None else self._kv_rows(v_out, m, "v_out")
+        _check(self.lib.gdn_kv8_gather(self.handle, layer, m, pp, kp, ks, vp, vs,
+                                       _raw_stream(self.device) if stream is None
+                                       else stream.cuda_stream))
+
+    def attention(self, layer: int, q, out, scale: float = 0.0, softcap: float = 0.0,
+                  window: int = 0, slopes=None, prefix=None, gate=None, stream=None):
+        """Attention of the step's tokens over their sequences' keys (gdn_kv8_attention): q,
+        out and gate [tokens, query heads, dim] bf16 (heads or columns of wider tensors are
+        fine), slopes f32 [query heads], prefix int32 [rows]. scale 0: 1 / sqrt(dim)."""
+        dev = self.device
+        size = (self.tokens, self.Hq, self.D)
+        qp, qs, qh = _heads(q, dev, size, _IS_BF16, "q")
+        op, os_, oh = _heads(out, dev, size, _IS_BF16, "out")
+        gp, gs, gh = (None, 0, 0) if gate is None else _heads(gate, dev, size, _IS_BF16, "gate")
+        sp = None if slopes is None else _dense(slopes, dev, (self.Hq,), _IS_F32, "slopes")
+        pp = None if prefix is None else _dense(prefix, dev, (self.rows,), _IS_I32, "prefix")
+        d = KV8AttnDesc(float(scale), float(softcap), int(window))
+        _check(self.lib.gdn_kv8_attention(self.handle, layer, ctypes.byref(d), qp, qs, qh, sp, pp,
+                                          gp, gs, gh, op, os_, oh,
+                                          _raw_stream(dev) if stream is None
+                                          else stream.cuda_stream))
+
+    def close(self):
+        if getattr(self, "handle", None):
+            _check(self.lib.gdn_kv8_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
+class Rope:
+    """Rotary positions of heads (gdn_rope_*). scaling: "none", "linear" (factor), "yarn"
+    (factor, original, fast, slow: pairs between `fast` and `slow` turns in `original`
+    positions) or "bands" (the same arguments). magnitude 0: 1, with yarn 0.1 ln(factor) + 1."""
+
+    def __init__(self, head_dim: int, rotary_dim: int | None = None, base: float = 1.0e7,
+                 interleaved: bool = False, scaling: str = "none", factor: float = 1.0,
+                 original: float = 0.0, fast: float = 32.0, slow: float = 1.0,
+                 magnitude: float = 0.0, device: int = 0):
+        self.lib = load()
+        self.handle = None
+        codes = {"none": 0, "linear": 1, "yarn": 2, "bands": 3}
+        if scaling not in codes:
+            raise ValueError(f"scaling must be one of {', '.join(codes)}, not {scaling!r}")
+        d = RopeDesc(head_dim, head_dim if rotary_dim is None else rotary_dim,
+                     int(bool(interleaved)), codes[scaling], float(base), float(factor),
+                     float(original), float(fast), float(slow), float(magnitude))
+        h = _VP()
+        _check(self.lib.gdn_rope_create(ctypes.byref(d), device, ctypes.byref(h)))
+        self.handle = h
+        self.D, self.device = head_dim, device
+
+    def forward(self, pos, q, k=None, q_out=None, k_out=None, q_norm_w=None, k_norm_w=None,
+                eps: float = 1e-6, inverse: bool = False, stream=None):
+        """q [tokens, heads, dim] and k, bf16 or f32, at positions pos [tokens] int32 -> q_out,
+        k_out (None: in place); norm weights bf16 [dim] for the norms before the turn. A token
+        at a negative position is copied. inverse: turns back."""
+        dev = self.device
+        (T,) = pos.size()
+        pp = _dense(pos, dev, (T,), _IS_I32, "pos")
+        f32 = q.dtype in _IS_F32
+        types = _IS_F32 if f32 else _IS_BF16
+
+        def rows(x, out, w, what):
+            size = (T, x.size(1), self.D)
+            xp, xs, xh = _heads(x, dev, size, types, what)
+            op, os_, oh = (xp, xs, xh) if out is None else _heads(out, dev, size, types,
+                                                                  what + "_out")
+            wp = None if w is None else _dense(w, dev, (self.D,), _IS_BF16, what + "_norm_w")
+            return RopeRows(xp, op, size[1], xs, xh, os_, oh, wp)
+
+        if k is None and (k_out is not None or k_norm_w is not None):
+            raise ValueError("k_out and k_norm_w go with k")
+        qr = rows(q, q_out, q_norm_w, "q")
+        kr = None if k is None else ctypes.byref(rows(k, k_out, k_norm_w, "k"))
+        _check(self.lib.gdn_rope_forward(self.handle, T, pp, ctypes.byref(qr), kr, int(f32),
+                                         float(eps), int(bool(inverse)),
+                                         _raw_stream(dev) if stream is None
+                                         else stream.cuda_stream))
+
+    def close(self):
+        if getattr(self, "handle", None):
+            _check(self.lib.gdn_rope_destroy(self.handle))
+            self.handle = None
+
+    def __del__(self):
+        try:
+            self.close()
+        except Exception:
+            pass
+
+
 class Executor:
     """ModelExecutor (src/scheduler/executor.rs:21-49) over pool slots: the
     decoder stack h = embed[tok]; h += mixer_l(rms_norm(h, w_l)) per layer;
@@ -955,7 +1188,7 @@ def _wrap_device(ptr: int, numel: int, dtype, device: int):
     class _Holder:
         def __init__(self, p, n, nbytes):
             self.__cuda_array_interface__ = {
-                "shape": (n,), "typestr": {torch.float32: "<f4", torch.int16: "<i2"}[dtype],
+                "shape": (n,), "typestr": {torch.float32: "<f4", torch.int16: "<i2", torch.int32: "<i4"}[dtype],
                 "data": (p, False), "version": 3, "strides": None,
             }
     esz = torch.empty(0, dtype=dtype).element_size()
