@@ -468,6 +468,9 @@ struct BlockNormArgs {
 hipError_t launch_block_norm(const BlockNormArgs& a);
 
 // The 8-bit paged cache (gdn_kv8.hip, gdn_attn8.hip). Device state and the last step's plan.
+struct Kv8Row {
+  int32_t slot, pos, fresh, cu;  // tokens before the step and in it (0: none or refused), first token
+};
 struct Kv8Plan {
   int num_slots, num_pages, max_pages, Hq, Hkv, D;
   int n, T, max_row;            // of the step: rows, tokens, most tokens of a row
@@ -480,11 +483,20 @@ struct Kv8Plan {
   int32_t* cu;                  // [n + 1]
   int32_t* pos;                 // [T]
   int32_t* map;                 // [T]
-  int32_t* row_slot;            // [n] -1: no tokens
-  int32_t* row_pos;             // [n] tokens before the step
-  int32_t* row_new;             // [n] tokens of the step, 0 where refused
+  int32_t* tok_row;             // [T] row, -1: of a refused row, -2: behind the last token
+  Kv8Row* rows;                 // [n]
   int32_t* blocks;              // [n + 1] pages that the rows before touch
+  int32_t* parts;               // [n] attention's chunks (of a kv head) of the rows before, at most
 };
+// Attention of few new tokens (below kKv8TileTokens in a row): groups of 16 / G tokens, their
+// pages in chunks of kv8_chunk_pages, a partial result each. Rows of several groups take
+// longer chunks, so that a row has no more partials than a single token's and its groups.
+constexpr int kKv8TileTokens = 16;
+__host__ __device__ inline int kv8_chunk_pages(int groups) {
+  int c = 4;
+  for (int g = 1; g < groups; g *= 2) c *= 2;
+  return c;
+}
 constexpr int kKv8Rows = 4096;  // rows of a step
 struct Kv8StepArgs {
   Kv8Plan p;

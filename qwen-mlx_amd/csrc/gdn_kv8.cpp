@@ -139,8 +139,8 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) {
   const size_t heads = (size_t)2 * d.num_kv_heads * d.num_pages;
   const size_t table = (size_t)d.num_slots * d.max_pages_per_slot;
   const int R = gdn::kKv8Rows;
-  const size_t words = table + 2 * (size_t)d.num_slots + d.num_pages + 2 + 5 * (size_t)(R + 1) +
-                       2 * (size_t)d.max_step_tokens;
+  const size_t words = table + 2 * (size_t)d.num_slots + d.num_pages + 6 + 7 * (size_t)(R + 1) +
+                       3 * (size_t)d.max_step_tokens;
   const size_t ws = gdn::kv8_attn_workspace_bytes(d);
   bool ok = true;
   for (int l = 0; l < d.num_layers && ok; ++l) {
@@ -170,6 +170,7 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) {
       at += n;
       return r;
     };
+    p.rows = reinterpret_cast<gdn::Kv8Row*>(take(4 * (size_t)R));  // 16-byte aligned
     p.table = take(table);
     p.owned = take(d.num_slots);
     p.mark = take(d.num_slots);
@@ -177,12 +178,11 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) {
     p.free_count = take(1);
     p.status = reinterpret_cast<uint32_t*>(take(1));
     p.cu = take(R + 1);
-    p.row_slot = take(R + 1);
-    p.row_pos = take(R + 1);
-    p.row_new = take(R + 1);
     p.blocks = take(R + 1);
+    p.parts = take(R + 1);
     p.pos = take(d.max_step_tokens);
     p.map = take(d.max_step_tokens);
+    p.tok_row = take(d.max_step_tokens);
     std::vector<int32_t> init(d.num_pages);
     for (int i = 0; i < d.num_pages; ++i) init[i] = d.num_pages - 1 - i;  // pop lowest first
     const std::vector<int32_t> mark(d.num_slots, INT_MAX);

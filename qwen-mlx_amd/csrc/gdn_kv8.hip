@@ -6,9 +6,10 @@
 // 1 KiB in one piece:
 //   K (key kk, dim d): [kk/16][d/64][(d%64)/16][kk%16][d%16] -- a lane's 16 bytes are 16
 //       dims of a key: the A operand (16 keys, 32-deep k = dims) of two products
-//   V (key kk, dim d): [d/16][(kk/4)%4][d%16][kk/16][kk%4] -- a lane's 16 bytes are 16 keys
-//       of a dim, four of each 16-key group: the A operand (16 dims, 32-deep k = keys) of two
-//       products, keys in the order in which the score accumulators hold them
+//   V (key kk, dim d): [kk/32][d/16][(kk/4)%2][d%16][(kk/8)%2][(kk/16)%2][kk%4] -- a lane's 16
+//       bytes are 16 keys of a dim, every other four of 32: the A operand of two products (32
+//       dims, 16-deep k = keys), keys in the order in which the score accumulators hold them;
+//       with its halves exchanged between the wave's halves, of two of 16 dims, 32 keys deep
 // One exponent per page, K or V, and head: exps[page][2][Hkv], in the low 8 bits of a word.
 #include "gdn_common.h"
 
@@ -26,8 +27,9 @@ typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 __device__ __forceinline__ int k_byte(int kk, int d, int D) {
   return ((kk >> 4) * (D >> 6) + (d >> 6)) * 1024 + (((d >> 4) & 3) * 16 + (kk & 15)) * 16 + (d & 15);
 }
-__device__ __forceinline__ int v_byte(int kk, int d) {
-  return (d >> 4) * 1024 + (((kk >> 2) & 3) * 16 + (d & 15)) * 16 + (kk >> 4) * 4 + (kk & 3);
+__device__ __forceinline__ int v_byte(int kk, int d, int D) {
+  return (kk >> 5) * 32 * D + (d >> 4) * 512 + (((kk >> 2) & 1) * 16 + (d & 15)) * 16 +
+         ((kk >> 3) & 1) * 8 + ((kk >> 4) & 1) * 4 + (kk & 3);
 }
 
 // 2^e of a normal f32, e in [-126, 127]
@@ -103,7 +105,7 @@ __device__ __forceinline__ int block_scan(int v, int* red, int& total) {
 
 // Tokens t of the step, each its row by search in cu (LDS or memory).
 __device__ __forceinline__ void map_token(const Kv8Plan& p, const int32_t* cu, int t) {
-  int pos = -1, place = -1;
+  int pos = -1, place = -1, row = -2;
   if (t < cu[p.n]) {
     int lo = 0, hi = p.n;  // the row: cu[row] <= t < cu[row + 1]
     while (hi - lo > 1) {
@@ -113,14 +115,17 @@ __device__ __forceinline__ void map_token(const Kv8Plan& p, const int32_t* cu, i
       else
         hi = mid;
     }
-    const int slot = p.row_slot[lo];
-    if (slot >= 0) {
-      pos = p.row_pos[lo] + t - cu[lo];
-      place = p.table[(size_t)slot * p.max_pages + pos / kPage] * kPage + pos % kPage;
+    const Kv8Row r = p.rows[lo];
+    row = -1;
+    if (r.fresh > 0) {
+      row = lo;
+      pos = r.pos + t - r.cu;
+      place = p.table[(size_t)r.slot * p.max_pages + pos / kPage] * kPage + pos % kPage;
     }
   }
   p.pos[t] = pos;
   p.map[t] = place;
+  p.tok_row[t] = row;
 }
 
 constexpr int kMapHere = 8192;  // tokens that the plan's own work-group maps
@@ -240,28 +245,38 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     if (m > 0) atomicMax(&taken, before);  // admitted rows come before refused ones
     move(m, slot[i], have[i], 1, avail - 1 - b, -1, false);
   }
-  int nblk = 0;
+  // pages that the row's tokens fall into, and attention's chunks
+  const int tpg = 16 / (p.Hq / p.Hkv);
+  int touched[R], chunks[R], nblk = 0, nchunk = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = tid * R + i;
     const int tok = ok[i] ? fresh[i] : 0;
-    nblk += tok > 0 ? (len[i] + tok - 1) / kPage - len[i] / kPage + 1 : 0;
+    touched[i] = tok > 0 ? (len[i] + tok - 1) / kPage - len[i] / kPage + 1 : 0;
+    chunks[i] = 0;
+    if (tok > 0 && tok < kKv8TileTokens) {
+      const int groups = (tok + tpg - 1) / tpg, cp = kv8_chunk_pages(groups);
+      chunks[i] = groups * ((need[i] + cp - 1) / cp);
+    }
+    nblk += touched[i];
+    nchunk += chunks[i];
     if (r >= p.n) continue;
-    p.row_slot[r] = ok[i] ? slot[i] : -1;
-    p.row_pos[r] = len[i];
-    p.row_new[r] = tok;
+    p.rows[r] = Kv8Row{ok[i] ? slot[i] : -1, len[i], tok, cu[i]};
     if (ok[i]) p.owned[slot[i]] = need[i];
     if (lens_out) lens_out[r] = ok[i] ? len[i] + tok : len[i];
     if (slot[i] >= 0 && slot[i] < p.num_slots) p.mark[slot[i]] = INT32_MAX;
   }
+  int none;
+  int c1 = block_scan<TH>(nchunk, red, none);
   int b0 = block_scan<TH>(nblk, red, total);  // and orders the tables for the tokens
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = tid * R + i;
     if (r >= p.n) continue;
     p.blocks[r] = b0;
-    const int tok = ok[i] ? fresh[i] : 0;
-    b0 += tok > 0 ? (len[i] + tok - 1) / kPage - len[i] / kPage + 1 : 0;
+    p.parts[r] = c1;
+    b0 += touched[i];
+    c1 += chunks[i];
   }
   if (tid == 0) {
     p.blocks[p.n] = total;
@@ -314,7 +329,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   const int e = blockIdx.x;
   if (e >= p.blocks[p.n]) return;
   const int r = row_of(p.blocks, p.n, e);
-  const int slot = p.row_slot[r], len = p.row_pos[r], fresh = p.row_new[r];
+  const Kv8Row row = p.rows[r];
+  const int slot = row.slot, len = row.pos, fresh = row.fresh;
   const int blk = len / kPage + e - p.blocks[r];
   const int first = blk * kPage;
   const int old = max(len - first, 0);                  // tokens that are there
@@ -325,7 +341,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   const uint16_t* const src = isv ? a.v : a.k;
   const int64_t stride = isv ? a.vs : a.ks;
   // row of token `first` in the packed tensors
-  const int64_t row0 = (int64_t)p.cu[r] + first - len;
+  const int64_t row0 = (int64_t)row.cu + first - len;
   const int was = old ? a.exps[head] : 0;
 
   u32x4 x[kPer][4];
@@ -356,7 +372,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
       if (4 * g + k < old) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          const int at = isv ? v_byte(4 * g + k, 8 * c + d) : k_byte(4 * g + k, 8 * c + d, D);
+          const int at = isv ? v_byte(4 * g + k, 8 * c + d, D) : k_byte(4 * g + k, 8 * c + d, D);
           const uint32_t b = tile[at] & 0x7fu;
           nan |= b == 0x7fu;
           mo = max(mo, b == 0x7fu ? 0u : b);
@@ -406,7 +422,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
       if (4 * g + k < old) {
 #pragma unroll
         for (int d = 0; d < 8; ++d) {
-          const int at = isv ? v_byte(4 * g + k, 8 * c + d) : k_byte(4 * g + k, 8 * c + d, D);
+          const int at = isv ? v_byte(4 * g + k, 8 * c + d, D) : k_byte(4 * g + k, 8 * c + d, D);
           f[d] = e4m3_value(tile[at]) * again;
         }
       } else {
@@ -424,7 +440,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
         const int w = d >> 2, s = 8 * (d & 3);
-        *reinterpret_cast<uint32_t*>(tile + v_byte(4 * g, 8 * c + d)) =
+        *reinterpret_cast<uint32_t*>(tile + v_byte(4 * g, 8 * c + d, D)) =
             ((b[0][w] >> s) & 0xffu) | ((b[1][w] >> s) & 0xffu) << 8 |
             ((b[2][w] >> s) & 0xffu) << 16 | ((b[3][w] >> s) & 0xffu) << 24;
       }
@@ -480,7 +496,7 @@ __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8GatherArgs a, int64_
       float f[8];
       if (z) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = e4m3_value(tile[v_byte(kk, d + i)]) * s;
+        for (int i = 0; i < 8; ++i) f[i] = e4m3_value(tile[v_byte(kk, d + i, p.D)]) * s;
       } else {
         const u32x2 b = *reinterpret_cast<const u32x2*>(tile + k_byte(kk, d, p.D));
 #pragma unroll
