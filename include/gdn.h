@@ -924,9 +924,11 @@ typedef struct gdn_kv8_attn_desc {
  *
  * Products and sums are f32; the softmax's weights enter the product with the values in f16
  * (11 bits), and out is rounded once. The bits are the same every time and do not
- * depend on the step's other rows; they may differ between steps that cut a
- * sequence differently. A NaN among the keys that a token sees makes its head NaN,
- * one among the values their dimension; tokens that do not see it are not touched. */
+ * depend on what the step's other rows are; the kernel and the places where keys are
+ * split follow the row's tokens and the step's bounds (n, max_tokens), so that steps of
+ * other bounds may differ by rounding. A NaN among the keys or values of a kv head
+ * that a token sees makes its query heads there NaN; tokens that do not see it are
+ * not touched. */
 gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc* desc,
                              const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
                              const float* slopes, const int32_t* prefix, const uint16_t* gate,

@@ -4,9 +4,12 @@
 // over the visible j, with one pass over the keys and the running maximum and sum of
 // the softmax.
 //
-// Scores and P V run on MFMA. e4m3 numbers convert exactly into bf16 (for q . k with q as
-// it is) and into f16 (for P V: P in [0, 1] as f16 keeps 11 bits, three more than
-// bf16), both without their page's exponent: the keys' exponent multiplies the scores, the
+// Scores and P V run on MFMA. For q . k the keys go in as they are held, against q in two
+// e4m3 parts under a power of two of its head: a bf16 number's 8 significant bits are the 4 of
+// its rounding and the 4 that are left, times 16 (numbers below 2^-14 of the head's
+// largest lose bits, 2^-22 of it at most). For P V the values convert exactly into f16, and P,
+// in [0, 2^8] as the running maximum follows by steps of 2^8, is rounded to it: 11 bits, three
+// more than bf16. The pages' exponents stay outside: the keys' multiplies the scores, the
 // values' is the unit of the running outputs, which are rescaled where it changes.
 #include "gdn_common.h"
 
@@ -15,28 +18,22 @@ namespace gdn {
 namespace {
 
 constexpr int kPage = 64;
+constexpr int kBlock = 32;  // keys of a step of the running softmax: half a page
 constexpr int kNanFlag = 1 << 16;
+constexpr float kStep = 8.f;  // log2 steps of the running maximum
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
 
 __device__ __forceinline__ float pow2(int e) { return __uint_as_float((uint32_t)(e + 127) << 23); }
 
-// 8 e4m3 bytes to 8 bf16 / 8 f16 (both exact)
-__device__ __forceinline__ bf16x8 to_bf16(uint32_t a, uint32_t b) {
-  u32x4 r;
-  r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, false));
-  r[1] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(a, 1.0f, true));
-  r[2] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, false));
-  r[3] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_bf16_fp8(b, 1.0f, true));
-  return __builtin_bit_cast(bf16x8, r);
-}
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+
+// 8 e4m3 bytes to 8 f16 (exact)
 __device__ __forceinline__ f16x8 to_f16(uint32_t a, uint32_t b) {
   u32x4 r;
   r[0] = __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_scalef32_pk_f16_fp8(a, 1.0f, false));
@@ -47,6 +44,39 @@ __device__ __forceinline__ f16x8 to_f16(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t pk_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+}
+
+// Scores of 16 keys for 16 columns: K as held (a lane's NK 16-byte pieces of its key), q in
+// two parts (NK pieces of each in turn).
+template <int NK>
+__device__ __forceinline__ f32x4 scores16(const u32x4* k, const u32x4* q) {
+  f32x4 s = {0.f, 0.f, 0.f, 0.f};
+  if constexpr (NK >= 2) {
+    constexpr int kOne = 0x7f7f7f7f, kLow = 0x7b7b7b7b;  // 2^0 and 2^-4
+    auto both = [](u32x4 a, u32x4 b) {
+      return (i32x8){(int)a[0], (int)a[1], (int)a[2], (int)a[3],
+                     (int)b[0], (int)b[1], (int)b[2], (int)b[3]};
+    };
+#pragma unroll
+    for (int i = 0; i < NK; i += 2) {
+      const i32x8 kk = both(k[i], k[i + 1]);
+      s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, both(q[2 * i], q[2 * i + 2]), s, 0, 0,
+                                                           0, kOne, 0, kOne);
+      s = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(kk, both(q[2 * i + 1], q[2 * i + 3]), s, 0,
+                                                           0, 0, kOne, 0, kLow);
+    }
+  } else {
+    f32x4 lo = {0.f, 0.f, 0.f, 0.f};
+    auto word = [](uint32_t a, uint32_t b) { return (long)(((uint64_t)b << 32) | a); };
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      const long kk = word(k[0][2 * h], k[0][2 * h + 1]);
+      s = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(kk, word(q[0][2 * h], q[0][2 * h + 1]), s, 0, 0, 0);
+      lo = __builtin_amdgcn_mfma_f32_16x16x32_fp8_fp8(kk, word(q[1][2 * h], q[1][2 * h + 1]), lo, 0, 0, 0);
+    }
+    s += lo * 0.0625f;
+  }
+  return s;
 }
 
 // Maximum over the four lanes of a column (lane ^ 16, lane ^ 32, both).
@@ -88,12 +118,12 @@ struct Found {
   Kv8Row row;
 };
 
-// The row that item g lies in, where a row has items(r, row) of them, by the wave. `before`
-// and b0: items of the rows before row b0 (a multiple of 64).
+// The row that item g lies in, where a row has items(r, row) of them, by the wave.
 template <typename F>
-__device__ __forceinline__ Found find_row(const Kv8Plan& p, int g, int b0, int before, F items) {
+__device__ __forceinline__ Found find_row(const Kv8Plan& p, int g, F items) {
   const int lane = threadIdx.x & 63;
-  for (int b = b0; b < p.n; b += 64) {
+  int before = 0;
+  for (int b = 0; b < p.n; b += 64) {
     const int r = b + lane;
     const Kv8Row row = r < p.n ? p.rows[r] : Kv8Row{-1, 0, 0, 0};
     const int mine = row.fresh > 0 ? items(r, row) : 0;
@@ -129,14 +159,19 @@ __device__ __forceinline__ Span span_of(int p0, int p1, int window, int pf, int 
   return s;
 }
 
+// 1 / (1 + e^-x), off by some 2^-22 of itself
+__device__ __forceinline__ float sigmoid(float x) {
+  return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
+}
+
 // Four outputs of a head from dim on: times sigmoid(gate) where there is one, rounded once.
 __device__ __forceinline__ void store4(const Kv8AttnArgs& a, int64_t t, int h, int dim, float* o) {
   if (a.gate) {
     const u32x2 g = *reinterpret_cast<const u32x2*>(a.gate + t * a.gs + h * a.ghs + dim);
-    o[0] *= sigmoid_f32(bf_lo(g.x));
-    o[1] *= sigmoid_f32(bf_hi(g.x));
-    o[2] *= sigmoid_f32(bf_lo(g.y));
-    o[3] *= sigmoid_f32(bf_hi(g.y));
+    o[0] *= sigmoid(bf_lo(g.x));
+    o[1] *= sigmoid(bf_hi(g.x));
+    o[2] *= sigmoid(bf_lo(g.y));
+    o[3] *= sigmoid(bf_hi(g.y));
   }
   *reinterpret_cast<u32x2*>(a.out + t * a.os + h * a.ohs + dim) =
       (u32x2){f2bf2(o[0], o[1]), f2bf2(o[2], o[3])};
@@ -179,8 +214,55 @@ __device__ __forceinline__ Group group_of(const Kv8AttnArgs& a, const Kv8Row& ro
   return x;
 }
 
-// The running softmax of 16 columns: lane (g4, c) holds keys 16 kg + 4 g4 + r of a page for
-// column c, and dims 16 d + 4 g4 + r of its outputs in units of 2^unit.
+// A lane's NK pieces of 16 dims of its column's q (16 g4 + 64 i on) in two e4m3 parts, in turn;
+// returns the exponent of the column.
+template <int NK>
+__device__ __forceinline__ int q_parts(const uint16_t* q, bool valid, u32x4* out) {
+  u32x4 x[NK][2];
+  uint32_t mx = 0;
+#pragma unroll
+  for (int i = 0; i < NK; ++i)
+#pragma unroll
+    for (int b = 0; b < 2; ++b) {
+      x[i][b] = valid ? *reinterpret_cast<const u32x4*>(q + 64 * i + 8 * b) : (u32x4){0u, 0u, 0u, 0u};
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        const uint32_t lo = x[i][b][w] & 0x7fffu, hi = (x[i][b][w] >> 16) & 0x7fffu;
+        mx = max(mx, max(lo >= 0x7f80u ? 0u : lo, hi >= 0x7f80u ? 0u : hi));
+      }
+    }
+  // bf16 patterns are in the order of their sizes, and so are they as f32
+  const uint32_t bits = __float_as_uint(max_xor16_32(__uint_as_float(mx << 16)));
+  // the least e with the largest <= 448 * 2^e (448 = 1.75 * 2^8)
+  const int e = max((int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -100);
+  const float inv = pow2(-e);
+#pragma unroll
+  for (int i = 0; i < NK; ++i) {
+    u32x4 hi, lo;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {  // 4 dims a word
+      const uint32_t a = x[i][w >> 1][2 * (w & 1)], b = x[i][w >> 1][2 * (w & 1) + 1];
+      const float f[4] = {bf_lo(a) * inv, bf_hi(a) * inv, bf_lo(b) * inv, bf_hi(b) * inv};
+      int h = __builtin_amdgcn_cvt_pk_fp8_f32(f[0], f[1], 0, false);
+      h = __builtin_amdgcn_cvt_pk_fp8_f32(f[2], f[3], h, true);
+      const float r[4] = {(f[0] - __builtin_amdgcn_cvt_f32_fp8(h, 0)) * 16.f,
+                          (f[1] - __builtin_amdgcn_cvt_f32_fp8(h, 1)) * 16.f,
+                          (f[2] - __builtin_amdgcn_cvt_f32_fp8(h, 2)) * 16.f,
+                          (f[3] - __builtin_amdgcn_cvt_f32_fp8(h, 3)) * 16.f};
+      int l = __builtin_amdgcn_cvt_pk_fp8_f32(r[0], r[1], 0, false);
+      l = __builtin_amdgcn_cvt_pk_fp8_f32(r[2], r[3], l, true);
+      hi[w] = (uint32_t)h;
+      lo[w] = (uint32_t)l;
+    }
+    out[2 * i] = hi;
+    out[2 * i + 1] = lo;
+  }
+  return e;
+}
+
+// The running softmax of 16 columns over blocks of 32 keys: lane (g4, c) holds keys 4 g4 + r and
+// 16 + 4 g4 + r of a block for column c, and dims 16 d + 4 g4 + r of its outputs in units of
+// 2^unit.
 template <int D>
 struct Online {
   float m, l;
@@ -195,40 +277,44 @@ struct Online {
     for (int d = 0; d < D / 16; ++d) O[d] = (f32x4){0.f, 0.f, 0.f, 0.f};
   }
 
-  // Scores S of the page at key0 to weights P; ek, ev: the exponents of its keys and values
-  __device__ __forceinline__ void weights(const f32x4* S, const Score& sc, const Group& x, int key0,
-                                          int ek, int ev, u32x4* P, uint32_t& seen) {
+  // Scores S of the block at key0 to weights P; e: the exponent of its keys and q, ev: of its values
+  __device__ __forceinline__ u32x4 weights(const f32x4* S, const Score& sc, const Group& x, int key0,
+                                           int e, int ev, uint32_t& seen) {
     const int g4 = (threadIdx.x & 63) >> 4;
-    float s[16], bm = -INFINITY;
-    const float mul = sc.mul * pow2(ek);
+    float s[8];
+    const float mul = __builtin_amdgcn_ldexpf(sc.mul, e);
 #pragma unroll
-    for (int i = 0; i < 16; ++i) s[i] = S[i >> 2][i & 3] * mul;
-    if (sc.cap > 0.f) {
+    for (int i = 0; i < 8; ++i) s[i] = S[i >> 2][i & 3] * mul;
+    if (__builtin_expect(sc.cap > 0.f, 0)) {
+      asm volatile("");  // a branch: the caps are many instructions
 #pragma unroll
-      for (int i = 0; i < 16; ++i) s[i] = capped(s[i], sc.cap);
+      for (int i = 0; i < 8; ++i) s[i] = capped(s[i], sc.cap);
     }
-    if (sc.sloped) {
+    if (__builtin_expect(sc.sloped, 0)) {
+      asm volatile("");
 #pragma unroll
-      for (int i = 0; i < 16; ++i)
+      for (int i = 0; i < 8; ++i)
         s[i] = fmaf(-sc.slope, (float)(x.cpos - (key0 + 16 * (i >> 2) + 4 * g4 + (i & 3))), s[i]);
     }
-    seen = 0xffffu;
-    // wave-uniform: every token of the group sees every key of the page
-    const bool all = (key0 + kPage - 1 <= x.pos0 && key0 > x.pos0 + x.nt - 1 - sc.window) ||
-                     key0 + kPage <= x.pf;
-    if (!all) {
+    seen = 0xffu;
+    // wave-uniform: every token of the group sees every key of the block
+    const bool all = (key0 + kBlock - 1 <= x.pos0 && key0 > x.pos0 + x.nt - 1 - sc.window) ||
+                     key0 + kBlock <= x.pf;
+    if (__builtin_expect(!all, 0)) {
+      asm volatile("");
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
+      for (int i = 0; i < 8; ++i) {
         const int key = key0 + 16 * (i >> 2) + 4 * g4 + (i & 3);
         const bool see = (key <= x.cpos && key > x.lo) || (key < x.pf && x.valid);
         s[i] = see ? s[i] : -INFINITY;
         seen &= ~((see ? 0u : 1u) << i);
       }
     }
-#pragma unroll
-    for (int i = 0; i < 16; ++i) bm = fmaxf(bm, s[i]);
+    float bm = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
+                     fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     bm = max_xor16_32(bm);
-    if (__any(bm > m) || ev != unit) {
+    // m follows the maximum once it is passed by 2^kStep: weights are at most that
+    if (__builtin_expect(__any(bm > m + kStep) || ev != unit, 0)) {
       const float mn = fmaxf(m, bm);
       float corr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;  // m = -inf: 0
       m = mn;
@@ -240,42 +326,56 @@ struct Online {
     }
     const float mref = m == -INFINITY ? 0.f : m;
 #pragma unroll
-    for (int kg = 0; kg < 4; ++kg) {
-      float e[4];
-#pragma unroll
-      for (int r = 0; r < 4; ++r) e[r] = __builtin_amdgcn_exp2f(s[4 * kg + r] - mref);
-      l += (e[0] + e[1]) + (e[2] + e[3]);
-      P[kg >> 1][(kg & 1) * 2] = pk_f16(e[0], e[1]);
-      P[kg >> 1][(kg & 1) * 2 + 1] = pk_f16(e[2], e[3]);
-    }
+    for (int i = 0; i < 8; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - mref);
+    l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    return (u32x4){pk_f16(s[0], s[1]), pk_f16(s[2], s[3]), pk_f16(s[4], s[5]), pk_f16(s[6], s[7])};
   }
 
-  // O[d] += the operand's 16 dims x 32 keys (half p of the page) . P
-  __device__ __forceinline__ void values(int d, u32x2 v, u32x4 P, const Group& x, int key0, int p,
-                                         bool has_nan, uint32_t seen) {
-    const int g4 = (threadIdx.x & 63) >> 4;
-    if (key0 + kPage > x.total) {  // keys past the row's end may hold anything
-      const int n = x.total - (key0 + 32 * p + 4 * g4);
-      v.x = first_keys(v.x, n);
-      v.y = first_keys(v.y, n - 16);
-    }
-    f16x8 f = to_f16(v.x, v.y);
-    if (has_nan) {
-      // NaN values reach the columns that see their keys, and no others: they leave the
-      // product, and another one counts them
-      f16x8 bad, eye;
+  // O += the block's values (raw bytes v, as loaded) . P. `total`: the row's keys.
+  __device__ __forceinline__ void values(u32x4* v, u32x4 P, int key0, int total, bool has_nan,
+                                         uint32_t seen) {
+    if (__builtin_expect(key0 + kBlock > total, 0)) {  // keys past the row's end may hold anything
+      const int g4 = (threadIdx.x & 63) >> 4;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        bad[i] = f[i] == f[i] ? (_Float16)0.f : (_Float16)1.f;
-        f[i] = f[i] == f[i] ? f[i] : (_Float16)0.f;
-        eye[i] = (seen >> (8 * p + i)) & 1u ? (_Float16)1.f : (_Float16)0.f;
+      for (int w = 0; w < 4; ++w) {
+        const int n = total - key0 - 4 * ((g4 & 1) + 2 * (w >> 1) + 4 * (w & 1));
+#pragma unroll
+        for (int i = 0; i < D / 32; ++i) v[i][w] = first_keys(v[i][w], n);
       }
-      const f32x4 cnt = __builtin_amdgcn_mfma_f32_16x16x32_f16(bad, eye, (f32x4){0.f, 0.f, 0.f, 0.f},
-                                                               0, 0, 0);
-#pragma unroll
-      for (int r = 0; r < 4; ++r) O[d][r] = cnt[r] > 0.f ? __builtin_nanf("") : O[d][r];
     }
-    O[d] = __builtin_amdgcn_mfma_f32_16x16x32_f16(f, __builtin_bit_cast(f16x8, P), O[d], 0, 0, 0);
+    if (__builtin_expect(has_nan, 0)) {
+      // NaN values leave the product; a column that sees one of their keys gets a NaN sum
+      u32x4 keys = {0u, 0u, 0u, 0u};  // top bits of the bytes of keys with a NaN in the lane's dims
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i)
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t top = ((v[i][w] & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+          v[i][w] &= ~((top >> 7) * 0xffu);
+          keys[w] |= top;
+        }
+      const int g4 = (threadIdx.x & 63) >> 4;
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+#pragma unroll
+        for (int off = 1; off < 16; off <<= 1) keys[w] |= __shfl_xor(keys[w], off, 64);
+        keys[w] |= __shfl_xor(keys[w], 32, 64);  // the other 16 dims, same keys
+      }
+      const uint32_t k0 = g4 & 2 ? keys[2] : keys[0], k1 = g4 & 2 ? keys[3] : keys[1];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+        if (((seen >> i) & 1u & (k0 >> (8 * i + 7))) | ((seen >> (4 + i)) & 1u & (k1 >> (8 * i + 7))))
+          l = __builtin_nanf("");
+    }
+    const f16x8 ph = __builtin_bit_cast(f16x8, P);
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) {
+      u32x2 va, vb;
+      v_operands(v[i], va, vb);
+      O[2 * i] = __builtin_amdgcn_mfma_f32_16x16x32_f16(to_f16(va.x, va.y), ph, O[2 * i], 0, 0, 0);
+      O[2 * i + 1] =
+          __builtin_amdgcn_mfma_f32_16x16x32_f16(to_f16(vb.x, vb.y), ph, O[2 * i + 1], 0, 0, 0);
+    }
   }
 
   __device__ __forceinline__ float sum() const {
@@ -302,7 +402,6 @@ __device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& 
   Chunks c{0, 1, 0};
   if (row.fresh <= 0 || row.fresh >= kKv8TileTokens) return c;
   c.groups = (row.fresh + tpg - 1) / tpg;
-  c.cp = kv8_chunk_pages(c.groups);
   const int total = row.pos + row.fresh;
   const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
   // the first and the last group's pages; one between them may see a page more where the
@@ -313,95 +412,136 @@ __device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& 
     most = max(most, span_of(p0, min(p0 + tpg, total) - 1, a.window, pf, total).count());
   }
   most = min(most + (c.groups > 1 && a.window > 0 ? 1 : 0), (total + kPage - 1) / kPage);
+  // whole pages for each of a chunk's waves
+  const int waves = kv8_chunk_waves(a.p.n, a.p.Hkv);
+  const int cp = (most - 1) / kv8_chunks(a.p.n, a.p.Hkv, a.p.D, c.groups) + 1;
+  c.cp = (cp + waves - 1) / waves * waves;
   c.nch = (most + c.cp - 1) / c.cp;
   return c;
 }
 
 }  // namespace
 
-// One wave per work-group; worker w of P takes the chunks [w k, (w + 1) k) of all rows' items,
-// k = ceil(items / P), each chunk its own partial: a token's result depends on its own row
-// alone. The next page's keys are loaded as soon as this page's scores are formed, its
-// values after this page's products, across chunks of a segment.
-template <int D>
-__global__ __launch_bounds__(64, D == 256 ? 1 : 2) void attn8_chunk_kernel(Kv8AttnArgs a, float* __restrict__ part) {
+// Work-group g takes the chunks g, g + grid, ... of all rows' items; its W waves every W-th page
+// of a chunk each, and they join in LDS: one partial a chunk. A wave loads the next page's
+// keys as soon as this page's scores are formed, its values after this page's products: 32
+// KiB in flight for each of the two waves of a SIMD (at D = 256).
+template <int D, int W>
+__global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(Kv8AttnArgs a, float* __restrict__ part) {
   constexpr int NK = D / 64, DB = D / 16;
   __shared__ u32x4 qlds[2 * NK][64];
-  __shared__ int before[kKv8Rows / 64];
+  __shared__ f32x4 os[W > 1 ? W : 1][W > 1 ? 16 : 1][D / 4];  // each wave's outputs: column, dims
+  __shared__ float ms[W][16], ls[W][16];
   const Kv8Plan& p = a.p;
-  const int lane = threadIdx.x, g4 = lane >> 4, c = lane & 15;
+  const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, c = lane & 15;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, tpg = 16 / G;
   auto items = [&](int r, const Kv8Row& row) {
     const Chunks k = chunks_of(a, row, r, tpg);
     return k.groups * k.nch * p.Hkv;
   };
-  int all = 0;
-  for (int b = 0; b < p.n; b += 64) {
-    const int r = b + lane;
-    int mine = 0;
-    if (r < p.n) mine = items(r, p.rows[r]);
-    if (lane == 0) before[b >> 6] = all;
-    all += __builtin_amdgcn_readlane(wave_scan(mine), 63);
-  }
-  const int k = (all + gridDim.x - 1) / gridDim.x;
-  int g = blockIdx.x * k;
-  const int gend = min(all, g + k);
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront", "local");
-  __builtin_amdgcn_wave_barrier();
-  while (g < gend) {
-    int b = 0;
-    while (b + 64 < p.n && before[(b >> 6) + 1] <= g) b += 64;
-    const Found f = find_row(p, g, b, before[b >> 6], items);
+  for (int g = blockIdx.x;; g += gridDim.x) {
+    const Found f = find_row(p, g, items);
+    if (f.r < 0) break;
     const Chunks ch = chunks_of(a, f.row, f.r, tpg);
-    const int local = g - f.first, seg = local / ch.nch, c0 = local - seg * ch.nch;
+    const int local = g - f.first, seg = local / ch.nch, chunk = local - seg * ch.nch;
     const int grp = seg / p.Hkv, j = seg - grp * p.Hkv;
-    const int nc = min(gend - g, ch.nch - c0);  // chunks of this segment
-    g += nc;
     const Group x = group_of(a, f.row, f.r, grp, j, G, tpg, c);
     const Score sc = score_of(a, x);
-    const int count = x.span.count();
-    const int v1 = min((c0 + nc) * ch.cp, count);
-    float* const out = part + ((size_t)p.parts[f.r] * p.Hkv + (size_t)seg * ch.nch) * (16 * (D + 4));
+    const int v1 = min((chunk + 1) * ch.cp, x.span.count());
+    if (W > 1 && g != (int)blockIdx.x) __syncthreads();  // the chunk before is written out
+    int eq;  // every wave forms q: its exponent is in registers
     {
-      const uint16_t* const q = a.q + x.t * a.qs + x.h * a.qhs + 16 * g4;
+      u32x4 q[2 * NK];
+      eq = q_parts<NK>(a.q + x.t * a.qs + x.h * a.qhs + 16 * g4, x.valid, q);
+      if (w == 0) {
 #pragma unroll
-      for (int i = 0; i < 2 * NK; ++i)
-        qlds[i][lane] = x.valid ? *reinterpret_cast<const u32x4*>(q + 64 * (i >> 1) + 8 * (i & 1))
-                                : (u32x4){0u, 0u, 0u, 0u};
+        for (int i = 0; i < 2 * NK; ++i) qlds[i][lane] = q[i];
+      }
     }
     const int32_t* const trow = p.table + (size_t)f.row.slot * p.max_pages;
-    // ids and exponents of 64 pages, one a lane
-    int vbase = 0, pid = 0, eks = 0, evs = 0;
+    // ids and exponents of 64 of the chunk's pages, one a lane
+    int vbase = chunk * ch.cp, pid = 0, eks = 0, evs = 0;
     auto ids = [&](int v) {
       vbase = v;
       pid = v + lane < v1 ? trow[x.span.page(v + lane)] : 0;
       const int32_t* const e = a.exps + (size_t)pid * 2 * p.Hkv + j;
       eks = e[0];
       evs = e[p.Hkv];
+      // waited for here: a wait behind the branch that reloads them would be one for every
+      // page load in flight, taken or not
+      asm volatile("" ::"v"(pid), "v"(eks), "v"(evs));
     };
-    const uint8_t* const base = a.pages + (size_t)j * (kPage * D) + lane * 16;
+    const uint8_t* const base = a.pages + (size_t)j * (kPage * D);
     const size_t page_bytes = (size_t)2 * p.Hkv * kPage * D, v_shift = (size_t)p.Hkv * kPage * D;
-    u32x4 kf[4 * NK], vf[DB];
+    // a page's halves of 32 keys, 32 * D contiguous bytes each of K and V
+    u32x4 kf[2][2 * NK], vf[2][DB / 2];
     auto page_of = [&](int v) {
       return base + (size_t)(uint32_t)__builtin_amdgcn_readlane(pid, v - vbase) * page_bytes;
     };
-    auto load_k = [&](const uint8_t* s) {
+    auto load = [&](const uint8_t* s, u32x4(&f)[DB / 2]) {
 #pragma unroll
-      for (int i = 0; i < 4 * NK; ++i)
-        kf[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(s) + i * 64);
+      for (int i = 0; i < DB / 2; ++i)
+        f[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(s) + i * 64 + lane);
     };
-    auto load_v = [&](const uint8_t* s) {
-#pragma unroll
-      for (int i = 0; i < DB; ++i)
-        vf[i] = __builtin_nontemporal_load(reinterpret_cast<const u32x4*>(s + v_shift) + i * 64);
-    };
+    constexpr int kHalf = kBlock * D;
     Online<D> on;
     on.clear();
-    auto flush = [&](int chunk) {
-      const float l = on.sum();
+    ids(vbase);
+    int v = vbase + w;
+    if (v < v1) {
+      const uint8_t* const cur = page_of(v);
+      load(cur, kf[0]);
+      load(cur + v_shift, vf[0]);
+      load(cur + kHalf, kf[1]);
+      load(cur + v_shift + kHalf, vf[1]);
+    }
+    lds_barrier();  // q
+    // page v, with the loads of the wave's next one behind its products; the last page (a call
+    // of its own) has none to issue: loads under a branch would be waited for as a whole
+    auto page = [&](auto lastc) {
+      constexpr bool last = decltype(lastc)::value;
+      const int key0 = x.span.page(v) * kPage;
+      const int ek = (int)(int8_t)__builtin_amdgcn_readlane(eks, v - vbase);
+      const int wv = __builtin_amdgcn_readlane(evs, v - vbase), ev = (int)(int8_t)wv;
+      const uint8_t* nxt = nullptr;
+      if constexpr (!last) {
+        if (v + W - vbase >= 64) ids(v + W);
+        nxt = page_of(v + W);
+      }
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        asm volatile("" ::: "memory");  // q is re-read from LDS for every block
+        f32x4 S[2];
+        {
+          u32x4 q[2 * NK];
+#pragma unroll
+          for (int i = 0; i < 2 * NK; ++i) q[i] = qlds[i][lane];
+          S[0] = scores16<NK>(kf[h], q);
+          S[1] = scores16<NK>(kf[h] + NK, q);
+        }
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!last) load(nxt + h * kHalf, kf[h]);
+        __builtin_amdgcn_sched_barrier(0);
+        uint32_t seen;
+        const u32x4 P = on.weights(S, sc, x, key0 + kBlock * h, eq + ek, ev, seen);
+        on.values(vf[h], P, key0 + kBlock * h, x.total, (wv & kNanFlag) != 0, seen);
+        __builtin_amdgcn_sched_barrier(0);
+        if constexpr (!last) load(nxt + v_shift + h * kHalf, vf[h]);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+    };
+    if (v < v1) {
+      for (; v + W < v1; v += W) page(std::false_type{});
+      page(std::true_type{});
+    }
+    float* const out = part + (((size_t)p.parts[f.r] * p.Hkv + (size_t)seg * ch.nch + chunk) * 16) *
+                                  (D + 4);
+    const float lw = on.sum();
+    if constexpr (W == 1) {
+      if (!x.valid) continue;
       if (ch.nch == 1) {
-        if (!x.valid) return;
-        const float inv = __builtin_amdgcn_ldexpf(1.0f / l, on.unit);
+        const float inv = __builtin_amdgcn_ldexpf(1.0f / lw, on.unit);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           float o[4];
@@ -409,83 +549,70 @@ __global__ __launch_bounds__(64, D == 256 ? 1 : 2) void attn8_chunk_kernel(Kv8At
           for (int r = 0; r < 4; ++r) o[r] = on.O[d][r] * inv;
           store4(a, x.t, x.h, 16 * d + 4 * g4, o);
         }
-      } else if (x.valid) {
-        float* const pr = out + ((size_t)chunk * 16 + c) * (D + 4);
+      } else {
+        float* const pr = out + c * (D + 4);
         if (g4 == 0) {
           pr[0] = on.m;
-          pr[1] = l;
+          pr[1] = lw;
         }
         const float one = __builtin_amdgcn_ldexpf(1.0f, on.unit);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
           *reinterpret_cast<f32x4*>(pr + 4 + 16 * d + 4 * g4) = on.O[d] * one;
       }
-      on.clear();
-    };
-    int v = c0 * ch.cp;
-    if (v < v1) {
-      ids(v);
-      const uint8_t* cur = page_of(v);
-      load_k(cur);
-      load_v(cur);
+      continue;
     }
-    for (int chunk = c0; chunk < c0 + nc; ++chunk) {
-      const int vend = min((chunk + 1) * ch.cp, v1);
-      for (; v < vend; ++v) {
-        const int key0 = x.span.page(v) * kPage;
-        const int ek = (int)(int8_t)__builtin_amdgcn_readlane(eks, v - vbase);
-        const int wv = __builtin_amdgcn_readlane(evs, v - vbase), ev = (int)(int8_t)wv;
-        if (v + 1 < v1 && v + 1 - vbase >= 64) ids(v + 1);
-        const uint8_t* const nxt = page_of(min(v + 1, v1 - 1));
-        f32x4 S[4];
+    // the waves' results under their common maximum
+    if (g4 == 0) ms[w][c] = on.m;
+    lds_barrier();
+    float M = ms[0][c];
 #pragma unroll
-        for (int kg = 0; kg < 4; ++kg) S[kg] = (f32x4){0.f, 0.f, 0.f, 0.f};
-        asm volatile("" ::: "memory");  // q is re-read from LDS for every page
+    for (int i = 1; i < W; ++i) M = fmaxf(M, ms[i][c]);
+    const float fac = on.m == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : exp2f(on.m - M);
+    if (g4 == 0) ls[w][c] = lw * fac;
+    const float fo = __builtin_amdgcn_ldexpf(fac, on.unit);
+    if (x.valid) {
 #pragma unroll
-        for (int i = 0; i < NK; ++i) {
-          const bf16x8 q0 = __builtin_bit_cast(bf16x8, qlds[2 * i][lane]);
-          const bf16x8 q1 = __builtin_bit_cast(bf16x8, qlds[2 * i + 1][lane]);
+      for (int d = 0; d < DB; ++d) os[w][c][4 * d + g4] = on.O[d] * fo;
+    }
+    lds_barrier();
+    const int cols = x.nt * G;
+    for (int i = tid; i < cols * (D / 4); i += 64 * W) {
+      const int col = i / (D / 4), d = i - col * (D / 4);
+      float l = ls[0][col], m = ms[0][col];
+      f32x4 o = os[0][col][d];
 #pragma unroll
-          for (int kg = 0; kg < 4; ++kg) {
-            const u32x4 kr = kf[kg * NK + i];
-            S[kg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(kr[0], kr[1]), q0, S[kg], 0, 0, 0);
-            S[kg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(to_bf16(kr[2], kr[3]), q1, S[kg], 0, 0, 0);
-          }
-        }
-        __builtin_amdgcn_sched_barrier(0);
-        if (v + 1 < v1) load_k(nxt);
-        __builtin_amdgcn_sched_barrier(0);
-        u32x4 P[2];
-        uint32_t seen;
-        on.weights(S, sc, x, key0, ek, ev, P, seen);
-        const bool has_nan = (wv & kNanFlag) != 0;
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int i = 0; i < DB / 2; ++i) {
-            u32x2 va, vb;
-            v_operands(vf[h * (DB / 2) + i], va, vb);
-            on.values(2 * i, va, P[h], x, key0, h, has_nan, seen);
-            on.values(2 * i + 1, vb, P[h], x, key0, h, has_nan, seen);
-          }
-        __builtin_amdgcn_sched_barrier(0);
-        if (v + 1 < v1) load_v(nxt);
-        __builtin_amdgcn_sched_barrier(0);
+      for (int k = 1; k < W; ++k) {
+        l += ls[k][col];
+        m = fmaxf(m, ms[k][col]);
+        o += os[k][col][d];
       }
-      flush(chunk);
+      if (ch.nch == 1) {
+        o *= 1.0f / l;
+        const int tok = col / G;
+        float of[4] = {o[0], o[1], o[2], o[3]};
+        store4(a, (int64_t)f.row.cu + grp * tpg + tok, j * G + col - tok * G, 4 * d, of);
+      } else {
+        float* const pr = out + (size_t)col * (D + 4);
+        *reinterpret_cast<f32x4*>(pr + 4 + 4 * d) = o;
+        if (d == 0) {
+          pr[0] = m;
+          pr[1] = l;
+        }
+      }
     }
   }
 }
 
-// grid (T, Hq), block 256: the chunks of a token's head, each wave every fourth one, then the
-// waves' sums in order. Also the zeros of refused rows' tokens. Tokens of tiles and of single
-// chunks are written already.
-template <int D>
-__global__ __launch_bounds__(256) void attn8_combine_kernel(Kv8AttnArgs a,
-                                                            const float* __restrict__ part) {
-  constexpr int DPL = D / 64;
+// grid (T, Hq), block 64 W: a token's chunks, chunk i in sum i % 16, wave w the sums w, w + W,
+// ..; then the sums in order, so that W changes no bits. Also the zeros of refused rows'
+// tokens. Tokens of tiles and of single chunks are written already.
+template <int D, int W>
+__global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
+                                                               const float* __restrict__ part) {
+  constexpr int DPL = D / 64, kPer = 16 / W;
   typedef float fvec __attribute__((ext_vector_type(DPL)));
-  __shared__ float sum[4][D];
+  __shared__ float sum[16][D];
   const Kv8Plan& p = a.p;
   const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -504,39 +631,57 @@ __global__ __launch_bounds__(256) void attn8_combine_kernel(Kv8AttnArgs a,
   const float* const pc = part + (((size_t)p.parts[r] * p.Hkv + (size_t)(grp * p.Hkv + j) * ch.nch) *
                                       16 + c) * (D + 4);
   constexpr size_t kStride = (size_t)16 * (D + 4);
-  float M = -INFINITY;
-  for (int i = lane; i < ch.nch; i += 64) M = fmaxf(M, pc[i * kStride]);
+  const int n = min(64, ch.nch);
+  fvec v[kPer];
+  auto rows = [&](int i0) {  // the wave's chunks of i0 .. i0 + 15
+#pragma unroll
+    for (int i = 0; i < kPer; ++i)
+      v[i] = *reinterpret_cast<const fvec*>(pc + min(i0 + wave + W * i, ch.nch - 1) * kStride + 4 +
+                                            DPL * lane);
+  };
+  rows(0);
+  // maxima and sums of 64 chunks, one a lane
+  float mi = lane < n ? pc[lane * kStride] : -INFINITY;
+  float li = lane < n ? pc[lane * kStride + 1] : 0.f;
+  float M = mi;
+  for (int i = lane + 64; i < ch.nch; i += 64) M = fmaxf(M, pc[i * kStride]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
   if (M == -INFINITY) M = 0.f;  // NaN scores alone
   float L = 0.f;
-  fvec A = (fvec)(0.f);
-  for (int i0 = 0; i0 < ch.nch; i0 += 64) {
-    const int n = min(64, ch.nch - i0);
-    const float* const ps = pc + (size_t)i0 * kStride;
-    const float w = lane < n ? exp2f(ps[lane * kStride] - M) : 0.f;
-    const float l = lane < n ? ps[lane * kStride + 1] : 0.f;
-    L += l != 0.f ? w * l : 0.f;
-    for (int i = wave; i < n; i += 4) {
-      const float wi = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(w), i));
-      const float li = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(l), i));
-      // a chunk without a visible key may hold anything
-      const fvec v = *reinterpret_cast<const fvec*>(ps + i * kStride + 4 + DPL * lane);
-      if (li != 0.f) A += v * wi;
+  fvec A[kPer];
+#pragma unroll
+  for (int i = 0; i < kPer; ++i) A[i] = (fvec)(0.f);
+  for (int b = 0; b < ch.nch; b += 64) {
+    if (b) {
+      mi = b + lane < ch.nch ? pc[(b + lane) * kStride] : -INFINITY;
+      li = b + lane < ch.nch ? pc[(b + lane) * kStride + 1] : 0.f;
+    }
+    const float wi = exp2f(mi - M);
+    L += li != 0.f ? wi * li : 0.f;
+    for (int i0 = b; i0 < min(b + 64, ch.nch); i0 += 16) {
+      if (i0) rows(i0);
+#pragma unroll
+      for (int i = 0; i < kPer; ++i) {
+        const int l = i0 - b + wave + W * i;
+        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), l));
+        const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(li), l));
+        if (s != 0.f) A[i] += v[i] * f;  // chunks without a visible key hold nothing
+      }
     }
   }
   L = wave_sum(L);
 #pragma unroll
-  for (int i = 0; i < DPL; ++i) sum[wave][DPL * lane + i] = A[i];
+  for (int i = 0; i < kPer; ++i)
+#pragma unroll
+    for (int d = 0; d < DPL; ++d) sum[wave + W * i][DPL * lane + d] = A[i][d];
   __syncthreads();
   if (tid < D / 4) {
     const float inv = 1.0f / L;
-    float o[4];
+    f32x4 s = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < 4; ++i) {
-      const int d = 4 * tid + i;
-      o[i] = ((sum[0][d] + sum[1][d]) + (sum[2][d] + sum[3][d])) * inv;
-    }
+    for (int i = 0; i < 16; ++i) s += *reinterpret_cast<const f32x4*>(&sum[i][4 * tid]);
+    float o[4] = {s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv};
     store4(a, t, h, 4 * tid, o);
   }
 }
@@ -550,18 +695,14 @@ __global__ __launch_bounds__(64) void attn8_rows_kernel(Kv8AttnArgs a) {
   const int lane = threadIdx.x, g4 = lane >> 4, c = lane & 15;
   const int G = p.Hq / p.Hkv, tpg = 16 / G, j = blockIdx.y;
   const int g = blockIdx.x;
-  const Found f = find_row(p, g, 0, 0, [&](int, const Kv8Row& row) {
+  const Found f = find_row(p, g, [&](int, const Kv8Row& row) {
     return row.fresh < kKv8TileTokens ? 0 : (row.fresh + tpg - 1) / tpg;
   });
   if (f.r < 0) return;
   const Group x = group_of(a, f.row, f.r, g - f.first, j, G, tpg, c);
   const Score sc = score_of(a, x);
   u32x4 q[2 * NK];
-#pragma unroll
-  for (int i = 0; i < 2 * NK; ++i)
-    q[i] = x.valid ? *reinterpret_cast<const u32x4*>(a.q + x.t * a.qs + x.h * a.qhs + 64 * (i >> 1) +
-                                                     16 * g4 + 8 * (i & 1))
-                   : (u32x4){0u, 0u, 0u, 0u};
+  const int eq = q_parts<NK>(a.q + x.t * a.qs + x.h * a.qhs + 16 * g4, x.valid, q);
   Online<D> on;
   on.clear();
   const int32_t* const trow = p.table + (size_t)f.row.slot * p.max_pages;
@@ -570,32 +711,24 @@ __global__ __launch_bounds__(64) void attn8_rows_kernel(Kv8AttnArgs a) {
     const size_t hk = ((size_t)trow[blk] * 2) * p.Hkv + j, hv = hk + p.Hkv;
     const u32x4* const kp = reinterpret_cast<const u32x4*>(a.pages + hk * (kPage * D)) + lane;
     const u32x4* const vp = reinterpret_cast<const u32x4*>(a.pages + hv * (kPage * D)) + lane;
-    const int wv = a.exps[hv];
-    f32x4 S[4];
+    const int ek = (int)(int8_t)a.exps[hk], wv = a.exps[hv];
 #pragma unroll
-    for (int kg = 0; kg < 4; ++kg) {
-      S[kg] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int h2 = 0; h2 < 2; ++h2) {
+      f32x4 S[2];
 #pragma unroll
-      for (int i = 0; i < NK; ++i) {
-        const u32x4 kr = kp[(kg * NK + i) * 64];
-        S[kg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            to_bf16(kr[0], kr[1]), __builtin_bit_cast(bf16x8, q[2 * i]), S[kg], 0, 0, 0);
-        S[kg] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(
-            to_bf16(kr[2], kr[3]), __builtin_bit_cast(bf16x8, q[2 * i + 1]), S[kg], 0, 0, 0);
+      for (int kg = 0; kg < 2; ++kg) {
+        u32x4 kr[NK];
+#pragma unroll
+        for (int i = 0; i < NK; ++i) kr[i] = kp[((2 * h2 + kg) * NK + i) * 64];
+        S[kg] = scores16<NK>(kr, q);
       }
+      u32x4 vr[DB / 2];
+#pragma unroll
+      for (int i = 0; i < DB / 2; ++i) vr[i] = vp[(h2 * (DB / 2) + i) * 64];
+      uint32_t seen;
+      const u32x4 P = on.weights(S, sc, x, key0 + kBlock * h2, eq + ek, (int)(int8_t)wv, seen);
+      on.values(vr, P, key0 + kBlock * h2, x.total, (wv & kNanFlag) != 0, seen);
     }
-    u32x4 P[2];
-    uint32_t seen;
-    on.weights(S, sc, x, key0, (int)(int8_t)a.exps[hk], (int)(int8_t)wv, P, seen);
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int i = 0; i < DB / 2; ++i) {
-        u32x2 va, vb;
-        v_operands(vp[(h * (DB / 2) + i) * 64], va, vb);
-        on.values(2 * i, va, P[h], x, key0, h, (wv & kNanFlag) != 0, seen);
-        on.values(2 * i + 1, vb, P[h], x, key0, h, (wv & kNanFlag) != 0, seen);
-      }
   }
   const float l = on.sum();
   if (!x.valid) return;
@@ -610,17 +743,12 @@ __global__ __launch_bounds__(64) void attn8_rows_kernel(Kv8AttnArgs a) {
 }
 
 size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
-  // chunks of a kv head over all rows of few tokens: a row has no more than its groups and one
-  // for every kv8_chunk_pages(1) of its pages, which are its own
+  // a group has kv8_chunks() partials for each kv head or less, which over all groups are
+  // kv8_waves() or one each
   const int64_t few = (int64_t)d.num_slots * (kKv8TileTokens - 1);
-  const int64_t chunks = (few < d.max_step_tokens ? few : d.max_step_tokens) +
-                         d.num_pages / kv8_chunk_pages(1) + 1;
-  return (size_t)chunks * d.num_kv_heads * 16 * (d.head_dim + 4) * sizeof(float);
+  const int64_t groups = few < d.max_step_tokens ? few : d.max_step_tokens;
+  return (size_t)(kv8_waves(d.head_dim) + groups * d.num_kv_heads) * 16 * (d.head_dim + 4) * sizeof(float);
 }
-
-// Waves that a step of few tokens in a row is split over: those that run side by side.
-template <int D>
-constexpr int kWorkers = D == 256 ? 1024 : 2048;
 
 template <int D>
 static hipError_t launch_attn8(const Kv8AttnArgs& a) {
@@ -633,9 +761,19 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
     hipLaunchKernelGGL(attn8_rows_kernel<D>, grid, dim3(64), 0, a.stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
-  hipLaunchKernelGGL(attn8_chunk_kernel<D>, dim3(kWorkers<D>), dim3(64), 0, a.stream, a, part);
+  // as many as the rows can have, up to four rounds of the chip's waves
+  const int W = kv8_chunk_waves(p.n, p.Hkv);
+  const int64_t most = kv8_waves(D) / W + (int64_t)p.Hkv * min(p.T, p.n * (kKv8TileTokens - 1));
+  const dim3 grid((unsigned)(most < 8192 / W ? most : 8192 / W));
+  if (W == 1)
+    hipLaunchKernelGGL((attn8_chunk_kernel<D, 1>), grid, dim3(64), 0, a.stream, a, part);
+  else
+    hipLaunchKernelGGL((attn8_chunk_kernel<D, 4>), grid, dim3(256), 0, a.stream, a, part);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  hipLaunchKernelGGL(attn8_combine_kernel<D>, dim3(p.T, p.Hq), dim3(256), 0, a.stream, a, part);
+  if (p.T * p.Hq <= 512)  // a wave for each sum where the work-groups are few
+    hipLaunchKernelGGL((attn8_combine_kernel<D, 16>), dim3(p.T, p.Hq), dim3(1024), 0, a.stream, a, part);
+  else
+    hipLaunchKernelGGL((attn8_combine_kernel<D, 4>), dim3(p.T, p.Hq), dim3(256), 0, a.stream, a, part);
   return hipGetLastError();
 }
 

@@ -488,14 +488,20 @@ struct Kv8Plan {
   int32_t* blocks;              // [n + 1] pages that the rows before touch
   int32_t* parts;               // [n] attention's chunks (of a kv head) of the rows before, at most
 };
-// Attention of few new tokens (below kKv8TileTokens in a row): groups of 16 / G tokens, their
-// pages in chunks of kv8_chunk_pages, a partial result each. Rows of several groups take
-// longer chunks, so that a row has no more partials than a single token's and its groups.
+// Attention of few new tokens (below kKv8TileTokens in a row): groups of 16 / G tokens, the pages
+// that a group sees in kv8_chunks() pieces or less, a partial result each, shared by `waves`
+// waves. By the step's bounds and the row alone: about kv8_waves() waves where every row has
+// enough pages, and four a piece where segments (rows x kv heads) are few.
 constexpr int kKv8TileTokens = 16;
-__host__ __device__ inline int kv8_chunk_pages(int groups) {
-  int c = 4;
-  for (int g = 1; g < groups; g *= 2) c *= 2;
-  return c;
+// those that run side by side: one a SIMD at D = 256 (512 registers), two at less
+__host__ __device__ constexpr int kv8_waves(int D) { return D == 256 ? 1024 : 2048; }
+constexpr int kKv8FewSegments = 32;
+__host__ __device__ inline int kv8_chunk_waves(int n, int Hkv) {
+  return n * Hkv <= kKv8FewSegments ? 4 : 1;
+}
+__host__ __device__ inline int kv8_chunks(int n, int Hkv, int D, int groups) {
+  const int c = kv8_waves(D) / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
+  return c < 1 ? 1 : c;
 }
 constexpr int kKv8Rows = 4096;  // rows of a step
 struct Kv8StepArgs {

@@ -255,8 +255,8 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     touched[i] = tok > 0 ? (len[i] + tok - 1) / kPage - len[i] / kPage + 1 : 0;
     chunks[i] = 0;
     if (tok > 0 && tok < kKv8TileTokens) {
-      const int groups = (tok + tpg - 1) / tpg, cp = kv8_chunk_pages(groups);
-      chunks[i] = groups * ((need[i] + cp - 1) / cp);
+      const int groups = (tok + tpg - 1) / tpg;
+      chunks[i] = groups * min(need[i], kv8_chunks(p.n, p.Hkv, p.D, groups));
     }
     nblk += touched[i];
     nchunk += chunks[i];

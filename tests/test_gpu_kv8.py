@@ -341,7 +341,7 @@ def test_nan_reaches_those_that_see_it(gpu):
     p.kv.attention(0, q, out)
     bad = torch.isnan(out)
     want = torch.zeros_like(bad)
-    want[70:, 2:, 7] = True   # head 1's queries that see the value, its dimension
+    want[70:, 2:] = True      # head 1's queries that see the value
     want[90:, :2] = True      # head 0's queries that see the key
     assert torch.equal(bad, want)
     clean_k, clean_v = k.clone(), v.clone()
@@ -356,7 +356,7 @@ def test_nan_reaches_those_that_see_it(gpu):
     p.kv.attention(0, q, out, window=5)
     bad = torch.isnan(out)
     want.zero_()
-    want[70:75, 2:, 7] = True
+    want[70:75, 2:] = True
     want[90:95, :2] = True
     assert torch.equal(bad, want)
     # the row is cut back before them: single tokens do not see what is left in the page
@@ -370,33 +370,46 @@ def test_nan_reaches_those_that_see_it(gpu):
 
 
 def test_rows_do_not_depend_on_each_other(gpu):
-    """A row's bits in a step with others and alone."""
+    """A row's bits beside rows of other lengths, contents and sizes, under the same bounds of
+    the step; and the same step twice."""
     import torch
     import gdn_amd
     rng = np.random.default_rng(14)
     hq, hk, d = 16, 2, 256
-    both, alone = (gdn_amd.KV8Cache(1, 8, 120, 40, hq, hk, d, 4096) for _ in range(2))
-    slots, lens = [6, 1, 3, 0], [1500, 40, 700, 0]
-    fill = [bf(rng, sum(lens), hk, d)[0] for _ in range(2)]
-    for kv in (both, alone):
-        kv.step(i32(slots), i32([0] * 4), i32(lens), sum(lens))
-        kv.append(0, *fill)
-    for ntok in ([1, 1, 1, 1], [5, 300, 1, 33]):
-        T = sum(ntok)
-        q, k, v = (bf(rng, T, h, d)[0] for h in (hq, hk, hk))
-        out, one = torch.empty_like(q), torch.empty_like(q)
-        both.step(i32(slots), i32(lens), i32(ntok), T)
-        both.append(0, k, v)
-        both.attention(0, q, out)
-        at = 0
-        for s, a, b in zip(slots, lens, ntok):
-            alone.step(i32([s]), i32([a]), i32([b]), b)
-            alone.append(0, k[at:at + b], v[at:at + b])
-            alone.attention(0, q[at:at + b], one[at:at + b])
-            at += b
-        assert torch.equal(out, one), ntok
-    both.close()
-    alone.close()
+    kv = gdn_amd.KV8Cache(1, 40, 300, 40, hq, hk, d, 4096)
+    mine, len0 = 7, 1500
+    first = [bf(rng, len0, hk, d)[0] for _ in range(2)]
+    for n in (2, 30):  # few segments and many
+        for new in (1, 5, 90):
+            q, k, v = (bf(rng, new, h, d)[0] for h in (hq, hk, hk))
+            outs = []
+            for other in range(3):
+                slots = [s for s in rng.permutation(40).tolist() if s != mine][:n]
+                slots[rng.integers(n)] = mine
+                lens = rng.integers(0, 300, n).tolist()
+                ntok = rng.integers(1, 3, n).tolist()
+                at = slots.index(mine)
+                lens[at], ntok[at] = len0, new
+                T, cu = 300, [0]
+                for x in ntok:
+                    cu.append(cu[-1] + x)
+                kv.step(i32([mine]), i32([0]), i32([len0]), len0)
+                kv.append(0, *first)
+                kv.step(i32(range(40)), i32([len0 if s == mine else 0 for s in range(40)]),
+                        i32([0] * 40), 0)
+                kv.step(i32(slots), i32(lens), i32(ntok), T, 90)
+                wide = [bf(rng, T, h, d)[0] for h in (hq, hk, hk)]
+                for w, x in zip(wide, (q, k, v)):
+                    w[cu[at]:cu[at] + new] = x
+                kv.append(0, *wide[1:])
+                for _ in range(2):
+                    out = torch.empty_like(wide[0])
+                    kv.attention(0, wide[0], out)
+                    outs.append(out[cu[at]:cu[at] + new])
+            assert kv.check() == 0
+            for o in outs[1:]:
+                assert torch.equal(outs[0], o), (n, new)
+    kv.close()
 
 
 def test_strides_streams_and_layers(gpu):
