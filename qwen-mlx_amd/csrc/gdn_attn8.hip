@@ -25,6 +25,7 @@ constexpr float kStep = 8.f;  // log2 steps of the running maximum
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef float f32x2 __attribute__((ext_vector_type(2)));
@@ -83,6 +84,12 @@ __device__ __forceinline__ f32x4 scores16(const u32x4* k, const u32x4* q) {
 __device__ __forceinline__ float max_xor16_32(float v) {
   const auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+  return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+
+// Maximum over a lane and lane ^ 32.
+__device__ __forceinline__ float max_xor32(float v) {
   const auto b = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
   return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
 }
@@ -214,17 +221,19 @@ __device__ __forceinline__ Group group_of(const Kv8AttnArgs& a, const Kv8Row& ro
   return x;
 }
 
-// A lane's NK pieces of 16 dims of its column's q (16 g4 + 64 i on) in two e4m3 parts, in turn;
-// returns the exponent of the column.
-template <int NK>
-__device__ __forceinline__ int q_parts(const uint16_t* q, bool valid, u32x4* out) {
-  u32x4 x[NK][2];
+// A lane's dims of its column's q, pieces of 16 (piece i from step * i on, pairs of them side by
+// side with PAIR) in two e4m3 parts, in turn; returns the exponent of the column. The column
+// lies in lanes l, l ^ 32 and, without PAIR, l ^ 16.
+template <int N, bool PAIR>
+__device__ __forceinline__ int q_pieces(const uint16_t* q, bool valid, u32x4* out) {
+  u32x4 x[N][2];
   uint32_t mx = 0;
 #pragma unroll
-  for (int i = 0; i < NK; ++i)
+  for (int i = 0; i < N; ++i)
 #pragma unroll
     for (int b = 0; b < 2; ++b) {
-      x[i][b] = valid ? *reinterpret_cast<const u32x4*>(q + 64 * i + 8 * b) : (u32x4){0u, 0u, 0u, 0u};
+      const int at = PAIR ? 64 * (i >> 1) + 16 * (i & 1) : 64 * i;
+      x[i][b] = valid ? *reinterpret_cast<const u32x4*>(q + at + 8 * b) : (u32x4){0u, 0u, 0u, 0u};
 #pragma unroll
       for (int w = 0; w < 4; ++w) {
         const uint32_t lo = x[i][b][w] & 0x7fffu, hi = (x[i][b][w] >> 16) & 0x7fffu;
@@ -232,12 +241,13 @@ __device__ __forceinline__ int q_parts(const uint16_t* q, bool valid, u32x4* out
       }
     }
   // bf16 patterns are in the order of their sizes, and so are they as f32
-  const uint32_t bits = __float_as_uint(max_xor16_32(__uint_as_float(mx << 16)));
+  const float size = __uint_as_float(mx << 16);
+  const uint32_t bits = __float_as_uint(PAIR ? max_xor32(size) : max_xor16_32(size));
   // the least e with the largest <= 448 * 2^e (448 = 1.75 * 2^8)
   const int e = max((int)(bits >> 23) - 135 + ((bits & 0x7fffffu) > 0x600000u ? 1 : 0), -100);
   const float inv = pow2(-e);
 #pragma unroll
-  for (int i = 0; i < NK; ++i) {
+  for (int i = 0; i < N; ++i) {
     u32x4 hi, lo;
 #pragma unroll
     for (int w = 0; w < 4; ++w) {  // 4 dims a word
@@ -258,6 +268,15 @@ __device__ __forceinline__ int q_parts(const uint16_t* q, bool valid, u32x4* out
     out[2 * i + 1] = lo;
   }
   return e;
+}
+// of 16 columns: dims 64 i + 16 g4 ..; of 32: dims 64 i + 32 hf .. (q already moved there)
+template <int NK>
+__device__ __forceinline__ int q_parts(const uint16_t* q, bool valid, u32x4* out) {
+  return q_pieces<NK, false>(q, valid, out);
+}
+template <int NK>
+__device__ __forceinline__ int q_parts32(const uint16_t* q, bool valid, u32x4* out) {
+  return q_pieces<2 * NK, true>(q, valid, out);
 }
 
 // The running softmax of 16 columns over blocks of 32 keys: lane (g4, c) holds keys 4 g4 + r and
@@ -604,18 +623,16 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
   }
 }
 
-// grid (T, Hq), block 64 W: a token's chunks, chunk i in sum i % 16, wave w the sums w, w + W,
-// ..; then the sums in order, so that W changes no bits. Also the zeros of refused rows'
-// tokens. Tokens of tiles and of single chunks are written already.
+// A token's head: its chunks, chunk i in sum i % 16, wave w the sums w, w + W, ..; then the sums
+// in order, so that W changes no bits. Also the zeros of refused rows' tokens. Tokens of tiles
+// and of single chunks are written already. By the work-group.
 template <int D, int W>
-__global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
-                                                               const float* __restrict__ part) {
+__device__ __forceinline__ void combine_token(const Kv8AttnArgs& a, const float* __restrict__ part, int t,
+                                              int h, int tid, int lane, int wave, int G, int tpg,
+                                              float (*sum)[D]) {
   constexpr int DPL = D / 64, kPer = 16 / W;
   typedef float fvec __attribute__((ext_vector_type(DPL)));
-  __shared__ float sum[16][D];
   const Kv8Plan& p = a.p;
-  const int t = blockIdx.x, h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = p.tok_row[t];
   if (r == -2) return;
   if (r < 0) {
@@ -624,25 +641,27 @@ __global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
     return;
   }
   const Kv8Row row = p.rows[r];
-  const int G = p.Hq / p.Hkv, tpg = 16 / G;
   const Chunks ch = chunks_of(a, row, r, tpg);
   if (ch.nch < 2) return;
   const int k = t - row.cu, grp = k / tpg, j = h / G, c = (k - grp * tpg) * G + h - j * G;
   const float* const pc = part + (((size_t)p.parts[r] * p.Hkv + (size_t)(grp * p.Hkv + j) * ch.nch) *
                                       16 + c) * (D + 4);
   constexpr size_t kStride = (size_t)16 * (D + 4);
-  const int n = min(64, ch.nch);
-  fvec v[kPer];
-  auto rows = [&](int i0) {  // the wave's chunks of i0 .. i0 + 15
+  // 64 chunks' rows go out before their maxima and sums, one a lane, are waited for
+  fvec v[4][kPer];
+  auto rows = [&](int b) {
 #pragma unroll
-    for (int i = 0; i < kPer; ++i)
-      v[i] = *reinterpret_cast<const fvec*>(pc + min(i0 + wave + W * i, ch.nch - 1) * kStride + 4 +
-                                            DPL * lane);
+    for (int q = 0; q < 4; ++q)
+      if (b + 16 * q < ch.nch) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i)
+          v[q][i] = *reinterpret_cast<const fvec*>(
+              pc + min(b + 16 * q + wave + W * i, ch.nch - 1) * kStride + 4 + DPL * lane);
+      }
   };
   rows(0);
-  // maxima and sums of 64 chunks, one a lane
-  float mi = lane < n ? pc[lane * kStride] : -INFINITY;
-  float li = lane < n ? pc[lane * kStride + 1] : 0.f;
+  float mi = lane < ch.nch ? pc[lane * kStride] : -INFINITY;
+  float li = lane < ch.nch ? pc[lane * kStride + 1] : 0.f;
   float M = mi;
   for (int i = lane + 64; i < ch.nch; i += 64) M = fmaxf(M, pc[i * kStride]);
 #pragma unroll
@@ -654,21 +673,23 @@ __global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
   for (int i = 0; i < kPer; ++i) A[i] = (fvec)(0.f);
   for (int b = 0; b < ch.nch; b += 64) {
     if (b) {
+      rows(b);
       mi = b + lane < ch.nch ? pc[(b + lane) * kStride] : -INFINITY;
       li = b + lane < ch.nch ? pc[(b + lane) * kStride + 1] : 0.f;
     }
     const float wi = exp2f(mi - M);
     L += li != 0.f ? wi * li : 0.f;
-    for (int i0 = b; i0 < min(b + 64, ch.nch); i0 += 16) {
-      if (i0) rows(i0);
 #pragma unroll
-      for (int i = 0; i < kPer; ++i) {
-        const int l = i0 - b + wave + W * i;
-        const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), l));
-        const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(li), l));
-        if (s != 0.f) A[i] += v[i] * f;  // chunks without a visible key hold nothing
+    for (int q = 0; q < 4; ++q)
+      if (b + 16 * q < ch.nch) {
+#pragma unroll
+        for (int i = 0; i < kPer; ++i) {
+          const int l = 16 * q + wave + W * i;
+          const float f = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(wi), l));
+          const float s = __int_as_float(__builtin_amdgcn_readlane(__float_as_int(li), l));
+          if (s != 0.f) A[i] += v[q][i] * f;  // chunks without a visible key hold nothing
+        }
       }
-    }
   }
   L = wave_sum(L);
 #pragma unroll
@@ -684,61 +705,395 @@ __global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
     float o[4] = {s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv};
     store4(a, t, h, 4 * tid, o);
   }
+  __syncthreads();  // sum is free for the next token
 }
 
-// One wave per (group of up to 16 / G tokens of a row of many, kv head) through all pages that its
-// tokens see.
-template <int D>
-__global__ __launch_bounds__(64) void attn8_rows_kernel(Kv8AttnArgs a) {
-  constexpr int NK = D / 64, DB = D / 16;
+// grid (ceil(T / per), Hq), block 64 W: per tokens of a head, one after the other.
+template <int D, int W>
+__global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
+                                                               const float* __restrict__ part,
+                                                               int per) {
+  __shared__ float sum[16][D];
   const Kv8Plan& p = a.p;
-  const int lane = threadIdx.x, g4 = lane >> 4, c = lane & 15;
-  const int G = p.Hq / p.Hkv, tpg = 16 / G, j = blockIdx.y;
-  const int g = blockIdx.x;
-  const Found f = find_row(p, g, [&](int, const Kv8Row& row) {
-    return row.fresh < kKv8TileTokens ? 0 : (row.fresh + tpg - 1) / tpg;
+  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = p.Hq / p.Hkv, tpg = 16 / G;
+  for (int first = blockIdx.x * per, i = 0; i < per && first + i < p.T; ++i) {
+    if (per > 1) {  // on to the next token that has something to do, 64 at a time
+      const int tl = first + i + lane;
+      const int rl = tl < p.T && i + lane < per ? p.tok_row[tl] : -2;
+      const uint64_t any = __ballot(rl == -1 || (rl >= 0 && p.rows[max(rl, 0)].fresh < kKv8TileTokens));
+      if (!any) {
+        i += 63;
+        continue;
+      }
+      i += __ffsll((unsigned long long)any) - 1;
+    }
+    combine_token<D, W>(a, part, first + i, h, tid, lane, wave, G, tpg, sum);
+  }
+}
+
+// Prompts. Work-group (tile, kv head): a tile is NW * NC * (32 / G) consecutive tokens of a row.
+// Wave w takes the NC groups of 32 / G tokens from w NC on; a group's (token, query head) pairs
+// are 32 columns. A page of K and V is copied into LDS by DMA a page ahead, two buffers of each,
+// and read by all waves. Rows of the products are 32 keys or dims, so that an operand read
+// from LDS, and a value's conversion, serves 32 NC columns.
+//
+// Lane (hf, c), hf = lane / 32, holds keys 8 i + 4 hf + r of a block of 32 (i, r = 0 .. 3) for
+// column c of each group, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^unit.
+//
+// With one wave a SIMD (the outputs of 64 columns at D = 256 are 256 registers) the overlap of
+// products and softmax is laid out in program order, a block apart: the products of block
+// k + 1's scores beside the exponentials of block k, those of block k's values beside the
+// maxima of block k + 1.
+template <int D, int NW, int NC>
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(Kv8AttnArgs a) {
+  constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
+  constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
+  static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
+  constexpr bool kLowInLds = D == 256;
+  __shared__ u32x4 lk0[kTile16], lk1[kTile16], lv0[kTile16], lv1[kTile16];
+  __shared__ u32x4 lq[kLowInLds ? NW * NC : 1][kLowInLds ? 2 * NK : 1][64];
+  const Kv8Plan& p = a.p;
+  const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, c = lane & 31;
+  const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = NW * NC * tpw, j = blockIdx.y;
+  const Found f = find_row(p, blockIdx.x, [&](int, const Kv8Row& row) {
+    return row.fresh < kKv8TileTokens ? 0 : (row.fresh + tpt - 1) / tpt;
   });
   if (f.r < 0) return;
-  const Group x = group_of(a, f.row, f.r, g - f.first, j, G, tpg, c);
-  const Score sc = score_of(a, x);
-  u32x4 q[2 * NK];
-  const int eq = q_parts<NK>(a.q + x.t * a.qs + x.h * a.qhs + 16 * g4, x.valid, q);
-  Online<D> on;
-  on.clear();
-  const int32_t* const trow = p.table + (size_t)f.row.slot * p.max_pages;
-  for (int v = 0; v < x.span.count(); ++v) {
-    const int blk = x.span.page(v), key0 = blk * kPage;
-    const size_t hk = ((size_t)trow[blk] * 2) * p.Hkv + j, hv = hk + p.Hkv;
-    const u32x4* const kp = reinterpret_cast<const u32x4*>(a.pages + hk * (kPage * D)) + lane;
-    const u32x4* const vp = reinterpret_cast<const u32x4*>(a.pages + hv * (kPage * D)) + lane;
-    const int ek = (int)(int8_t)a.exps[hk], wv = a.exps[hv];
+  const Kv8Row row = f.row;
+  const int tiles = (row.fresh + tpt - 1) / tpt;
+  const int k0 = (tiles - 1 - (blockIdx.x - f.first)) * tpt;  // longest first
+  const int total = row.pos + row.fresh;
+  const int pf = a.prefix ? min(max(a.prefix[f.r], 0), total) : 0;
+  const int p0 = row.pos + k0;  // the tile's first position
+  const Span span = span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total);
+  const int count = span.count();
+  // the wave's positions
+  const int w0 = p0 + w * NC * tpw, wn = min(max(total - w0, 0), NC * tpw);
+  const int ctok = c / G, h = j * G + c - ctok * G;
+  int cpos[NC], eq[NC];
+  int64_t t[NC];
+  uint32_t seen[NC];
+  float m[NC], l[NC], mk[NC];
+  f32x16 O[NC][NT], S[NC];
 #pragma unroll
-    for (int h2 = 0; h2 < 2; ++h2) {
-      f32x4 S[2];
+  for (int n = 0; n < NC; ++n) {
+    const int at = w0 + n * tpw + ctok;
+    const bool valid = ctok < tpw && at < total;
+    cpos[n] = valid ? at : -1;
+    t[n] = (int64_t)row.cu + (valid ? at - row.pos : 0);
+    m[n] = -INFINITY;
+    l[n] = 0.f;
 #pragma unroll
-      for (int kg = 0; kg < 2; ++kg) {
-        u32x4 kr[NK];
+    for (int i = 0; i < NT; ++i)
 #pragma unroll
-        for (int i = 0; i < NK; ++i) kr[i] = kp[((2 * h2 + kg) * NK + i) * 64];
-        S[kg] = scores16<NK>(kr, q);
-      }
-      u32x4 vr[DB / 2];
+      for (int r = 0; r < 16; ++r) O[n][i][r] = 0.f;
+  }
+  int unit = 0;
+  const float sm = a.softcap > 0.f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
+  const float cap = a.softcap * 1.4426950408889634f;
+  const float slope = a.slopes ? a.slopes[ctok < tpw ? h : 0] * 1.4426950408889634f : 0.f;
+  const int window = a.window > 0 ? a.window : INT32_MAX / 2;
+  const bool odd = a.softcap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
+
+  const int32_t* const trow = p.table + (size_t)row.slot * p.max_pages;
+  int vbase = 0, pid = 0, eks = 0, evs = 0;
+  auto ids = [&](int v) __attribute__((always_inline)) {
+    vbase = v;
+    pid = v + lane < count ? trow[span.page(v + lane)] : 0;
+    const int32_t* const e = a.exps + (size_t)pid * 2 * p.Hkv + j;
+    eks = e[0];
+    evs = e[p.Hkv];
+    asm volatile("" ::"v"(pid), "v"(eks), "v"(evs));
+  };
+  ids(0);
+  const uint8_t* const base = a.pages + (size_t)j * (kPage * D);
+  const size_t page_bytes = (size_t)2 * p.Hkv * kPage * D, v_shift = (size_t)p.Hkv * kPage * D;
+  // K or V of page v into a buffer: a wave copies its share of the 1 KiB pieces
+  auto copy = [&](int v, u32x4* dst, size_t shift) __attribute__((always_inline)) {
+    const uint8_t* const src = base + shift + lane * 16 +
+        (size_t)(uint32_t)__builtin_amdgcn_readlane(pid, min(v, count - 1) - vbase) * page_bytes;
 #pragma unroll
-      for (int i = 0; i < DB / 2; ++i) vr[i] = vp[(h2 * (DB / 2) + i) * 64];
-      uint32_t seen;
-      const u32x4 P = on.weights(S, sc, x, key0 + kBlock * h2, eq + ek, (int)(int8_t)wv, seen);
-      on.values(vr, P, key0 + kBlock * h2, x.total, (wv & kNanFlag) != 0, seen);
+    for (int i = 0; i < kLoads; ++i)
+      __builtin_amdgcn_global_load_lds(
+          (const void __attribute__((address_space(1)))*)(src + (w * kLoads + i) * 1024),
+          (void __attribute__((address_space(3)))*)(dst + (w * kLoads + i) * 64), 16, 0, 0);
+  };
+  copy(0, lk0, 0);
+  copy(0, lv0, v_shift);
+  copy(1, lk1, 0);
+  copy(1, lv1, v_shift);
+
+  // q: dims 64 i + 32 hf .. + 31 of column c, in two e4m3 parts
+  u32x4 qh[NC][2 * NK], ql[kLowInLds ? 1 : NC][kLowInLds ? 1 : 2 * NK];
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    u32x4 q[4 * NK];
+    eq[n] = q_parts32<NK>(a.q + t[n] * a.qs + h * a.qhs + 32 * hf, cpos[n] >= 0, q);
+#pragma unroll
+    for (int i = 0; i < 2 * NK; ++i) {
+      qh[n][i] = q[2 * i];
+      if constexpr (kLowInLds)
+        lq[w * NC + n][i][lane] = q[2 * i + 1];
+      else
+        ql[n][i] = q[2 * i + 1];
     }
   }
-  const float l = on.sum();
-  if (!x.valid) return;
-  const float inv = __builtin_amdgcn_ldexpf(1.0f / l, on.unit);
+  // this lane's pieces: of key c of 32 (NK KiB for 16 keys), and of dim c of 32
+  const int kat = (c >> 4) * NK * 64 + 32 * hf + (c & 15);
+  const int vat = (c >> 4) * 32 + 16 * hf + (c & 15);
+
+  auto both = [](u32x4 x, u32x4 y) __attribute__((always_inline)) {
+    return (i32x8){(int)x[0], (int)x[1], (int)x[2], (int)x[3],
+                   (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
+  };
+  // scores of half hb of the page in lk
+  auto scores = [&](const u32x4* lk, int hb, f32x16* Sn) __attribute__((always_inline)) {
+    constexpr int kOne = 0x7f7f7f7f, kLow = 0x7b7b7b7b;  // 2^0 and 2^-4
 #pragma unroll
-  for (int d = 0; d < DB; ++d) {
-    float o[4];
+    for (int n = 0; n < NC; ++n)
 #pragma unroll
-    for (int r = 0; r < 4; ++r) o[r] = on.O[d][r] * inv;
-    store4(a, x.t, x.h, 16 * d + 4 * g4, o);
+      for (int i = 0; i < 16; ++i) Sn[n][i] = 0.f;
+    asm volatile("" ::: "memory");  // q's low parts are re-read from LDS for every block
+#pragma unroll
+    for (int i = 0; i < NK; ++i) {
+      const int at = kat + (2 * hb * NK + i) * 64;
+      const i32x8 kk = both(lk[at], lk[at + 16]);
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+            kk, both(qh[n][2 * i], qh[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kOne);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const i32x8 qq = kLowInLds
+                             ? both(lq[w * NC + n][2 * i][lane], lq[w * NC + n][2 * i + 1][lane])
+                             : both(ql[kLowInLds ? 0 : n][kLowInLds ? 0 : 2 * i],
+                                    ql[kLowInLds ? 0 : n][kLowInLds ? 0 : 2 * i + 1]);
+        Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kk, qq, Sn[n], 0, 0, 0, kOne, 0, kLow);
+      }
+    }
+  };
+  // Scores of the block at kb that need more than a factor: x = mk * S in any case
+  auto prepare = [&](f32x16* Sn, int kb, int ek) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      mk[n] = __builtin_amdgcn_ldexpf(sm, eq[n] + ek);
+      seen[n] = 0xffffu;
+    }
+    const bool all = (kb + kBlock - 1 <= w0 && kb > w0 + wn - 1 - window) || kb + kBlock <= pf;
+    if (__builtin_expect(odd || !all, 0)) {
+      asm volatile("");
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const int lo = cpos[n] - window, cpf = cpos[n] >= 0 ? pf : 0;
+        uint32_t see_all = 0;
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+          const int key = kb + 8 * (i >> 2) + 4 * hf + (i & 3);
+          float y = Sn[n][i] * mk[n];
+          if (cap > 0.f) y = capped(y, cap);
+          y = fmaf(-slope, (float)(cpos[n] - key), y);
+          const bool see = (key <= cpos[n] && key > lo) || key < cpf;
+          Sn[n][i] = see ? y : -INFINITY;
+          see_all |= (see ? 1u : 0u) << i;
+        }
+        seen[n] = see_all;
+        mk[n] = 1.f;
+      }
+    }
+  };
+  auto maxima = [&](const f32x16* Sn, float* bm) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      float x = fmaxf(Sn[n][0], Sn[n][1]);
+#pragma unroll
+      for (int i = 2; i < 16; ++i) x = fmaxf(x, Sn[n][i]);
+      bm[n] = max_xor32(x) * mk[n];
+    }
+  };
+  // the running maximum follows once it is passed by 2^kStep; ev: the exponent of the block's values
+  auto follow = [&](const float* bm, int ev) __attribute__((always_inline)) {
+    bool up = ev != unit;
+#pragma unroll
+    for (int n = 0; n < NC; ++n) up |= __any(bm[n] > m[n] + kStep);
+    if (__builtin_expect(up, 0)) {
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        const float mn = fmaxf(m[n], bm[n]);
+        float corr = mn > m[n] ? __builtin_amdgcn_exp2f(m[n] - mn) : 1.0f;  // m = -inf: 0
+        m[n] = mn;
+        l[n] *= corr;
+        corr = __builtin_amdgcn_ldexpf(corr, unit - ev);
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+          O[n][i] *= corr;
+          __builtin_amdgcn_sched_barrier(0);  // not all of them in registers of their own at once
+        }
+      }
+      unit = ev;
+    }
+  };
+  u32x4 P[NC][2];
+  auto weights = [&](const f32x16* Sc) __attribute__((always_inline)) {
+#pragma unroll
+    for (int n = 0; n < NC; ++n) {
+      const float mref = m[n] == -INFINITY ? 0.f : m[n];
+      float e[16], sum = 0.f;
+#pragma unroll
+      for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(Sc[n][i], mk[n], -mref));
+#pragma unroll
+      for (int i = 0; i < 16; i += 4) sum += (e[i] + e[i + 1]) + (e[i + 2] + e[i + 3]);
+      l[n] += sum;
+      // keys 4 hf + r and 16 + 4 hf + r, then those 8 further on: the order of the values' bytes
+      P[n][0] = (u32x4){pk_f16(e[0], e[1]), pk_f16(e[2], e[3]), pk_f16(e[8], e[9]), pk_f16(e[10], e[11])};
+      P[n][1] = (u32x4){pk_f16(e[4], e[5]), pk_f16(e[6], e[7]), pk_f16(e[12], e[13]), pk_f16(e[14], e[15])};
+    }
+  };
+  auto values = [&](const u32x4* lv, int hb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < NT; ++i) {
+      const u32x4 vr = lv[vat + (hb * (D / 16) + 2 * i) * 32];
+      const f16x8 f0 = to_f16(vr[0], vr[1]), f1 = to_f16(vr[2], vr[3]);
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        O[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f0, __builtin_bit_cast(f16x8, P[n][0]), O[n][i], 0, 0, 0);
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+        O[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1, __builtin_bit_cast(f16x8, P[n][1]), O[n][i], 0, 0, 0);
+    }
+  };
+  // Half hb of page v, from kb on, before its product where keys past the row's end may hold
+  // anything or some hold NaN: those bytes become zeros in LDS (each wave writes all that it
+  // reads, the same as the others), and a column that sees the key of a NaN, read from the page
+  // itself, gets a NaN sum.
+  auto clean = [&](int v, u32x4* lv, int hb, int kb, const uint32_t* seen_) __attribute__((always_inline)) {
+    const u32x4* const src = reinterpret_cast<const u32x4*>(
+        base + v_shift + (size_t)(uint32_t)__builtin_amdgcn_readlane(pid, v - vbase) * page_bytes);
+    u32x4 nan_keys = {0u, 0u, 0u, 0u};
+#pragma nounroll
+    for (int i = 0; i < NT; ++i) {
+      const int at = vat + (hb * (D / 16) + 2 * i) * 32;
+      u32x4 vr = src[at];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) {
+        // the word's four keys, from 4 (hf + 2 (k / 2) + 4 (k % 2)) on
+        const uint32_t x = first_keys(vr[k], total - kb - 4 * (hf + 2 * (k >> 1) + 4 * (k & 1)));
+        const uint32_t top = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        nan_keys[k] |= top;
+        vr[k] = x & ~((top >> 7) * 0xffu);
+      }
+      lv[at] = vr;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+#pragma unroll
+      for (int off = 1; off < 32; off <<= 1) nan_keys[k] |= __shfl_xor(nan_keys[k], off, 64);
+#pragma unroll
+      for (int n = 0; n < NC; ++n)
+#pragma unroll
+        for (int q = 0; q < 4; ++q)  // scores 4 (k / 2 + 2 (k % 2)) .. are those keys'
+          if ((nan_keys[k] >> (8 * q + 7)) & (seen_[n] >> (4 * ((k >> 1) + 2 * (k & 1)) + q)) & 1u)
+            l[n] = __builtin_nanf("");
+    }
+  };
+
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the first two pages
+  lds_barrier();
+  const bool idle = wn == 0;  // no tokens for this wave: copies and barriers only
+  float bm[NC];
+  auto exps_of = [&](int v, int& ek, int& ev, bool& nan) __attribute__((always_inline)) {
+    const int at = min(v, count - 1) - vbase;
+    ek = (int)(int8_t)__builtin_amdgcn_readlane(eks, at);
+    const int wv = __builtin_amdgcn_readlane(evs, at);
+    ev = (int)(int8_t)wv;
+    nan = (wv & kNanFlag) != 0;
+  };
+  int ek, ev;
+  bool nan;
+  exps_of(0, ek, ev, nan);
+  if (!idle) {
+    scores(lk0, 0, S);
+    prepare(S, span.page(0) * kPage, ek);
+    maxima(S, bm);
+    follow(bm, ev);
+  }
+  // Page v in buffers b. On entry the scores and maxima of its first half are formed, its K and V
+  // have landed, and the next page's are on their way, K first.
+  auto page = [&](int v, auto bc) __attribute__((always_inline)) {
+    constexpr int b = decltype(bc)::value;
+    u32x4* const lk = b ? lk1 : lk0;
+    u32x4* const lv = b ? lv1 : lv0;
+    const u32x4* const lkn = b ? lk0 : lk1;
+    const int key0 = span.page(v) * kPage;
+    f32x16 Sn[NC];
+    uint32_t was[NC];
+    if (!idle) {
+      scores(lk, 1, Sn);
+      weights(S);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) was[n] = seen[n];
+      prepare(Sn, key0 + kBlock, ek);
+      if (__builtin_expect(nan || key0 + kBlock > total, 0)) clean(v, lv, 0, key0, was);
+      values(lv, 0);
+      maxima(Sn, bm);
+      follow(bm, ev);
+    }
+    // the next page's K has landed everywhere, and no wave reads this page's any more
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kLoads);  // vmcnt(kLoads)
+    lds_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
+    if (min(v + 2, count - 1) - vbase >= 64) ids(v);
+    copy(v + 2, lk, 0);
+    __builtin_amdgcn_sched_barrier(0);
+    int ekn, evn;
+    bool nann;
+    exps_of(v + 1, ekn, evn, nann);
+    if (!idle) {
+      // behind the last page: scores of a page that was copied again, which nothing uses
+      scores(lkn, 0, S);
+      weights(Sn);
+#pragma unroll
+      for (int n = 0; n < NC; ++n) was[n] = seen[n];
+      prepare(S, span.page(min(v + 1, count - 1)) * kPage, ekn);
+      if (__builtin_expect(nan || key0 + kPage > total, 0)) clean(v, lv, 1, key0 + kBlock, was);
+      values(lv, 1);
+      maxima(S, bm);
+      if (v + 1 < count) follow(bm, evn);
+    }
+    // the next page's V has landed everywhere, and no wave reads this page's any more
+    __builtin_amdgcn_s_waitcnt(0x0F70 | kLoads);
+    lds_barrier();
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
+    copy(v + 2, lv, v_shift);
+    __builtin_amdgcn_sched_barrier(0);
+    ek = ekn;
+    ev = evn;
+    nan = nann;
+  };
+  int v = 0;
+#pragma nounroll
+  for (; v + 2 <= count; v += 2) {
+    page(v, std::integral_constant<int, 0>{});
+    page(v + 1, std::integral_constant<int, 1>{});
+  }
+  if (v < count) page(v, std::integral_constant<int, 0>{});
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // the last copies (repeats) land before the LDS is given back
+#pragma unroll
+  for (int n = 0; n < NC; ++n) {
+    const float ln = l[n] + __shfl_xor(l[n], 32, 64);
+    if (cpos[n] < 0) continue;
+    const float inv = __builtin_amdgcn_ldexpf(1.0f / ln, unit);
+#pragma unroll
+    for (int i = 0; i < NT; ++i)
+#pragma unroll
+      for (int g = 0; g < 4; ++g) {
+        float o[4];
+#pragma unroll
+        for (int r = 0; r < 4; ++r) o[r] = O[n][i][4 * g + r] * inv;
+        store4(a, t[n], h, 32 * i + 8 * g + 4 * hf, o);
+      }
   }
 }
 
@@ -753,12 +1108,14 @@ size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
 template <int D>
 static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   const Kv8Plan& p = a.p;
-  const int tpg = 16 / (p.Hq / p.Hkv);
   float* const part = static_cast<float*>(a.workspace);
   hipError_t e;
   if (p.max_row >= kKv8TileTokens) {
-    const dim3 grid(min(p.T, p.T / tpg + min(p.n, p.T)), p.Hkv);
-    hipLaunchKernelGGL(attn8_rows_kernel<D>, grid, dim3(64), 0, a.stream, a);
+    constexpr int NW = 4, NC = 1;
+    const int tpt = NW * NC * (32 / (p.Hq / p.Hkv));
+    // rows of tiles have kKv8TileTokens or more
+    const dim3 grid(p.T / tpt + min(p.n, p.T / kKv8TileTokens), p.Hkv);
+    hipLaunchKernelGGL((attn8_tile_kernel<D, NW, NC>), grid, dim3(64 * NW), 0, a.stream, a);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   // as many as the rows can have, up to four rounds of the chip's waves
@@ -770,10 +1127,12 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   else
     hipLaunchKernelGGL((attn8_chunk_kernel<D, 4>), grid, dim3(256), 0, a.stream, a, part);
   if ((e = hipGetLastError()) != hipSuccess) return e;
+  const int per = (p.T + 511) / 512;  // long steps hold few such tokens
+  const dim3 tokens((p.T + per - 1) / per, p.Hq);
   if (p.T * p.Hq <= 512)  // a wave for each sum where the work-groups are few
-    hipLaunchKernelGGL((attn8_combine_kernel<D, 16>), dim3(p.T, p.Hq), dim3(1024), 0, a.stream, a, part);
+    hipLaunchKernelGGL((attn8_combine_kernel<D, 16>), tokens, dim3(1024), 0, a.stream, a, part, per);
   else
-    hipLaunchKernelGGL((attn8_combine_kernel<D, 4>), dim3(p.T, p.Hq), dim3(256), 0, a.stream, a, part);
+    hipLaunchKernelGGL((attn8_combine_kernel<D, 4>), tokens, dim3(256), 0, a.stream, a, part, per);
   return hipGetLastError();
 }
 
