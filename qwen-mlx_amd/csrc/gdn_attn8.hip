@@ -20,6 +20,7 @@ namespace {
 constexpr int kPage = 64;
 constexpr int kBlock = 32;  // keys of a step of the running softmax: half a page
 constexpr int kNanFlag = 1 << 16;
+constexpr int kSplitPages = 8;  // of a tile's split at least
 constexpr float kStep = 8.f;  // log2 steps of the running maximum
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -279,6 +280,19 @@ __device__ __forceinline__ int q_parts32(const uint16_t* q, bool valid, u32x4* o
   return q_pieces<2 * NK, true>(q, valid, out);
 }
 
+// sc * 2^e; an e that leaves nothing of any score stays a factor
+__device__ __forceinline__ float factor_of(float sc, int e) {
+  return __builtin_amdgcn_ldexpf(sc, max(e, -110));
+}
+
+// Bits of those of a lane's `count` scores whose keys lie below n, four keys side by side every
+// STEP from 0 on.
+template <int STEP>
+__device__ __forceinline__ uint32_t first_scores(int n, int count) {
+  const int k = min(max(n, 0), STEP * count / 4);
+  return (1u << (4 * (k / STEP) + min(k % STEP, 4))) - 1u;
+}
+
 // The running softmax of 16 columns over blocks of 32 keys: lane (g4, c) holds keys 4 g4 + r and
 // 16 + 4 g4 + r of a block for column c, and dims 16 d + 4 g4 + r of its outputs in units of
 // 2^unit.
@@ -301,9 +315,10 @@ struct Online {
                                            int e, int ev, uint32_t& seen) {
     const int g4 = (threadIdx.x & 63) >> 4;
     float s[8];
-    const float mul = __builtin_amdgcn_ldexpf(sc.mul, e);
+    const float mul = factor_of(sc.mul, e);
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = S[i >> 2][i & 3] * mul;
+    const int k0 = key0 + 4 * g4;  // score i is of key k0 + 16 (i / 4) + i % 4
     if (__builtin_expect(sc.cap > 0.f, 0)) {
       asm volatile("");  // a branch: the caps are many instructions
 #pragma unroll
@@ -311,9 +326,9 @@ struct Online {
     }
     if (__builtin_expect(sc.sloped, 0)) {
       asm volatile("");
+      const float far = sc.slope * (float)(k0 - x.cpos);
 #pragma unroll
-      for (int i = 0; i < 8; ++i)
-        s[i] = fmaf(-sc.slope, (float)(x.cpos - (key0 + 16 * (i >> 2) + 4 * g4 + (i & 3))), s[i]);
+      for (int i = 0; i < 8; ++i) s[i] += fmaf(sc.slope, (float)(16 * (i >> 2) + (i & 3)), far);
     }
     seen = 0xffu;
     // wave-uniform: every token of the group sees every key of the block
@@ -321,13 +336,10 @@ struct Online {
                      key0 + kBlock <= x.pf;
     if (__builtin_expect(!all, 0)) {
       asm volatile("");
+      auto below = [](int n) { return first_scores<16>(n, 8); };  // of keys below k0 + n
+      seen = (below(x.cpos + 1 - k0) & ~below(x.lo + 1 - k0)) | below(x.valid ? x.pf - k0 : 0);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int key = key0 + 16 * (i >> 2) + 4 * g4 + (i & 3);
-        const bool see = (key <= x.cpos && key > x.lo) || (key < x.pf && x.valid);
-        s[i] = see ? s[i] : -INFINITY;
-        seen &= ~((see ? 0u : 1u) << i);
-      }
+      for (int i = 0; i < 8; ++i) s[i] = (seen >> i) & 1u ? s[i] : -INFINITY;
     }
     float bm = fmaxf(fmaxf(fmaxf(s[0], s[1]), fmaxf(s[2], s[3])),
                      fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
@@ -437,6 +449,32 @@ __device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& 
   c.cp = (cp + waves - 1) / waves * waves;
   c.nch = (most + c.cp - 1) / c.cp;
   return c;
+}
+
+// Items of a row of tiles: (tile from the last one on, split). By row alone where pages are cut.
+struct Splits {
+  int tiles, cp, n;
+};
+__device__ __forceinline__ Splits splits_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpt,
+                                            int most_splits) {
+  Splits s{0, 1, 0};
+  if (row.fresh < kKv8TileTokens) return s;
+  s.tiles = (row.fresh + tpt - 1) / tpt;
+  s.n = 1;
+  s.cp = INT32_MAX / 2;
+  if (most_splits > 1) {
+    const int total = row.pos + row.fresh;
+    const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
+    int most = 0;  // of the first and the last tile's pages, as in chunks_of
+    for (int g = 0; g < s.tiles; g += max(s.tiles - 1, 1)) {
+      const int p0 = row.pos + g * tpt;
+      most = max(most, span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total).count());
+    }
+    most = min(most + (s.tiles > 1 && a.window > 0 ? 1 : 0), (total + kPage - 1) / kPage);
+    s.cp = max((most - 1) / most_splits + 1, kSplitPages);
+    s.n = (most + s.cp - 1) / s.cp;
+  }
+  return s;
 }
 
 }  // namespace
@@ -621,49 +659,57 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
       }
     }
   }
+  // tokens of refused rows: zeros, each work-group its share of the step's
+  for (int t0 = blockIdx.x * 64; t0 < p.T; t0 += gridDim.x * 64) {
+    uint64_t none = __ballot(t0 + lane < p.T && p.tok_row[t0 + lane] == -1);
+    for (; none; none &= none - 1) {
+      const int64_t t = t0 + __ffsll((unsigned long long)none) - 1;
+      for (int i = tid; i < p.Hq * (D / 4); i += 64 * W)
+        *reinterpret_cast<u32x2*>(a.out + t * a.os + (i / (D / 4)) * a.ohs + i % (D / 4) * 4) = (u32x2){0u, 0u};
+    }
+  }
 }
 
-// A token's head: its chunks, chunk i in sum i % 16, wave w the sums w, w + W, ..; then the sums
-// in order, so that W changes no bits. Also the zeros of refused rows' tokens. Tokens of tiles
-// and of single chunks are written already. By the work-group.
+// Rows of few tokens: grid (n * per, Hq), block 64 W; token k < per of row r, a head: its chunks,
+// chunk i in sum i % 16, wave w the sums w, w + W, ..; then the sums in order. Rows of a single
+// chunk are written already.
 template <int D, int W>
-__device__ __forceinline__ void combine_token(const Kv8AttnArgs& a, const float* __restrict__ part, int t,
-                                              int h, int tid, int lane, int wave, int G, int tpg,
-                                              float (*sum)[D]) {
+__global__ __launch_bounds__(64 * W) void attn8_join_kernel(Kv8AttnArgs a, const float* __restrict__ part,
+                                                            int per) {
   constexpr int DPL = D / 64, kPer = 16 / W;
+  constexpr size_t kStride = (size_t)16 * (D + 4);  // of a token's chunks
   typedef float fvec __attribute__((ext_vector_type(DPL)));
+  __shared__ float sum[16][D];
   const Kv8Plan& p = a.p;
-  const int r = p.tok_row[t];
-  if (r == -2) return;
-  if (r < 0) {
-    if (tid < D / 4)
-      *reinterpret_cast<u32x2*>(a.out + (int64_t)t * a.os + h * a.ohs + 4 * tid) = (u32x2){0u, 0u};
-    return;
-  }
+  const int tid = threadIdx.x, lane = tid & 63, h = blockIdx.y;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int r = blockIdx.x / per, k = blockIdx.x - r * per;
   const Kv8Row row = p.rows[r];
-  const Chunks ch = chunks_of(a, row, r, tpg);
-  if (ch.nch < 2) return;
-  const int k = t - row.cu, grp = k / tpg, j = h / G, c = (k - grp * tpg) * G + h - j * G;
-  const float* const pc = part + (((size_t)p.parts[r] * p.Hkv + (size_t)(grp * p.Hkv + j) * ch.nch) *
-                                      16 + c) * (D + 4);
-  constexpr size_t kStride = (size_t)16 * (D + 4);
+  const int parts = p.parts[r];
+  if (k >= row.fresh) return;
+  const int G = p.Hq / p.Hkv, tpg = 16 / G, j = h / G, grp = k / tpg, c = (k - grp * tpg) * G + h - j * G;
+  const int nch = chunks_of(a, row, r, tpg).nch;
+  if (nch < 2) return;
+  const int64_t t = (int64_t)row.cu + k;
+  const float* const pc =
+      part + ((size_t)parts * p.Hkv + (size_t)(grp * p.Hkv + j) * nch) * kStride + c * (D + 4);
   // 64 chunks' rows go out before their maxima and sums, one a lane, are waited for
   fvec v[4][kPer];
-  auto rows = [&](int b) {
+  auto rows = [&](int b) __attribute__((always_inline)) {
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (b + 16 * q < ch.nch) {
+      if (b + 16 * q < nch) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i)
           v[q][i] = *reinterpret_cast<const fvec*>(
-              pc + min(b + 16 * q + wave + W * i, ch.nch - 1) * kStride + 4 + DPL * lane);
+              pc + min(b + 16 * q + wave + W * i, nch - 1) * kStride + 4 + DPL * lane);
       }
   };
   rows(0);
-  float mi = lane < ch.nch ? pc[lane * kStride] : -INFINITY;
-  float li = lane < ch.nch ? pc[lane * kStride + 1] : 0.f;
+  float mi = lane < nch ? pc[lane * kStride] : -INFINITY;
+  float li = lane < nch ? pc[lane * kStride + 1] : 0.f;
   float M = mi;
-  for (int i = lane + 64; i < ch.nch; i += 64) M = fmaxf(M, pc[i * kStride]);
+  for (int i = lane + 64; i < nch; i += 64) M = fmaxf(M, pc[i * kStride]);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) M = fmaxf(M, __shfl_xor(M, off, 64));
   if (M == -INFINITY) M = 0.f;  // NaN scores alone
@@ -671,17 +717,17 @@ __device__ __forceinline__ void combine_token(const Kv8AttnArgs& a, const float*
   fvec A[kPer];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) A[i] = (fvec)(0.f);
-  for (int b = 0; b < ch.nch; b += 64) {
+  for (int b = 0; b < nch; b += 64) {
     if (b) {
       rows(b);
-      mi = b + lane < ch.nch ? pc[(b + lane) * kStride] : -INFINITY;
-      li = b + lane < ch.nch ? pc[(b + lane) * kStride + 1] : 0.f;
+      mi = b + lane < nch ? pc[(b + lane) * kStride] : -INFINITY;
+      li = b + lane < nch ? pc[(b + lane) * kStride + 1] : 0.f;
     }
     const float wi = exp2f(mi - M);
     L += li != 0.f ? wi * li : 0.f;
 #pragma unroll
     for (int q = 0; q < 4; ++q)
-      if (b + 16 * q < ch.nch) {
+      if (b + 16 * q < nch) {
 #pragma unroll
         for (int i = 0; i < kPer; ++i) {
           const int l = 16 * q + wave + W * i;
@@ -705,31 +751,47 @@ __device__ __forceinline__ void combine_token(const Kv8AttnArgs& a, const float*
     float o[4] = {s[0] * inv, s[1] * inv, s[2] * inv, s[3] * inv};
     store4(a, t, h, 4 * tid, o);
   }
-  __syncthreads();  // sum is free for the next token
 }
 
-// grid (ceil(T / per), Hq), block 64 W: per tokens of a head, one after the other.
-template <int D, int W>
-__global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
-                                                               const float* __restrict__ part,
-                                                               int per) {
-  __shared__ float sum[16][D];
+// Rows of tiles whose pages are split: grid (tiles at most, Hkv, D / 32), block 256, 32 dims of a
+// tile's 128 columns: 8 lanes a column, its splits in order.
+template <int D>
+__global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, const float* __restrict__ part,
+                                                               int most_splits) {
+  constexpr int kCols = 32 * kKv8TileWaves;
+  constexpr size_t kStride = (size_t)kCols * (D + 4);
   const Kv8Plan& p = a.p;
-  const int h = blockIdx.y, tid = threadIdx.x, lane = tid & 63;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = p.Hq / p.Hkv, tpg = 16 / G;
-  for (int first = blockIdx.x * per, i = 0; i < per && first + i < p.T; ++i) {
-    if (per > 1) {  // on to the next token that has something to do, 64 at a time
-      const int tl = first + i + lane;
-      const int rl = tl < p.T && i + lane < per ? p.tok_row[tl] : -2;
-      const uint64_t any = __ballot(rl == -1 || (rl >= 0 && p.rows[max(rl, 0)].fresh < kKv8TileTokens));
-      if (!any) {
-        i += 63;
-        continue;
+  const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = kKv8TileWaves * tpw, j = blockIdx.y;
+  const Found f = find_row(p, blockIdx.x, [&](int, const Kv8Row& row) {
+    return row.fresh < kKv8TileTokens ? 0 : (row.fresh + tpt - 1) / tpt;
+  });
+  if (f.r < 0) return;
+  const int n = splits_of(a, f.row, f.r, tpt, most_splits).n;
+  if (n < 2) return;
+  const int tile = blockIdx.x - f.first;
+  const float* const base =
+      part + ((size_t)(p.tiles[f.r] + tile) * p.Hkv + j) * most_splits * kStride;
+  const int dim = 32 * blockIdx.z + 4 * (threadIdx.x & 7);
+  for (int col = threadIdx.x >> 3; col < kCols; col += 32) {
+    const int c = col & 31, ctok = c / G, tok = tile * tpt + (col >> 5) * tpw + ctok;
+    if (ctok >= tpw || tok >= f.row.fresh) continue;
+    const float* const pc = base + (size_t)col * (D + 4);
+    float M = -INFINITY, L = 0.f;
+    for (int s = 0; s < n; ++s) M = fmaxf(M, pc[s * kStride]);
+    if (M == -INFINITY) M = 0.f;  // NaN scores alone
+    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int s = 0; s < n; ++s) {
+      const float w = exp2f(pc[s * kStride] - M), l = pc[s * kStride + 1];
+      const f32x4 v = *reinterpret_cast<const f32x4*>(pc + s * kStride + 4 + dim);
+      if (l != 0.f) {  // a split without a visible key holds nothing
+        L += w * l;
+        A += v * w;
       }
-      i += __ffsll((unsigned long long)any) - 1;
     }
-    combine_token<D, W>(a, part, first + i, h, tid, lane, wave, G, tpg, sum);
+    const float inv = 1.0f / L;
+    float o[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
+    store4(a, (int64_t)f.row.cu + tok, j * G + c - ctok * G, dim, o);
   }
 }
 
@@ -747,7 +809,7 @@ __global__ __launch_bounds__(64 * W) void attn8_combine_kernel(Kv8AttnArgs a,
 // k + 1's scores beside the exponentials of block k, those of block k's values beside the
 // maxima of block k + 1.
 template <int D, int NW, int NC>
-__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(Kv8AttnArgs a) {
+__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part) {
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
   static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
@@ -758,18 +820,23 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, c = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = NW * NC * tpw, j = blockIdx.y;
-  const Found f = find_row(p, blockIdx.x, [&](int, const Kv8Row& row) {
-    return row.fresh < kKv8TileTokens ? 0 : (row.fresh + tpt - 1) / tpt;
+  const int most_splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
+  const Found f = find_row(p, blockIdx.x, [&](int r, const Kv8Row& row) {
+    const Splits s = splits_of(a, row, r, tpt, most_splits);
+    return s.tiles * s.n;
   });
   if (f.r < 0) return;
   const Kv8Row row = f.row;
-  const int tiles = (row.fresh + tpt - 1) / tpt;
-  const int k0 = (tiles - 1 - (blockIdx.x - f.first)) * tpt;  // longest first
+  const Splits sp = splits_of(a, row, f.r, tpt, most_splits);
+  const int local = blockIdx.x - f.first, split = local % sp.n;
+  const int tile = sp.tiles - 1 - local / sp.n;  // longest first
+  const int k0 = tile * tpt;
   const int total = row.pos + row.fresh;
   const int pf = a.prefix ? min(max(a.prefix[f.r], 0), total) : 0;
   const int p0 = row.pos + k0;  // the tile's first position
   const Span span = span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total);
-  const int count = span.count();
+  const int v0 = split * sp.cp;
+  const int count = min(span.count(), sp.n > 1 ? v0 + sp.cp : INT32_MAX);  // pages [v0, count)
   // the wave's positions
   const int w0 = p0 + w * NC * tpw, wn = min(max(total - w0, 0), NC * tpw);
   const int ctok = c / G, h = j * G + c - ctok * G;
@@ -808,7 +875,17 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
     evs = e[p.Hkv];
     asm volatile("" ::"v"(pid), "v"(eks), "v"(evs));
   };
-  ids(0);
+  // the tile's partial results, if its pages are split: columns (wave, c)
+  float* const out = part + (((size_t)(p.tiles[f.r] + tile) * p.Hkv + j) * most_splits + split) *
+                                ((size_t)32 * NW * NC * (D + 4));
+  if (v0 >= count) {  // nothing in this split (the tile is shorter than the row's last one)
+    for (int i = tid; i < 32 * NW * NC; i += 64 * NW) {
+      out[(size_t)i * (D + 4)] = -INFINITY;
+      out[(size_t)i * (D + 4) + 1] = 0.f;
+    }
+    return;
+  }
+  ids(v0);
   const uint8_t* const base = a.pages + (size_t)j * (kPage * D);
   const size_t page_bytes = (size_t)2 * p.Hkv * kPage * D, v_shift = (size_t)p.Hkv * kPage * D;
   // K or V of page v into a buffer: a wave copies its share of the 1 KiB pieces
@@ -821,10 +898,10 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
           (const void __attribute__((address_space(1)))*)(src + (w * kLoads + i) * 1024),
           (void __attribute__((address_space(3)))*)(dst + (w * kLoads + i) * 64), 16, 0, 0);
   };
-  copy(0, lk0, 0);
-  copy(0, lv0, v_shift);
-  copy(1, lk1, 0);
-  copy(1, lv1, v_shift);
+  copy(v0, lk0, 0);
+  copy(v0, lv0, v_shift);
+  copy(v0 + 1, lk1, 0);
+  copy(v0 + 1, lv1, v_shift);
 
   // q: dims 64 i + 32 hf .. + 31 of column c, in two e4m3 parts
   u32x4 qh[NC][2 * NK], ql[kLowInLds ? 1 : NC][kLowInLds ? 1 : 2 * NK];
@@ -879,28 +956,38 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   auto prepare = [&](f32x16* Sn, int kb, int ek) __attribute__((always_inline)) {
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      mk[n] = __builtin_amdgcn_ldexpf(sm, eq[n] + ek);
+      mk[n] = factor_of(sm, eq[n] + ek);
       seen[n] = 0xffffu;
     }
-    const bool all = (kb + kBlock - 1 <= w0 && kb > w0 + wn - 1 - window) || kb + kBlock <= pf;
-    if (__builtin_expect(odd || !all, 0)) {
+    const int kl = kb + 4 * hf;  // score i is of key kl + 8 (i / 4) + i % 4
+    if (__builtin_expect(odd, 0)) {
       asm volatile("");
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-        const int lo = cpos[n] - window, cpf = cpos[n] >= 0 ? pf : 0;
-        uint32_t see_all = 0;
 #pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          const int key = kb + 8 * (i >> 2) + 4 * hf + (i & 3);
-          float y = Sn[n][i] * mk[n];
-          if (cap > 0.f) y = capped(y, cap);
-          y = fmaf(-slope, (float)(cpos[n] - key), y);
-          const bool see = (key <= cpos[n] && key > lo) || key < cpf;
-          Sn[n][i] = see ? y : -INFINITY;
-          see_all |= (see ? 1u : 0u) << i;
-        }
-        seen[n] = see_all;
+        for (int i = 0; i < 16; ++i) Sn[n][i] *= mk[n];
         mk[n] = 1.f;
+        if (cap > 0.f) {
+#pragma unroll
+          for (int i = 0; i < 16; ++i) Sn[n][i] = capped(Sn[n][i], cap);
+        }
+        if (a.slopes) {
+          const float far = slope * (float)(kl - cpos[n]);
+#pragma unroll
+          for (int i = 0; i < 16; ++i) Sn[n][i] += fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), far);
+        }
+      }
+    }
+    const bool all = (kb + kBlock - 1 <= w0 && kb > w0 + wn - 1 - window) || kb + kBlock <= pf;
+    if (__builtin_expect(!all, 0)) {
+      asm volatile("");
+#pragma unroll
+      for (int n = 0; n < NC; ++n) {
+        auto below = [](int k) { return first_scores<8>(k, 16); };  // of keys below kl + k
+        seen[n] = (below(cpos[n] + 1 - kl) & ~below(cpos[n] - window + 1 - kl)) |
+                  below(cpos[n] >= 0 ? pf - kl : 0);
+#pragma unroll
+        for (int i = 0; i < 16; ++i) Sn[n][i] = (seen[n] >> i) & 1u ? Sn[n][i] : -INFINITY;
       }
     }
   };
@@ -1012,10 +1099,10 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   };
   int ek, ev;
   bool nan;
-  exps_of(0, ek, ev, nan);
+  exps_of(v0, ek, ev, nan);
   if (!idle) {
     scores(lk0, 0, S);
-    prepare(S, span.page(0) * kPage, ek);
+    prepare(S, span.page(v0) * kPage, ek);
     maxima(S, bm);
     follow(bm, ev);
   }
@@ -1072,7 +1159,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
     ev = evn;
     nan = nann;
   };
-  int v = 0;
+  int v = v0;
 #pragma nounroll
   for (; v + 2 <= count; v += 2) {
     page(v, std::integral_constant<int, 0>{});
@@ -1084,6 +1171,21 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   for (int n = 0; n < NC; ++n) {
     const float ln = l[n] + __shfl_xor(l[n], 32, 64);
     if (cpos[n] < 0) continue;
+    if (sp.n > 1) {
+      float* const pr = out + (size_t)((w * NC + n) * 32 + c) * (D + 4);
+      if (hf == 0) {
+        pr[0] = m[n];
+        pr[1] = ln;
+      }
+      const float one = __builtin_amdgcn_ldexpf(1.0f, unit);
+#pragma unroll
+      for (int i = 0; i < NT; ++i)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+          *reinterpret_cast<f32x4*>(pr + 4 + 32 * i + 8 * g + 4 * hf) =
+              (f32x4){O[n][i][4 * g], O[n][i][4 * g + 1], O[n][i][4 * g + 2], O[n][i][4 * g + 3]} * one;
+      continue;
+    }
     const float inv = __builtin_amdgcn_ldexpf(1.0f / ln, unit);
 #pragma unroll
     for (int i = 0; i < NT; ++i)
@@ -1097,25 +1199,33 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   }
 }
 
-size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
-  // a group has kv8_chunks() partials for each kv head or less, which over all groups are
-  // kv8_waves() or one each
+// Partials of the chunks: a group has kv8_chunks() for each kv head or less, which over all
+// groups are kv8_waves() or one each.
+size_t kv8_attn_chunk_floats(const gdn_kv8_desc& d) {
   const int64_t few = (int64_t)d.num_slots * (kKv8TileTokens - 1);
   const int64_t groups = few < d.max_step_tokens ? few : d.max_step_tokens;
-  return (size_t)(kv8_waves(d.head_dim) + groups * d.num_kv_heads) * 16 * (d.head_dim + 4) * sizeof(float);
+  return (size_t)(kv8_waves(d.head_dim) + groups * d.num_kv_heads) * 16 * (d.head_dim + 4);
+}
+
+size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
+  // tiles times splits, where there is more than one, are kv8_tile_groups() or less
+  const size_t tiles = (size_t)kv8_tile_groups(d.head_dim) * 32 * kKv8TileWaves * (d.head_dim + 4);
+  return (kv8_attn_chunk_floats(d) + tiles) * sizeof(float);
 }
 
 template <int D>
 static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   const Kv8Plan& p = a.p;
   float* const part = static_cast<float*>(a.workspace);
+  float* const tpart = part + a.tile_part;
   hipError_t e;
+  int splits = 1;
   if (p.max_row >= kKv8TileTokens) {
-    constexpr int NW = 4, NC = 1;
-    const int tpt = NW * NC * (32 / (p.Hq / p.Hkv));
-    // rows of tiles have kKv8TileTokens or more
-    const dim3 grid(p.T / tpt + min(p.n, p.T / kKv8TileTokens), p.Hkv);
-    hipLaunchKernelGGL((attn8_tile_kernel<D, NW, NC>), grid, dim3(64 * NW), 0, a.stream, a);
+    const int G = p.Hq / p.Hkv;
+    splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
+    const dim3 grid(kv8_most_tiles(p.n, p.T, G) * splits, p.Hkv);
+    hipLaunchKernelGGL((attn8_tile_kernel<D, kKv8TileWaves, 1>), grid, dim3(64 * kKv8TileWaves), 0,
+                       a.stream, a, tpart);
     if ((e = hipGetLastError()) != hipSuccess) return e;
   }
   // as many as the rows can have, up to four rounds of the chip's waves
@@ -1127,12 +1237,17 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   else
     hipLaunchKernelGGL((attn8_chunk_kernel<D, 4>), grid, dim3(256), 0, a.stream, a, part);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  const int per = (p.T + 511) / 512;  // long steps hold few such tokens
-  const dim3 tokens((p.T + per - 1) / per, p.Hq);
-  if (p.T * p.Hq <= 512)  // a wave for each sum where the work-groups are few
-    hipLaunchKernelGGL((attn8_combine_kernel<D, 16>), tokens, dim3(1024), 0, a.stream, a, part, per);
+  const int per = min(p.max_row, kKv8TileTokens - 1);
+  const dim3 few(p.n * per, p.Hq);
+  if (p.n * per * p.Hq <= 512)  // a wave for each sum where the work-groups are few
+    hipLaunchKernelGGL((attn8_join_kernel<D, 16>), few, dim3(1024), 0, a.stream, a, part, per);
   else
-    hipLaunchKernelGGL((attn8_combine_kernel<D, 4>), tokens, dim3(256), 0, a.stream, a, part, per);
+    hipLaunchKernelGGL((attn8_join_kernel<D, 4>), few, dim3(256), 0, a.stream, a, part, per);
+  if (splits > 1) {
+    if ((e = hipGetLastError()) != hipSuccess) return e;
+    const dim3 tiles(kv8_most_tiles(p.n, p.T, p.Hq / p.Hkv), p.Hkv, D / 32);
+    hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, tiles, dim3(256), 0, a.stream, a, tpart, splits);
+  }
   return hipGetLastError();
 }
 

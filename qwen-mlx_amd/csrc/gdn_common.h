@@ -487,6 +487,7 @@ struct Kv8Plan {
   Kv8Row* rows;                 // [n]
   int32_t* blocks;              // [n + 1] pages that the rows before touch
   int32_t* parts;               // [n] attention's chunks (of a kv head) of the rows before, at most
+  int32_t* tiles;               // [n] its tiles of the rows before
 };
 // Attention of few new tokens (below kKv8TileTokens in a row): groups of 16 / G tokens, the pages
 // that a group sees in kv8_chunks() pieces or less, a partial result each, shared by `waves`
@@ -502,6 +503,19 @@ __host__ __device__ inline int kv8_chunk_waves(int n, int Hkv) {
 __host__ __device__ inline int kv8_chunks(int n, int Hkv, int D, int groups) {
   const int c = kv8_waves(D) / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
   return c < 1 ? 1 : c;
+}
+// Rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens, their pages in kv8_splits() pieces
+// or less, where the step's bounds let the tiles be few: about kv8_tile_groups() work-groups.
+constexpr int kKv8TileWaves = 4;
+__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 256 ? 512 : 1024; }
+__host__ __device__ inline int kv8_most_tiles(int n, int T, int G) {
+  const int a = T / (kKv8TileWaves * (32 / G)), b = T / kKv8TileTokens;
+  return a + (n < b ? n : b);
+}
+__host__ __device__ inline int kv8_splits(int n, int T, int Hkv, int G, int D) {
+  const int64_t most = (int64_t)kv8_most_tiles(n, T, G) * Hkv;
+  const int64_t s = kv8_tile_groups(D) / (most > 0 ? most : 1);
+  return s < 1 ? 1 : (int)s;
 }
 constexpr int kKv8Rows = 4096;  // rows of a step
 struct Kv8StepArgs {
@@ -549,9 +563,11 @@ struct Kv8AttnArgs {
   uint16_t* out;
   int64_t os, ohs;
   void* workspace;
+  size_t tile_part;             // floats of the chunks' partials in it, before the tiles'
   hipStream_t stream;
 };
 size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d);
+size_t kv8_attn_chunk_floats(const gdn_kv8_desc& d);
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a);
 
 // Rotary positions (gdn_rope.hip).

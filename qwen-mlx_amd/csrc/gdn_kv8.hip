@@ -245,9 +245,9 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     if (m > 0) atomicMax(&taken, before);  // admitted rows come before refused ones
     move(m, slot[i], have[i], 1, avail - 1 - b, -1, false);
   }
-  // pages that the row's tokens fall into, and attention's chunks
-  const int tpg = 16 / (p.Hq / p.Hkv);
-  int touched[R], chunks[R], nblk = 0, nchunk = 0;
+  // pages that the row's tokens fall into, attention's chunks and tiles
+  const int tpg = 16 / (p.Hq / p.Hkv), tpt = kKv8TileWaves * (32 / (p.Hq / p.Hkv));
+  int touched[R], chunks[R], tiles[R], nblk = 0, nchunk = 0, ntile = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = tid * R + i;
@@ -258,8 +258,10 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
       const int groups = (tok + tpg - 1) / tpg;
       chunks[i] = groups * min(need[i], kv8_chunks(p.n, p.Hkv, p.D, groups));
     }
+    tiles[i] = tok >= kKv8TileTokens ? (tok + tpt - 1) / tpt : 0;
     nblk += touched[i];
     nchunk += chunks[i];
+    ntile += tiles[i];
     if (r >= p.n) continue;
     p.rows[r] = Kv8Row{ok[i] ? slot[i] : -1, len[i], tok, cu[i]};
     if (ok[i]) p.owned[slot[i]] = need[i];
@@ -268,6 +270,7 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
   }
   int none;
   int c1 = block_scan<TH>(nchunk, red, none);
+  int t1 = p.max_row >= kKv8TileTokens ? block_scan<TH>(ntile, red, none) : 0;
   int b0 = block_scan<TH>(nblk, red, total);  // and orders the tables for the tokens
 #pragma unroll
   for (int i = 0; i < R; ++i) {
@@ -275,6 +278,8 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     if (r >= p.n) continue;
     p.blocks[r] = b0;
     p.parts[r] = c1;
+    p.tiles[r] = t1;
+    t1 += tiles[i];
     b0 += touched[i];
     c1 += chunks[i];
   }

@@ -325,6 +325,25 @@ def test_long_rows_and_loud_pages(gpu):
     p.kv.close()
 
 
+@pytest.mark.parametrize("hq,hk,dim", [(8, 1, 256), (12, 4, 128), (3, 3, 64)])
+def test_prompts_behind_long_contexts(gpu, hq, hk, dim):
+    """Few tiles whose keys are split: pieces that a tile does not reach, windows that leave
+    some out, tokens of tiles and of groups in one step, enough tokens for every kernel that
+    joins pieces."""
+    rng = np.random.default_rng(17)
+    p = Pair(5, 120, 60, hq=hq, hk=hk, dim=dim, tokens=4200)
+    p.step([0, 1], [0, 0], [2900, 1200])
+    p.append(rng)
+    p.step([0, 4, 1], [2900, 0, 1200], [35, 17, 3])
+    p.append(rng)
+    p.attention(rng, label="split tiles", gate=True)
+    p.attention(rng, label="split tiles, window", window=300, softcap=20.0)
+    p.step([1, 3, 0], [1203, 0, 2935], [16, 700, 1], tokens=900)
+    p.append(rng)
+    p.attention(rng, label="long step", slopes=[0.01] * hq)
+    p.kv.close()
+
+
 def test_nan_reaches_those_that_see_it(gpu):
     """A NaN key or value of a later token, of one outside the window, behind a cut."""
     import torch
