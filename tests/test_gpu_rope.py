@@ -111,6 +111,33 @@ def test_in_place_views_and_the_way_back(gpu):
     r.close()
 
 
+@pytest.mark.parametrize("dim,rot,interleaved", [(64, 32, False), (64, 32, True), (96, 46, False)])
+@pytest.mark.parametrize("T", [3, 600])
+def test_what_does_not_turn_keeps_its_bits(gpu, dim, rot, interleaved, T):
+    """Infinities and NaN among the dimensions behind rotary_dim and in tokens at negative
+    positions stay where they are; a turned pair takes only its own."""
+    import torch
+    import gdn_amd
+    inf, nan = float("inf"), float("nan")
+    x = torch.randn(T, 3, dim, device="cuda:0").bfloat16()
+    x[0, 1, rot], x[0, 2, rot + 3], x[1, 0, 0], x[1, 1, dim - 1] = inf, nan, nan, -inf
+    x[2, 0, 1] = nan
+    pos = torch.arange(T, dtype=torch.int32, device="cuda:0")
+    pos[1] = -1
+    out = torch.empty_like(x)
+    r = gdn_amd.Rope(dim, rot, 1.0e4, interleaved)
+    r.forward(pos, x, q_out=out)
+    bits = lambda t: t.view(torch.int16)  # noqa: E731
+    assert torch.equal(bits(out[:, :, rot:]), bits(x[:, :, rot:]))
+    assert torch.equal(bits(out[1]), bits(x[1]))
+    bad = torch.isnan(out[:, :, :rot])
+    bad[1] = False
+    want = torch.zeros_like(bad)
+    want[2, 0, [0, 1] if interleaved else [1, 1 + rot // 2]] = True
+    assert torch.equal(bad, want)
+    r.close()
+
+
 def test_refused_calls(gpu):
     import torch
     import gdn_amd
