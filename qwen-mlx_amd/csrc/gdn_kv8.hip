@@ -318,14 +318,38 @@ hipError_t launch_kv8_step(const Kv8StepArgs& a) {
 
 // --------------------------------------------------------------------- append --
 
+namespace {
+
+// The largest of the 16-bit halves' low 15 bits, both by v_pk_max_u16.
+__device__ __forceinline__ uint32_t pk_max(uint32_t a, uint32_t b) {
+  typedef uint16_t u16x2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(uint32_t, __builtin_elementwise_max(__builtin_bit_cast(u16x2, a),
+                                                                __builtin_bit_cast(u16x2, b)));
+}
+
+// Top bits of the NaN bytes of a word of e4m3.
+__device__ __forceinline__ uint32_t nan_bytes(uint32_t w) {
+  return ((w & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+}
+
+// Four bytes times 2^k (a factor), rounded anew.
+__device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
+  return e4m3_pair(__builtin_amdgcn_cvt_f32_fp8(w, 0) * f, __builtin_amdgcn_cvt_f32_fp8(w, 1) * f) |
+         e4m3_pair(__builtin_amdgcn_cvt_f32_fp8(w, 2) * f, __builtin_amdgcn_cvt_f32_fp8(w, 3) * f) << 16;
+}
+
+}  // namespace
+
 // grid (pages that the step can touch, Hkv, 2), block 256: one page's K (z = 0) or V tile of
-// a head. The new rows come into registers, the tile's old bytes into LDS; their largest
+// a head. The new rows and the tile's old bytes come into registers; their largest
 // magnitudes (as integers: bf16 and e4m3 patterns are in the order of their values) give the
-// exponent; the tile is put together in LDS and written whole. An item is 4 keys x 8
-// dims: 8 bytes of each key in K's order, a word of 4 keys for each dim in V's.
+// exponent. A page that is new or whose exponent changes is put together in LDS and written
+// whole; otherwise only the new rows' bytes are. An item is 4 keys x 8 dims: 8 bytes of each
+// key in K's order, a word of 4 keys for each dim in V's.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   constexpr int kChunks = D / 8, kItems = 16 * kChunks, kPer = (kItems + 255) / 256;
+  constexpr int kOld = kPage * D / 16 / 256;  // 16-byte pieces of a tile a thread
   __shared__ u32x4 tile4[kPage * D / 16];
   __shared__ uint32_t red[2][4];
   uint8_t* const tile = reinterpret_cast<uint8_t*>(tile4);
@@ -349,7 +373,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   const int64_t row0 = (int64_t)row.cu + first - len;
   const int was = old ? a.exps[head] : 0;
 
-  u32x4 x[kPer][4];
+  u32x4 x[kPer][4], ob[kOld];
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int it = tid + 256 * i, c = it % kChunks, g = it / kChunks;
@@ -361,38 +385,48 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
         x[i][k] = *reinterpret_cast<const u32x4*>(src + (row0 + kk) * stride + j * D + 8 * c);
     }
   }
-  if (old) {
-    for (int i = tid; i < kPage * D / 16; i += 256) tile4[i] = dst[i];
-    __syncthreads();
-  }
-  // largest finite magnitudes: of the new rows as bf16, of the old ones as e4m3 patterns
-  uint32_t mx = 0, mo = 0;
+  // bf16 magnitudes of the new rows, e4m3 ones of the old; infinities and NaN do not count
+  uint32_t mx2 = 0, mo2 = 0;
   bool nan = false;
+  if (old) {
 #pragma unroll
-  for (int i = 0; i < kPer; ++i) {
-    const int it = tid + 256 * i, c = it % kChunks, g = it / kChunks;
-    if (it >= kItems) break;
+    for (int i = 0; i < kOld; ++i) ob[i] = dst[tid + 256 * i];
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      if (4 * g + k < old) {
+    for (int i = 0; i < kOld; ++i) {
+      // the piece's keys: K one (16 dims of it), V four words of four
+      const int at = tid + 256 * i;
+      const int kkey = at / D * 16 + at % 16;
+      const int v0 = at / (2 * D) * 32 + 4 * (at / 16 % 2);
 #pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const int at = isv ? v_byte(4 * g + k, 8 * c + d, D) : k_byte(4 * g + k, 8 * c + d, D);
-          const uint32_t b = tile[at] & 0x7fu;
-          nan |= b == 0x7fu;
-          mo = max(mo, b == 0x7fu ? 0u : b);
-        }
-      } else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          const uint32_t lo = x[i][k][w] & 0x7fffu, hi = (x[i][k][w] >> 16) & 0x7fffu;
-          nan |= lo >= 0x7f80u || hi >= 0x7f80u;
-          mx = max(mx, max(lo >= 0x7f80u ? 0u : lo, hi >= 0x7f80u ? 0u : hi));
-        }
+      for (int w = 0; w < 4; ++w) {
+        const int n = isv ? old - (v0 + 8 * (w >> 1) + 16 * (w & 1)) : kkey < old ? 4 : 0;
+        const uint32_t b = n >= 4 ? ob[i][w] : n <= 0 ? 0u : ob[i][w] & ((1u << (8 * n)) - 1u);
+        ob[i][w] = b;  // nothing behind the old rows
+        const uint32_t top = nan_bytes(b);
+        nan |= top != 0;
+        const uint32_t m = b & 0x7f7f7f7fu & ~((top >> 7) * 0xffu);
+        mo2 = pk_max(mo2, pk_max(m & 0x00ff00ffu, (m >> 8) & 0x00ff00ffu));
       }
     }
   }
-  uint32_t both = mx << 8 | mo;  // one reduction each way: pairs do not mix below
+#pragma unroll
+  for (int i = 0; i < kPer; ++i)
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+#pragma unroll
+      for (int w = 0; w < 4; ++w) {
+        uint32_t m = x[i][k][w] & 0x7fff7fffu;
+        if ((m & 0x7f80u) == 0x7f80u) {
+          nan = true;
+          m &= 0xffff0000u;
+        }
+        if ((m & 0x7f800000u) == 0x7f800000u) {
+          nan = true;
+          m &= 0xffffu;
+        }
+        mx2 = pk_max(mx2, m);
+      }
+  uint32_t both = max(mx2 & 0xffffu, mx2 >> 16) << 8 | max(mo2 & 0xffffu, mo2 >> 16);
 #pragma unroll
   for (int off = 32; off > 0; off >>= 1) {
     const uint32_t u = __shfl_xor(both, off, 64);
@@ -404,8 +438,7 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
     red[1][tid >> 6] = wave_nan;
   }
   __syncthreads();
-  mx = mo = 0;
-  uint32_t any_nan = 0;
+  uint32_t mx = 0, mo = 0, any_nan = 0;
 #pragma unroll
   for (int i = 0; i < 4; ++i) {
     mx = max(mx, red[0][i] >> 8);
@@ -415,48 +448,57 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   const int eo = (int)(int8_t)was;
   const float vold = old ? e4m3_value(mo) * pow2(eo) : 0.f;
   const int en = exponent_of(__float_as_uint(fmaxf(__uint_as_float(mx << 16), vold)));
-  const float inv = pow2(-en), again = old ? pow2(eo - en) : 0.f;
+  const float inv = pow2(-en);
+  const bool whole = old == 0 || en != eo;
+  if (whole && old) {  // the old rows first, the new ones' bytes over them
+    const float f = pow2(eo - en);
+#pragma unroll
+    for (int i = 0; i < kOld; ++i)
+      tile4[tid + 256 * i] =
+          (u32x4){again4(ob[i][0], f), again4(ob[i][1], f), again4(ob[i][2], f), again4(ob[i][3], f)};
+    __syncthreads();
+  }
+  uint8_t* const to = whole ? tile : reinterpret_cast<uint8_t*>(dst);
 #pragma unroll
   for (int i = 0; i < kPer; ++i) {
     const int it = tid + 256 * i, c = it % kChunks, g = it / kChunks;
     if (it >= kItems) break;
+    if (old && (4 * g + 3 < old || 4 * g >= last)) continue;
     uint32_t b[4][2];  // per key 8 bytes
 #pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      float f[8];
-      if (4 * g + k < old) {
-#pragma unroll
-        for (int d = 0; d < 8; ++d) {
-          const int at = isv ? v_byte(4 * g + k, 8 * c + d, D) : k_byte(4 * g + k, 8 * c + d, D);
-          f[d] = e4m3_value(tile[at]) * again;
-        }
-      } else {
-#pragma unroll
-        for (int w = 0; w < 4; ++w) {
-          f[2 * w] = bf_lo(x[i][k][w]) * inv;
-          f[2 * w + 1] = bf_hi(x[i][k][w]) * inv;
-        }
-      }
+    for (int k = 0; k < 4; ++k)
 #pragma unroll
       for (int w = 0; w < 2; ++w)
-        b[k][w] = e4m3_pair(f[4 * w], f[4 * w + 1]) | e4m3_pair(f[4 * w + 2], f[4 * w + 3]) << 16;
-    }
+        b[k][w] = e4m3_pair(bf_lo(x[i][k][2 * w]) * inv, bf_hi(x[i][k][2 * w]) * inv) |
+                  e4m3_pair(bf_lo(x[i][k][2 * w + 1]) * inv, bf_hi(x[i][k][2 * w + 1]) * inv) << 16;
+    const bool all = old == 0 || (4 * g >= old && 4 * g + 3 < last);  // the item's four keys
     if (isv) {
 #pragma unroll
       for (int d = 0; d < 8; ++d) {
         const int w = d >> 2, s = 8 * (d & 3);
-        *reinterpret_cast<uint32_t*>(tile + v_byte(4 * g, 8 * c + d, D)) =
-            ((b[0][w] >> s) & 0xffu) | ((b[1][w] >> s) & 0xffu) << 8 |
-            ((b[2][w] >> s) & 0xffu) << 16 | ((b[3][w] >> s) & 0xffu) << 24;
+        uint8_t* const at = to + v_byte(4 * g, 8 * c + d, D);
+        if (all) {
+          *reinterpret_cast<uint32_t*>(at) =
+              ((b[0][w] >> s) & 0xffu) | ((b[1][w] >> s) & 0xffu) << 8 |
+              ((b[2][w] >> s) & 0xffu) << 16 | ((b[3][w] >> s) & 0xffu) << 24;
+        } else {
+#pragma unroll
+          for (int k = 0; k < 4; ++k)
+            if (4 * g + k >= old && 4 * g + k < last) at[k] = (uint8_t)(b[k][w] >> s);
+        }
       }
     } else {
 #pragma unroll
       for (int k = 0; k < 4; ++k)
-        *reinterpret_cast<u32x2*>(tile + k_byte(4 * g + k, 8 * c, D)) = (u32x2){b[k][0], b[k][1]};
+        if (all || (4 * g + k >= old && 4 * g + k < last))
+          *reinterpret_cast<u32x2*>(to + k_byte(4 * g + k, 8 * c, D)) = (u32x2){b[k][0], b[k][1]};
     }
   }
-  __syncthreads();
-  for (int i = tid; i < kPage * D / 16; i += 256) dst[i] = tile4[i];
+  if (whole) {
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kOld; ++i) dst[tid + 256 * i] = tile4[tid + 256 * i];
+  }
   if (tid == 0) a.exps[head] = (en & 0xff) | (any_nan ? kNanFlag : 0);
 }
 
@@ -478,50 +520,46 @@ hipError_t launch_kv8_append(const Kv8AppendArgs& a) {
 
 namespace {
 
-// grid of 256 threads' work-groups from `from` on: 8 dims of a head of a token a thread.
+// grid (ceil(m / 64) from `from` on, Hkv * D / 32, 2), block 256: 64 places, 32 dims of a head, K
+// (z = 0) or V; 8 dims of a place a thread. Places that run through a page, as a sequence's do,
+// share the cache lines of V's bytes.
 __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8GatherArgs a, int64_t from) {
   const Kv8Plan& p = a.p;
-  const int chunks = p.Hkv * p.D / 8;
-  const int64_t at = (from + blockIdx.x) * 256 + threadIdx.x;
-  const int64_t t = at / chunks;
-  if (t >= a.m) return;
-  const int c = (int)(at - t * chunks), j = c / (p.D / 8), d = (c - j * (p.D / 8)) * 8;
+  const int z = blockIdx.z, parts = p.D / 32, j = blockIdx.y / parts;
+  const int d = (blockIdx.y - j * parts) * 32 + 8 * (threadIdx.x & 3);
+  uint16_t* const out = z ? a.v_out : a.k_out;
+  const int64_t t = (from + blockIdx.x) * 64 + (threadIdx.x >> 2);
+  if (!out || t >= a.m) return;
   const int place = a.map[t];
-  const bool there = place >= 0 && place < p.num_pages * kPage;
-  const int page = there ? place / kPage : 0, kk = place & (kPage - 1);
+  u32x4 o = {0u, 0u, 0u, 0u};
+  if (place >= 0 && place < p.num_pages * kPage) {
+    const int kk = place & (kPage - 1);
+    const size_t head = ((size_t)(place / kPage) * 2 + z) * p.Hkv + j;
+    const uint8_t* const tile = a.pages + head * ((size_t)kPage * p.D);
+    const float s = pow2((int)(int8_t)a.exps[head]);
+    float f[8];
+    if (z) {
 #pragma unroll
-  for (int z = 0; z < 2; ++z) {
-    uint16_t* const out = z ? a.v_out : a.k_out;
-    if (!out) continue;
-    u32x4 o = {0u, 0u, 0u, 0u};
-    if (there) {
-      const size_t head = ((size_t)page * 2 + z) * p.Hkv + j;
-      const uint8_t* const tile = a.pages + head * ((size_t)kPage * p.D);
-      const float s = pow2((int)(int8_t)a.exps[head]);
-      float f[8];
-      if (z) {
+      for (int i = 0; i < 8; ++i) f[i] = e4m3_value(tile[v_byte(kk, d + i, p.D)]) * s;
+    } else {
+      const u32x2 b = *reinterpret_cast<const u32x2*>(tile + k_byte(kk, d, p.D));
 #pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = e4m3_value(tile[v_byte(kk, d + i, p.D)]) * s;
-      } else {
-        const u32x2 b = *reinterpret_cast<const u32x2*>(tile + k_byte(kk, d, p.D));
-#pragma unroll
-        for (int i = 0; i < 8; ++i) f[i] = e4m3_value((b[i >> 2] >> (8 * (i & 3))) & 0xffu) * s;
-      }
-      // four significant bits: exact in bf16
-      o = (u32x4){f2bf2(f[0], f[1]), f2bf2(f[2], f[3]), f2bf2(f[4], f[5]), f2bf2(f[6], f[7])};
+      for (int i = 0; i < 8; ++i) f[i] = e4m3_value((b[i >> 2] >> (8 * (i & 3))) & 0xffu) * s;
     }
-    *reinterpret_cast<u32x4*>(out + t * (z ? a.vs : a.ks) + j * p.D + d) = o;
+    // four significant bits: exact in bf16
+    o = (u32x4){f2bf2(f[0], f[1]), f2bf2(f[2], f[3]), f2bf2(f[4], f[5]), f2bf2(f[6], f[7])};
   }
+  *reinterpret_cast<u32x4*>(out + t * (z ? a.vs : a.ks) + j * p.D + d) = o;
 }
 
 }  // namespace
 
 hipError_t launch_kv8_gather(const Kv8GatherArgs& a) {
-  const int64_t groups = ((int64_t)a.m * (a.p.Hkv * a.p.D / 8) + 255) / 256;
-  constexpr int64_t kGroups = 1 << 22;  // of a launch: a grid holds less than 2^32 threads
+  const int64_t groups = ((int64_t)a.m + 63) / 64;
+  constexpr int64_t kGroups = 1 << 16;
   for (int64_t g = 0; g < groups; g += kGroups) {
-    const unsigned n = (unsigned)(groups - g < kGroups ? groups - g : kGroups);
-    hipLaunchKernelGGL(kv8_gather_kernel, dim3(n), dim3(256), 0, a.stream, a, g);
+    const dim3 grid((unsigned)(groups - g < kGroups ? groups - g : kGroups), a.p.Hkv * (a.p.D / 32), 2);
+    hipLaunchKernelGGL(kv8_gather_kernel, grid, dim3(256), 0, a.stream, a, g);
     const hipError_t e = hipGetLastError();
     if (e != hipSuccess) return e;
   }

@@ -19,7 +19,7 @@ struct Raw {
     const u32x4* s = F32 ? reinterpret_cast<const u32x4*>(static_cast<const float*>(p) + i)
                          : reinterpret_cast<const u32x4*>(static_cast<const uint16_t*>(p) + i);
 #pragma unroll
-    for (int k = 0; k < (F32 ? 2 : 1); ++k) v[k] = s[k];
+    for (int k = 0; k < (F32 ? 2 : 1); ++k) v[k] = __builtin_nontemporal_load(s + k);
   }
   __device__ __forceinline__ void zero() {
 #pragma unroll
@@ -46,11 +46,12 @@ template <bool F32>
 __device__ __forceinline__ void store8(void* p, int64_t i, const float* f) {
   if constexpr (F32) {
     v4f* d = reinterpret_cast<v4f*>(static_cast<float*>(p) + i);
-    d[0] = (v4f){f[0], f[1], f[2], f[3]};
-    d[1] = (v4f){f[4], f[5], f[6], f[7]};
+    __builtin_nontemporal_store((v4f){f[0], f[1], f[2], f[3]}, d);
+    __builtin_nontemporal_store((v4f){f[4], f[5], f[6], f[7]}, d + 1);
   } else {
-    *reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i) =
-        (u32x4){f2bf2(f[0], f[1]), f2bf2(f[2], f[3]), f2bf2(f[4], f[5]), f2bf2(f[6], f[7])};
+    __builtin_nontemporal_store(
+        (u32x4){f2bf2(f[0], f[1]), f2bf2(f[2], f[3]), f2bf2(f[4], f[5]), f2bf2(f[6], f[7])},
+        reinterpret_cast<u32x4*>(static_cast<uint16_t*>(p) + i));
   }
 }
 
