@@ -337,12 +337,13 @@ def _heads(t, dev: int, size, types, what: str):
     if t.size() != size or t.get_device() != dev or t.dtype not in types:
         _refuse(t, dev, size, types, what)
     a, b, c = t.stride()
-    if c != 1 and size[2] > 1:
+    if c != 1:
         raise ValueError(f"{what} must have contiguous heads")
-    if size[1] == 1:
-        b = size[2]
-    if size[0] == 1:
-        a = size[1] * b
+    n, h, d = size
+    if h == 1:
+        b = d
+    if n == 1:
+        a = h * b
     return t.data_ptr(), a, b
 
 
@@ -993,27 +994,31 @@ class Rope:
         """q [tokens, heads, dim] and k, bf16 or f32, at positions pos [tokens] int32 -> q_out,
         k_out (None: in place); norm weights bf16 [dim] for the norms before the turn. A token
         at a negative position is copied. inverse: turns back."""
-        dev = self.device
-        (T,) = pos.size()
-        pp = _dense(pos, dev, (T,), _IS_I32, "pos")
+        dev, D = self.device, self.D
+        tsize = pos.size()
+        pp = _dense(pos, dev, tsize, _IS_I32, "pos")
+        T, qh = tsize[0], q.size(1)
         f32 = q.dtype in _IS_F32
         types = _IS_F32 if f32 else _IS_BF16
-
-        def rows(x, out, w, what):
-            size = (T, x.size(1), self.D)
-            xp, xs, xh = _heads(x, dev, size, types, what)
-            op, os_, oh = (xp, xs, xh) if out is None else _heads(out, dev, size, types,
-                                                                  what + "_out")
-            wp = None if w is None else _dense(w, dev, (self.D,), _IS_BF16, what + "_norm_w")
-            return RopeRows(xp, op, size[1], xs, xh, os_, oh, wp)
-
-        if k is None and (k_out is not None or k_norm_w is not None):
+        size = (T, qh, D)
+        xp, xs, xh = op, os_, oh = _heads(q, dev, size, types, "q")
+        if q_out is not None:
+            op, os_, oh = _heads(q_out, dev, size, types, "q_out")
+        wp = None if q_norm_w is None else _dense(q_norm_w, dev, (D,), _IS_BF16, "q_norm_w")
+        qr = RopeRows(xp, op, qh, xs, xh, os_, oh, wp)
+        kr = None
+        if k is not None:
+            kh = k.size(1)
+            size = (T, kh, D)
+            xp, xs, xh = op, os_, oh = _heads(k, dev, size, types, "k")
+            if k_out is not None:
+                op, os_, oh = _heads(k_out, dev, size, types, "k_out")
+            wp = None if k_norm_w is None else _dense(k_norm_w, dev, (D,), _IS_BF16, "k_norm_w")
+            kr = ctypes.byref(RopeRows(xp, op, kh, xs, xh, os_, oh, wp))
+        elif k_out is not None or k_norm_w is not None:
             raise ValueError("k_out and k_norm_w go with k")
-        qr = rows(q, q_out, q_norm_w, "q")
-        kr = None if k is None else ctypes.byref(rows(k, k_out, k_norm_w, "k"))
-        _check(self.lib.gdn_rope_forward(self.handle, T, pp, ctypes.byref(qr), kr, int(f32),
-                                         float(eps), int(bool(inverse)),
-                                         _raw_stream(dev) if stream is None
+        _check(self.lib.gdn_rope_forward(self.handle, T, pp, ctypes.byref(qr), kr, f32, eps,
+                                         bool(inverse), _raw_stream(dev) if stream is None
                                          else stream.cuda_stream))
 
     def close(self):
