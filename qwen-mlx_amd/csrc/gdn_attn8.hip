@@ -9,8 +9,9 @@
 // its rounding and the 4 that are left, times 16 (numbers below 2^-14 of the head's
 // largest lose bits, 2^-22 of it at most). For P V the values convert exactly into f16, and P,
 // in [0, 2^8] as the running maximum follows by steps of 2^8, is rounded to it: 11 bits, three
-// more than bf16. The pages' exponents stay outside: the keys' multiplies the scores, the
-// values' is the unit of the running outputs, which are rescaled where it changes.
+// more than bf16. The pages' exponents stay outside: the keys' multiplies the scores; the
+// outputs run in units of 2^(unit - 6), and P carries 2^(6 + the values' exponent - unit), which
+// f16 has room for from 2^0 to 2^7: only beyond that are the outputs rescaled.
 #include "gdn_common.h"
 
 namespace gdn {
@@ -22,6 +23,11 @@ constexpr int kBlock = 32;  // keys of a step of the running softmax: half a pag
 constexpr int kNanFlag = 1 << 16;
 constexpr int kSplitPages = 8;  // of a tile's split at least
 constexpr float kStep = 8.f;  // log2 steps of the running maximum
+constexpr int kUnit = 6;      // the outputs' unit is 2^(unit - kUnit)
+// Whether values of exponent ev go on in a unit: P's factor 2^(kUnit + ev - unit) is in [2^0, 2^7]
+__device__ __forceinline__ bool unit_holds(int ev, int unit) {
+  return ev - unit >= -kUnit && ev - unit <= 1;
+}
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
 typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
@@ -295,7 +301,7 @@ __device__ __forceinline__ uint32_t first_scores(int n, int count) {
 
 // The running softmax of 16 columns over blocks of 32 keys: lane (g4, c) holds keys 4 g4 + r and
 // 16 + 4 g4 + r of a block for column c, and dims 16 d + 4 g4 + r of its outputs in units of
-// 2^unit.
+// 2^(unit - kUnit).
 template <int D>
 struct Online {
   float m, l;
@@ -345,20 +351,23 @@ struct Online {
                      fmaxf(fmaxf(s[4], s[5]), fmaxf(s[6], s[7])));
     bm = max_xor16_32(bm);
     // m follows the maximum once it is passed by 2^kStep: weights are at most that
-    if (__builtin_expect(__any(bm > m + kStep) || ev != unit, 0)) {
+    if (__builtin_expect(__any(bm > m + kStep) || !unit_holds(ev, unit), 0)) {
       const float mn = fmaxf(m, bm);
       float corr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;  // m = -inf: 0
       m = mn;
       l *= corr;
-      corr = __builtin_amdgcn_ldexpf(corr, unit - ev);
-      unit = ev;
+      if (!unit_holds(ev, unit)) {
+        corr = __builtin_amdgcn_ldexpf(corr, unit - (ev + 2));
+        unit = ev + 2;  // room either way
+      }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) O[d] *= corr;
     }
-    const float mref = m == -INFINITY ? 0.f : m;
+    const int up = kUnit + ev - unit;
+    const float mref = (m == -INFINITY ? 0.f : m) - (float)up;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - mref);
-    l += ((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7]));
+    l = fmaf(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])), pow2(-up), l);
     return (u32x4){pk_f16(s[0], s[1]), pk_f16(s[2], s[3]), pk_f16(s[4], s[5]), pk_f16(s[6], s[7])};
   }
 
@@ -598,7 +607,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
     if constexpr (W == 1) {
       if (!x.valid) continue;
       if (ch.nch == 1) {
-        const float inv = __builtin_amdgcn_ldexpf(1.0f / lw, on.unit);
+        const float inv = __builtin_amdgcn_ldexpf(1.0f / lw, on.unit - kUnit);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
           float o[4];
@@ -612,7 +621,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
           pr[0] = on.m;
           pr[1] = lw;
         }
-        const float one = __builtin_amdgcn_ldexpf(1.0f, on.unit);
+        const float one = __builtin_amdgcn_ldexpf(1.0f, on.unit - kUnit);
 #pragma unroll
         for (int d = 0; d < DB; ++d)
           *reinterpret_cast<f32x4*>(pr + 4 + 16 * d + 4 * g4) = on.O[d] * one;
@@ -627,7 +636,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
     for (int i = 1; i < W; ++i) M = fmaxf(M, ms[i][c]);
     const float fac = on.m == -INFINITY ? (lw == 0.f ? 0.f : 1.f) : exp2f(on.m - M);
     if (g4 == 0) ls[w][c] = lw * fac;
-    const float fo = __builtin_amdgcn_ldexpf(fac, on.unit);
+    const float fo = __builtin_amdgcn_ldexpf(fac, on.unit - kUnit);
     if (x.valid) {
 #pragma unroll
       for (int d = 0; d < DB; ++d) os[w][c][4 * d + g4] = on.O[d] * fo;
@@ -802,7 +811,7 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, co
 // from LDS, and a value's conversion, serves 32 NC columns.
 //
 // Lane (hf, c), hf = lane / 32, holds keys 8 i + 4 hf + r of a block of 32 (i, r = 0 .. 3) for
-// column c of each group, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^unit.
+// column c of each group, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^(unit - kUnit).
 //
 // With one wave a SIMD (the outputs of 64 columns at D = 256 are 256 registers) the overlap of
 // products and softmax is laid out in program order, a block apart: the products of block
@@ -1002,40 +1011,44 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   };
   // the running maximum follows once it is passed by 2^kStep; ev: the exponent of the block's values
   auto follow = [&](const float* bm, int ev) __attribute__((always_inline)) {
-    bool up = ev != unit;
+    bool up = !unit_holds(ev, unit);
 #pragma unroll
     for (int n = 0; n < NC; ++n) up |= __any(bm[n] > m[n] + kStep);
     if (__builtin_expect(up, 0)) {
+      const int to = unit_holds(ev, unit) ? unit : ev + 2;  // room either way
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
         const float mn = fmaxf(m[n], bm[n]);
         float corr = mn > m[n] ? __builtin_amdgcn_exp2f(m[n] - mn) : 1.0f;  // m = -inf: 0
         m[n] = mn;
         l[n] *= corr;
-        corr = __builtin_amdgcn_ldexpf(corr, unit - ev);
+        corr = __builtin_amdgcn_ldexpf(corr, unit - to);
 #pragma unroll
         for (int i = 0; i < NT; ++i) {
           O[n][i] *= corr;
           __builtin_amdgcn_sched_barrier(0);  // not all of them in registers of their own at once
         }
       }
-      unit = ev;
+      unit = to;
     }
   };
   u32x4 P[NC][2];
-  auto weights = [&](const f32x16* Sc) __attribute__((always_inline)) {
+  auto weights = [&](const f32x16* Sc, int ev) __attribute__((always_inline)) {
+    const int up = kUnit + ev - unit;
 #pragma unroll
     for (int n = 0; n < NC; ++n) {
-      const float mref = m[n] == -INFINITY ? 0.f : m[n];
+      const float mref = (m[n] == -INFINITY ? 0.f : m[n]) - (float)up;
       float e[16], sum = 0.f;
 #pragma unroll
       for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(Sc[n][i], mk[n], -mref));
 #pragma unroll
       for (int i = 0; i < 16; i += 4) sum += (e[i] + e[i + 1]) + (e[i + 2] + e[i + 3]);
-      l[n] += sum;
+      l[n] = fmaf(sum, pow2(-up), l[n]);
       // keys 4 hf + r and 16 + 4 hf + r, then those 8 further on: the order of the values' bytes
       P[n][0] = (u32x4){pk_f16(e[0], e[1]), pk_f16(e[2], e[3]), pk_f16(e[8], e[9]), pk_f16(e[10], e[11])};
       P[n][1] = (u32x4){pk_f16(e[4], e[5]), pk_f16(e[6], e[7]), pk_f16(e[12], e[13]), pk_f16(e[14], e[15])};
+      // here, beside the scores' products, not behind the branches that follow
+      asm volatile("" : "+v"(P[n][0]), "+v"(P[n][1]));
     }
   };
   auto values = [&](const u32x4* lv, int hb) __attribute__((always_inline)) {
@@ -1118,7 +1131,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
     uint32_t was[NC];
     if (!idle) {
       scores(lk, 1, Sn);
-      weights(S);
+      weights(S, ev);
 #pragma unroll
       for (int n = 0; n < NC; ++n) was[n] = seen[n];
       prepare(Sn, key0 + kBlock, ek);
@@ -1140,7 +1153,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
     if (!idle) {
       // behind the last page: scores of a page that was copied again, which nothing uses
       scores(lkn, 0, S);
-      weights(Sn);
+      weights(Sn, ev);
 #pragma unroll
       for (int n = 0; n < NC; ++n) was[n] = seen[n];
       prepare(S, span.page(min(v + 1, count - 1)) * kPage, ekn);
@@ -1177,7 +1190,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
         pr[0] = m[n];
         pr[1] = ln;
       }
-      const float one = __builtin_amdgcn_ldexpf(1.0f, unit);
+      const float one = __builtin_amdgcn_ldexpf(1.0f, unit - kUnit);
 #pragma unroll
       for (int i = 0; i < NT; ++i)
 #pragma unroll
@@ -1186,7 +1199,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
               (f32x4){O[n][i][4 * g], O[n][i][4 * g + 1], O[n][i][4 * g + 2], O[n][i][4 * g + 3]} * one;
       continue;
     }
-    const float inv = __builtin_amdgcn_ldexpf(1.0f / ln, unit);
+    const float inv = __builtin_amdgcn_ldexpf(1.0f / ln, unit - kUnit);
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
