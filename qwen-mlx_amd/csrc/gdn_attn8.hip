@@ -822,9 +822,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
   static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
-  constexpr bool kLowInLds = D == 256;
   __shared__ u32x4 lk0[kTile16], lk1[kTile16], lv0[kTile16], lv1[kTile16];
-  __shared__ u32x4 lq[kLowInLds ? NW * NC : 1][kLowInLds ? 2 * NK : 1][64];
   const Kv8Plan& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, c = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -913,7 +911,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
   copy(v0 + 1, lv1, v_shift);
 
   // q: dims 64 i + 32 hf .. + 31 of column c, in two e4m3 parts
-  u32x4 qh[NC][2 * NK], ql[kLowInLds ? 1 : NC][kLowInLds ? 1 : 2 * NK];
+  u32x4 qh[NC][2 * NK], ql[NC][2 * NK];
 #pragma unroll
   for (int n = 0; n < NC; ++n) {
     u32x4 q[4 * NK];
@@ -921,10 +919,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
 #pragma unroll
     for (int i = 0; i < 2 * NK; ++i) {
       qh[n][i] = q[2 * i];
-      if constexpr (kLowInLds)
-        lq[w * NC + n][i][lane] = q[2 * i + 1];
-      else
-        ql[n][i] = q[2 * i + 1];
+      ql[n][i] = q[2 * i + 1];
     }
   }
   // this lane's pieces: of key c of 32 (NK KiB for 16 keys), and of dim c of 32
@@ -942,7 +937,6 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) Sn[n][i] = 0.f;
-    asm volatile("" ::: "memory");  // q's low parts are re-read from LDS for every block
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
       const int at = kat + (2 * hb * NK + i) * 64;
@@ -952,13 +946,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
         Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
             kk, both(qh[n][2 * i], qh[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kOne);
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        const i32x8 qq = kLowInLds
-                             ? both(lq[w * NC + n][2 * i][lane], lq[w * NC + n][2 * i + 1][lane])
-                             : both(ql[kLowInLds ? 0 : n][kLowInLds ? 0 : 2 * i],
-                                    ql[kLowInLds ? 0 : n][kLowInLds ? 0 : 2 * i + 1]);
-        Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kk, qq, Sn[n], 0, 0, 0, kOne, 0, kLow);
-      }
+      for (int n = 0; n < NC; ++n)
+        Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
+            kk, both(ql[n][2 * i], ql[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kLow);
     }
   };
   // Scores of the block at kb that need more than a factor: x = mk * S in any case
