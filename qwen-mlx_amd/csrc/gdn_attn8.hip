@@ -813,12 +813,12 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, co
 // Lane (hf, c), hf = lane / 32, holds keys 8 i + 4 hf + r of a block of 32 (i, r = 0 .. 3) for
 // column c of each group, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^(unit - kUnit).
 //
-// With one wave a SIMD (the outputs of 64 columns at D = 256 are 256 registers) the overlap of
-// products and softmax is laid out in program order, a block apart: the products of block
-// k + 1's scores beside the exponentials of block k, those of block k's values beside the
-// maxima of block k + 1.
+// Two waves a SIMD or more, each in at most 256 registers (at D = 256 its outputs are 128 of them,
+// q's parts 64): one's products run beside the other's softmax, so that a wave's own steps stay
+// in order. One wave a SIMD with the steps of two blocks side by side took 665 us where this
+// takes 531 (8,192 tokens of 24 query heads over 4 of 256 dims).
 template <int D, int NW, int NC>
-__global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part) {
+__global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part) {
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
   static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
@@ -1100,67 +1100,36 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 1 : 2) void attn8_tile_kernel(K
     ev = (int)(int8_t)wv;
     nan = (wv & kNanFlag) != 0;
   };
-  int ek, ev;
-  bool nan;
-  exps_of(v0, ek, ev, nan);
-  if (!idle) {
-    scores(lk0, 0, S);
-    prepare(S, span.page(v0) * kPage, ek);
-    maxima(S, bm);
-    follow(bm, ev);
-  }
-  // Page v in buffers b. On entry the scores and maxima of its first half are formed, its K and V
-  // have landed, and the next page's are on their way, K first.
+  // Page v in buffers b, which has landed; the next page's copies are on their way.
   auto page = [&](int v, auto bc) __attribute__((always_inline)) {
     constexpr int b = decltype(bc)::value;
     u32x4* const lk = b ? lk1 : lk0;
     u32x4* const lv = b ? lv1 : lv0;
-    const u32x4* const lkn = b ? lk0 : lk1;
     const int key0 = span.page(v) * kPage;
-    f32x16 Sn[NC];
-    uint32_t was[NC];
+    int ek, ev;
+    bool nan;
+    exps_of(v, ek, ev, nan);
     if (!idle) {
-      scores(lk, 1, Sn);
-      weights(S, ev);
 #pragma unroll
-      for (int n = 0; n < NC; ++n) was[n] = seen[n];
-      prepare(Sn, key0 + kBlock, ek);
-      if (__builtin_expect(nan || key0 + kBlock > total, 0)) clean(v, lv, 0, key0, was);
-      values(lv, 0);
-      maxima(Sn, bm);
-      follow(bm, ev);
+      for (int hb = 0; hb < 2; ++hb) {
+        const int kb = key0 + hb * kBlock;
+        scores(lk, hb, S);
+        prepare(S, kb, ek);
+        maxima(S, bm);
+        follow(bm, ev);
+        weights(S, ev);
+        if (__builtin_expect(nan || kb + kBlock > total, 0)) clean(v, lv, hb, kb, seen);
+        values(lv, hb);
+      }
     }
-    // the next page's K has landed everywhere, and no wave reads this page's any more
-    __builtin_amdgcn_s_waitcnt(0x0F70 | kLoads);  // vmcnt(kLoads)
+    // the next page has landed everywhere, and no wave reads this one any more
+    __builtin_amdgcn_s_waitcnt(0x0F70);
     lds_barrier();
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
     if (min(v + 2, count - 1) - vbase >= 64) ids(v);
     copy(v + 2, lk, 0);
-    __builtin_amdgcn_sched_barrier(0);
-    int ekn, evn;
-    bool nann;
-    exps_of(v + 1, ekn, evn, nann);
-    if (!idle) {
-      // behind the last page: scores of a page that was copied again, which nothing uses
-      scores(lkn, 0, S);
-      weights(Sn, ev);
-#pragma unroll
-      for (int n = 0; n < NC; ++n) was[n] = seen[n];
-      prepare(S, span.page(min(v + 1, count - 1)) * kPage, ekn);
-      if (__builtin_expect(nan || key0 + kPage > total, 0)) clean(v, lv, 1, key0 + kBlock, was);
-      values(lv, 1);
-      maxima(S, bm);
-      if (v + 1 < count) follow(bm, evn);
-    }
-    // the next page's V has landed everywhere, and no wave reads this page's any more
-    __builtin_amdgcn_s_waitcnt(0x0F70 | kLoads);
-    lds_barrier();
-    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "workgroup", "global");
     copy(v + 2, lv, v_shift);
     __builtin_amdgcn_sched_barrier(0);
-    ek = ekn;
-    ev = evn;
-    nan = nann;
   };
   int v = v0;
 #pragma nounroll
