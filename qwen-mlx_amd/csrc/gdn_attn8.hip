@@ -128,7 +128,7 @@ __device__ __forceinline__ int wave_scan(int s) {
 }
 
 struct Found {
-  int r, first;  // row and its first item; r = -1: none
+  int r, first;  // row and its first item; r = -1: none, and first the items of all rows
   Kv8Row row;
 };
 
@@ -154,7 +154,19 @@ __device__ __forceinline__ Found find_row(const Kv8Plan& p, int g, F items) {
     }
     before += total;
   }
-  return Found{-1, 0, {-1, 0, 0, 0}};
+  return Found{-1, before, {-1, 0, 0, 0}};
+}
+
+// Zeros for those of the 64 tokens from t0 on whose rows are refused, by `threads` threads.
+__device__ __forceinline__ void zero_refused(const Kv8AttnArgs& a, int64_t t0, int tid, int threads) {
+  const int64_t mine = t0 + (threadIdx.x & 63);
+  const int quads = a.p.D / 4;
+  uint64_t none = __ballot(mine < a.p.T && a.p.tok_row[mine] == -1);
+  for (; none; none &= none - 1) {
+    const int64_t t = t0 + __ffsll((unsigned long long)none) - 1;
+    for (int i = tid; i < a.p.Hq * quads; i += threads)
+      *reinterpret_cast<u32x2*>(a.out + t * a.os + (i / quads) * a.ohs + i % quads * 4) = (u32x2){0u, 0u};
+  }
 }
 
 // Visible keys of a group of tokens, as pages: [0, pre) then [lo, end).
@@ -440,7 +452,7 @@ struct Chunks {
 };
 __device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpg) {
   Chunks c{0, 1, 0};
-  if (row.fresh <= 0 || row.fresh >= kKv8TileTokens) return c;
+  if (row.fresh <= 0) return c;
   c.groups = (row.fresh + tpg - 1) / tpg;
   const int total = row.pos + row.fresh;
   const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
@@ -460,18 +472,21 @@ __device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& 
   return c;
 }
 
-// Items of a row of tiles: (tile from the last one on, split). By row alone where pages are cut.
+// Items of a row in a step of tiles: (tile from the last one on, split). By row alone where pages
+// are cut, and by the step's bounds, which rows of fewer than kKv8TileTokens tokens have their own
+// of: they are few tiles with as many pages as any.
 struct Splits {
   int tiles, cp, n;
 };
 __device__ __forceinline__ Splits splits_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpt,
-                                            int most_splits) {
+                                            const Kv8Splits& most_splits) {
   Splits s{0, 1, 0};
-  if (row.fresh < kKv8TileTokens) return s;
+  if (row.fresh <= 0) return s;
   s.tiles = (row.fresh + tpt - 1) / tpt;
   s.n = 1;
   s.cp = INT32_MAX / 2;
-  if (most_splits > 1) {
+  const int pieces = row.fresh < kKv8TileTokens ? most_splits.few : most_splits.many;
+  if (pieces > 1) {
     const int total = row.pos + row.fresh;
     const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
     int most = 0;  // of the first and the last tile's pages, as in chunks_of
@@ -480,10 +495,20 @@ __device__ __forceinline__ Splits splits_of(const Kv8AttnArgs& a, const Kv8Row& 
       most = max(most, span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total).count());
     }
     most = min(most + (s.tiles > 1 && a.window > 0 ? 1 : 0), (total + kPage - 1) / kPage);
-    s.cp = max((most - 1) / most_splits + 1, kSplitPages);
+    s.cp = max((most - 1) / pieces + 1, kSplitPages);
     s.n = (most + s.cp - 1) / s.cp;
   }
   return s;
+}
+// Partial results of a tile's splits: 128 columns of D + 4 floats each
+template <int D>
+__device__ __forceinline__ float* split_part(const Kv8Plan& p, float* part, const Kv8Splits& most, int r,
+                                             int fresh, int tile, int j) {
+  constexpr size_t kStride = (size_t)32 * kKv8TileWaves * (D + 4);
+  if (fresh >= kKv8TileTokens)
+    return part + ((size_t)(p.tiles[r] + tile) * p.Hkv + j) * most.many * kStride;
+  const size_t at = (size_t)r * kv8_few_tiles(p.Hq / p.Hkv) + tile;
+  return part + (kv8_tile_groups(D) + (at * p.Hkv + j) * most.few) * kStride;
 }
 
 }  // namespace
@@ -669,14 +694,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
     }
   }
   // tokens of refused rows: zeros, each work-group its share of the step's
-  for (int t0 = blockIdx.x * 64; t0 < p.T; t0 += gridDim.x * 64) {
-    uint64_t none = __ballot(t0 + lane < p.T && p.tok_row[t0 + lane] == -1);
-    for (; none; none &= none - 1) {
-      const int64_t t = t0 + __ffsll((unsigned long long)none) - 1;
-      for (int i = tid; i < p.Hq * (D / 4); i += 64 * W)
-        *reinterpret_cast<u32x2*>(a.out + t * a.os + (i / (D / 4)) * a.ohs + i % (D / 4) * 4) = (u32x2){0u, 0u};
-    }
-  }
+  for (int64_t t0 = blockIdx.x * 64; t0 < p.T; t0 += gridDim.x * 64) zero_refused(a, t0, tid, 64 * W);
 }
 
 // Rows of few tokens: grid (n * per, Hq), block 64 W; token k < per of row r, a head: its chunks,
@@ -762,24 +780,21 @@ __global__ __launch_bounds__(64 * W) void attn8_join_kernel(Kv8AttnArgs a, const
   }
 }
 
-// Rows of tiles whose pages are split: grid (tiles at most, Hkv, D / 32), block 256, 32 dims of a
-// tile's 128 columns: 8 lanes a column, its splits in order.
+// Tiles whose pages are split: grid (tiles at most, Hkv, D / 32), block 256, 32 dims of a tile's 128
+// columns: 8 lanes a column, its splits in order.
 template <int D>
-__global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, const float* __restrict__ part,
-                                                               int most_splits) {
+__global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, float* __restrict__ part,
+                                                               Kv8Splits most_splits) {
   constexpr int kCols = 32 * kKv8TileWaves;
   constexpr size_t kStride = (size_t)kCols * (D + 4);
   const Kv8Plan& p = a.p;
   const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = kKv8TileWaves * tpw, j = blockIdx.y;
-  const Found f = find_row(p, blockIdx.x, [&](int, const Kv8Row& row) {
-    return row.fresh < kKv8TileTokens ? 0 : (row.fresh + tpt - 1) / tpt;
-  });
+  const Found f = find_row(p, blockIdx.x, [&](int, const Kv8Row& row) { return (row.fresh + tpt - 1) / tpt; });
   if (f.r < 0) return;
   const int n = splits_of(a, f.row, f.r, tpt, most_splits).n;
   if (n < 2) return;
   const int tile = blockIdx.x - f.first;
-  const float* const base =
-      part + ((size_t)(p.tiles[f.r] + tile) * p.Hkv + j) * most_splits * kStride;
+  const float* const base = split_part<D>(p, part, most_splits, f.r, f.row.fresh, tile, j);
   const int dim = 32 * blockIdx.z + 4 * (threadIdx.x & 7);
   for (int col = threadIdx.x >> 3; col < kCols; col += 32) {
     const int c = col & 31, ctok = c / G, tok = tile * tpt + (col >> 5) * tpw + ctok;
@@ -818,7 +833,8 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, co
 // in order. One wave a SIMD with the steps of two blocks side by side took 665 us where this
 // takes 531 (8,192 tokens of 24 query heads over 4 of 256 dims).
 template <int D, int NW, int NC>
-__global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part) {
+__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
+                                                           Kv8Splits most_splits) {
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
   static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
@@ -827,12 +843,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, f
   const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, c = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = NW * NC * tpw, j = blockIdx.y;
-  const int most_splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
   const Found f = find_row(p, blockIdx.x, [&](int r, const Kv8Row& row) {
     const Splits s = splits_of(a, row, r, tpt, most_splits);
     return s.tiles * s.n;
   });
-  if (f.r < 0) return;
+  if (f.r < 0) {  // a work-group to spare (the last one is): tokens of refused rows, zeros
+    const int first = ((int)(blockIdx.x - f.first) * gridDim.y + j) * NW + w;
+    const int step = ((int)gridDim.x - f.first) * gridDim.y * NW;
+    for (int64_t t0 = (int64_t)first * 64; t0 < p.T; t0 += (int64_t)step * 64)
+      zero_refused(a, t0, lane, 64);
+    return;
+  }
   const Kv8Row row = f.row;
   const Splits sp = splits_of(a, row, f.r, tpt, most_splits);
   const int local = blockIdx.x - f.first, split = local % sp.n;
@@ -883,8 +904,8 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, f
     asm volatile("" ::"v"(pid), "v"(eks), "v"(evs));
   };
   // the tile's partial results, if its pages are split: columns (wave, c)
-  float* const out = part + (((size_t)(p.tiles[f.r] + tile) * p.Hkv + j) * most_splits + split) *
-                                ((size_t)32 * NW * NC * (D + 4));
+  float* const out = split_part<D>(p, part, most_splits, f.r, row.fresh, tile, j) +
+                     (size_t)split * (32 * NW * NC * (D + 4));
   if (v0 >= count) {  // nothing in this split (the tile is shorter than the row's last one)
     for (int i = tid; i < 32 * NW * NC; i += 64 * NW) {
       out[(size_t)i * (D + 4)] = -INFINITY;
@@ -930,25 +951,31 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, f
     return (i32x8){(int)x[0], (int)x[1], (int)x[2], (int)x[3],
                    (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
   };
-  // scores of half hb of the page in lk
+  // scores of half hb of the page in lk, a fragment read ahead
   auto scores = [&](const u32x4* lk, int hb, f32x16* Sn) __attribute__((always_inline)) {
     constexpr int kOne = 0x7f7f7f7f, kLow = 0x7b7b7b7b;  // 2^0 and 2^-4
+    auto key = [&](int i) __attribute__((always_inline)) {
+      const int at = kat + (2 * hb * NK + i) * 64;
+      return both(lk[at], lk[at + 16]);
+    };
 #pragma unroll
     for (int n = 0; n < NC; ++n)
 #pragma unroll
       for (int i = 0; i < 16; ++i) Sn[n][i] = 0.f;
+    i32x8 kk[2] = {key(0), NK > 1 ? key(1) : key(0)};
+    __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-      const int at = kat + (2 * hb * NK + i) * 64;
-      const i32x8 kk = both(lk[at], lk[at + 16]);
 #pragma unroll
       for (int n = 0; n < NC; ++n)
         Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            kk, both(qh[n][2 * i], qh[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kOne);
+            kk[i & 1], both(qh[n][2 * i], qh[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kOne);
 #pragma unroll
       for (int n = 0; n < NC; ++n)
         Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            kk, both(ql[n][2 * i], ql[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kLow);
+            kk[i & 1], both(ql[n][2 * i], ql[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kLow);
+      if (i + 2 < NK) kk[i & 1] = key(i + 2);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Scores of the block at kb that need more than a factor: x = mk * S in any case
@@ -963,18 +990,17 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, f
       asm volatile("");
 #pragma unroll
       for (int n = 0; n < NC; ++n) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) Sn[n][i] *= mk[n];
-        mk[n] = 1.f;
         if (cap > 0.f) {
 #pragma unroll
-          for (int i = 0; i < 16; ++i) Sn[n][i] = capped(Sn[n][i], cap);
+          for (int i = 0; i < 16; ++i) Sn[n][i] = capped(Sn[n][i] * mk[n], cap);
+          mk[n] = 1.f;
         }
-        if (a.slopes) {
-          const float far = slope * (float)(kl - cpos[n]);
+        // slopes of zeros where there are none: a scale that is not positive comes here too
+        const float far = slope * (float)(kl - cpos[n]);
 #pragma unroll
-          for (int i = 0; i < 16; ++i) Sn[n][i] += fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), far);
-        }
+        for (int i = 0; i < 16; ++i)
+          Sn[n][i] = fmaf(Sn[n][i], mk[n], fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), far));
+        mk[n] = 1.f;
       }
     }
     const bool all = (kb + kBlock - 1 <= w0 && kb > w0 + wn - 1 - window) || kb + kBlock <= pf;
@@ -1041,17 +1067,28 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, f
       asm volatile("" : "+v"(P[n][0]), "+v"(P[n][1]));
     }
   };
+  // O += P V of half hb of the page in lv: fragments are read two ahead (the first two before the
+  // weights are formed) and converted beside the products
+  u32x4 vr[2];
+  auto values_ahead = [&](const u32x4* lv, int hb) __attribute__((always_inline)) {
+#pragma unroll
+    for (int i = 0; i < 2; ++i) vr[i] = lv[vat + (hb * (D / 16) + 2 * i) * 32];
+  };
   auto values = [&](const u32x4* lv, int hb) __attribute__((always_inline)) {
+    f16x8 f0 = to_f16(vr[0][0], vr[0][1]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-      const u32x4 vr = lv[vat + (hb * (D / 16) + 2 * i) * 32];
-      const f16x8 f0 = to_f16(vr[0], vr[1]), f1 = to_f16(vr[2], vr[3]);
 #pragma unroll
       for (int n = 0; n < NC; ++n)
         O[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f0, __builtin_bit_cast(f16x8, P[n][0]), O[n][i], 0, 0, 0);
+      const f16x8 f1 = to_f16(vr[i & 1][2], vr[i & 1][3]);
+      if (i + 2 < NT) vr[i & 1] = lv[vat + (hb * (D / 16) + 2 * (i + 2)) * 32];
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
       for (int n = 0; n < NC; ++n)
         O[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1, __builtin_bit_cast(f16x8, P[n][1]), O[n][i], 0, 0, 0);
+      if (i + 1 < NT) f0 = to_f16(vr[(i + 1) & 1][0], vr[(i + 1) & 1][1]);
+      __builtin_amdgcn_sched_barrier(0);
     }
   };
   // Half hb of page v, from kb on, before its product where keys past the row's end may hold
@@ -1113,13 +1150,21 @@ __global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, f
 #pragma unroll
       for (int hb = 0; hb < 2; ++hb) {
         const int kb = key0 + hb * kBlock;
+        __builtin_amdgcn_s_setprio(1);
         scores(lk, hb, S);
+        __builtin_amdgcn_s_setprio(0);
         prepare(S, kb, ek);
         maxima(S, bm);
         follow(bm, ev);
+        values_ahead(lv, hb);
         weights(S, ev);
-        if (__builtin_expect(nan || kb + kBlock > total, 0)) clean(v, lv, hb, kb, seen);
+        if (__builtin_expect(nan || kb + kBlock > total, 0)) {
+          clean(v, lv, hb, kb, seen);
+          values_ahead(lv, hb);
+        }
+        __builtin_amdgcn_s_setprio(1);
         values(lv, hb);
+        __builtin_amdgcn_s_setprio(0);
       }
     }
     // the next page has landed everywhere, and no wave reads this one any more
@@ -1180,8 +1225,9 @@ size_t kv8_attn_chunk_floats(const gdn_kv8_desc& d) {
 }
 
 size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
-  // tiles times splits, where there is more than one, are kv8_tile_groups() or less
-  const size_t tiles = (size_t)kv8_tile_groups(d.head_dim) * 32 * kKv8TileWaves * (d.head_dim + 4);
+  // tiles times splits, where there is more than one, are kv8_tile_groups() or less, of the rows
+  // of few tokens as of the others
+  const size_t tiles = (size_t)2 * kv8_tile_groups(d.head_dim) * 32 * kKv8TileWaves * (d.head_dim + 4);
   return (kv8_attn_chunk_floats(d) + tiles) * sizeof(float);
 }
 
@@ -1189,37 +1235,37 @@ template <int D>
 static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   const Kv8Plan& p = a.p;
   float* const part = static_cast<float*>(a.workspace);
-  float* const tpart = part + a.tile_part;
   hipError_t e;
-  int splits = 1;
   if (p.max_row >= kKv8TileTokens) {
+    float* const tpart = part + a.tile_part;
     const int G = p.Hq / p.Hkv;
-    splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
-    const dim3 grid(kv8_most_tiles(p.n, p.T, G) * splits, p.Hkv);
+    const Kv8Splits splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
+    const int many = kv8_most_tiles(p.n, p.T, G), few = min(p.n, p.T) * kv8_few_tiles(G);
+    const dim3 grid(many * splits.many + few * splits.few + 1, p.Hkv);
     hipLaunchKernelGGL((attn8_tile_kernel<D, kKv8TileWaves, 1>), grid, dim3(64 * kKv8TileWaves), 0,
-                       a.stream, a, tpart);
-    if ((e = hipGetLastError()) != hipSuccess) return e;
+                       a.stream, a, tpart, splits);
+    if (splits.many > 1 || splits.few > 1) {
+      if ((e = hipGetLastError()) != hipSuccess) return e;
+      hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, dim3(many + few, p.Hkv, D / 32), dim3(256), 0,
+                         a.stream, a, tpart, splits);
+    }
+    return hipGetLastError();
   }
   // as many as the rows can have, up to four rounds of the chip's waves
   const int W = kv8_chunk_waves(p.n, p.Hkv);
-  const int64_t most = kv8_waves(D) / W + (int64_t)p.Hkv * min(p.T, p.n * (kKv8TileTokens - 1));
+  const int64_t most = kv8_waves(D) / W + (int64_t)p.Hkv * min(p.T, p.n * p.max_row);
   const dim3 grid((unsigned)(most < 8192 / W ? most : 8192 / W));
   if (W == 1)
     hipLaunchKernelGGL((attn8_chunk_kernel<D, 1>), grid, dim3(64), 0, a.stream, a, part);
   else
     hipLaunchKernelGGL((attn8_chunk_kernel<D, 4>), grid, dim3(256), 0, a.stream, a, part);
   if ((e = hipGetLastError()) != hipSuccess) return e;
-  const int per = min(p.max_row, kKv8TileTokens - 1);
+  const int per = p.max_row;
   const dim3 few(p.n * per, p.Hq);
   if (p.n * per * p.Hq <= 512)  // a wave for each sum where the work-groups are few
     hipLaunchKernelGGL((attn8_join_kernel<D, 16>), few, dim3(1024), 0, a.stream, a, part, per);
   else
     hipLaunchKernelGGL((attn8_join_kernel<D, 4>), few, dim3(256), 0, a.stream, a, part, per);
-  if (splits > 1) {
-    if ((e = hipGetLastError()) != hipSuccess) return e;
-    const dim3 tiles(kv8_most_tiles(p.n, p.T, p.Hq / p.Hkv), p.Hkv, D / 32);
-    hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, tiles, dim3(256), 0, a.stream, a, tpart, splits);
-  }
   return hipGetLastError();
 }
 

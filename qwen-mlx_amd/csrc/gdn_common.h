@@ -504,18 +504,26 @@ __host__ __device__ inline int kv8_chunks(int n, int Hkv, int D, int groups) {
   const int c = kv8_waves(D) / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
   return c < 1 ? 1 : c;
 }
-// Rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens, their pages in kv8_splits() pieces
-// or less, where the step's bounds let the tiles be few: about kv8_tile_groups() work-groups.
+// Steps with rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens of a row, their pages in
+// kv8_splits() pieces or less, where the step's bounds let the tiles be few: about
+// kv8_tile_groups() work-groups, and as many again of the rows of fewer than kKv8TileTokens.
 constexpr int kKv8TileWaves = 4;
-__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 256 ? 512 : 1024; }
+__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 256 ? 512 : 1536; }
 __host__ __device__ inline int kv8_most_tiles(int n, int T, int G) {
   const int a = T / (kKv8TileWaves * (32 / G)), b = T / kKv8TileTokens;
   return a + (n < b ? n : b);
 }
-__host__ __device__ inline int kv8_splits(int n, int T, int Hkv, int G, int D) {
-  const int64_t most = (int64_t)kv8_most_tiles(n, T, G) * Hkv;
-  const int64_t s = kv8_tile_groups(D) / (most > 0 ? most : 1);
-  return s < 1 ? 1 : (int)s;
+__host__ __device__ inline int kv8_few_tiles(int G) {  // of a row of few tokens at most
+  const int tpt = kKv8TileWaves * (32 / G);
+  return (kKv8TileTokens - 2) / tpt + 1;
+}
+struct Kv8Splits {
+  int many, few;  // at most, of a tile of a row of many tokens and of one of few
+};
+__host__ __device__ inline Kv8Splits kv8_splits(int n, int T, int Hkv, int G, int D) {
+  const int64_t many = (int64_t)kv8_most_tiles(n, T, G) * Hkv, few = (int64_t)n * kv8_few_tiles(G) * Hkv;
+  const int64_t a = kv8_tile_groups(D) / (many > 0 ? many : 1), b = kv8_tile_groups(D) / few;
+  return {a < 1 ? 1 : (int)a, b < 1 ? 1 : (int)b};
 }
 constexpr int kKv8Rows = 4096;  // rows of a step
 struct Kv8StepArgs {
