@@ -780,69 +780,91 @@ __global__ __launch_bounds__(64 * W) void attn8_join_kernel(Kv8AttnArgs a, const
   }
 }
 
-// Tiles whose pages are split: grid (tiles at most, Hkv, D / 32), block 256, 32 dims of a tile's 128
-// columns: 8 lanes a column, its splits in order.
+// Tiles whose pages are split: grid (those of rows of few tokens, if any may be split, then those
+// of the others, if any may, Hkv, kKv8TileWaves), block 256: a wave's 32 columns, 8 lanes each, its
+// splits in order.
 template <int D>
 __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, float* __restrict__ part,
                                                                Kv8Splits most_splits) {
-  constexpr int kCols = 32 * kKv8TileWaves;
-  constexpr size_t kStride = (size_t)kCols * (D + 4);
+  constexpr size_t kStride = (size_t)32 * kKv8TileWaves * (D + 4);
   const Kv8Plan& p = a.p;
   const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = kKv8TileWaves * tpw, j = blockIdx.y;
-  const Found f = find_row(p, blockIdx.x, [&](int, const Kv8Row& row) { return (row.fresh + tpt - 1) / tpt; });
-  if (f.r < 0) return;
-  const int n = splits_of(a, f.row, f.r, tpt, most_splits).n;
+  const int ft = kv8_few_tiles(G), few = most_splits.few > 1 ? p.n * ft : 0;
+  int r, tile;
+  Kv8Row row;
+  if ((int)blockIdx.x < few) {
+    r = blockIdx.x / ft;
+    tile = blockIdx.x - r * ft;
+    row = p.rows[r];
+    if (row.fresh >= kKv8TileTokens) return;
+  } else {
+    const Found f = find_row(p, blockIdx.x - few, [&](int, const Kv8Row& x) {
+      return x.fresh >= kKv8TileTokens ? (x.fresh + tpt - 1) / tpt : 0;
+    });
+    if (f.r < 0) return;
+    r = f.r;
+    tile = blockIdx.x - few - f.first;
+    row = f.row;
+  }
+  const int wave = blockIdx.z, c = threadIdx.x >> 3, ctok = c / G;
+  const int tok = tile * tpt + wave * tpw + ctok;
+  if (ctok >= tpw || tok >= row.fresh) return;
+  const int n = splits_of(a, row, r, tpt, most_splits).n;
   if (n < 2) return;
-  const int tile = blockIdx.x - f.first;
-  const float* const base = split_part<D>(p, part, most_splits, f.r, f.row.fresh, tile, j);
-  const int dim = 32 * blockIdx.z + 4 * (threadIdx.x & 7);
-  for (int col = threadIdx.x >> 3; col < kCols; col += 32) {
-    const int c = col & 31, ctok = c / G, tok = tile * tpt + (col >> 5) * tpw + ctok;
-    if (ctok >= tpw || tok >= f.row.fresh) continue;
-    const float* const pc = base + (size_t)col * (D + 4);
-    float M = -INFINITY, L = 0.f;
-    for (int s = 0; s < n; ++s) M = fmaxf(M, pc[s * kStride]);
-    if (M == -INFINITY) M = 0.f;  // NaN scores alone
-    f32x4 A = {0.f, 0.f, 0.f, 0.f};
+  const int dim = 4 * (threadIdx.x & 7);  // and those 32, 64, .. further on
+  const float* const pc = split_part<D>(p, part, most_splits, r, row.fresh, tile, j) +
+                          (size_t)(wave * 32 + c) * (D + 4);
+  float M = -INFINITY, L = 0.f;
 #pragma unroll 4
-    for (int s = 0; s < n; ++s) {
-      const float w = exp2f(pc[s * kStride] - M), l = pc[s * kStride + 1];
-      const f32x4 v = *reinterpret_cast<const f32x4*>(pc + s * kStride + 4 + dim);
-      if (l != 0.f) {  // a split without a visible key holds nothing
-        L += w * l;
-        A += v * w;
-      }
-    }
-    const float inv = 1.0f / L;
-    float o[4] = {A[0] * inv, A[1] * inv, A[2] * inv, A[3] * inv};
-    store4(a, (int64_t)f.row.cu + tok, j * G + c - ctok * G, dim, o);
+  for (int s = 0; s < n; ++s) M = fmaxf(M, pc[s * kStride]);
+  if (M == -INFINITY) M = 0.f;  // NaN scores alone
+  f32x4 A[D / 32];
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) A[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+#pragma unroll(512 / D)
+  for (int s = 0; s < n; ++s) {
+    const float f = exp2f(pc[s * kStride] - M), l = pc[s * kStride + 1];
+    f32x4 v[D / 32];
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) v[i] = *reinterpret_cast<const f32x4*>(pc + s * kStride + 4 + dim + 32 * i);
+    if (l == 0.f) continue;  // a split without a visible key holds nothing
+    L += f * l;
+#pragma unroll
+    for (int i = 0; i < D / 32; ++i) A[i] += v[i] * f;
+  }
+  const float inv = 1.0f / L;
+#pragma unroll
+  for (int i = 0; i < D / 32; ++i) {
+    float o[4] = {A[i][0] * inv, A[i][1] * inv, A[i][2] * inv, A[i][3] * inv};
+    store4(a, (int64_t)row.cu + tok, j * G + c - ctok * G, dim + 32 * i, o);
   }
 }
 
-// Prompts. Work-group (tile, kv head): a tile is NW * NC * (32 / G) consecutive tokens of a row.
-// Wave w takes the NC groups of 32 / G tokens from w NC on; a group's (token, query head) pairs
-// are 32 columns. A page of K and V is copied into LDS by DMA a page ahead, two buffers of each,
-// and read by all waves. Rows of the products are 32 keys or dims, so that an operand read
-// from LDS, and a value's conversion, serves 32 NC columns.
+// Prompts. Work-group (tile, kv head): a tile is NW * (32 / G) consecutive tokens of a row, wave w
+// takes 32 / G of them from w (32 / G) on; the (token, query head) pairs are its 32 columns. A page
+// of K and V is copied into LDS by DMA a page ahead, two buffers of each, and read by all waves.
+// Rows of the products are 32 keys or dims, so that an operand read from LDS, and a value's
+// conversion, serves 32 columns.
 //
 // Lane (hf, c), hf = lane / 32, holds keys 8 i + 4 hf + r of a block of 32 (i, r = 0 .. 3) for
-// column c of each group, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^(unit - kUnit).
+// column c, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^(unit - kUnit).
 //
-// Two waves a SIMD or more, each in at most 256 registers (at D = 256 its outputs are 128 of them,
-// q's parts 64): one's products run beside the other's softmax, so that a wave's own steps stay
-// in order. One wave a SIMD with the steps of two blocks side by side took 665 us where this
-// takes 531 (8,192 tokens of 24 query heads over 4 of 256 dims).
-template <int D, int NW, int NC>
-__global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
-                                                           Kv8Splits most_splits) {
+// Two waves a SIMD or more, each in at most 256 registers: at D = 256 its outputs are 128 of them,
+// q's parts 64, and what only rare branches need is kept in LDS.
+template <int D, int NW>
+__global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
+                                                                Kv8Splits most_splits) {
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
   static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
   __shared__ u32x4 lk0[kTile16], lk1[kTile16], lv0[kTile16], lv1[kTile16];
+  // a lane's column: its position (-1: none), its slope, the exponent of its q
+  struct Column { int pos; float slope; int eq, pad; };
+  __shared__ Column columns[D == 256 ? 64 * NW : 1];
   const Kv8Plan& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, hf = lane >> 5, c = lane & 31;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = NW * NC * tpw, j = blockIdx.y;
+  const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = NW * tpw, j = blockIdx.y;
   const Found f = find_row(p, blockIdx.x, [&](int r, const Kv8Row& row) {
     const Splits s = splits_of(a, row, r, tpt, most_splits);
     return s.tiles * s.n;
@@ -858,39 +880,27 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
   const Splits sp = splits_of(a, row, f.r, tpt, most_splits);
   const int local = blockIdx.x - f.first, split = local % sp.n;
   const int tile = sp.tiles - 1 - local / sp.n;  // longest first
-  const int k0 = tile * tpt;
   const int total = row.pos + row.fresh;
   const int pf = a.prefix ? min(max(a.prefix[f.r], 0), total) : 0;
-  const int p0 = row.pos + k0;  // the tile's first position
+  const int p0 = row.pos + tile * tpt;  // the tile's first position
   const Span span = span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total);
   const int v0 = split * sp.cp;
   const int count = min(span.count(), sp.n > 1 ? v0 + sp.cp : INT32_MAX);  // pages [v0, count)
-  // the wave's positions
-  const int w0 = p0 + w * NC * tpw, wn = min(max(total - w0, 0), NC * tpw);
-  const int ctok = c / G, h = j * G + c - ctok * G;
-  int cpos[NC], eq[NC];
-  int64_t t[NC];
-  uint32_t seen[NC];
-  float m[NC], l[NC], mk[NC];
-  f32x16 O[NC][NT], S[NC];
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const int at = w0 + n * tpw + ctok;
-    const bool valid = ctok < tpw && at < total;
-    cpos[n] = valid ? at : -1;
-    t[n] = (int64_t)row.cu + (valid ? at - row.pos : 0);
-    m[n] = -INFINITY;
-    l[n] = 0.f;
-#pragma unroll
-    for (int i = 0; i < NT; ++i)
-#pragma unroll
-      for (int r = 0; r < 16; ++r) O[n][i][r] = 0.f;
+  // the tile's partial results, if its pages are split: columns (wave, c)
+  float* const out = split_part<D>(p, part, most_splits, f.r, row.fresh, tile, j) +
+                     (size_t)split * (32 * NW * (D + 4));
+  if (v0 >= count) {  // nothing in this split (the tile is shorter than the row's last one)
+    for (int i = tid; i < 32 * NW; i += 64 * NW) {
+      out[(size_t)i * (D + 4)] = -INFINITY;
+      out[(size_t)i * (D + 4) + 1] = 0.f;
+    }
+    return;
   }
-  int unit = 0;
-  const float sm = a.softcap > 0.f ? a.scale / a.softcap : a.scale * 1.4426950408889634f;
-  const float cap = a.softcap * 1.4426950408889634f;
-  const float slope = a.slopes ? a.slopes[ctok < tpw ? h : 0] * 1.4426950408889634f : 0.f;
+  // the wave's positions
+  const int w0 = p0 + w * tpw, wn = min(max(total - w0, 0), tpw);
   const int window = a.window > 0 ? a.window : INT32_MAX / 2;
+  const float sm = __int_as_float(__builtin_amdgcn_readfirstlane(
+      __float_as_int(a.softcap > 0.f ? a.scale / a.softcap : a.scale * 1.4426950408889634f)));
   const bool odd = a.softcap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
 
   const int32_t* const trow = p.table + (size_t)row.slot * p.max_pages;
@@ -903,27 +913,23 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
     evs = e[p.Hkv];
     asm volatile("" ::"v"(pid), "v"(eks), "v"(evs));
   };
-  // the tile's partial results, if its pages are split: columns (wave, c)
-  float* const out = split_part<D>(p, part, most_splits, f.r, row.fresh, tile, j) +
-                     (size_t)split * (32 * NW * NC * (D + 4));
-  if (v0 >= count) {  // nothing in this split (the tile is shorter than the row's last one)
-    for (int i = tid; i < 32 * NW * NC; i += 64 * NW) {
-      out[(size_t)i * (D + 4)] = -INFINITY;
-      out[(size_t)i * (D + 4) + 1] = 0.f;
-    }
-    return;
-  }
   ids(v0);
   const uint8_t* const base = a.pages + (size_t)j * (kPage * D);
   const size_t page_bytes = (size_t)2 * p.Hkv * kPage * D, v_shift = (size_t)p.Hkv * kPage * D;
+  auto page_of = [&](int v) __attribute__((always_inline)) {
+    uint64_t at = (uint64_t)base +
+                  (size_t)(uint32_t)__builtin_amdgcn_readlane(pid, min(v, count - 1) - vbase) * page_bytes;
+    asm("" : "+s"(at));  // lanes add their 32-bit offsets to it
+    return reinterpret_cast<const uint8_t*>(at);
+  };
   // K or V of page v into a buffer: a wave copies its share of the 1 KiB pieces
   auto copy = [&](int v, u32x4* dst, size_t shift) __attribute__((always_inline)) {
-    const uint8_t* const src = base + shift + lane * 16 +
-        (size_t)(uint32_t)__builtin_amdgcn_readlane(pid, min(v, count - 1) - vbase) * page_bytes;
+    const uint8_t* const src = page_of(v) + shift + w * (kLoads * 1024);
+    const uint32_t mine = lane * 16;
 #pragma unroll
     for (int i = 0; i < kLoads; ++i)
       __builtin_amdgcn_global_load_lds(
-          (const void __attribute__((address_space(1)))*)(src + (w * kLoads + i) * 1024),
+          (const void __attribute__((address_space(1)))*)(src + i * 1024 + mine),
           (void __attribute__((address_space(3)))*)(dst + (w * kLoads + i) * 64), 16, 0, 0);
   };
   copy(v0, lk0, 0);
@@ -932,143 +938,142 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
   copy(v0 + 1, lv1, v_shift);
 
   // q: dims 64 i + 32 hf .. + 31 of column c, in two e4m3 parts
-  u32x4 qh[NC][2 * NK], ql[NC][2 * NK];
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
+  u32x4 qh[2 * NK], ql[2 * NK];
+  Column mine;
+  {
+    const int ctok = c / G, h = j * G + c - ctok * G;
+    const bool valid = ctok < wn;
+    const int64_t t = (int64_t)row.cu + (valid ? w0 + ctok - row.pos : 0);
     u32x4 q[4 * NK];
-    eq[n] = q_parts32<NK>(a.q + t[n] * a.qs + h * a.qhs + 32 * hf, cpos[n] >= 0, q);
+    const int eq = q_parts32<NK>(a.q + t * a.qs + h * a.qhs + 32 * hf, valid, q);
 #pragma unroll
     for (int i = 0; i < 2 * NK; ++i) {
-      qh[n][i] = q[2 * i];
-      ql[n][i] = q[2 * i + 1];
+      qh[i] = q[2 * i];
+      ql[i] = q[2 * i + 1];
     }
+    mine = Column{valid ? w0 + ctok : -1,
+                          a.slopes && valid ? a.slopes[h] * 1.4426950408889634f : 0.f, eq, 0};
+    if constexpr (D == 256) columns[tid] = mine;
   }
+  // at D = 256 from LDS, found anew at each use, which holds no register
+  auto column = [&]() __attribute__((always_inline)) {
+    if constexpr (D < 256) return mine;
+    int at;
+    asm volatile("v_mbcnt_lo_u32_b32 %0, -1, 0\n\tv_mbcnt_hi_u32_b32 %0, -1, %0" : "=v"(at));
+    return columns[64 * w + at];
+  };
   // this lane's pieces: of key c of 32 (NK KiB for 16 keys), and of dim c of 32
   const int kat = (c >> 4) * NK * 64 + 32 * hf + (c & 15);
   const int vat = (c >> 4) * 32 + 16 * hf + (c & 15);
+
+  float m = -INFINITY, l = 0.f, mk;
+  uint32_t seen;
+  int unit = 0;
+  f32x16 O[NT], S;
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) O[i][r] = 0.f;
 
   auto both = [](u32x4 x, u32x4 y) __attribute__((always_inline)) {
     return (i32x8){(int)x[0], (int)x[1], (int)x[2], (int)x[3],
                    (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
   };
-  // scores of half hb of the page in lk, a fragment read ahead
-  auto scores = [&](const u32x4* lk, int hb, f32x16* Sn) __attribute__((always_inline)) {
+  // S: scores of half hb of the page in lk, fragments read two ahead
+  auto scores = [&](const u32x4* lk, int hb) __attribute__((always_inline)) {
     constexpr int kOne = 0x7f7f7f7f, kLow = 0x7b7b7b7b;  // 2^0 and 2^-4
     auto key = [&](int i) __attribute__((always_inline)) {
       const int at = kat + (2 * hb * NK + i) * 64;
       return both(lk[at], lk[at + 16]);
     };
 #pragma unroll
-    for (int n = 0; n < NC; ++n)
-#pragma unroll
-      for (int i = 0; i < 16; ++i) Sn[n][i] = 0.f;
+    for (int i = 0; i < 16; ++i) S[i] = 0.f;
     i32x8 kk[2] = {key(0), NK > 1 ? key(1) : key(0)};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
     for (int i = 0; i < NK; ++i) {
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-        Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            kk[i & 1], both(qh[n][2 * i], qh[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kOne);
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-        Sn[n] = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(
-            kk[i & 1], both(ql[n][2 * i], ql[n][2 * i + 1]), Sn[n], 0, 0, 0, kOne, 0, kLow);
+      S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kk[i & 1], both(qh[2 * i], qh[2 * i + 1]), S,
+                                                          0, 0, 0, kOne, 0, kOne);
+      S = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(kk[i & 1], both(ql[2 * i], ql[2 * i + 1]), S,
+                                                          0, 0, 0, kOne, 0, kLow);
       if (i + 2 < NK) kk[i & 1] = key(i + 2);
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // Scores of the block at kb that need more than a factor: x = mk * S in any case
-  auto prepare = [&](f32x16* Sn, int kb, int ek) __attribute__((always_inline)) {
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      mk[n] = factor_of(sm, eq[n] + ek);
-      seen[n] = 0xffffu;
-    }
+  // S and mk: scores of the block at kb, keys that a column does not see as -inf, are mk * S
+  auto prepare = [&](int kb, int ek) __attribute__((always_inline)) {
+    mk = factor_of(sm, column().eq + ek);
+    seen = 0xffffu;
     const int kl = kb + 4 * hf;  // score i is of key kl + 8 (i / 4) + i % 4
     if (__builtin_expect(odd, 0)) {
-      asm volatile("");
+      asm volatile("");  // a branch, as below: rare and long
+      const float cap = a.softcap * 1.4426950408889634f;
+      if (cap > 0.f) {
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        if (cap > 0.f) {
-#pragma unroll
-          for (int i = 0; i < 16; ++i) Sn[n][i] = capped(Sn[n][i] * mk[n], cap);
-          mk[n] = 1.f;
+        for (int i = 0; i < 16; ++i) {
+          S[i] = capped(S[i] * mk, cap);
+          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
         }
-        // slopes of zeros where there are none: a scale that is not positive comes here too
-        const float far = slope * (float)(kl - cpos[n]);
-#pragma unroll
-        for (int i = 0; i < 16; ++i)
-          Sn[n][i] = fmaf(Sn[n][i], mk[n], fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), far));
-        mk[n] = 1.f;
+        mk = 1.f;
       }
+      // slopes of zero where there are none: a scale that is not positive comes here too
+      const Column col = column();
+      const float slope = col.slope, far = slope * (float)(kl - col.pos);
+#pragma unroll
+      for (int i = 0; i < 16; ++i) {
+        S[i] = fmaf(S[i], mk, fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), far));
+        if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few registers at once
+      }
+      mk = 1.f;
     }
     const bool all = (kb + kBlock - 1 <= w0 && kb > w0 + wn - 1 - window) || kb + kBlock <= pf;
     if (__builtin_expect(!all, 0)) {
       asm volatile("");
+      const int cpos = column().pos;
+      auto below = [](int k) { return first_scores<8>(k, 16); };  // of keys below kl + k
+      seen = (below(cpos + 1 - kl) & ~below(cpos - window + 1 - kl)) | below(cpos >= 0 ? pf - kl : 0);
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        auto below = [](int k) { return first_scores<8>(k, 16); };  // of keys below kl + k
-        seen[n] = (below(cpos[n] + 1 - kl) & ~below(cpos[n] - window + 1 - kl)) |
-                  below(cpos[n] >= 0 ? pf - kl : 0);
-#pragma unroll
-        for (int i = 0; i < 16; ++i) Sn[n][i] = (seen[n] >> i) & 1u ? Sn[n][i] : -INFINITY;
-      }
-    }
-  };
-  auto maxima = [&](const f32x16* Sn, float* bm) __attribute__((always_inline)) {
-#pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      float x = fmaxf(Sn[n][0], Sn[n][1]);
-#pragma unroll
-      for (int i = 2; i < 16; ++i) x = fmaxf(x, Sn[n][i]);
-      bm[n] = max_xor32(x) * mk[n];
+      for (int i = 0; i < 16; ++i) S[i] = (seen >> i) & 1u ? S[i] : -INFINITY;
     }
   };
   // the running maximum follows once it is passed by 2^kStep; ev: the exponent of the block's values
-  auto follow = [&](const float* bm, int ev) __attribute__((always_inline)) {
-    bool up = !unit_holds(ev, unit);
+  auto follow = [&](int ev) __attribute__((always_inline)) {
+    float bm = fmaxf(S[0], S[1]);
 #pragma unroll
-    for (int n = 0; n < NC; ++n) up |= __any(bm[n] > m[n] + kStep);
-    if (__builtin_expect(up, 0)) {
+    for (int i = 2; i < 16; ++i) bm = fmaxf(bm, S[i]);
+    bm = max_xor32(bm) * mk;
+    if (__builtin_expect(!unit_holds(ev, unit) || __any(bm > m + kStep), 0)) {
       const int to = unit_holds(ev, unit) ? unit : ev + 2;  // room either way
+      const float mn = fmaxf(m, bm);
+      float corr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;  // m = -inf: 0
+      m = mn;
+      l *= corr;
+      corr = __builtin_amdgcn_ldexpf(corr, unit - to);
 #pragma unroll
-      for (int n = 0; n < NC; ++n) {
-        const float mn = fmaxf(m[n], bm[n]);
-        float corr = mn > m[n] ? __builtin_amdgcn_exp2f(m[n] - mn) : 1.0f;  // m = -inf: 0
-        m[n] = mn;
-        l[n] *= corr;
-        corr = __builtin_amdgcn_ldexpf(corr, unit - to);
-#pragma unroll
-        for (int i = 0; i < NT; ++i) {
-          O[n][i] *= corr;
-          __builtin_amdgcn_sched_barrier(0);  // not all of them in registers of their own at once
-        }
+      for (int i = 0; i < NT; ++i) {
+        O[i] *= corr;
+        __builtin_amdgcn_sched_barrier(0);  // not all of them in registers of their own at once
       }
       unit = to;
     }
   };
-  u32x4 P[NC][2];
-  auto weights = [&](const f32x16* Sc, int ev) __attribute__((always_inline)) {
+  u32x4 P[2];
+  auto weights = [&](int ev) __attribute__((always_inline)) {
     const int up = kUnit + ev - unit;
+    const float mref = (m == -INFINITY ? 0.f : m) - (float)up;
+    float e[16], sum = 0.f;
 #pragma unroll
-    for (int n = 0; n < NC; ++n) {
-      const float mref = (m[n] == -INFINITY ? 0.f : m[n]) - (float)up;
-      float e[16], sum = 0.f;
+    for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(S[i], mk, -mref));
 #pragma unroll
-      for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(Sc[n][i], mk[n], -mref));
-#pragma unroll
-      for (int i = 0; i < 16; i += 4) sum += (e[i] + e[i + 1]) + (e[i + 2] + e[i + 3]);
-      l[n] = fmaf(sum, pow2(-up), l[n]);
-      // keys 4 hf + r and 16 + 4 hf + r, then those 8 further on: the order of the values' bytes
-      P[n][0] = (u32x4){pk_f16(e[0], e[1]), pk_f16(e[2], e[3]), pk_f16(e[8], e[9]), pk_f16(e[10], e[11])};
-      P[n][1] = (u32x4){pk_f16(e[4], e[5]), pk_f16(e[6], e[7]), pk_f16(e[12], e[13]), pk_f16(e[14], e[15])};
-      // here, beside the scores' products, not behind the branches that follow
-      asm volatile("" : "+v"(P[n][0]), "+v"(P[n][1]));
-    }
+    for (int i = 0; i < 16; i += 4) sum += (e[i] + e[i + 1]) + (e[i + 2] + e[i + 3]);
+    l = fmaf(sum, pow2(-up), l);
+    // keys 4 hf + r and 16 + 4 hf + r, then those 8 further on: the order of the values' bytes
+    P[0] = (u32x4){pk_f16(e[0], e[1]), pk_f16(e[2], e[3]), pk_f16(e[8], e[9]), pk_f16(e[10], e[11])};
+    P[1] = (u32x4){pk_f16(e[4], e[5]), pk_f16(e[6], e[7]), pk_f16(e[12], e[13]), pk_f16(e[14], e[15])};
+    asm volatile("" : "+v"(P[0]), "+v"(P[1]));  // here, not behind the branches that follow
   };
-  // O += P V of half hb of the page in lv: fragments are read two ahead (the first two before the
-  // weights are formed) and converted beside the products
+  // O += P V of half hb of the page in lv: fragments are read two ahead (the first two apart) and
+  // converted beside the products
   u32x4 vr[2];
   auto values_ahead = [&](const u32x4* lv, int hb) __attribute__((always_inline)) {
 #pragma unroll
@@ -1078,15 +1083,11 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
     f16x8 f0 = to_f16(vr[0][0], vr[0][1]);
 #pragma unroll
     for (int i = 0; i < NT; ++i) {
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-        O[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f0, __builtin_bit_cast(f16x8, P[n][0]), O[n][i], 0, 0, 0);
+      O[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f0, __builtin_bit_cast(f16x8, P[0]), O[i], 0, 0, 0);
       const f16x8 f1 = to_f16(vr[i & 1][2], vr[i & 1][3]);
       if (i + 2 < NT) vr[i & 1] = lv[vat + (hb * (D / 16) + 2 * (i + 2)) * 32];
       __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-      for (int n = 0; n < NC; ++n)
-        O[n][i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1, __builtin_bit_cast(f16x8, P[n][1]), O[n][i], 0, 0, 0);
+      O[i] = __builtin_amdgcn_mfma_f32_32x32x16_f16(f1, __builtin_bit_cast(f16x8, P[1]), O[i], 0, 0, 0);
       if (i + 1 < NT) f0 = to_f16(vr[(i + 1) & 1][0], vr[(i + 1) & 1][1]);
       __builtin_amdgcn_sched_barrier(0);
     }
@@ -1095,53 +1096,46 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
   // anything or some hold NaN: those bytes become zeros in LDS (each wave writes all that it
   // reads, the same as the others), and a column that sees the key of a NaN, read from the page
   // itself, gets a NaN sum.
-  auto clean = [&](int v, u32x4* lv, int hb, int kb, const uint32_t* seen_) __attribute__((always_inline)) {
-    const u32x4* const src = reinterpret_cast<const u32x4*>(
-        base + v_shift + (size_t)(uint32_t)__builtin_amdgcn_readlane(pid, v - vbase) * page_bytes);
+  auto clean = [&](int v, u32x4* lv, int hb, int kb) __attribute__((always_inline)) {
+    const uint8_t* const src = page_of(v) + v_shift;
     u32x4 nan_keys = {0u, 0u, 0u, 0u};
 #pragma nounroll
     for (int i = 0; i < NT; ++i) {
-      const int at = vat + (hb * (D / 16) + 2 * i) * 32;
-      u32x4 vr = src[at];
+      const uint32_t at = vat + (hb * (D / 16) + 2 * i) * 32;
+      u32x4 x = *reinterpret_cast<const u32x4*>(src + at * 16);
 #pragma unroll
       for (int k = 0; k < 4; ++k) {
         // the word's four keys, from 4 (hf + 2 (k / 2) + 4 (k % 2)) on
-        const uint32_t x = first_keys(vr[k], total - kb - 4 * (hf + 2 * (k >> 1) + 4 * (k & 1)));
-        const uint32_t top = ((x & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
+        const uint32_t y = first_keys(x[k], total - kb - 4 * (hf + 2 * (k >> 1) + 4 * (k & 1)));
+        const uint32_t top = ((y & 0x7f7f7f7fu) + 0x01010101u) & 0x80808080u;
         nan_keys[k] |= top;
-        vr[k] = x & ~((top >> 7) * 0xffu);
+        x[k] = y & ~((top >> 7) * 0xffu);
       }
-      lv[at] = vr;
+      lv[at] = x;
     }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
 #pragma unroll
       for (int off = 1; off < 32; off <<= 1) nan_keys[k] |= __shfl_xor(nan_keys[k], off, 64);
 #pragma unroll
-      for (int n = 0; n < NC; ++n)
-#pragma unroll
-        for (int q = 0; q < 4; ++q)  // scores 4 (k / 2 + 2 (k % 2)) .. are those keys'
-          if ((nan_keys[k] >> (8 * q + 7)) & (seen_[n] >> (4 * ((k >> 1) + 2 * (k & 1)) + q)) & 1u)
-            l[n] = __builtin_nanf("");
+      for (int q = 0; q < 4; ++q)  // scores 4 (k / 2 + 2 (k % 2)) .. are those keys'
+        if ((nan_keys[k] >> (8 * q + 7)) & (seen >> (4 * ((k >> 1) + 2 * (k & 1)) + q)) & 1u)
+          l = __builtin_nanf("");
     }
   };
-
-  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the first two pages
-  lds_barrier();
-  const bool idle = wn == 0;  // no tokens for this wave: copies and barriers only
-  float bm[NC];
   auto exps_of = [&](int v, int& ek, int& ev, bool& nan) __attribute__((always_inline)) {
-    const int at = min(v, count - 1) - vbase;
+    const int at = v - vbase;
     ek = (int)(int8_t)__builtin_amdgcn_readlane(eks, at);
     const int wv = __builtin_amdgcn_readlane(evs, at);
     ev = (int)(int8_t)wv;
     nan = (wv & kNanFlag) != 0;
   };
-  // Page v in buffers b, which has landed; the next page's copies are on their way.
-  auto page = [&](int v, auto bc) __attribute__((always_inline)) {
-    constexpr int b = decltype(bc)::value;
-    u32x4* const lk = b ? lk1 : lk0;
-    u32x4* const lv = b ? lv1 : lv0;
+  __builtin_amdgcn_s_waitcnt(0x0F70);  // vmcnt(0): the first two pages
+  lds_barrier();
+  const bool idle = wn == 0;  // no tokens for this wave: copies and barriers only
+  // Page v in lk and lv, which has landed; the next page's copies are on their way. Products go
+  // before another wave's softmax.
+  auto page = [&](int v, u32x4* lk, u32x4* lv) __attribute__((always_inline)) {
     const int key0 = span.page(v) * kPage;
     int ek, ev;
     bool nan;
@@ -1151,15 +1145,14 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
       for (int hb = 0; hb < 2; ++hb) {
         const int kb = key0 + hb * kBlock;
         __builtin_amdgcn_s_setprio(1);
-        scores(lk, hb, S);
+        scores(lk, hb);
         __builtin_amdgcn_s_setprio(0);
-        prepare(S, kb, ek);
-        maxima(S, bm);
-        follow(bm, ev);
+        prepare(kb, ek);
+        follow(ev);
         values_ahead(lv, hb);
-        weights(S, ev);
+        weights(ev);
         if (__builtin_expect(nan || kb + kBlock > total, 0)) {
-          clean(v, lv, hb, kb, seen);
+          clean(v, lv, hb, kb);
           values_ahead(lv, hb);
         }
         __builtin_amdgcn_s_setprio(1);
@@ -1179,41 +1172,41 @@ __global__ __launch_bounds__(64 * NW, D == 64 ? 4 : 2) void attn8_tile_kernel(Kv
   int v = v0;
 #pragma nounroll
   for (; v + 2 <= count; v += 2) {
-    page(v, std::integral_constant<int, 0>{});
-    page(v + 1, std::integral_constant<int, 1>{});
+    page(v, lk0, lv0);
+    page(v + 1, lk1, lv1);
   }
-  if (v < count) page(v, std::integral_constant<int, 0>{});
+  if (v < count) page(v, lk0, lv0);
   __builtin_amdgcn_s_waitcnt(0x0F70);  // the last copies (repeats) land before the LDS is given back
-#pragma unroll
-  for (int n = 0; n < NC; ++n) {
-    const float ln = l[n] + __shfl_xor(l[n], 32, 64);
-    if (cpos[n] < 0) continue;
-    if (sp.n > 1) {
-      float* const pr = out + (size_t)((w * NC + n) * 32 + c) * (D + 4);
-      if (hf == 0) {
-        pr[0] = m[n];
-        pr[1] = ln;
-      }
-      const float one = __builtin_amdgcn_ldexpf(1.0f, unit - kUnit);
-#pragma unroll
-      for (int i = 0; i < NT; ++i)
-#pragma unroll
-        for (int g = 0; g < 4; ++g)
-          *reinterpret_cast<f32x4*>(pr + 4 + 32 * i + 8 * g + 4 * hf) =
-              (f32x4){O[n][i][4 * g], O[n][i][4 * g + 1], O[n][i][4 * g + 2], O[n][i][4 * g + 3]} * one;
-      continue;
+  l += __shfl_xor(l, 32, 64);
+  const int cpos = column().pos;
+  if (cpos < 0) return;
+  if (sp.n > 1) {
+    float* const pr = out + (size_t)(w * 32 + c) * (D + 4);
+    if (hf == 0) {
+      pr[0] = m;
+      pr[1] = l;
     }
-    const float inv = __builtin_amdgcn_ldexpf(1.0f / ln, unit - kUnit);
+    const float one = __builtin_amdgcn_ldexpf(1.0f, unit - kUnit);
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
-      for (int g = 0; g < 4; ++g) {
-        float o[4];
-#pragma unroll
-        for (int r = 0; r < 4; ++r) o[r] = O[n][i][4 * g + r] * inv;
-        store4(a, t[n], h, 32 * i + 8 * g + 4 * hf, o);
-      }
+      for (int g = 0; g < 4; ++g)
+        *reinterpret_cast<f32x4*>(pr + 4 + 32 * i + 8 * g + 4 * hf) =
+            (f32x4){O[i][4 * g], O[i][4 * g + 1], O[i][4 * g + 2], O[i][4 * g + 3]} * one;
+    return;
   }
+  const int64_t t = (int64_t)row.cu + cpos - row.pos;
+  const int h = j * G + c - (cpos - w0) * G;
+  const float inv = __builtin_amdgcn_ldexpf(1.0f / l, unit - kUnit);
+#pragma unroll
+  for (int i = 0; i < NT; ++i)
+#pragma unroll
+    for (int g = 0; g < 4; ++g) {
+      float o[4];
+#pragma unroll
+      for (int r = 0; r < 4; ++r) o[r] = O[i][4 * g + r] * inv;
+      store4(a, t, h, 32 * i + 8 * g + 4 * hf, o);
+    }
 }
 
 // Partials of the chunks: a group has kv8_chunks() for each kv head or less, which over all
@@ -1240,13 +1233,14 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
     float* const tpart = part + a.tile_part;
     const int G = p.Hq / p.Hkv;
     const Kv8Splits splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
-    const int many = kv8_most_tiles(p.n, p.T, G), few = min(p.n, p.T) * kv8_few_tiles(G);
-    const dim3 grid(many * splits.many + few * splits.few + 1, p.Hkv);
-    hipLaunchKernelGGL((attn8_tile_kernel<D, kKv8TileWaves, 1>), grid, dim3(64 * kKv8TileWaves), 0,
+    const int many = kv8_most_tiles(p.n, p.T, G), few = p.n * kv8_few_tiles(G);
+    const dim3 grid(many * splits.many + min(few, p.T) * splits.few + 1, p.Hkv);
+    hipLaunchKernelGGL((attn8_tile_kernel<D, kKv8TileWaves>), grid, dim3(64 * kKv8TileWaves), 0,
                        a.stream, a, tpart, splits);
     if (splits.many > 1 || splits.few > 1) {
       if ((e = hipGetLastError()) != hipSuccess) return e;
-      hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, dim3(many + few, p.Hkv, D / 32), dim3(256), 0,
+      hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, dim3((splits.many > 1 ? many : 0) + (splits.few > 1 ? few : 0), p.Hkv, kKv8TileWaves),
+                         dim3(256), 0,
                          a.stream, a, tpart, splits);
     }
     return hipGetLastError();

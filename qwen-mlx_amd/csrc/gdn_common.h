@@ -508,7 +508,7 @@ __host__ __device__ inline int kv8_chunks(int n, int Hkv, int D, int groups) {
 // kv8_splits() pieces or less, where the step's bounds let the tiles be few: about
 // kv8_tile_groups() work-groups, and as many again of the rows of fewer than kKv8TileTokens.
 constexpr int kKv8TileWaves = 4;
-__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 256 ? 512 : 1536; }
+__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 256 ? 512 : 1280; }
 __host__ __device__ inline int kv8_most_tiles(int n, int T, int G) {
   const int a = T / (kKv8TileWaves * (32 / G)), b = T / kKv8TileTokens;
   return a + (n < b ? n : b);
