@@ -781,8 +781,8 @@ __global__ __launch_bounds__(64 * W) void attn8_join_kernel(Kv8AttnArgs a, const
 }
 
 // Tiles whose pages are split: grid (those of rows of few tokens, if any may be split, then those
-// of the others, if any may, Hkv, kKv8TileWaves), block 256: a wave's 32 columns, 8 lanes each, its
-// splits in order.
+// of the others, if any may, Hkv, kKv8TileWaves), block 256: a wave's 32 columns by eights, 8 lanes for
+// every fourth split of each, those in order and then the four sums.
 template <int D>
 __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, float* __restrict__ part,
                                                                Kv8Splits most_splits) {
@@ -806,37 +806,49 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
     tile = blockIdx.x - few - f.first;
     row = f.row;
   }
-  const int wave = blockIdx.z, c = threadIdx.x >> 3, ctok = c / G;
-  const int tok = tile * tpt + wave * tpw + ctok;
-  if (ctok >= tpw || tok >= row.fresh) return;
   const int n = splits_of(a, row, r, tpt, most_splits).n;
   if (n < 2) return;
+  const int wave = blockIdx.z;
   const int dim = 4 * (threadIdx.x & 7);  // and those 32, 64, .. further on
-  const float* const pc = split_part<D>(p, part, most_splits, r, row.fresh, tile, j) +
-                          (size_t)(wave * 32 + c) * (D + 4);
-  float M = -INFINITY, L = 0.f;
+  const int g = (threadIdx.x >> 3) & 3;
+  const float* const base = split_part<D>(p, part, most_splits, r, row.fresh, tile, j);
+  auto over_four = [](float x, auto join) {
+    x = join(x, __shfl_xor(x, 8, 64));
+    return join(x, __shfl_xor(x, 16, 64));
+  };
+  auto add = [](float x, float y) { return x + y; };
+#pragma nounroll
+  for (int c = threadIdx.x >> 5; c < 32; c += 8) {
+    const int ctok = c / G, tok = tile * tpt + wave * tpw + ctok;
+    if (ctok >= tpw || tok >= row.fresh) return;  // and so are those behind it
+    const float* const pc = base + (size_t)(wave * 32 + c) * (D + 4);
+    float M = -INFINITY, L = 0.f;
 #pragma unroll 4
-  for (int s = 0; s < n; ++s) M = fmaxf(M, pc[s * kStride]);
-  if (M == -INFINITY) M = 0.f;  // NaN scores alone
-  f32x4 A[D / 32];
+    for (int s = g; s < n; s += 4) M = fmaxf(M, pc[s * kStride]);
+    M = over_four(M, [](float x, float y) { return fmaxf(x, y); });
+    if (M == -INFINITY) M = 0.f;  // NaN scores alone
+    f32x4 A[D / 32];
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) A[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    for (int i = 0; i < D / 32; ++i) A[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
 #pragma unroll(512 / D)
-  for (int s = 0; s < n; ++s) {
-    const float f = exp2f(pc[s * kStride] - M), l = pc[s * kStride + 1];
-    f32x4 v[D / 32];
+    for (int s = g; s < n; s += 4) {
+      const float f = exp2f(pc[s * kStride] - M), l = pc[s * kStride + 1];
+      f32x4 v[D / 32];
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) v[i] = *reinterpret_cast<const f32x4*>(pc + s * kStride + 4 + dim + 32 * i);
-    if (l == 0.f) continue;  // a split without a visible key holds nothing
-    L += f * l;
+      for (int i = 0; i < D / 32; ++i) v[i] = *reinterpret_cast<const f32x4*>(pc + s * kStride + 4 + dim + 32 * i);
+      if (l == 0.f) continue;  // a split without a visible key holds nothing
+      L += f * l;
 #pragma unroll
-    for (int i = 0; i < D / 32; ++i) A[i] += v[i] * f;
-  }
-  const float inv = 1.0f / L;
+      for (int i = 0; i < D / 32; ++i) A[i] += v[i] * f;
+    }
+    const float inv = 1.0f / over_four(L, add);
 #pragma unroll
-  for (int i = 0; i < D / 32; ++i) {
-    float o[4] = {A[i][0] * inv, A[i][1] * inv, A[i][2] * inv, A[i][3] * inv};
-    store4(a, (int64_t)row.cu + tok, j * G + c - ctok * G, dim + 32 * i, o);
+    for (int i = 0; i < D / 32; ++i) {
+      float o[4];
+#pragma unroll
+      for (int k = 0; k < 4; ++k) o[k] = over_four(A[i][k], add) * inv;
+      if (i % 4 == g) store4(a, (int64_t)row.cu + tok, j * G + c - ctok * G, dim + 32 * i, o);
+    }
   }
 }
 
@@ -1224,6 +1236,15 @@ size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
   return (kv8_attn_chunk_floats(d) + tiles) * sizeof(float);
 }
 
+// Pieces that the pages of at most `tiles` work-groups are cut into. Two lie on a CU side by side
+// (D = 64: four): tiles for half of the places or fewer are cut to fill them, 1,024 tokens behind
+// 4,096 (D = 256, 130 tiles) 117 us in 3 pieces and 148 in 5; more tiles into two rounds of work,
+// 19 ragged rows (D = 256, 320 at most) 268 us whole and 209 in 3; those of 64 dims (356) 107 us in
+// 2 pieces, 93 in 3, 94 in 5.
+static int tile_pieces(int64_t tiles, int D) {
+  return max(1, (int)((D == 64 ? 1280 : tiles <= 256 ? 512 : 1024) / tiles));
+}
+
 template <int D>
 static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   const Kv8Plan& p = a.p;
@@ -1232,8 +1253,10 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   if (p.max_row >= kKv8TileTokens) {
     float* const tpart = part + a.tile_part;
     const int G = p.Hq / p.Hkv;
-    const Kv8Splits splits = kv8_splits(p.n, p.T, p.Hkv, G, D);
     const int many = kv8_most_tiles(p.n, p.T, G), few = p.n * kv8_few_tiles(G);
+    // 63 single tokens at 4,096 beside a prompt of 512 (D = 256): 73 us, from 512 work-groups 94
+    const Kv8Splits splits{tile_pieces((int64_t)many * p.Hkv, D),
+                           max(1, (D == 256 ? 384 : 768) / (few * p.Hkv))};
     const dim3 grid(many * splits.many + min(few, p.T) * splits.few + 1, p.Hkv);
     hipLaunchKernelGGL((attn8_tile_kernel<D, kKv8TileWaves>), grid, dim3(64 * kKv8TileWaves), 0,
                        a.stream, a, tpart, splits);

@@ -495,7 +495,7 @@ struct Kv8Plan {
 // enough pages, and four a piece where segments (rows x kv heads) are few.
 constexpr int kKv8TileTokens = 16;
 // those that run side by side: one a SIMD at D = 256 (512 registers), two at less
-__host__ __device__ constexpr int kv8_waves(int D) { return D == 256 ? 1024 : 2048; }
+__host__ __device__ constexpr int kv8_waves(int D) { return D == 64 ? 1280 : 1024; }
 constexpr int kKv8FewSegments = 32;
 __host__ __device__ inline int kv8_chunk_waves(int n, int Hkv) {
   return n * Hkv <= kKv8FewSegments ? 4 : 1;
@@ -504,11 +504,11 @@ __host__ __device__ inline int kv8_chunks(int n, int Hkv, int D, int groups) {
   const int c = kv8_waves(D) / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
   return c < 1 ? 1 : c;
 }
-// Steps with rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens of a row, their pages in
-// kv8_splits() pieces or less, where the step's bounds let the tiles be few: about
-// kv8_tile_groups() work-groups, and as many again of the rows of fewer than kKv8TileTokens.
+// Steps with rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens of a row, their pages cut
+// into pieces where the step's bounds let the tiles be few, of at most kv8_tile_groups()
+// work-groups, and those of the rows of fewer than kKv8TileTokens into pieces of as many.
 constexpr int kKv8TileWaves = 4;
-__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 256 ? 512 : 1280; }
+__host__ __device__ constexpr int kv8_tile_groups(int D) { return D == 64 ? 1280 : 1024; }
 __host__ __device__ inline int kv8_most_tiles(int n, int T, int G) {
   const int a = T / (kKv8TileWaves * (32 / G)), b = T / kKv8TileTokens;
   return a + (n < b ? n : b);
@@ -520,11 +520,6 @@ __host__ __device__ inline int kv8_few_tiles(int G) {  // of a row of few tokens
 struct Kv8Splits {
   int many, few;  // at most, of a tile of a row of many tokens and of one of few
 };
-__host__ __device__ inline Kv8Splits kv8_splits(int n, int T, int Hkv, int G, int D) {
-  const int64_t many = (int64_t)kv8_most_tiles(n, T, G) * Hkv, few = (int64_t)n * kv8_few_tiles(G) * Hkv;
-  const int64_t a = kv8_tile_groups(D) / (many > 0 ? many : 1), b = kv8_tile_groups(D) / few;
-  return {a < 1 ? 1 : (int)a, b < 1 ? 1 : (int)b};
-}
 constexpr int kKv8Rows = 4096;  // rows of a step
 struct Kv8StepArgs {
   Kv8Plan p;
