@@ -922,11 +922,13 @@ typedef struct gdn_kv8_attn_desc {
  * DEVICE arrays (or NULL). Tokens of refused rows get zeros; rows behind the last
  * token are left as they are.
  *
- * Products and sums are f32; the softmax's weights enter the product with the values in f16
- * (11 bits), and out is rounded once. The bits are the same every time and do not
+ * Products and sums are f32; dimensions of q below 2^-13 of its head's largest are rounded
+ * by at most 2^-21 of that, the softmax's weights enter the product with the values in
+ * f16 (11 bits), and out is rounded once. The bits are the same every time and do not
  * depend on what the step's other rows are; the kernel and the places where keys are
- * split follow the row's tokens and the step's bounds (n, max_tokens), so that steps of
- * other bounds may differ by rounding. A NaN among the keys or values of a kv head
+ * split follow the row's tokens and the step's bounds (n, max_tokens, max_row_tokens), so
+ * that steps of other bounds may differ by rounding. An infinity or NaN in a head of q
+ * makes that head's output NaN. A NaN among the keys or values of a kv head
  * that a token sees makes its query heads there NaN; tokens that do not see it are
  * not touched. */
 gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc* desc,

@@ -112,8 +112,9 @@ class Ref:
         The tolerance adds what the contract allows: bf16's half step 2^-8 of the result; the
         weights' half step 2^-11 of sum p|v| (f16), or 2^-25 of each |v| below f16's normal
         numbers; f32 sums of D products in a score (D 2^-24 of sum |q k|), of f32 scores
-        (2^-22 of their size, of the cap where there is one, of the distance term), each
-        moving weights by twice its size; f32 sums over the keys, n 2^-24 of sum p|v|; some
+        (2^-22 of their size, of the cap where there is one, of the distance term) and q's
+        dimensions below 2^-13 of its head's largest to 2^-21 of that, each moving weights by
+        twice its size; f32 sums over the keys, n 2^-24 of sum p|v|; some
         roundings of f32 in the norm and gate (2^-20)."""
         Hq = q.shape[1]
         G = Hq // self.heads
@@ -134,6 +135,9 @@ class Ref:
                     sc = qk.sum(1) * scale
                     err = np.abs(qk).sum(1) * abs(scale) * self.dim * 2.0 ** -24
                     err += 2.0 ** -22 * np.abs(sc)
+                    most = np.abs(q[c + t, h]).max()
+                    low = np.abs(q[c + t, h]) < 2.0 ** -13 * most
+                    err += 2.0 ** -21 * most * abs(scale) * np.abs(k[:, low]).sum(1)
                     if softcap:
                         sc = softcap * np.tanh(sc / softcap)
                         err += 2.0 ** -21 * softcap

@@ -590,3 +590,169 @@ def test_steps_without_tokens(gpu):
     kv.gather(0, i32(range(64)), out, None)
     assert not out.any()
     kv.close()
+
+
+@pytest.mark.parametrize("hq,hk,dim", [(16, 1, 64), (6, 2, 128), (16, 2, 256)])
+def test_few_tokens_beside_prompts(gpu, hq, hk, dim):
+    """Rows of 1 to 15 tokens in steps with longer ones, in two tiles where 16 query heads share
+    keys, their pages in many pieces; options; a refused row among them."""
+    rng = np.random.default_rng(18)
+    p = Pair(7, 110, 40, hq=hq, hk=hk, dim=dim, tokens=2700)
+    p.step([0, 1, 5], [0, 0, 0], [2300, 300, 64])
+    p.append(rng)
+    p.step([5, 0, 2, 1, 9, 3], [64, 2300, 0, 300, 0, 0], [1, 15, 20, 9, 3, 2], tokens=52)
+    assert p.kv.check() == 1
+    p.append(rng)
+    p.ref.flags = 0
+    p.attention(rng, label="few beside many", gate=True)
+    p.attention(rng, label="few beside many, window", window=200, softcap=10.0)
+    p.attention(rng, label="few beside many, prefix", prefix=[3, 500, 0, 9, 7, 40], window=30,
+                slopes=[0.02 * (h - 2) for h in range(hq)])
+    p.step([0, 2], [2315, 20], [1, 18], tokens=30)
+    p.append(rng)
+    p.attention(rng, label="one beside many")
+    p.kv.close()
+
+
+@pytest.mark.parametrize("n,longest", [(4096, 1), (700, 30)])
+def test_attention_of_many_rows(gpu, n, longest):
+    rng = np.random.default_rng(19)
+    p = Pair(n, 3 * n, 3, hq=2, hk=1, dim=64, tokens=60 * n)
+    slots = rng.permutation(n).tolist()
+    lens = rng.integers(0, 80, n).tolist()
+    p.step(slots, [0] * n, lens)
+    p.append(rng)
+    ntok = [1] * n
+    ntok[n // 2] = longest
+    p.step(slots, lens, ntok)
+    p.append(rng)
+    p.attention(rng, label=f"{n} rows")
+    p.kv.close()
+
+
+@pytest.mark.parametrize("dim", [64, 256])
+def test_queries_of_every_size(gpu, dim):
+    """A head's dimensions from its largest down to 2^-30 of it, where the largest meet keys of
+    zero, so that the small ones make the scores."""
+    import torch
+    rng = np.random.default_rng(20)
+    p = Pair(2, 12, 6, hq=4, hk=2, dim=dim)
+    small = torch.arange(dim, device="cuda:0") % 31
+    done = []
+
+    def keys(x):
+        if not done:
+            x[:, :, small < 12] = 0
+            x[:, :, small >= 12] *= 64
+        done.append(x)
+
+    for step in ([0, 1], [0, 0], [20, 130]), ([0, 1], [20, 130], [20, 1]), ([1, 0], [131, 40], [2, 1]):
+        p.step(*step)
+        done.clear()
+        p.append(rng, change=keys)
+        t = p.kv.tokens
+        q, _ = bf(rng, t, 4, dim)
+        q = (q.float() * 2.0 ** (14 - small)).to(torch.bfloat16)
+        out = torch.zeros_like(q)
+        p.kv.attention(0, q, out, scale=0.05)
+        want, tol = p.ref.attention(num(q), scale=0.05)
+        assert np.all(np.abs(num(out) - want) <= tol)
+    p.kv.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+def test_infinities_and_nan_in_queries_stay_in_their_heads(gpu, dim):
+    import torch
+    rng = np.random.default_rng(21)
+    p = Pair(2, 12, 6, hq=8, hk=2, dim=dim)
+    for step in ([1, 0], [0, 0], [70, 33]), ([0, 1], [33, 70], [1, 3]):  # tiles, chunks
+        p.step(*step)
+        p.append(rng)
+        t = p.kv.tokens
+        q, _ = bf(rng, t, 8, dim)
+        clean = torch.zeros_like(q)
+        p.kv.attention(0, q, clean)
+        odd = q.clone()
+        want = torch.zeros(t, 8, dtype=torch.bool, device="cuda:0")
+        for at, h, value in ((0, 0, "inf"), (1, 3, "nan"), (t - 1, 7, "-inf"), (2, 4, "nan")):
+            odd[at, h, (5 * h) % dim] = float(value)
+            want[at, h] = True
+        out = torch.zeros_like(q)
+        p.kv.attention(0, odd, out)
+        assert torch.equal(torch.isnan(out).all(2), want)
+        assert torch.equal(out[~want], clean[~want])
+    p.kv.close()
+
+
+def test_offsets_past_32_bits(gpu):
+    """More than 4 GiB of pages in a layer, the last of them in use."""
+    rng = np.random.default_rng(22)
+    pages = 17000
+    p = Pair(3, pages, pages, hq=16, hk=8, dim=256, tokens=200)
+    assert pages * 2 * 8 * 64 * 256 > 2 ** 32 + 2 ** 27
+    p.step([0], [(pages - 6) * 64], [0])
+    p.step([1, 2], [0, 0], [100, 20])
+    p.append(rng)
+    p.check_held()
+    p.attention(rng, label="far pages")
+    p.step([2, 1], [20, 100], [1, 5])
+    p.append(rng)
+    p.check_held()
+    p.attention(rng, label="far pages, tokens")
+    p.kv.close()
+
+
+def test_graphs_that_share_a_cache(gpu):
+    """Two captured steps of one cache, of tokens and of prompts, replayed in turn with eager
+    steps between them; every replay against a twin cache's eager calls."""
+    import torch
+    import gdn_amd
+    rng = np.random.default_rng(23)
+    hq, hk, d = 8, 2, 64
+    twin = [gdn_amd.KV8Cache(1, 6, 60, 20, hq, hk, d, 256) for _ in range(2)]
+    plans = [dict(slots=i32([4, 0]), tok=i32([1, 2]), T=4, most=2),
+             dict(slots=i32([1, 5, 3]), tok=i32([40, 7, 0]), T=60, most=40)]
+    bufs = []
+    for kv in twin:
+        mine = []
+        for pl in plans:
+            b = {w: torch.zeros(pl["T"], h, d, device="cuda:0", dtype=torch.bfloat16)
+                 for w, h in (("q", hq), ("k", hk), ("v", hk), ("out", hq))}
+            b["lens"] = torch.zeros_like(pl["slots"])
+            mine.append(b)
+        bufs.append(mine)
+
+    def step(kv, pl, b):
+        kv.step(pl["slots"], b["lens"], pl["tok"], pl["T"], pl["most"], lens_out=b["lens"])
+        kv.append(0, b["k"], b["v"])
+        kv.attention(0, b["q"], b["out"])
+
+    for kv, mine in zip(twin, bufs):  # both once before the capture
+        for pl, b in zip(plans, mine):
+            step(kv, pl, b)
+    torch.cuda.synchronize()
+    graphs = []
+    for pl, b in zip(plans, bufs[0]):
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g):
+            step(twin[0], pl, b)
+        graphs.append(g)
+    for i in range(8):
+        which = (0, 1, 1, 0, 0, 1, 0, 1)[i]
+        for w, h in (("q", hq), ("k", hk), ("v", hk)):
+            x = bf(rng, plans[which]["T"], h, d)[0]
+            for mine in bufs:
+                mine[which][w].copy_(x)
+        if i == 4:  # an eager step between the replays
+            step(twin[0], plans[which], bufs[0][which])
+        else:
+            graphs[which].replay()
+        step(twin[1], plans[which], bufs[1][which])
+        torch.cuda.synchronize()
+        a, b = bufs[0][which], bufs[1][which]
+        assert a["lens"].tolist() == b["lens"].tolist()
+        used = int(plans[which]["tok"].sum())
+        assert torch.equal(a["out"][:used], b["out"][:used]), i
+    for kv in twin:
+        assert kv.check() == 0
+        kv.close()
