@@ -861,10 +861,16 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
 // Lane (hf, c), hf = lane / 32, holds keys 8 i + 4 hf + r of a block of 32 (i, r = 0 .. 3) for
 // column c, and dims 32 t + 8 i + 4 hf + r of its outputs in units of 2^(unit - kUnit).
 //
-// Two waves a SIMD or more, each in at most 256 registers: at D = 256 its outputs are 128 of them,
-// q's parts 64, and what only rare branches need is kept in LDS.
+// As many waves a SIMD as the outputs and q's parts (128 + 64 registers at D = 256) leave room for,
+// 2, 3 and 4 at 256, 128 and 64 dims; one's products run beside the others' softmax, so that a
+// wave's own steps stay in order. 8,192 tokens of 16 query heads over 2 of 256 dims: one wave a
+// SIMD with the steps of two blocks side by side 665 us, two 500; products and softmax of half
+// the waves in turn, by barriers, 508. At that rate (1.1 PFLOP/s, of which a third of the
+// instructions' work is the scores' second part) the clock, not a unit, is what gives: the f16
+// products alone run at 1.6 GHz on such numbers, and at 2.1 on zeros. 19 rows of 1 .. 571 tokens
+// of 32 query heads over 8 of 128 dims: 255 us in two waves a SIMD, 231 in three.
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
+__global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
                                                                 Kv8Splits most_splits) {
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
