@@ -466,7 +466,7 @@ __device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& 
   most = min(most + (c.groups > 1 && a.window > 0 ? 1 : 0), (total + kPage - 1) / kPage);
   // whole pages for each of a chunk's waves
   const int waves = kv8_chunk_waves(a.p.n, a.p.Hkv);
-  const int cp = (most - 1) / kv8_chunks(a.p.n, a.p.Hkv, a.p.D, c.groups) + 1;
+  const int cp = (most - 1) / kv8_chunks(a.p.n, a.p.Hkv, c.groups) + 1;
   c.cp = (cp + waves - 1) / waves * waves;
   c.nch = (most + c.cp - 1) / c.cp;
   return c;
@@ -699,11 +699,13 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
 
 // Rows of few tokens: grid (n * per, Hq), block 64 W; token k < per of row r, a head: its chunks,
 // chunk i in sum i % 16, wave w the sums w, w + W, ..; then the sums in order. Rows of a single
-// chunk are written already.
-template <int D, int W>
-__global__ __launch_bounds__(64 * W) void attn8_join_kernel(Kv8AttnArgs a, const float* __restrict__ part,
-                                                            int per) {
-  constexpr int DPL = D / 64, kPer = 16 / W;
+// chunk are written already. Bound by latency, the row, its chunks and their rows one after the
+// other: 4 waves with four sums each take a token's 128 chunks of 16 heads of 256 dims in 6 us,
+// 16 waves with one sum each, which a work-group has to wait for, in 7.5.
+template <int D>
+__global__ __launch_bounds__(256) void attn8_join_kernel(Kv8AttnArgs a, const float* __restrict__ part,
+                                                         int per) {
+  constexpr int W = 4, DPL = D / 64, kPer = 16 / W;
   constexpr size_t kStride = (size_t)16 * (D + 4);  // of a token's chunks
   typedef float fvec __attribute__((ext_vector_type(DPL)));
   __shared__ float sum[16][D];
@@ -865,9 +867,9 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
 // 2, 3 and 4 at 256, 128 and 64 dims; one's products run beside the others' softmax, so that a
 // wave's own steps stay in order. 8,192 tokens of 16 query heads over 2 of 256 dims: one wave a
 // SIMD with the steps of two blocks side by side 665 us, two 500; products and softmax of half
-// the waves in turn, by barriers, 508. At that rate (1.1 PFLOP/s, of which a third of the
-// instructions' work is the scores' second part) the clock, not a unit, is what gives: the f16
-// products alone run at 1.6 GHz on such numbers, and at 2.1 on zeros. 19 rows of 1 .. 571 tokens
+// the waves in turn, by barriers, 508. At that rate (1.1 PFLOP/s, a quarter of the matrix time
+// on top for the scores' second part) the clock, not a unit, is what gives: the f16
+// products alone run at 1.6 GHz on such numbers, and at 2.2 on constants. 19 rows of 1 .. 571 tokens
 // of 32 query heads over 8 of 128 dims: 255 us in two waves a SIMD, 231 in three.
 template <int D, int NW>
 __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
@@ -1228,11 +1230,11 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
 }
 
 // Partials of the chunks: a group has kv8_chunks() for each kv head or less, which over all
-// groups are kv8_waves() or one each.
+// groups are kKv8Waves or one each.
 size_t kv8_attn_chunk_floats(const gdn_kv8_desc& d) {
   const int64_t few = (int64_t)d.num_slots * (kKv8TileTokens - 1);
   const int64_t groups = few < d.max_step_tokens ? few : d.max_step_tokens;
-  return (size_t)(kv8_waves(d.head_dim) + groups * d.num_kv_heads) * 16 * (d.head_dim + 4);
+  return (size_t)(kKv8Waves + groups * d.num_kv_heads) * 16 * (d.head_dim + 4);
 }
 
 size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
@@ -1276,7 +1278,7 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   }
   // as many as the rows can have, up to four rounds of the chip's waves
   const int W = kv8_chunk_waves(p.n, p.Hkv);
-  const int64_t most = kv8_waves(D) / W + (int64_t)p.Hkv * min(p.T, p.n * p.max_row);
+  const int64_t most = kKv8Waves / W + (int64_t)p.Hkv * min(p.T, p.n * p.max_row);
   const dim3 grid((unsigned)(most < 8192 / W ? most : 8192 / W));
   if (W == 1)
     hipLaunchKernelGGL((attn8_chunk_kernel<D, 1>), grid, dim3(64), 0, a.stream, a, part);
@@ -1285,10 +1287,7 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   if ((e = hipGetLastError()) != hipSuccess) return e;
   const int per = p.max_row;
   const dim3 few(p.n * per, p.Hq);
-  if (p.n * per * p.Hq <= 512)  // a wave for each sum where the work-groups are few
-    hipLaunchKernelGGL((attn8_join_kernel<D, 16>), few, dim3(1024), 0, a.stream, a, part, per);
-  else
-    hipLaunchKernelGGL((attn8_join_kernel<D, 4>), few, dim3(256), 0, a.stream, a, part, per);
+  hipLaunchKernelGGL(attn8_join_kernel<D>, few, dim3(256), 0, a.stream, a, part, per);
   return hipGetLastError();
 }
 

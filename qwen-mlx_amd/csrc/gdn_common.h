@@ -489,19 +489,24 @@ struct Kv8Plan {
   int32_t* parts;               // [n] attention's chunks (of a kv head) of the rows before, at most
   int32_t* tiles;               // [n] its tiles of the rows before
 };
-// Attention of few new tokens (below kKv8TileTokens in a row): groups of 16 / G tokens, the pages
-// that a group sees in kv8_chunks() pieces or less, a partial result each, shared by `waves`
-// waves. By the step's bounds and the row alone: about kv8_waves() waves where every row has
+// Attention of few new tokens (below kKv8TileTokens in every row): groups of 16 / G tokens, the
+// pages that a group sees in kv8_chunks() pieces or less, a partial result each, shared by `waves`
+// waves. By the step's bounds and the row alone: about kKv8Waves waves where every row has
 // enough pages, and four a piece where segments (rows x kv heads) are few.
+// Steps of 16 rows at 4,096 by chunks / by tiles: of 12 tokens 35 / 43 us (64 dims), 66 / 83 (128),
+// 73 / 67 (256); of 15 tokens 40 / 43, 85 / 84, 79 / 71; of 24 tokens 56 / 47, 105 / 98, 123 / 80.
 constexpr int kKv8TileTokens = 16;
-// those that run side by side: one a SIMD at D = 256 (512 registers), two at less
-__host__ __device__ constexpr int kv8_waves(int D) { return D == 64 ? 1280 : 1024; }
-constexpr int kKv8FewSegments = 32;
+// one a SIMD (at D = 256, of 512 registers, there is no room for more): 64 rows at 4,096 take 60 us
+// of 1,024 waves and 69 of 2,048, of 64 dims 33 and 35; 512 take 58 there, and 23 not 19 for 4 rows
+constexpr int kKv8Waves = 1024;
+// 8 segments of 128 dims, a row at 32,000: 22 us by four waves a piece, 28 by one; 16 segments of 256
+// dims at 4,096: 23 and 21
+constexpr int kKv8FewSegments = 8;
 __host__ __device__ inline int kv8_chunk_waves(int n, int Hkv) {
   return n * Hkv <= kKv8FewSegments ? 4 : 1;
 }
-__host__ __device__ inline int kv8_chunks(int n, int Hkv, int D, int groups) {
-  const int c = kv8_waves(D) / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
+__host__ __device__ inline int kv8_chunks(int n, int Hkv, int groups) {
+  const int c = kKv8Waves / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
   return c < 1 ? 1 : c;
 }
 // Steps with rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens of a row, their pages cut
