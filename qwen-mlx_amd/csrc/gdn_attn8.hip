@@ -825,24 +825,31 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
     if (ctok >= tpw || tok >= row.fresh) return;  // and so are those behind it
     const float* const pc = base + (size_t)(wave * 32 + c) * (D + 4);
     float M = -INFINITY, L = 0.f;
-#pragma unroll 4
-    for (int s = g; s < n; s += 4) M = fmaxf(M, pc[s * kStride]);
-    M = over_four(M, [](float x, float y) { return fmaxf(x, y); });
-    if (M == -INFINITY) M = 0.f;  // NaN scores alone
     f32x4 A[D / 32];
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) A[i] = (f32x4){0.f, 0.f, 0.f, 0.f};
+    // the sums so far times 2^(M - to) as the maximum goes on to `to`; NaN scores alone leave it
+    auto rise = [&](float to) {
+      const float f = exp2f(M - (to == -INFINITY ? 0.f : to));
+      L *= f;
+#pragma unroll
+      for (int i = 0; i < D / 32; ++i) A[i] *= f;
+      M = to;
+    };
 #pragma unroll(512 / D)
     for (int s = g; s < n; s += 4) {
-      const float f = exp2f(pc[s * kStride] - M), l = pc[s * kStride + 1];
+      const float m = pc[s * kStride], l = pc[s * kStride + 1];
       f32x4 v[D / 32];
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) v[i] = *reinterpret_cast<const f32x4*>(pc + s * kStride + 4 + dim + 32 * i);
       if (l == 0.f) continue;  // a split without a visible key holds nothing
+      rise(fmaxf(M, m));
+      const float f = exp2f(m - (M == -INFINITY ? 0.f : M));
       L += f * l;
 #pragma unroll
       for (int i = 0; i < D / 32; ++i) A[i] += v[i] * f;
     }
+    rise(over_four(M, [](float x, float y) { return fmaxf(x, y); }));
     const float inv = 1.0f / over_four(L, add);
 #pragma unroll
     for (int i = 0; i < D / 32; ++i) {
