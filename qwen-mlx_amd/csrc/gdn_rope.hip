@@ -3,7 +3,8 @@
 //   (y_a, y_b) -> (y_a cos - y_b sin, y_a sin + y_b cos) of pair i at pos * f_i
 // The angle in turns is a product in 64 bits, of which the fraction goes on in f32: at
 // position 10^6 an f32 product would be off by 2^-5 turns.
-// Bound by HBM: each element is read and written once.
+// Bound by HBM: each element is read and written once; 16,384 tokens of 18 bf16 heads of 256 dims,
+// 302 MB, 59 us (5.1 TB/s where a large copy reaches 5.2), 64 of them 4 us.
 #include "gdn_common.h"
 
 namespace gdn {
