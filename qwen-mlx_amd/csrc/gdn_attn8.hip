@@ -235,7 +235,7 @@ __device__ __forceinline__ Group group_of(const Kv8AttnArgs& a, const Kv8Row& ro
   x.t = (int64_t)row.cu + k0 + (x.valid ? ctok : 0);
   x.cpos = x.valid ? x.pos0 + ctok : -1;
   x.pf = a.prefix ? min(max(a.prefix[r], 0), x.total) : 0;
-  x.lo = a.window > 0 ? x.cpos - a.window : -1;  // keys above it
+  x.lo = a.window > 0 ? max(x.cpos - a.window, -1) : -1;  // keys above it
   x.span = span_of(x.pos0, x.pos0 + x.nt - 1, a.window, x.pf, x.total);
   return x;
 }
@@ -1063,7 +1063,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
       asm volatile("");
       const int cpos = column().pos;
       auto below = [](int k) { return first_scores<8>(k, 16); };  // of keys below kl + k
-      seen = (below(cpos + 1 - kl) & ~below(cpos - window + 1 - kl)) | below(cpos >= 0 ? pf - kl : 0);
+      seen = (below(cpos + 1 - kl) & ~below(max(cpos - window, -1) + 1 - kl)) |
+             below(cpos >= 0 ? pf - kl : 0);
 #pragma unroll
       for (int i = 0; i < 16; ++i) S[i] = (seen >> i) & 1u ? S[i] : -INFINITY;
     }

@@ -756,3 +756,19 @@ def test_graphs_that_share_a_cache(gpu):
     for kv in twin:
         assert kv.check() == 0
         kv.close()
+
+
+@pytest.mark.parametrize("window", [2 ** 31 - 1, 2 ** 30, 1000])
+def test_windows_longer_than_any_row(gpu, window):
+    import torch
+    rng = np.random.default_rng(24)
+    p = Pair(2, 12, 6, hq=4, hk=2, dim=64)
+    for step in ([1, 0], [0, 0], [70, 33]), ([0, 1], [33, 70], [1, 3]):  # tiles, chunks
+        p.step(*step)
+        p.append(rng)
+        q, _ = bf(rng, p.kv.tokens, 4, 64)
+        whole, out = torch.zeros_like(q), torch.zeros_like(q)
+        p.kv.attention(0, q, whole)
+        p.kv.attention(0, q, out, window=window)
+        assert torch.equal(whole, out)
+    p.kv.close()
