@@ -867,6 +867,11 @@ gdn_status gdn_kv8_describe(const gdn_kv8* kv, gdn_kv8_desc* desc);
  * refused for it counts). A refused row keeps its pages; its tokens are skipped:
  * they have no place, and attention gives them zeros.
  *
+ * gdn_kv8_append and gdn_kv8_attention follow the bounds of the last gdn_kv8_step call
+ * and the plan that the last step left on the GPU: outside a graph they go behind a step
+ * outside a graph. Behind a replay of another step's graph its rows inside those bounds are
+ * worked on, the others left out.
+ *
  * lens_out (or NULL; may be lens) receives lens[i] + ntok[i], a refused or
  * padding row's lens[i]. */
 gdn_status gdn_kv8_step(gdn_kv8* kv, int32_t n, const int32_t* slots, const int32_t* lens,

@@ -139,7 +139,8 @@ __device__ __forceinline__ Found find_row(const Kv8Plan& p, int g, F items) {
   int before = 0;
   for (int b = 0; b < p.n; b += 64) {
     const int r = b + lane;
-    const Kv8Row row = r < p.n ? p.rows[r] : Kv8Row{-1, 0, 0, 0};
+    Kv8Row row = r < p.n ? p.rows[r] : Kv8Row{-1, 0, 0, 0};
+    row.fresh = kv8_tokens(p, row);
     const int mine = row.fresh > 0 ? items(r, row) : 0;
     const int s = wave_scan(mine);
     const int total = __builtin_amdgcn_readlane(s, 63);
@@ -718,7 +719,7 @@ __global__ __launch_bounds__(256) void attn8_join_kernel(Kv8AttnArgs a, const fl
   const int r = blockIdx.x / per, k = blockIdx.x - r * per;
   const Kv8Row row = p.rows[r];
   const int parts = p.parts[r];
-  if (k >= row.fresh) return;
+  if (k >= kv8_tokens(p, row)) return;
   const int G = p.Hq / p.Hkv, tpg = 16 / G, j = h / G, grp = k / tpg, c = (k - grp * tpg) * G + h - j * G;
   const int nch = chunks_of(a, row, r, tpg).nch;
   if (nch < 2) return;
@@ -803,6 +804,7 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
     r = blockIdx.x / ft;
     tile = blockIdx.x - r * ft;
     row = p.rows[r];
+    row.fresh = kv8_tokens(p, row);
     if (row.fresh >= kKv8TileTokens) return;
   } else {
     const Found f = find_row(p, blockIdx.x - few, [&](int, const Kv8Row& x) {

@@ -485,10 +485,16 @@ struct Kv8Plan {
   int32_t* map;                 // [T]
   int32_t* tok_row;             // [T] row, -1: of a refused row, -2: behind the last token
   Kv8Row* rows;                 // [n]
+  int32_t* used;                // [1] n; rows behind it hold nothing
   int32_t* blocks;              // [n + 1] pages that the rows before touch
   int32_t* parts;               // [n] attention's chunks (of a kv head) of the rows before, at most
   int32_t* tiles;               // [n] its tiles of the rows before
 };
+// Tokens of a row inside the bounds that a call was given. The plan may be another step's than
+// these, a replayed graph's: what does not fit them is left out, so that no access leaves a tensor.
+__host__ __device__ inline int kv8_tokens(const Kv8Plan& p, const Kv8Row& r) {
+  return r.fresh > 0 && r.fresh <= p.max_row && r.cu + r.fresh <= p.T ? r.fresh : 0;
+}
 // Attention of few new tokens (below kKv8TileTokens in every row): groups of 16 / G tokens, the
 // pages that a group sees in kv8_chunks() pieces or less, a partial result each, shared by `waves`
 // waves. By the step's bounds and the row alone: about kKv8Waves waves where every row has

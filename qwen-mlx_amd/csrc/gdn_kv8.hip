@@ -148,7 +148,7 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
   bool ok[R];
   uint32_t flags = 0;
   if (tid == 0) taken = 0;
-  const int count = *p.free_count;
+  const int count = *p.free_count, used = *p.used;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = tid * R + i;
@@ -285,9 +285,11 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     b0 += touched[i];
     c1 += chunks[i];
   }
+  for (int r = p.n + tid; r < used; r += TH) p.rows[r] = Kv8Row{-1, 0, 0, 0};
   if (tid == 0) {
     p.blocks[p.n] = total;
     *p.free_count = avail - taken;
+    *p.used = p.n;
   }
   if (flags) atomicOr(p.status, flags);
   if (p.T <= kMapHere)
@@ -364,7 +366,8 @@ __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   if (e >= p.blocks[p.n]) return;
   const int r = row_of(p.blocks, p.n, e);
   const Kv8Row row = p.rows[r];
-  const int slot = row.slot, len = row.pos, fresh = row.fresh;
+  const int slot = row.slot, len = row.pos, fresh = kv8_tokens(p, row);
+  if (fresh == 0) return;
   const int blk = len / kPage + e - p.blocks[r];
   const int first = blk * kPage;
   const int old = max(len - first, 0);                  // tokens that are there

@@ -772,3 +772,46 @@ def test_windows_longer_than_any_row(gpu, window):
         p.kv.attention(0, q, out, window=window)
         assert torch.equal(whole, out)
     p.kv.close()
+
+
+def test_eager_calls_behind_another_steps_replay(gpu):
+    """Append and attention under one step's bounds where a replayed graph has planned another:
+    its rows that fit are worked on, nothing outside the tensors or the pages is touched."""
+    import torch
+    import gdn_amd
+    rng = np.random.default_rng(25)
+    hq, hk, d = 4, 2, 64
+    kv = gdn_amd.KV8Cache(1, 8, 40, 10, hq, hk, d, 256)
+    wide = dict(slots=i32([0, 1, 2]), lens=i32([0, 0, 0]), tok=i32([9, 30, 80]))
+    kv.step(wide["slots"], wide["lens"], wide["tok"], 120, 80)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv.step(wide["slots"], wide["lens"], wide["tok"], 120, 80)
+    # rows of a step that releases the slots, so that nothing behind its n may be followed
+    kv.step(i32([5, 4, 3, 2, 1, 0]), i32([70, 0, 0, 0, 0, 0]), i32([2, 1, 1, 0, 0, 0]), 20, 20)
+    graph.replay()  # three rows, of which the first fits 20 tokens, and none 8 rows
+    q, k, v = (bf(rng, 24, h, d)[0] for h in (hq, hk, hk))
+    out = torch.full_like(q, 7.0)
+    kv.append(0, k[:20], v[:20])
+    kv.attention(0, q[:20], out[:20])
+    ko = torch.zeros(9, hk, d, device="cuda:0", dtype=torch.bfloat16)
+    kv.gather(0, kv.views()["map"][:9].contiguous(), ko, None)
+    torch.cuda.synchronize()
+    assert (ko - k[:9]).abs().max() <= k.abs().max() * 2.0 ** -4
+    assert torch.all(out[9:] == 7.0) and not torch.any(out[:9] == 7.0)
+    # fewer rows on the GPU than the bounds say
+    alone = i32([6]), i32([0]), i32([1])
+    kv.step(*alone, 1, 1)
+    torch.cuda.synchronize()
+    one = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(one):
+        kv.step(*alone, 1, 1)
+    kv.step(i32(range(8)), i32([0] * 8), i32([3] * 8), 24, 3)
+    one.replay()
+    out.fill_(7.0)
+    kv.append(0, k, v)
+    kv.attention(0, q, out)
+    torch.cuda.synchronize()
+    assert torch.all(out[1:] == 7.0) and not torch.any(out[:1] == 7.0)
+    kv.close()
