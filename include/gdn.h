@@ -924,8 +924,8 @@ typedef struct gdn_kv8_attn_desc {
  * out [max_tokens] rows of num_q_heads x head_dim bf16, token and head strides in
  * elements; q and gate 16-byte aligned with strides that are multiples of 8, out
  * 8-byte aligned with multiples of 4. slopes [num_q_heads] f32 and prefix [n] are
- * DEVICE arrays (or NULL). Tokens of refused rows get zeros; rows behind the last
- * token are left as they are.
+ * DEVICE arrays (or NULL). out's heads must not run into each other, nor overlap q or gate.
+ * Tokens of refused rows get zeros; rows behind the last token are left as they are.
  *
  * Products and sums are f32; dimensions of q below 2^-13 of its head's largest are rounded
  * by at most 2^-21 of that, the softmax's weights enter the product with the values in
@@ -983,7 +983,7 @@ gdn_status gdn_rope_destroy(gdn_rope* rope);
  * are normalised and copied; a token at a negative position is copied as it is.
  * inverse: turns back (the gradient of the turn). Pointers 16-byte aligned, token
  * and head strides multiples of 8 elements; an output may be its input with the
- * same strides, other overlaps are not allowed. Allocates nothing, may be captured. */
+ * same strides, its heads must not run into each other, other overlaps are not allowed. Allocates nothing, may be captured. */
 typedef struct gdn_rope_rows {
   const void* in;
   void* out;

@@ -8,7 +8,9 @@
 #include <cmath>
 #include <cstdarg>
 #include <cstdio>
+#include <memory>
 #include <new>
+#include <stdexcept>
 #include <vector>
 
 #include "gdn.h"
@@ -54,15 +56,16 @@ bool aligned(const void* p, uintptr_t n) { return reinterpret_cast<uintptr_t>(p)
 
 // Rows of `heads` heads of `dim` elements, tokens `stride` and heads `head_stride` apart,
 // the heads inside a token's row or the tokens inside a head's plane; every head starts
-// at a multiple of `unit` elements.
+// at a multiple of `unit` elements. With `tokens` (an output's) no plane runs into the next.
 bool rows_ok(const void* p, int64_t stride, int64_t head_stride, int heads, int dim, int unit,
-             int elem) {
+             int elem, int64_t tokens = 1) {
   if (!aligned(p, (uintptr_t)unit * elem > 16 ? 16 : (uintptr_t)unit * elem) ||
       stride % unit != 0 || stride < dim)
     return false;
   if (heads <= 1) return true;
   return head_stride % unit == 0 && head_stride >= dim &&
-         (head_stride >= stride || stride >= (heads - 1) * head_stride + dim);
+         ((head_stride >= stride && head_stride >= (tokens - 1) * stride + dim) ||
+          stride >= (heads - 1) * head_stride + dim);
 }
 
 }  // namespace
@@ -108,7 +111,7 @@ gdn_status check_layer(const gdn_kv8* kv, int32_t layer, const char* what) {
 
 extern "C" {
 
-gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) {
+gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) try {
   if (!desc || !out) return kfail(GDN_ERR_INVALID, "gdn_kv8_create: desc/out is NULL");
   *out = nullptr;
   const gdn_kv8_desc& d = *desc;
@@ -132,9 +135,11 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) {
     (void)hipGetLastError();
     return kfail(GDN_ERR_INVALID, "gdn_kv8_create: no device %d", d.device);
   }
-  gdn_kv8* kv = new (std::nothrow) gdn_kv8;
-  if (!kv) return kfail(GDN_ERR_OOM, "gdn_kv8_create: host memory");
+  std::unique_ptr<gdn_kv8, void (*)(gdn_kv8*)> held(new gdn_kv8, kv8_free);
+  gdn_kv8* const kv = held.get();
   kv->d = d;
+  kv->pages.reserve(d.num_layers);
+  kv->exps.reserve(d.num_layers);
   const size_t page_bytes = (size_t)2 * d.num_kv_heads * kPageTokens * d.head_dim;
   const size_t heads = (size_t)2 * d.num_kv_heads * d.num_pages;
   const size_t table = (size_t)d.num_slots * d.max_pages_per_slot;
@@ -201,12 +206,15 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) {
   }
   if (!ok) {
     (void)hipGetLastError();
-    kv8_free(kv);
     return kfail(GDN_ERR_OOM, "gdn_kv8_create: %d layers x %d pages of %zu bytes, workspace of %zu",
                  d.num_layers, d.num_pages, page_bytes, ws);
   }
-  *out = kv;
+  *out = held.release();
   return GDN_OK;
+} catch (const std::bad_alloc&) {
+  return kfail(GDN_ERR_OOM, "gdn_kv8_create: host memory");
+} catch (const std::length_error&) {
+  return kfail(GDN_ERR_OOM, "gdn_kv8_create: host memory");
 }
 
 gdn_status gdn_kv8_destroy(gdn_kv8* kv) {
@@ -355,7 +363,7 @@ gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc
   if (gate && !rows_ok(gate, gate_stride, gate_head_stride, H, D, 8, 2))
     return kfail(GDN_ERR_INVALID, "gdn_kv8_attention: gate needs 16-byte alignment and strides "
                  "that hold %d heads of %d in multiples of 8", H, D);
-  if (!rows_ok(out, out_stride, out_head_stride, H, D, 4, 2))
+  if (!rows_ok(out, out_stride, out_head_stride, H, D, 4, 2, kv->p.T))
     return kfail(GDN_ERR_INVALID, "gdn_kv8_attention: out needs 8-byte alignment and strides that "
                  "hold %d heads of %d in multiples of 4", H, D);
   if (!aligned(slopes, 4) || !aligned(prefix, 4))
@@ -386,7 +394,7 @@ gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc
   return e == hipSuccess ? GDN_OK : hip_fail(e, "gdn_kv8_attention launch");
 }
 
-gdn_status gdn_rope_create(const gdn_rope_desc* desc, int32_t device, gdn_rope** out) {
+gdn_status gdn_rope_create(const gdn_rope_desc* desc, int32_t device, gdn_rope** out) try {
   if (!desc || !out) return kfail(GDN_ERR_INVALID, "gdn_rope_create: desc/out is NULL");
   *out = nullptr;
   const gdn_rope_desc& d = *desc;
@@ -409,8 +417,8 @@ gdn_status gdn_rope_create(const gdn_rope_desc* desc, int32_t device, gdn_rope**
     (void)hipGetLastError();
     return kfail(GDN_ERR_INVALID, "gdn_rope_create: no device %d", device);
   }
-  gdn_rope* r = new (std::nothrow) gdn_rope;
-  if (!r) return kfail(GDN_ERR_OOM, "gdn_rope_create: host memory");
+  std::unique_ptr<gdn_rope> held(new gdn_rope);
+  gdn_rope* const r = held.get();
   r->d = d;
   r->device = device;
   const double pi = 3.14159265358979323846, rot = d.rotary_dim, base = d.base, f = d.factor;
@@ -443,11 +451,12 @@ gdn_status gdn_rope_create(const gdn_rope_desc* desc, int32_t device, gdn_rope**
       hipDeviceSynchronize() != hipSuccess) {
     (void)hipGetLastError();
     if (r->turns) (void)hipFree(r->turns);
-    delete r;
     return kfail(GDN_ERR_OOM, "gdn_rope_create: %zu bytes", sizeof(double) * turns.size());
   }
-  *out = r;
+  *out = held.release();
   return GDN_OK;
+} catch (const std::bad_alloc&) {
+  return kfail(GDN_ERR_OOM, "gdn_rope_create: host memory");
 }
 
 gdn_status gdn_rope_destroy(gdn_rope* rope) {
@@ -477,7 +486,7 @@ gdn_status gdn_rope_forward(const gdn_rope* rope, int32_t T, const int32_t* pos,
       return kfail(GDN_ERR_INVALID, "gdn_rope_forward: %s has %d heads", name, r->heads);
     if (r->heads == 0) continue;
     if (!r->in || !r->out || !rows_ok(r->in, r->in_stride, r->in_head_stride, r->heads, D, 8, elem) ||
-        !rows_ok(r->out, r->out_stride, r->out_head_stride, r->heads, D, 8, elem) ||
+        !rows_ok(r->out, r->out_stride, r->out_head_stride, r->heads, D, 8, elem, T) ||
         !aligned(r->norm_w, 16))
       return kfail(GDN_ERR_INVALID, "gdn_rope_forward: %s needs 16-byte alignment and strides that "
                    "hold %d heads of %d in multiples of 8", name, r->heads, D);

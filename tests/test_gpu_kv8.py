@@ -557,7 +557,9 @@ def test_refused_calls(gpu):
                 lambda: kv.attention(0, z(4, 8, 132, **bf16)[:, :, 4:], q),
                 lambda: kv.attention(0, z(4, 8, 130, **bf16)[:, :, :128], q),
                 lambda: kv.append(0, z(4, 260, **bf16)[:, 4:], k),
-                lambda: kv.attention(0, q, z(4, 8, 129, **bf16)[:, :, 1:])):
+                lambda: kv.attention(0, q, z(4, 8, 129, **bf16)[:, :, 1:]),
+                # heads' planes that run into each other
+                lambda: kv.attention(0, q, z(4 * 8 * 128, **bf16).as_strided((4, 8, 128), (128, 256, 1)))):
         with pytest.raises(E):
             bad()
     for bad in (lambda: kv.append(0, k[:3], k), lambda: kv.append(0, k.float(), k),

@@ -112,7 +112,7 @@ def test_in_place_views_and_the_way_back(gpu):
 
 
 @pytest.mark.parametrize("dim,rot,interleaved", [(64, 32, False), (64, 32, True), (96, 46, False)])
-@pytest.mark.parametrize("T", [3, 600])
+@pytest.mark.parametrize("T", [3, 600, 2100])
 def test_what_does_not_turn_keeps_its_bits(gpu, dim, rot, interleaved, T):
     """Infinities and NaN among the dimensions behind rotary_dim and in tokens at negative
     positions stay where they are; a turned pair takes only its own."""
@@ -151,7 +151,9 @@ def test_refused_calls(gpu):
                 lambda: r.forward(pos, q, q_norm_w=w, inverse=True),
                 lambda: r.forward(pos, torch.zeros(4, 2, 68, device="cuda:0",
                                                    dtype=torch.bfloat16)[:, :, :64]),
-                lambda: r.forward(pos, q[:, :0])):
+                lambda: r.forward(pos, q[:, :0]),
+                lambda: r.forward(pos, q, q_out=torch.zeros(
+                    512, device="cuda:0", dtype=torch.bfloat16).as_strided((4, 2, 64), (64, 128, 1)))):
         with pytest.raises(E):
             bad()
     for bad in (lambda: r.forward(pos[:3], q), lambda: r.forward(pos, q, q.float()),
@@ -161,4 +163,33 @@ def test_refused_calls(gpu):
         with pytest.raises(ValueError):
             bad()
     r.forward(pos[:0], q[:0])
+    r.close()
+
+
+@pytest.mark.parametrize("hq,hk,dim,rot", [(16, 2, 256, 64), (3, 0, 96, 46), (9, 2, 512, 512),
+                                           (33, 8, 80, 80), (1, 1, 8, 8)])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("f32", [False, True])
+def test_long_steps_are_their_tokens(gpu, hq, hk, dim, rot, interleaved, f32):
+    """2,051 tokens in one call, in place and not, against calls of 64 tokens and less."""
+    import torch
+    import gdn_amd
+    T, dt = 2051, torch.float32 if f32 else torch.bfloat16
+    g = torch.Generator(device="cuda:0").manual_seed(dim + rot)
+    q, k = (torch.randn(T, h, dim, device="cuda:0", generator=g).to(dt) for h in (hq, hk))
+    w = torch.randn(dim, device="cuda:0", generator=g).bfloat16()
+    pos = torch.randint(-1, 100000, (T,), device="cuda:0", generator=g, dtype=torch.int32)
+    r = gdn_amd.Rope(dim, rot, 1.0e4, interleaved)
+
+    def turn(a, b, qo, ko):
+        r.forward(pos[a:b], q[a:b], k[a:b] if hk else None, q_out=qo[a:b],
+                  k_out=ko[a:b] if hk else None, q_norm_w=w, k_norm_w=w if hk else None, eps=1e-5)
+
+    whole, parts = ([torch.full_like(x, 3.0) for x in (q, k)] for _ in range(2))
+    turn(0, T, *whole)
+    for a in range(0, T, 64):
+        turn(a, min(a + 64, T), *parts)
+    turn(0, T, q, k)
+    for a, b, c in zip(whole, parts, (q, k)):
+        assert torch.equal(a, b) and torch.equal(a, c)
     r.close()
