@@ -935,8 +935,6 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
   const int window = a.window > 0 ? a.window : INT32_MAX / 2;
   const float sm = __int_as_float(__builtin_amdgcn_readfirstlane(
       __float_as_int(a.softcap > 0.f ? a.scale / a.softcap : a.scale * 1.4426950408889634f)));
-  const bool odd = a.softcap > 0.f || a.slopes != nullptr || !(a.scale > 0.f);
-
   const int32_t* const trow = p.table + (size_t)row.slot * p.max_pages;
   int vbase = 0, pid = 0, eks = 0, evs = 0;
   auto ids = [&](int v) __attribute__((always_inline)) {
@@ -1000,7 +998,14 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
   const int kat = (c >> 4) * NK * 64 + 32 * hf + (c & 15);
   const int vat = (c >> 4) * 32 + 16 * hf + (c & 15);
 
-  float m = -INFINITY, l = 0.f, mk;
+  // A distance term can start the accumulators, divided by mk, but for a part that is the lane's:
+  // half the work of adding it to the scores (19 ragged rows of 64 dims 102 us, and 97). Not where a cap
+  // comes before it, nor beyond the sizes for which the quotient is an f32 number, with mk's power
+  // of two 2^-60 at least; and not with more dims, whose registers it has no room in.
+  const bool tilt = D == 64 && a.slopes && a.softcap == 0.f && sm >= 0x1p-40f && sm <= 0x1p40f &&
+                    __all(fabsf(column().slope) <= 0x1p20f);
+  const bool odd = a.softcap > 0.f || (a.slopes && !tilt) || !(a.scale > 0.f);
+  float m = -INFINITY, l = 0.f, mk, far = 0.f;
   uint32_t seen;
   int unit = 0;
   f32x16 O[NT], S;
@@ -1014,14 +1019,14 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
                    (int)y[0], (int)y[1], (int)y[2], (int)y[3]};
   };
   // S: scores of half hb of the page in lk, fragments read two ahead
-  auto scores = [&](const u32x4* lk, int hb) __attribute__((always_inline)) {
+  auto scores = [&](const u32x4* lk, int hb, auto start) __attribute__((always_inline)) {
     constexpr int kOne = 0x7f7f7f7f, kLow = 0x7b7b7b7b;  // 2^0 and 2^-4
     auto key = [&](int i) __attribute__((always_inline)) {
       const int at = kat + (2 * hb * NK + i) * 64;
       return both(lk[at], lk[at + 16]);
     };
 #pragma unroll
-    for (int i = 0; i < 16; ++i) S[i] = 0.f;
+    for (int i = 0; i < 16; ++i) S[i] = start(i);
     i32x8 kk[2] = {key(0), NK > 1 ? key(1) : key(0)};
     __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
@@ -1034,9 +1039,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
       __builtin_amdgcn_sched_barrier(0);
     }
   };
-  // S and mk: scores of the block at kb, keys that a column does not see as -inf, are mk * S
-  auto prepare = [&](int kb, int ek) __attribute__((always_inline)) {
-    mk = factor_of(sm, column().eq + ek);
+  // S, mk, far: scores of the block at kb, keys that a column does not see as -inf, are mk * S + far
+  auto prepare = [&](int kb) __attribute__((always_inline)) {
     seen = 0xffffu;
     const int kl = kb + 4 * hf;  // score i is of key kl + 8 (i / 4) + i % 4
     if (__builtin_expect(odd, 0)) {
@@ -1052,10 +1056,10 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
       }
       // slopes of zero where there are none: a scale that is not positive comes here too
       const Column col = column();
-      const float slope = col.slope, far = slope * (float)(kl - col.pos);
+      const float slope = col.slope, off = slope * (float)(kl - col.pos);
 #pragma unroll
       for (int i = 0; i < 16; ++i) {
-        S[i] = fmaf(S[i], mk, fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), far));
+        S[i] = fmaf(S[i], mk, fmaf(slope, (float)(8 * (i >> 2) + (i & 3)), off));
         if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few registers at once
       }
       mk = 1.f;
@@ -1076,7 +1080,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
     float bm = fmaxf(S[0], S[1]);
 #pragma unroll
     for (int i = 2; i < 16; ++i) bm = fmaxf(bm, S[i]);
-    bm = max_xor32(bm) * mk;
+    bm = max_xor32(fmaf(bm, mk, far));
     if (__builtin_expect(!unit_holds(ev, unit) || __any(bm > m + kStep), 0)) {
       const int to = unit_holds(ev, unit) ? unit : ev + 2;  // room either way
       const float mn = fmaxf(m, bm);
@@ -1095,17 +1099,26 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
   u32x4 P[2];
   auto weights = [&](int ev) __attribute__((always_inline)) {
     const int up = kUnit + ev - unit;
-    const float mref = (m == -INFINITY ? 0.f : m) - (float)up;
-    float e[16], sum = 0.f;
+    const float mref = (m == -INFINITY ? 0.f : m) - (float)up - far;
+    float e[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) e[i] = __builtin_amdgcn_exp2f(fmaf(S[i], mk, -mref));
-#pragma unroll
-    for (int i = 0; i < 16; i += 4) sum += (e[i] + e[i + 1]) + (e[i + 2] + e[i + 3]);
-    l = fmaf(sum, pow2(-up), l);
     // keys 4 hf + r and 16 + 4 hf + r, then those 8 further on: the order of the values' bytes
     P[0] = (u32x4){pk_f16(e[0], e[1]), pk_f16(e[2], e[3]), pk_f16(e[8], e[9]), pk_f16(e[10], e[11])};
     P[1] = (u32x4){pk_f16(e[4], e[5]), pk_f16(e[6], e[7]), pk_f16(e[12], e[13]), pk_f16(e[14], e[15])};
     asm volatile("" : "+v"(P[0]), "+v"(P[1]));  // here, not behind the branches that follow
+    // the sum is of the rounded weights, two an instruction (which keeps f16's small numbers)
+    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+    const f16x2 ones = {(_Float16)1.f, (_Float16)1.f};
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < 4; ++i)
+#pragma unroll
+      for (int k = 0; k < 2; ++k) {
+        const uint32_t two = P[k][i];
+        sum[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two), ones, sum[k], false);
+      }
+    l = fmaf(sum[0] + sum[1], pow2(-up), l);
   };
   // O += P V of half hb of the page in lv: fragments are read two ahead (the first two apart) and
   // converted beside the products
@@ -1180,9 +1193,18 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
       for (int hb = 0; hb < 2; ++hb) {
         const int kb = key0 + hb * kBlock;
         __builtin_amdgcn_s_setprio(1);
-        scores(lk, hb);
+        if (__builtin_expect(tilt, 0)) {
+          const Column col = column();
+          mk = __builtin_amdgcn_ldexpf(sm, max(col.eq + ek, -60));
+          far = col.slope * (float)(kb + 4 * hf - col.pos);
+          const float part = col.slope * __builtin_amdgcn_rcpf(mk);
+          scores(lk, hb, [&](int i) { return part * (float)(8 * (i >> 2) + (i & 3)); });
+        } else {
+          scores(lk, hb, [](int) { return 0.f; });
+          mk = factor_of(sm, column().eq + ek);
+        }
         __builtin_amdgcn_s_setprio(0);
-        prepare(kb, ek);
+        prepare(kb);
         follow(ev);
         values_ahead(lv, hb);
         weights(ev);

@@ -817,3 +817,19 @@ def test_eager_calls_behind_another_steps_replay(gpu):
     torch.cuda.synchronize()
     assert torch.all(out[1:] == 7.0) and not torch.any(out[:1] == 7.0)
     kv.close()
+
+
+@pytest.mark.parametrize("slope,scale", [(1.0, 0.125), (3e6, 0.125), (0.5, 1e-13), (0.25, -0.1),
+                                         (1e-9, 4.0)])
+def test_distance_terms_of_every_size(gpu, slope, scale):
+    """Slopes and scales either side of where the term starts the accumulators; a page of zeros
+    and queries of zeros, whose scores have no size of their own."""
+    rng = np.random.default_rng(26)
+    p = Pair(3, 12, 6, hq=4, hk=2, dim=64)
+    p.step([1], [0], [64])
+    p.append(rng, change=lambda x: x.zero_())
+    p.step([1, 0], [64, 0], [70, 33])
+    p.append(rng)
+    p.attention(rng, label="slopes", scale=scale, slopes=[slope, -slope, 0.0, slope / 3])
+    p.attention(rng, label="zero queries", std=0.0, scale=scale, slopes=[slope, 0.1, 0.0, slope / 3])
+    p.kv.close()
