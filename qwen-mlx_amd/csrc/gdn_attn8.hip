@@ -880,14 +880,15 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
 // As many waves a SIMD as the outputs and q's parts (128 + 64 registers at D = 256) leave room for,
 // 2, 3 and 4 at 256, 128 and 64 dims; one's products run beside the others' softmax, so that a
 // wave's own steps stay in order. 8,192 tokens of 16 query heads over 2 of 256 dims: one wave a
-// SIMD with the steps of two blocks side by side 665 us, two 500; products and softmax of half
-// the waves in turn, by barriers, 508. At that rate (1.1 PFLOP/s, a quarter of the matrix time
-// on top for the scores' second part) the clock, not a unit, is what gives: the f16
-// products alone run at 1.6 GHz on such numbers, and at 2.2 on constants. 19 rows of 1 .. 571 tokens
-// of 32 query heads over 8 of 128 dims: 255 us in two waves a SIMD, 231 in three.
+// SIMD with the steps of two blocks side by side 665 us, two 483; products and softmax of half
+// the waves in turn, by barriers, were as fast (508, where the rest took 500). At that rate (1.1
+// PFLOP/s, a quarter of the matrix time on top for the scores' second part) the clock, not a unit,
+// is what gives: the f16 products alone run at 1.6 GHz on such numbers, and at 2.2 on constants.
+// 19 rows of 1 .. 571 tokens of 32 query heads over 8 of 128 dims: 255 us in two waves a SIMD, 231
+// in three.
 template <int D, int NW>
-__global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn8_tile_kernel(Kv8AttnArgs a, float* __restrict__ part,
-                                                                Kv8Splits most_splits) {
+__global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn8_tile_kernel(
+    Kv8AttnArgs a, float* __restrict__ part, Kv8Splits most_splits) {
   constexpr int NK = D / 64, NT = D / 32, kTile16 = kPage * D / 16;  // 16-byte pieces of a tile
   constexpr int kLoads = kTile16 / 64 / NW;                          // of a wave for a tile
   static_assert(kTile16 % (64 * NW) == 0, "whole pieces for each wave");
@@ -999,9 +1000,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
   const int vat = (c >> 4) * 32 + 16 * hf + (c & 15);
 
   // A distance term can start the accumulators, divided by mk, but for a part that is the lane's:
-  // half the work of adding it to the scores (19 ragged rows of 64 dims 102 us, and 97). Not where a cap
-  // comes before it, nor beyond the sizes for which the quotient is an f32 number, with mk's power
-  // of two 2^-60 at least; and not with more dims, whose registers it has no room in.
+  // half the work of adding it to the scores (19 ragged rows of 64 dims 102 us, and 97). Not where
+  // a cap comes before it, nor beyond the sizes for which the quotient is an f32 number, with mk's
+  // power of two 2^-60 at least; and not with more dims, whose registers it has no room in.
   const bool tilt = D == 64 && a.slopes && a.softcap == 0.f && sm >= 0x1p-40f && sm <= 0x1p40f &&
                     __all(fabsf(column().slope) <= 0x1p20f);
   const bool odd = a.softcap > 0.f || (a.slopes && !tilt) || !(a.scale > 0.f);
@@ -1307,7 +1308,8 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
                        a.stream, a, tpart, splits);
     if (splits.many > 1 || splits.few > 1) {
       if ((e = hipGetLastError()) != hipSuccess) return e;
-      hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, dim3((splits.many > 1 ? many : 0) + (splits.few > 1 ? few : 0), p.Hkv, kKv8TileWaves),
+      const int cut = (splits.many > 1 ? many : 0) + (splits.few > 1 ? few : 0);
+      hipLaunchKernelGGL(attn8_join_tiles_kernel<D>, dim3(cut, p.Hkv, kKv8TileWaves),
                          dim3(256), 0,
                          a.stream, a, tpart, splits);
     }
