@@ -170,22 +170,6 @@ __device__ __forceinline__ void zero_refused(const Kv8AttnArgs& a, int64_t t0, i
   }
 }
 
-// Visible keys of a group of tokens, as pages: [0, pre) then [lo, end).
-struct Span {
-  int pre, lo, end;
-  __device__ __forceinline__ int count() const { return pre + end - lo; }
-  __device__ __forceinline__ int page(int v) const { return v < pre ? v : v - pre + lo; }
-};
-// p0, p1: first and last position; total: the row's length with the step; pf: its prefix
-__device__ __forceinline__ Span span_of(int p0, int p1, int window, int pf, int total) {
-  Span s;
-  const int keys = min(max(p1 + 1, pf), total);
-  s.end = (keys + kPage - 1) / kPage;
-  s.lo = window > 0 ? max(p0 - window + 1, 0) / kPage : 0;
-  s.pre = min((pf + kPage - 1) / kPage, s.lo);
-  return s;
-}
-
 // 1 / (1 + e^-x), off by some 2^-22 of itself
 __device__ __forceinline__ float sigmoid(float x) {
   return __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(-1.4426950408889634f * x));
@@ -222,7 +206,7 @@ struct Group {
   int h, cpos, lo, pf, total, pos0, nt;
   int64_t t;
   bool valid;
-  Span span;
+  Kv8Span span;
 };
 __device__ __forceinline__ Group group_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int g, int j,
                                           int G, int tpg, int c) {
@@ -237,7 +221,7 @@ __device__ __forceinline__ Group group_of(const Kv8AttnArgs& a, const Kv8Row& ro
   x.cpos = x.valid ? x.pos0 + ctok : -1;
   x.pf = a.prefix ? min(max(a.prefix[r], 0), x.total) : 0;
   x.lo = a.window > 0 ? max(x.cpos - a.window, -1) : -1;  // keys above it
-  x.span = span_of(x.pos0, x.pos0 + x.nt - 1, a.window, x.pf, x.total);
+  x.span = kv8_span(x.pos0, x.pos0 + x.nt - 1, a.window, x.pf, x.total);
   return x;
 }
 
@@ -447,59 +431,28 @@ __device__ __forceinline__ Score score_of(const Kv8AttnArgs& a, const Group& x) 
   return sc;
 }
 
-// Items of a row of few tokens: (group, kv head, chunk) in this order.
-struct Chunks {
-  int groups, cp, nch;
-};
-__device__ __forceinline__ Chunks chunks_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpg) {
-  Chunks c{0, 1, 0};
-  if (row.fresh <= 0) return c;
-  c.groups = (row.fresh + tpg - 1) / tpg;
+// Items of a row of few tokens: (group, kv head, chunk) in this order. Whole pages for each of a
+// chunk's waves.
+__device__ __forceinline__ Kv8Cut chunks_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpg) {
+  if (row.fresh <= 0) return Kv8Cut{0, 1, 0};
   const int total = row.pos + row.fresh;
   const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
-  // the first and the last group's pages; one between them may see a page more where the
-  // window's two ends fall into pages
-  int most = 0;
-  for (int g = 0; g < c.groups; g += max(c.groups - 1, 1)) {
-    const int p0 = row.pos + g * tpg;
-    most = max(most, span_of(p0, min(p0 + tpg, total) - 1, a.window, pf, total).count());
-  }
-  most = min(most + (c.groups > 1 && a.window > 0 ? 1 : 0), (total + kPage - 1) / kPage);
-  // whole pages for each of a chunk's waves
-  const int waves = kv8_chunk_waves(a.p.n, a.p.Hkv);
-  const int cp = (most - 1) / kv8_chunks(a.p.n, a.p.Hkv, c.groups) + 1;
-  c.cp = (cp + waves - 1) / waves * waves;
-  c.nch = (most + c.cp - 1) / c.cp;
-  return c;
+  return kv8_cut(row.pos, row.fresh, a.window, pf, tpg,
+                 kv8_chunks(a.p.n, a.p.Hkv, (row.fresh + tpg - 1) / tpg),
+                 kv8_chunk_waves(a.p.n, a.p.Hkv), 1);
 }
 
 // Items of a row in a step of tiles: (tile from the last one on, split). By row alone where pages
 // are cut, and by the step's bounds, which rows of fewer than kKv8TileTokens tokens have their own
 // of: they are few tiles with as many pages as any.
-struct Splits {
-  int tiles, cp, n;
-};
-__device__ __forceinline__ Splits splits_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpt,
+__device__ __forceinline__ Kv8Cut splits_of(const Kv8AttnArgs& a, const Kv8Row& row, int r, int tpt,
                                             const Kv8Splits& most_splits) {
-  Splits s{0, 1, 0};
-  if (row.fresh <= 0) return s;
-  s.tiles = (row.fresh + tpt - 1) / tpt;
-  s.n = 1;
-  s.cp = INT32_MAX / 2;
+  if (row.fresh <= 0) return Kv8Cut{0, 1, 0};
   const int pieces = row.fresh < kKv8TileTokens ? most_splits.few : most_splits.many;
-  if (pieces > 1) {
-    const int total = row.pos + row.fresh;
-    const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
-    int most = 0;  // of the first and the last tile's pages, as in chunks_of
-    for (int g = 0; g < s.tiles; g += max(s.tiles - 1, 1)) {
-      const int p0 = row.pos + g * tpt;
-      most = max(most, span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total).count());
-    }
-    most = min(most + (s.tiles > 1 && a.window > 0 ? 1 : 0), (total + kPage - 1) / kPage);
-    s.cp = max((most - 1) / pieces + 1, kSplitPages);
-    s.n = (most + s.cp - 1) / s.cp;
-  }
-  return s;
+  if (pieces <= 1) return Kv8Cut{(row.fresh + tpt - 1) / tpt, 1, 1};
+  const int total = row.pos + row.fresh;
+  const int pf = a.prefix ? min(max(a.prefix[r], 0), total) : 0;
+  return kv8_cut(row.pos, row.fresh, a.window, pf, tpt, pieces, 1, kSplitPages);
 }
 // Partial results of a tile's splits: 128 columns of D + 4 floats each
 template <int D>
@@ -532,18 +485,18 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, tpg = 16 / G;
   auto items = [&](int r, const Kv8Row& row) {
-    const Chunks k = chunks_of(a, row, r, tpg);
-    return k.groups * k.nch * p.Hkv;
+    const Kv8Cut k = chunks_of(a, row, r, tpg);
+    return k.items * k.n * p.Hkv;
   };
   for (int g = blockIdx.x;; g += gridDim.x) {
     const Found f = find_row(p, g, items);
     if (f.r < 0) break;
-    const Chunks ch = chunks_of(a, f.row, f.r, tpg);
-    const int local = g - f.first, seg = local / ch.nch, chunk = local - seg * ch.nch;
+    const Kv8Cut ch = chunks_of(a, f.row, f.r, tpg);
+    const int local = g - f.first, seg = local / ch.n, chunk = local - seg * ch.n;
     const int grp = seg / p.Hkv, j = seg - grp * p.Hkv;
     const Group x = group_of(a, f.row, f.r, grp, j, G, tpg, c);
     const Score sc = score_of(a, x);
-    const int v1 = min((chunk + 1) * ch.cp, x.span.count());
+    const int v1 = kv8_piece_end(ch, chunk, x.span.count());
     if (W > 1 && g != (int)blockIdx.x) __syncthreads();  // the chunk before is written out
     int eq;  // every wave forms q: its exponent is in registers
     {
@@ -630,12 +583,12 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
       for (; v + W < v1; v += W) page(std::false_type{});
       page(std::true_type{});
     }
-    float* const out = part + (((size_t)p.parts[f.r] * p.Hkv + (size_t)seg * ch.nch + chunk) * 16) *
+    float* const out = part + (((size_t)p.parts[f.r] * p.Hkv + (size_t)seg * ch.n + chunk) * 16) *
                                   (D + 4);
     const float lw = on.sum();
     if constexpr (W == 1) {
       if (!x.valid) continue;
-      if (ch.nch == 1) {
+      if (ch.n == 1) {
         const float inv = __builtin_amdgcn_ldexpf(1.0f / lw, on.unit - kUnit);
 #pragma unroll
         for (int d = 0; d < DB; ++d) {
@@ -682,7 +635,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
         m = fmaxf(m, ms[k][col]);
         o += os[k][col][d];
       }
-      if (ch.nch == 1) {
+      if (ch.n == 1) {
         o *= 1.0f / l;
         const int tok = col / G;
         float of[4] = {o[0], o[1], o[2], o[3]};
@@ -721,7 +674,7 @@ __global__ __launch_bounds__(256) void attn8_join_kernel(Kv8AttnArgs a, const fl
   const int parts = p.parts[r];
   if (k >= kv8_tokens(p, row)) return;
   const int G = p.Hq / p.Hkv, tpg = 16 / G, j = h / G, grp = k / tpg, c = (k - grp * tpg) * G + h - j * G;
-  const int nch = chunks_of(a, row, r, tpg).nch;
+  const int nch = chunks_of(a, row, r, tpg).n;
   if (nch < 2) return;
   const int64_t t = (int64_t)row.cu + k;
   const float* const pc =
@@ -901,8 +854,8 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int G = p.Hq / p.Hkv, tpw = 32 / G, tpt = NW * tpw, j = blockIdx.y;
   const Found f = find_row(p, blockIdx.x, [&](int r, const Kv8Row& row) {
-    const Splits s = splits_of(a, row, r, tpt, most_splits);
-    return s.tiles * s.n;
+    const Kv8Cut s = splits_of(a, row, r, tpt, most_splits);
+    return s.items * s.n;
   });
   if (f.r < 0) {  // a work-group to spare (the last one is): tokens of refused rows, zeros
     const int first = ((int)(blockIdx.x - f.first) * gridDim.y + j) * NW + w;
@@ -912,19 +865,19 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
     return;
   }
   const Kv8Row row = f.row;
-  const Splits sp = splits_of(a, row, f.r, tpt, most_splits);
+  const Kv8Cut sp = splits_of(a, row, f.r, tpt, most_splits);
   const int local = blockIdx.x - f.first, split = local % sp.n;
-  const int tile = sp.tiles - 1 - local / sp.n;  // longest first
+  const int tile = sp.items - 1 - local / sp.n;  // longest first
   const int total = row.pos + row.fresh;
   const int pf = a.prefix ? min(max(a.prefix[f.r], 0), total) : 0;
   const int p0 = row.pos + tile * tpt;  // the tile's first position
-  const Span span = span_of(p0, min(p0 + tpt, total) - 1, a.window, pf, total);
+  const Kv8Span span = kv8_span(p0, min(p0 + tpt, total) - 1, a.window, pf, total);
   const int v0 = split * sp.cp;
-  const int count = min(span.count(), sp.n > 1 ? v0 + sp.cp : INT32_MAX);  // pages [v0, count)
+  const int count = kv8_piece_end(sp, split, span.count());  // pages [v0, count)
   // the tile's partial results, if its pages are split: columns (wave, c)
   float* const out = split_part<D>(p, part, most_splits, f.r, row.fresh, tile, j) +
                      (size_t)split * (32 * NW * (D + 4));
-  if (v0 >= count) {  // nothing in this split (the tile is shorter than the row's last one)
+  if (v0 >= count) {  // nothing in this split (the tile sees fewer pages than others)
     for (int i = tid; i < 32 * NW; i += 64 * NW) {
       out[(size_t)i * (D + 4)] = -INFINITY;
       out[(size_t)i * (D + 4) + 1] = 0.f;

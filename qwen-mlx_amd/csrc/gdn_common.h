@@ -528,6 +528,51 @@ __host__ __device__ inline int kv8_few_tiles(int G) {  // of a row of few tokens
   const int tpt = kKv8TileWaves * (32 / G);
   return (kKv8TileTokens - 2) / tpt + 1;
 }
+// Visible keys of some consecutive tokens of a row, as pages: [0, pre) then [lo, end).
+struct Kv8Span {
+  int pre, lo, end;
+  __host__ __device__ int count() const { return pre + end - lo; }
+  __host__ __device__ int page(int v) const { return v < pre ? v : v - pre + lo; }
+};
+// p0, p1: first and last position; total: the row's length with the step; pf: its prefix
+__host__ __device__ inline Kv8Span kv8_span(int p0, int p1, int window, int pf, int total) {
+  Kv8Span s;
+  const int most = p1 + 1 > pf ? p1 + 1 : pf, keys = most < total ? most : total;
+  s.end = (keys + 63) / 64;
+  s.lo = window > 0 && p0 - window + 1 > 0 ? (p0 - window + 1) / 64 : 0;
+  const int pre = (pf + 63) / 64;
+  s.pre = pre < s.lo ? pre : s.lo;
+  return s;
+}
+// How a row's items of `per` tokens (groups, tiles) have their pages cut: into n pieces of cp pages,
+// cp a multiple of `unit` and at least `least`. By the first and the last item's pages: one between
+// them may see a page or two more where the window's ends fall into pages (a full one, where the
+// last has few tokens), which its last piece takes, as that runs to the item's end.
+struct Kv8Cut {
+  int items, cp, n;
+};
+__host__ __device__ inline Kv8Cut kv8_cut(int pos, int fresh, int window, int pf, int per, int pieces,
+                                          int unit, int least) {
+  Kv8Cut c{(fresh + per - 1) / per, 1, 1};
+  const int total = pos + fresh;
+  int most = 0;
+  for (int g = 0; g < c.items; g += c.items > 2 ? c.items - 1 : 1) {
+    const int p0 = pos + g * per, p1 = p0 + per < total ? p0 + per : total;
+    const int k = kv8_span(p0, p1 - 1, window, pf, total).count();
+    most = k > most ? k : most;
+  }
+  const int some = most + (c.items > 1 && window > 0 ? 1 : 0), all = (total + 63) / 64;
+  most = some < all ? some : all;
+  const int cp = ((most - 1) / pieces + unit) / unit * unit;
+  c.cp = cp > least ? cp : least;
+  c.n = (most + c.cp - 1) / c.cp;
+  return c;
+}
+// End of piece i of an item that sees `count` pages
+__host__ __device__ inline int kv8_piece_end(const Kv8Cut& c, int i, int count) {
+  const int end = (i + 1) * c.cp;
+  return i == c.n - 1 || end > count ? count : end;
+}
 struct Kv8Splits {
   int many, few;  // at most, of a tile of a row of many tokens and of one of few
 };

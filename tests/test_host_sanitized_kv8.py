@@ -1,0 +1,21 @@
+"""How attention over the 8-bit cache cuts a row's pages, over head layouts, lengths, windows and
+prefixes, on the CPU (``tests/host/kv8_test.cpp``) under AddressSanitizer and UBSan.
+"""
+import os
+import shutil
+import subprocess
+
+import pytest
+
+HOST = os.path.join(os.path.dirname(os.path.abspath(__file__)), "host")
+
+
+@pytest.mark.skipif(shutil.which("make") is None or not os.path.exists("/opt/rocm/bin/hipcc"),
+                    reason="needs make and hipcc")
+def test_pieces_of_a_row_hold_every_page_once():
+    r = subprocess.run(["make", "-C", HOST, "-j8", "run_kv8"], capture_output=True, text=True,
+                       timeout=600)
+    out = r.stdout + r.stderr
+    assert r.returncode == 0, out[-6000:]
+    assert "ALL OK" in out, out[-3000:]
+    assert "runtime error" not in out and "AddressSanitizer" not in out, out[-6000:]
