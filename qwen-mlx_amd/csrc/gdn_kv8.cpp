@@ -192,9 +192,11 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) try {
     p.tok_row = take(d.max_step_tokens);
     std::vector<int32_t> init(d.num_pages);
     for (int i = 0; i < d.num_pages; ++i) init[i] = d.num_pages - 1 - i;  // pop lowest first
-    const std::vector<int32_t> mark(d.num_slots, INT_MAX);
+    const std::vector<int32_t> mark(d.num_slots, INT_MAX), behind(R + 1, INT_MAX);
     ok = hipMemset(kv->ints, 0, sizeof(int32_t) * words) == hipSuccess &&
          hipMemset(p.table, 0xff, sizeof(int32_t) * table) == hipSuccess &&
+         hipMemcpy(p.blocks, behind.data(), sizeof(int32_t) * (R + 1), hipMemcpyHostToDevice) ==
+             hipSuccess &&
          hipMemcpy(p.free_pages, init.data(), sizeof(int32_t) * d.num_pages,
                    hipMemcpyHostToDevice) == hipSuccess &&
          hipMemcpy(p.mark, mark.data(), sizeof(int32_t) * d.num_slots, hipMemcpyHostToDevice) ==

@@ -60,7 +60,8 @@ __device__ __forceinline__ int exponent_of(uint32_t bits) {
 }
 
 // Row of item g in the prefix sums pre[0 .. n] (pre[n] > g): the last row whose items start
-// at or before g. By the wave, 64 rows at a time.
+// at or before g. By the wave, 64 rows at a time. Where the plan has fewer rows than n, an item
+// behind theirs falls to the first row behind them, which holds nothing.
 __device__ __forceinline__ int row_of(const int32_t* __restrict__ pre, int n, int g) {
   const int lane = threadIdx.x & 63;
   int r = 0;
@@ -285,7 +286,10 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     b0 += touched[i];
     c1 += chunks[i];
   }
-  for (int r = p.n + tid; r < used; r += TH) p.rows[r] = Kv8Row{-1, 0, 0, 0};
+  for (int r = p.n + tid; r < used; r += TH) {
+    p.rows[r] = Kv8Row{-1, 0, 0, 0};
+    p.blocks[r + 1] = INT32_MAX;  // behind every item
+  }
   if (tid == 0) {
     p.blocks[p.n] = total;
     *p.free_count = avail - taken;

@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from gdn_testlib import say
-from test_gpu_kv8 import Pair
+from test_gpu_kv8 import Pair, bf, i32
 
 pytestmark = pytest.mark.gpu
 
@@ -24,3 +24,66 @@ def test_windows_on_prompts_in_pieces(gpu, hq, dim, cached, new, window):
     p.append(rng)
     p.attention(rng, label=f"window {window}", window=window)
     p.kv.close()
+
+
+def captured_step(kv, slots, lens, ntok, tokens, most):
+    """A graph of a step on a cache, planned once before."""
+    import torch
+    args = i32(slots), i32(lens), i32(ntok)
+    kv.step(*args, tokens, most)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        kv.step(*args, tokens, most)
+    return graph, args
+
+
+def held(kv, places):
+    import torch
+    out = torch.full((2, len(places), kv.Hkv, kv.D), 9.0, dtype=torch.bfloat16, device="cuda:0")
+    kv.gather(0, places, out[0], out[1])
+    return out
+
+
+@pytest.mark.parametrize("rows,ntok", [
+    (12, [200, 3, 130, 64, 77]),  # more rows in the call than in the plan
+    (70, [1, 65, 0, 400, 2, 190] * 11),
+    (2, [70, 130, 200, 64, 9]),   # fewer
+    (5, [70, 130, 200, 64, 9]),
+    (65, [100] * 70)])
+def test_append_behind_another_steps_replay(gpu, rows, ntok):
+    """Rows of many pages planned by a graph, appended under bounds of `rows` rows, of which
+    an earlier step of single tokens was: the first `rows` hold what a cache that planned
+    them itself does, and the others' pages are as they were."""
+    import gdn_amd
+    import torch
+    rng = np.random.default_rng(rows)
+    hk, d, n, T = 2, 64, len(ntok), sum(ntok)
+    lens = rng.integers(0, 150, n).tolist()
+    slots = rng.permutation(200)[:n].tolist()
+    others = [s for s in range(200) if s not in slots][:rows]
+    fill = [bf(rng, sum(lens), hk, d)[0] for _ in range(2)]
+    kv, twin = (gdn_amd.KV8Cache(1, 200, 1200, 10, 4, hk, d, 8000) for _ in range(2))
+    for c in (kv, twin):
+        c.step(i32(slots), i32([0] * n), i32(lens), sum(lens))
+        c.append(0, *fill)
+    say("kv8 append behind a replay", rows, n)
+    graph, args = captured_step(kv, slots, lens, ntok, T, max(ntok))
+    twin.step(*args, T, max(ntok))
+    single = i32(others), i32([0] * rows), i32([1] * rows)
+    for c in (kv, twin):
+        c.step(*single, T, max(ntok))
+    graph.replay()
+    twin.step(*args, T, max(ntok))
+    places = twin.views()["map"][:T].clone()
+    assert torch.equal(places, kv.views()["map"][:T])
+    before = held(kv, places)
+    k, v = (bf(rng, T, hk, d)[0] for _ in range(2))
+    kv.append(0, k, v)
+    twin.append(0, k, v)
+    inside = sum(ntok[:rows])
+    assert torch.equal(held(kv, places)[:, :inside], held(twin, places)[:, :inside])
+    assert torch.equal(held(kv, places)[:, inside:], before[:, inside:])
+    for c in (kv, twin):
+        assert c.check() == 0
+        c.close()
