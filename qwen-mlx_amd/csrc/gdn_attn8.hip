@@ -483,7 +483,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
   const Kv8Plan& p = a.p;
   const int tid = threadIdx.x, lane = tid & 63, g4 = lane >> 4, c = lane & 15;
   const int w = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int G = p.Hq / p.Hkv, tpg = 16 / G;
+  const int G = p.Hq / p.Hkv, tpg = 16 / G, row_parts = kv8_row_parts(p.n, p.Hkv) * p.Hkv;
   auto items = [&](int r, const Kv8Row& row) {
     const Kv8Cut k = chunks_of(a, row, r, tpg);
     return k.items * k.n * p.Hkv;
@@ -583,8 +583,7 @@ __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(K
       for (; v + W < v1; v += W) page(std::false_type{});
       page(std::true_type{});
     }
-    float* const out = part + (((size_t)p.parts[f.r] * p.Hkv + (size_t)seg * ch.n + chunk) * 16) *
-                                  (D + 4);
+    float* const out = part + ((size_t)f.r * row_parts + seg * ch.n + chunk) * 16 * (D + 4);
     const float lw = on.sum();
     if constexpr (W == 1) {
       if (!x.valid) continue;
@@ -671,14 +670,13 @@ __global__ __launch_bounds__(256) void attn8_join_kernel(Kv8AttnArgs a, const fl
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = blockIdx.x / per, k = blockIdx.x - r * per;
   const Kv8Row row = p.rows[r];
-  const int parts = p.parts[r];
   if (k >= kv8_tokens(p, row)) return;
   const int G = p.Hq / p.Hkv, tpg = 16 / G, j = h / G, grp = k / tpg, c = (k - grp * tpg) * G + h - j * G;
   const int nch = chunks_of(a, row, r, tpg).n;
   if (nch < 2) return;
   const int64_t t = (int64_t)row.cu + k;
   const float* const pc =
-      part + ((size_t)parts * p.Hkv + (size_t)(grp * p.Hkv + j) * nch) * kStride + c * (D + 4);
+      part + ((size_t)(r * kv8_row_parts(p.n, p.Hkv) + grp * nch) * p.Hkv + j * nch) * kStride + c * (D + 4);
   // 64 chunks' rows go out before their maxima and sums, one a lane, are waited for
   fvec v[4][kPer];
   auto rows = [&](int b) __attribute__((always_inline)) {
@@ -1220,19 +1218,14 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
     }
 }
 
-// Partials of the chunks: a group has kv8_chunks() for each kv head or less, which over all
-// groups are kKv8Waves or one each.
-size_t kv8_attn_chunk_floats(const gdn_kv8_desc& d) {
-  const int64_t few = (int64_t)d.num_slots * (kKv8TileTokens - 1);
-  const int64_t groups = few < d.max_step_tokens ? few : d.max_step_tokens;
-  return (size_t)(kKv8Waves + groups * d.num_kv_heads) * 16 * (d.head_dim + 4);
-}
+// Partials of the chunks: all rows' and kv heads' kv8_row_parts()
+static size_t chunk_floats(int D) { return (size_t)kKv8Waves * 16 * (D + 4); }
 
 size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d) {
   // tiles times splits, where there is more than one, are kv8_tile_groups() or less, of the rows
   // of few tokens as of the others
   const size_t tiles = (size_t)2 * kv8_tile_groups(d.head_dim) * 32 * kKv8TileWaves * (d.head_dim + 4);
-  return (kv8_attn_chunk_floats(d) + tiles) * sizeof(float);
+  return (chunk_floats(d.head_dim) + tiles) * sizeof(float);
 }
 
 // Pieces that the pages of at most `tiles` work-groups are cut into. Two lie on a CU side by side
@@ -1250,7 +1243,7 @@ static hipError_t launch_attn8(const Kv8AttnArgs& a) {
   float* const part = static_cast<float*>(a.workspace);
   hipError_t e;
   if (p.max_row >= kKv8TileTokens) {
-    float* const tpart = part + a.tile_part;
+    float* const tpart = part + chunk_floats(D);
     const int G = p.Hq / p.Hkv;
     const int many = kv8_most_tiles(p.n, p.T, G), few = p.n * kv8_few_tiles(G);
     // 63 single tokens at 4,096 beside a prompt of 512 (D = 256): 73 us, from 512 work-groups 94

@@ -487,7 +487,6 @@ struct Kv8Plan {
   Kv8Row* rows;                 // [n]
   int32_t* used;                // [1] n of the plan on the GPU; rows behind it hold nothing
   int32_t* blocks;              // [n + 1] pages that the rows before touch; INT32_MAX behind
-  int32_t* parts;               // [n] attention's chunks (of a kv head) of the rows before, at most
   int32_t* tiles;               // [n] its tiles of the rows before
 };
 // Tokens of a row inside the bounds that a call was given. The plan may be another step's than
@@ -514,6 +513,11 @@ __host__ __device__ inline int kv8_chunk_waves(int n, int Hkv) {
 __host__ __device__ inline int kv8_chunks(int n, int Hkv, int groups) {
   const int c = kKv8Waves / (kv8_chunk_waves(n, Hkv) * n * Hkv * groups);
   return c < 1 ? 1 : c;
+}
+// Partial results that a row has room for, a kv head: its groups times kv8_chunks() or fewer, where
+// that is more than one. n * Hkv times this is kKv8Waves or less.
+__host__ __device__ inline int kv8_row_parts(int n, int Hkv) {
+  return kKv8Waves / (kv8_chunk_waves(n, Hkv) * n * Hkv);
 }
 // Steps with rows of more tokens: tiles of kKv8TileWaves * (32 / G) tokens of a row, their pages cut
 // into pieces where the step's bounds let the tiles be few, of at most kv8_tile_groups()
@@ -622,11 +626,9 @@ struct Kv8AttnArgs {
   uint16_t* out;
   int64_t os, ohs;
   void* workspace;
-  size_t tile_part;             // floats of the chunks' partials in it, before the tiles'
   hipStream_t stream;
 };
 size_t kv8_attn_workspace_bytes(const gdn_kv8_desc& d);
-size_t kv8_attn_chunk_floats(const gdn_kv8_desc& d);
 hipError_t launch_kv8_attn(const Kv8AttnArgs& a);
 
 // Rotary positions (gdn_rope.hip).

@@ -144,7 +144,7 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) try {
   const size_t heads = (size_t)2 * d.num_kv_heads * d.num_pages;
   const size_t table = (size_t)d.num_slots * d.max_pages_per_slot;
   const int R = gdn::kKv8Rows;
-  const size_t words = table + 2 * (size_t)d.num_slots + d.num_pages + 7 + 8 * (size_t)(R + 1) +
+  const size_t words = table + 2 * (size_t)d.num_slots + d.num_pages + 3 + 7 * (size_t)(R + 1) +
                        3 * (size_t)d.max_step_tokens;
   const size_t ws = gdn::kv8_attn_workspace_bytes(d);
   bool ok = true;
@@ -185,7 +185,6 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) try {
     p.status = reinterpret_cast<uint32_t*>(take(1));
     p.cu = take(R + 1);
     p.blocks = take(R + 1);
-    p.parts = take(R + 1);
     p.tiles = take(R + 1);
     p.pos = take(d.max_step_tokens);
     p.map = take(d.max_step_tokens);
@@ -390,7 +389,6 @@ gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc
   a.os = out_stride;
   a.ohs = out_head_stride;
   a.workspace = kv->workspace;
-  a.tile_part = gdn::kv8_attn_chunk_floats(kv->d);
   a.stream = static_cast<hipStream_t>(stream);
   const hipError_t e = gdn::launch_kv8_attn(a);
   return e == hipSuccess ? GDN_OK : hip_fail(e, "gdn_kv8_attention launch");

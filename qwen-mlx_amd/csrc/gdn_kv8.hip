@@ -248,22 +248,16 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     if (m > 0) atomicMax(&taken, before);  // admitted rows come before refused ones
     move(m, slot[i], have[i], 1, avail - 1 - b, -1, false);
   }
-  // pages that the row's tokens fall into, attention's chunks and tiles
-  const int tpg = 16 / (p.Hq / p.Hkv), tpt = kKv8TileWaves * (32 / (p.Hq / p.Hkv));
-  int touched[R], chunks[R], tiles[R], nblk = 0, nchunk = 0, ntile = 0;
+  // pages that the row's tokens fall into, attention's tiles
+  const int tpt = kKv8TileWaves * (32 / (p.Hq / p.Hkv));
+  int touched[R], tiles[R], nblk = 0, ntile = 0;
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = tid * R + i;
     const int tok = ok[i] ? fresh[i] : 0;
     touched[i] = tok > 0 ? (len[i] + tok - 1) / kPage - len[i] / kPage + 1 : 0;
-    chunks[i] = 0;
-    if (tok > 0 && tok < kKv8TileTokens) {
-      const int groups = (tok + tpg - 1) / tpg;
-      chunks[i] = groups * min(need[i], kv8_chunks(p.n, p.Hkv, groups));
-    }
     tiles[i] = tok >= kKv8TileTokens ? (tok + tpt - 1) / tpt : 0;
     nblk += touched[i];
-    nchunk += chunks[i];
     ntile += tiles[i];
     if (r >= p.n) continue;
     p.rows[r] = Kv8Row{ok[i] ? slot[i] : -1, len[i], tok, cu[i]};
@@ -272,7 +266,6 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     if (slot[i] >= 0 && slot[i] < p.num_slots) p.mark[slot[i]] = INT32_MAX;
   }
   int none;
-  int c1 = block_scan<TH>(nchunk, red, none);
   int t1 = p.max_row >= kKv8TileTokens ? block_scan<TH>(ntile, red, none) : 0;
   int b0 = block_scan<TH>(nblk, red, total);  // and orders the tables for the tokens
 #pragma unroll
@@ -280,11 +273,9 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     const int r = tid * R + i;
     if (r >= p.n) continue;
     p.blocks[r] = b0;
-    p.parts[r] = c1;
     p.tiles[r] = t1;
     t1 += tiles[i];
     b0 += touched[i];
-    c1 += chunks[i];
   }
   for (int r = p.n + tid; r < used; r += TH) {
     p.rows[r] = Kv8Row{-1, 0, 0, 0};

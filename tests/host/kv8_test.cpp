@@ -1,6 +1,6 @@
 // How attention over the 8-bit cache cuts a row's pages (gdn_common.h), against the mask's
 // definition: the pages of an item are the ones that hold a key that it sees, each once and
-// in order, and its pieces take each of them once.
+// in order, and its pieces take each of them once and have room for their results.
 #include <cstdio>
 #include <cstdlib>
 #include <random>
@@ -65,9 +65,13 @@ int main() {
       const int fresh = 1 + upto(1700), few = 1 + upto(gdn::kKv8TileTokens - 2);
       row(tile, pos, fresh, window, std::min(pf, pos + fresh), 2 + upto(20), 1, 8);
       row(tile, pos, few, window, std::min(pf, pos + few), 2 + upto(200), 1, 8);
-      const int n = 1 + upto(40), Hkv = 1 + upto(8), groups = (few + group - 1) / group;
+      const int n = 1 + upto(i % 7 ? 40 : 4095), Hkv = 1 + upto(i % 6 ? 8 : 255), groups = (few + group - 1) / group;
       row(group, pos, few, window, std::min(pf, pos + few), gdn::kv8_chunks(n, Hkv, groups),
           gdn::kv8_chunk_waves(n, Hkv), 1);
+      // room for the partial results of every row
+      const int chunks = gdn::kv8_chunks(n, Hkv, groups), room = gdn::kv8_row_parts(n, Hkv);
+      if ((chunks > 1 && groups * chunks > room) || n * Hkv * room > gdn::kKv8Waves)
+        fail("room", group, pos, few, window, n, chunks, room);
     }
   }
   std::printf("%ld items\nALL OK\n", checks);

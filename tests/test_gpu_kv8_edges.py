@@ -87,3 +87,32 @@ def test_append_behind_another_steps_replay(gpu, rows, ntok):
     for c in (kv, twin):
         assert c.check() == 0
         c.close()
+
+
+@pytest.mark.parametrize("rows", [4, 2, 64, 100])
+@pytest.mark.parametrize("longest", [1, 20])
+def test_attention_behind_another_steps_replay(gpu, rows, longest):
+    """64 rows planned by a graph, long ones first, under bounds of another number of rows, by
+    which keys are split otherwise: the rows inside them by the definition, the others'
+    tokens left as they were."""
+    rng = np.random.default_rng(rows)
+    n = 64
+    p = Pair(170, 560, 66, hq=4, hk=2, dim=64, tokens=17000)
+    slots = rng.permutation(170).tolist()
+    slots, others = slots[:n], slots[n:n + rows]
+    lens, ntok = [4096, 4000, 4096, 3000] + [5] * (n - 4), [longest] + [1] * (n - 1)
+    T = sum(ntok)
+    p.step(slots, [0] * n, lens)
+    p.append(rng)
+    say("kv8 attention behind a replay", rows, longest)
+    graph, _ = captured_step(p.kv, slots, lens, ntok, T, longest)
+    p.ref.step(slots, lens, ntok, T, longest)
+    p.step(others, [0] * rows, [1] * rows, max(T, rows), longest)
+    graph.replay()
+    p.ref.step(slots, lens, ntok, T, longest)
+    p.check_tables()
+    p.ref.plan = p.ref.plan[:rows]
+    p.ref.end = sum(ntok[:rows])
+    p.append(rng)
+    p.attention(rng, label=f"{rows} of {n} rows", gate=True)
+    p.kv.close()
