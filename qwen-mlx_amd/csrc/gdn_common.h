@@ -483,9 +483,9 @@ struct Kv8Plan {
   int32_t* cu;                  // [n + 1]
   int32_t* pos;                 // [T]
   int32_t* map;                 // [T]
-  int32_t* tok_row;             // [T] row, -1: of a refused row, -2: behind the last token
+  int32_t* tok_row;             // [T] row, -1: of a refused row, -2: behind the last token, and behind T
   Kv8Row* rows;                 // [n]
-  int32_t* used;                // [1] n of the plan on the GPU; rows behind it hold nothing
+  int32_t* used;                // [2] n of the plan on the GPU, rows behind it hold nothing; its T
   int32_t* blocks;              // [n + 1] pages that the rows before touch; INT32_MAX behind
   int32_t* tiles;               // [n] its tiles of the rows before
 };

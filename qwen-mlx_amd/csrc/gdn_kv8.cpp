@@ -144,7 +144,7 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) try {
   const size_t heads = (size_t)2 * d.num_kv_heads * d.num_pages;
   const size_t table = (size_t)d.num_slots * d.max_pages_per_slot;
   const int R = gdn::kKv8Rows;
-  const size_t words = table + 2 * (size_t)d.num_slots + d.num_pages + 3 + 7 * (size_t)(R + 1) +
+  const size_t words = table + 2 * (size_t)d.num_slots + d.num_pages + 4 + 7 * (size_t)(R + 1) +
                        3 * (size_t)d.max_step_tokens;
   const size_t ws = gdn::kv8_attn_workspace_bytes(d);
   bool ok = true;
@@ -181,7 +181,7 @@ gdn_status gdn_kv8_create(const gdn_kv8_desc* desc, gdn_kv8** out) try {
     p.mark = take(d.num_slots);
     p.free_pages = take(d.num_pages);
     p.free_count = take(1);
-    p.used = take(1);
+    p.used = take(2);
     p.status = reinterpret_cast<uint32_t*>(take(1));
     p.cu = take(R + 1);
     p.blocks = take(R + 1);

@@ -149,7 +149,7 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
   bool ok[R];
   uint32_t flags = 0;
   if (tid == 0) taken = 0;
-  const int count = *p.free_count, used = *p.used;
+  const int count = *p.free_count, used = p.used[0], used_t = p.used[1];
 #pragma unroll
   for (int i = 0; i < R; ++i) {
     const int r = tid * R + i;
@@ -281,10 +281,12 @@ __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* 
     p.rows[r] = Kv8Row{-1, 0, 0, 0};
     p.blocks[r + 1] = INT32_MAX;  // behind every item
   }
+  for (int t = p.T + tid; t < used_t; t += TH) p.tok_row[t] = -2;
   if (tid == 0) {
     p.blocks[p.n] = total;
     *p.free_count = avail - taken;
-    *p.used = p.n;
+    p.used[0] = p.n;
+    p.used[1] = p.T;
   }
   if (flags) atomicOr(p.status, flags);
   if (p.T <= kMapHere)

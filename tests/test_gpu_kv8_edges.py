@@ -116,3 +116,22 @@ def test_attention_behind_another_steps_replay(gpu, rows, longest):
     p.append(rng)
     p.attention(rng, label=f"{rows} of {n} rows", gate=True)
     p.kv.close()
+
+
+@pytest.mark.parametrize("new", [2, 20])
+def test_tokens_behind_a_replayed_plan_are_left_alone(gpu, new):
+    """A step whose later rows are refused, then the replay of a shorter one: the tokens that
+    were refused are none of the plan's any more, and their outputs stay."""
+    rng = np.random.default_rng(new)
+    p = Pair(4, 12, 6, hq=4, hk=2, dim=64, tokens=200)
+    p.step([1, 2], [0, 0], [70, 40])
+    p.append(rng)
+    graph, _ = captured_step(p.kv, [2, 1], [40, 70], [new, 1], new + 1, new)
+    p.ref.step([2, 1], [40, 70], [new, 1], new + 1, new)
+    p.step([0, 9, 9], [0, 0, 0], [1, new, new], 2 * new + 90, new)
+    graph.replay()
+    p.ref.step([2, 1], [40, 70], [new, 1], new + 1, new)
+    assert p.kv.check() == 1
+    p.append(rng)
+    p.attention(rng, label="a shorter plan")  # rows behind the plan's tokens stay as they were
+    p.kv.close()
