@@ -911,7 +911,7 @@ gdn_status gdn_kv8_gather(gdn_kv8* kv, int32_t layer, int32_t m, const int32_t* 
 
 typedef struct gdn_kv8_attn_desc {
   float scale;     /* factor on q . k; 0: 1 / sqrt(head_dim)                       */
-  float softcap;   /* > 0: scores become softcap * tanh(score / softcap)           */
+  float softcap;   /* 1e-30 .. 1e30: scores become softcap * tanh(score / softcap); 0: not */
   int32_t window;  /* > 0: a token sees the last `window` positions, its own included */
 } gdn_kv8_attn_desc;
 
@@ -927,14 +927,15 @@ typedef struct gdn_kv8_attn_desc {
  * DEVICE arrays (or NULL). out's heads must not run into each other, nor overlap q or gate.
  * Tokens of refused rows get zeros; rows behind the last token are left as they are.
  *
- * Products and sums are f32; dimensions of q below 2^-13 of its head's largest are rounded
- * by at most 2^-21 of that, the softmax's weights enter the product with the values in
- * f16 (11 bits), and out is rounded once. The bits are the same every time and do not
- * depend on what the step's other rows are; the kernel and the places where keys are
- * split follow the row's tokens and the step's bounds (n, max_tokens, max_row_tokens), so
- * that steps of other bounds may differ by rounding. An infinity or NaN in a head of q
- * makes that head's output NaN. A NaN among the keys or values of a kv head
- * that a token sees makes its query heads there NaN; tokens that do not see it are
+ * Products and sums are f32, a capped score within 2^-19 of itself; dimensions of q below
+ * 2^-13 of its head's largest are rounded by at most 2^-21 of that, the softmax's weights
+ * enter the product with the values in f16 (11 bits), and out is rounded once. The bits are
+ * the same every time and do not depend on what the step's other rows are; the kernel and
+ * the places where keys are split follow the row's tokens and the step's bounds (n,
+ * max_tokens, max_row_tokens), so that steps of other bounds may differ by rounding. An
+ * infinity or NaN in a head of q makes that head's output NaN. A NaN among the keys or
+ * values of a kv head that a token sees makes its query heads there NaN; tokens that do not
+ * see it are
  * not touched. */
 gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc* desc,
                              const uint16_t* q, int64_t q_stride, int64_t q_head_stride,

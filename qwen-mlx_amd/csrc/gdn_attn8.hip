@@ -12,6 +12,8 @@
 // more than bf16. The pages' exponents stay outside: the keys' multiplies the scores; the
 // outputs run in units of 2^(unit - 6), and P carries 2^(6 + the values' exponent - unit), which
 // f16 has room for from 2^0 to 2^7: only beyond that are the outputs rescaled.
+#include <cfloat>
+
 #include "gdn_common.h"
 
 namespace gdn {
@@ -110,10 +112,18 @@ struct Score {
   int window;     // or more than any position
 };
 
-// softcap * tanh(y): 1 - 2 / (1 + e^2y), off by some 2^-23 of the cap
+// cap * tanh(y), off by at most 2^-19 of itself. 1 - 2 / (1 + e^2y) is off by some 2^-21.3 of 1
+// everywhere, which is too much of a small y: below 1/4 the series y - y^3 / 3 + 2 y^5 / 15 - ..,
+// whose first term left out is 2^-26.8 of y there.
 __device__ __forceinline__ float capped(float y, float cap) {
   const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);  // e^2y; inf: 1
-  return cap * fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+  const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+  const float z = y * y;
+  float c = fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f);
+  c = fmaf(z, c, 2.0f / 15.0f);
+  c = fmaf(z, c, -1.0f / 3.0f);
+  const float near = fmaf(z * c, y, y);
+  return cap * (fabsf(y) < 0.25f ? near : far);
 }
 
 // Inclusive sum over the wave's lanes.
@@ -283,9 +293,10 @@ __device__ __forceinline__ int q_parts32(const uint16_t* q, bool valid, u32x4* o
   return q_pieces<2 * NK, true>(q, valid, out);
 }
 
-// sc * 2^e; an e that leaves nothing of any score stays a factor
+// sc * 2^e; an e that leaves nothing of any score stays a factor, and what has no room in f32 its
+// largest number, so that scores of zero stay zero
 __device__ __forceinline__ float factor_of(float sc, int e) {
-  return __builtin_amdgcn_ldexpf(sc, max(e, -110));
+  return __builtin_amdgcn_fmed3f(__builtin_amdgcn_ldexpf(sc, max(e, -110)), -FLT_MAX, FLT_MAX);
 }
 
 // Bits of those of a lane's `count` scores whose keys lie below n, four keys side by side every

@@ -352,6 +352,7 @@ gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc
   if (!kv->planned)
     return kfail(GDN_ERR_INVALID, "gdn_kv8_attention: no step planned (gdn_kv8_step)");
   if (!std::isfinite(desc->scale) || !std::isfinite(desc->softcap) || desc->softcap < 0.0f ||
+      (desc->softcap != 0.0f && (desc->softcap < 1e-30f || desc->softcap > 1e30f)) ||
       desc->window < 0)
     return kfail(GDN_ERR_INVALID, "gdn_kv8_attention: scale %g, softcap %g, window %d",
                  (double)desc->scale, (double)desc->softcap, desc->window);

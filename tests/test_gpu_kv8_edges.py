@@ -4,7 +4,7 @@ import numpy as np
 import pytest
 
 from gdn_testlib import say
-from test_gpu_kv8 import Pair, bf, i32
+from test_gpu_kv8 import Pair, bf, i32, num
 
 pytestmark = pytest.mark.gpu
 
@@ -135,3 +135,65 @@ def test_tokens_behind_a_replayed_plan_are_left_alone(gpu, new):
     p.append(rng)
     p.attention(rng, label="a shorter plan")  # rows behind the plan's tokens stay as they were
     p.kv.close()
+
+
+def capped_reference(ref, q, cap, scale):
+    """(out, tolerance) as Ref.attention's, but for a capped score, whose error is within 2^-19 of
+    itself: f32 roundings of its factors, and of the function, whose worst is near -1/4 where
+    2 / (1 + e^2y) is 1.25 with a relative error of 2 2^-23 (a reciprocal's and an exponential's
+    last places, two roundings), 10 2^-23 of the result."""
+    out, tol = np.zeros((2, ref.end) + q.shape[1:])
+    G = q.shape[1] // ref.heads
+    for s, a, b, c in ref.plan:
+        for t in range(b):
+            for h in range(q.shape[1]):
+                k, v = (x[:a + t + 1, h // G] for x in ref.held[s])
+                qk = q[c + t, h] * k
+                y = qk.sum(1) * scale / cap
+                sc = cap * np.tanh(y)
+                err = np.abs(qk).sum(1) * abs(scale) * ref.dim * 2.0 ** -24 / np.cosh(np.minimum(
+                    np.abs(y) * 0.99, 300)) ** 2
+                err += 2.0 ** -19 * np.abs(sc)
+                w = np.exp(sc - sc.max())
+                w /= w.sum()
+                o, av = w @ v, w @ np.abs(v)
+                out[c + t, h] = o
+                tol[c + t, h] = ((2.0 ** -11 + 2 * err.max() + (len(k) + 16) * 2.0 ** -24 + 2.0 ** -20) * av +
+                                 2.0 ** -25 * np.abs(v).sum(0) + 2.0 ** -8 * np.abs(o)) * (1 + 2.0 ** -7)
+    return out, tol
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("cap,loud", [(1e-30, 1e10), (1e-30, 1.0), (1e-3, 1.0), (0.5, 1.0), (6.0, 1.0),
+                                      (1e3, 1.0), (1e4, 1.0), (1e6, 1.0), (1e8, 1.0), (1e30, 1.0)])
+def test_caps_of_every_size(gpu, dim, cap, loud):
+    """Scores far above their cap and far below it, where it changes nothing, and a key of zeros,
+    in a step of tiles and in one of chunks."""
+    import torch
+    rng = np.random.default_rng(dim)
+    p = Pair(2, 12, 6, hq=4, hk=2, dim=dim)
+    scale = 3 * loud / dim ** 0.5
+    cap = float(np.float32(cap))
+    for step in ([1, 0], [0, 0], [130, 33]), ([0, 1], [33, 130], [1, 3]):
+        p.step(*step)
+        p.append(rng, change=lambda x: x[0].zero_())
+        q, qn = bf(rng, p.kv.tokens, 4, dim)
+        out = torch.zeros_like(q)
+        p.kv.attention(0, q, out, scale=scale, softcap=cap)
+        want, tol = capped_reference(p.ref, qn, cap, float(np.float32(scale)))
+        err = np.abs(num(out) - want)
+        say("kv8 cap", cap, "worst error / tolerance", float((err / np.maximum(tol, 1e-30)).max()))
+        assert np.all(err <= tol)
+    p.kv.close()
+
+
+def test_caps_that_are_refused(gpu):
+    import gdn_amd
+    import torch
+    kv = gdn_amd.KV8Cache(1, 2, 4, 4, 4, 2, 64, 8)
+    kv.step(i32([0]), i32([0]), i32([4]), 4)
+    q = torch.zeros(4, 4, 64, device="cuda:0", dtype=torch.bfloat16)
+    for cap in (1e-31, 1e-40, 1.1e30, 3e38, float("inf"), -1.0):
+        with pytest.raises(gdn_amd.GdnError, match="softcap"):
+            kv.attention(0, q, q.clone(), softcap=cap)
+    kv.close()
