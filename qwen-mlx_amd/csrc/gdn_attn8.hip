@@ -967,7 +967,9 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
   // power of two 2^-60 at least; and not with more dims, whose registers it has no room in.
   const bool tilt = D == 64 && a.slopes && a.softcap == 0.f && sm >= 0x1p-40f && sm <= 0x1p40f &&
                     __all(fabsf(column().slope) <= 0x1p20f);
-  const bool odd = a.softcap > 0.f || (a.slopes && !tilt) || !(a.scale > 0.f);
+  // Nor may masked scores, -inf, meet an mk that is not positive: factor_of()'s 2^-110 of a small
+  // scale is none any more, where zero queries meet a page of zeros.
+  const bool odd = a.softcap > 0.f || (a.slopes && !tilt) || !(tilt || sm >= 0x1p-16f);
   float m = -INFINITY, l = 0.f, mk, far = 0.f;
   uint32_t seen;
   int unit = 0;
@@ -1017,7 +1019,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
         }
         mk = 1.f;
       }
-      // slopes of zero where there are none: a scale that is not positive comes here too
+      // slopes of zero where there are none: a scale that is small or negative comes here too
       const Column col = column();
       const float slope = col.slope, off = slope * (float)(kl - col.pos);
 #pragma unroll

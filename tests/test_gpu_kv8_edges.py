@@ -197,3 +197,20 @@ def test_caps_that_are_refused(gpu):
         with pytest.raises(gdn_amd.GdnError, match="softcap"):
             kv.attention(0, q, q.clone(), softcap=cap)
     kv.close()
+
+
+@pytest.mark.parametrize("dim", [64, 128, 256])
+@pytest.mark.parametrize("scale", [1e-6, 1e-13, 1e-38, 1e-42, -1e-13])
+def test_scales_that_leave_nothing_of_the_scores(gpu, dim, scale):
+    """Queries of zeros and others, a page of zeros, in a step of tiles and in one of chunks."""
+    rng = np.random.default_rng(dim)
+    p = Pair(2, 12, 6, hq=4, hk=2, dim=dim)
+    p.step([1], [0], [64])
+    p.append(rng, change=lambda x: x.zero_())
+    for step in ([1, 0], [64, 0], [70, 33]), ([0, 1], [33, 134], [1, 3]):
+        p.step(*step)
+        p.append(rng)
+        p.attention(rng, label=f"scale {scale}", std=0.0, scale=scale)
+        p.attention(rng, label=f"scale {scale}", scale=scale)
+        p.attention(rng, label=f"scale {scale}, window", scale=scale, window=50)
+    p.kv.close()
