@@ -895,8 +895,8 @@ gdn_status gdn_kv8_views(const gdn_kv8* kv, gdn_kv8_view* view);
 gdn_status gdn_kv8_check(gdn_kv8* kv, void* stream, uint32_t* flags);
 
 /* Put the step's new keys and values [max_tokens, stride] (num_kv_heads x
- * head_dim bf16 each, 16-byte aligned, strides multiples of 8) into layer's
- * pages. A page's exponent follows the tokens that it holds with them; where it
+ * head_dim bf16 each, 16-byte aligned, strides multiples of 8 that hold a row) into
+ * layer's pages. A page's exponent follows the tokens that it holds with them; where it
  * changes, the older numbers are rounded anew from what was held. The same
  * call twice leaves the same bits. */
 gdn_status gdn_kv8_append(gdn_kv8* kv, int32_t layer, const uint16_t* k, int64_t k_stride,
@@ -904,7 +904,7 @@ gdn_status gdn_kv8_append(gdn_kv8* kv, int32_t layer, const uint16_t* k, int64_t
 
 /* The values held at m places map[i] (page * 64 + position % 64, DEVICE array) of a
  * layer -> k_out, v_out [m, stride] bf16 (exact; either may be NULL; 16-byte aligned,
- * strides multiples of 8). A place outside the cache gives zeros. */
+ * strides multiples of 8 that hold a row). A place outside the cache gives zeros. */
 gdn_status gdn_kv8_gather(gdn_kv8* kv, int32_t layer, int32_t m, const int32_t* map,
                           uint16_t* k_out, int64_t k_stride, uint16_t* v_out, int64_t v_stride,
                           void* stream);

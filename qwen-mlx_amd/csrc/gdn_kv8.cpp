@@ -68,6 +68,12 @@ bool rows_ok(const void* p, int64_t stride, int64_t head_stride, int heads, int 
           stride >= (heads - 1) * head_stride + dim);
 }
 
+// Rows of `heads` heads side by side, which do not run into the next row. A single row's stride
+// does not matter.
+bool packed_rows_ok(const void* p, int64_t stride, int heads, int dim, int64_t rows) {
+  return aligned(p, 16) && (rows <= 1 || (stride % 8 == 0 && stride >= (int64_t)heads * dim));
+}
+
 }  // namespace
 
 struct gdn_kv8 {
@@ -292,7 +298,7 @@ gdn_status gdn_kv8_append(gdn_kv8* kv, int32_t layer, const uint16_t* k, int64_t
   if (kv->p.T == 0) return GDN_OK;
   if (!k || !v) return kfail(GDN_ERR_INVALID, "gdn_kv8_append: NULL tensor pointer");
   const int D = kv->d.head_dim, H = kv->d.num_kv_heads;
-  if (!rows_ok(k, k_stride, D, H, D, 8, 2) || !rows_ok(v, v_stride, D, H, D, 8, 2))
+  if (!packed_rows_ok(k, k_stride, H, D, kv->p.T) || !packed_rows_ok(v, v_stride, H, D, kv->p.T))
     return kfail(GDN_ERR_INVALID, "gdn_kv8_append: k and v need 16-byte alignment and row strides "
                  ">= %d that are multiples of 8 (got %lld, %lld)", H * D, (long long)k_stride,
                  (long long)v_stride);
@@ -320,8 +326,8 @@ gdn_status gdn_kv8_gather(gdn_kv8* kv, int32_t layer, int32_t m, const int32_t* 
   if (!map || !aligned(map, 4) || (!k_out && !v_out))
     return kfail(GDN_ERR_INVALID, "gdn_kv8_gather: NULL or misaligned array");
   const int D = kv->d.head_dim, H = kv->d.num_kv_heads;
-  if ((k_out && !rows_ok(k_out, k_stride, D, H, D, 8, 2)) ||
-      (v_out && !rows_ok(v_out, v_stride, D, H, D, 8, 2)))
+  if ((k_out && !packed_rows_ok(k_out, k_stride, H, D, m)) ||
+      (v_out && !packed_rows_ok(v_out, v_stride, H, D, m)))
     return kfail(GDN_ERR_INVALID, "gdn_kv8_gather: outputs need 16-byte alignment and row strides "
                  ">= %d that are multiples of 8 (got %lld, %lld)", H * D, (long long)k_stride,
                  (long long)v_stride);

@@ -214,3 +214,28 @@ def test_scales_that_leave_nothing_of_the_scores(gpu, dim, scale):
         p.attention(rng, label=f"scale {scale}", scale=scale)
         p.attention(rng, label=f"scale {scale}, window", scale=scale, window=50)
     p.kv.close()
+
+
+def test_rows_that_run_into_each_other_are_refused(gpu):
+    """A stride of one head where a row has several: append and gather take whole rows. A single
+    row's stride does not matter."""
+    import gdn_amd
+    import torch
+    kv = gdn_amd.KV8Cache(1, 2, 4, 4, 4, 2, 64, 8)
+    kv.step(i32([0]), i32([0]), i32([4]), 4)
+    flat = torch.zeros(4 * 128, device="cuda:0", dtype=torch.bfloat16)
+    good = flat.view(4, 2, 64)
+    for stride in (64, 72, 120):
+        bad = flat.as_strided((4, 2, 64), (stride, 64, 1))
+        for call in (lambda: kv.append(0, bad, good), lambda: kv.append(0, good, bad),
+                     lambda: kv.gather(0, i32(range(4)), bad, None),
+                     lambda: kv.gather(0, i32(range(4)), None, bad)):
+            with pytest.raises(gdn_amd.GdnError, match="row strides"):
+                call()
+    kv.append(0, good, good)
+    for stride in (64, 8, 0, 1000):
+        one = flat.as_strided((1, 2, 64), (stride, 64, 1))
+        kv.gather(0, i32([0]), one, one.clone())
+        kv.step(i32([0]), i32([4]), i32([1]), 1)
+        kv.append(0, one, one)
+    kv.close()
