@@ -9,9 +9,12 @@
 // its rounding and the 4 that are left, times 16 (numbers below 2^-14 of the head's
 // largest lose bits, 2^-22 of it at most). For P V the values convert exactly into f16, and P,
 // in [0, 2^8] as the running maximum follows by steps of 2^8, is rounded to it: 11 bits, three
-// more than bf16. The pages' exponents stay outside: the keys' multiplies the scores; the
-// outputs run in units of 2^(unit - 6), and P carries 2^(6 + the values' exponent - unit), which
-// f16 has room for from 2^0 to 2^7: only beyond that are the outputs rescaled.
+// more than bf16, and small weights by at most 2^-29 of the maximum's. The softmax's sum is of the
+// rounded P, so that values that are all the same come out as they are. The pages' exponents stay
+// outside: the keys' multiplies the scores; the outputs run in units of 2^(unit - 6), and P carries
+// 2^(6 + the values' exponent - unit), 2^4 to 2^7: only beyond that are the outputs rescaled. With
+// more f16 has no room; from 2^0 on, a million keys of weights just too small for it were lost
+// beside one that weighs as much as 2^25 of them, 3% of the sum.
 #include <cfloat>
 
 #include "gdn_common.h"
@@ -26,9 +29,10 @@ constexpr int kNanFlag = 1 << 16;
 constexpr int kSplitPages = 8;  // of a tile's split at least
 constexpr float kStep = 8.f;  // log2 steps of the running maximum
 constexpr int kUnit = 6;      // the outputs' unit is 2^(unit - kUnit)
-// Whether values of exponent ev go on in a unit: P's factor 2^(kUnit + ev - unit) is in [2^0, 2^7]
+// Whether values of exponent ev go on in a unit: P's factor 2^(kUnit + ev - unit) is in [2^4, 2^7].
+// A new unit is ev itself.
 __device__ __forceinline__ bool unit_holds(int ev, int unit) {
-  return ev - unit >= -kUnit && ev - unit <= 1;
+  return ev - unit >= 4 - kUnit && ev - unit <= 7 - kUnit;
 }
 
 typedef uint32_t u32x4 __attribute__((ext_vector_type(4)));
@@ -54,6 +58,11 @@ __device__ __forceinline__ f16x8 to_f16(uint32_t a, uint32_t b) {
 }
 __device__ __forceinline__ uint32_t pk_f16(float a, float b) {
   return __builtin_bit_cast(uint32_t, __builtin_convertvector((f32x2){a, b}, f16x2));
+}
+// s + the two f16 numbers of a word, small ones among them, in one instruction
+__device__ __forceinline__ float add_f16(uint32_t two, float s) {
+  const f16x2 ones = {(_Float16)1.f, (_Float16)1.f};
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two), ones, s, false);
 }
 
 // Scores of 16 keys for 16 columns: K as held (a lane's NK 16-byte pieces of its key), q in
@@ -365,8 +374,8 @@ struct Online {
       m = mn;
       l *= corr;
       if (!unit_holds(ev, unit)) {
-        corr = __builtin_amdgcn_ldexpf(corr, unit - (ev + 2));
-        unit = ev + 2;  // room either way
+        corr = __builtin_amdgcn_ldexpf(corr, unit - ev);
+        unit = ev;
       }
 #pragma unroll
       for (int d = 0; d < D / 16; ++d) O[d] *= corr;
@@ -375,8 +384,9 @@ struct Online {
     const float mref = (m == -INFINITY ? 0.f : m) - (float)up;
 #pragma unroll
     for (int i = 0; i < 8; ++i) s[i] = __builtin_amdgcn_exp2f(s[i] - mref);
-    l = fmaf(((s[0] + s[1]) + (s[2] + s[3])) + ((s[4] + s[5]) + (s[6] + s[7])), pow2(-up), l);
-    return (u32x4){pk_f16(s[0], s[1]), pk_f16(s[2], s[3]), pk_f16(s[4], s[5]), pk_f16(s[6], s[7])};
+    const u32x4 P = {pk_f16(s[0], s[1]), pk_f16(s[2], s[3]), pk_f16(s[4], s[5]), pk_f16(s[6], s[7])};
+    l = fmaf(add_f16(P[2], add_f16(P[0], 0.f)) + add_f16(P[3], add_f16(P[1], 0.f)), pow2(-up), l);
+    return P;
   }
 
   // O += the block's values (raw bytes v, as loaded) . P. `total`: the row's keys.
@@ -1047,7 +1057,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
     for (int i = 2; i < 16; ++i) bm = fmaxf(bm, S[i]);
     bm = max_xor32(fmaf(bm, mk, far));
     if (__builtin_expect(!unit_holds(ev, unit) || __any(bm > m + kStep), 0)) {
-      const int to = unit_holds(ev, unit) ? unit : ev + 2;  // room either way
+      const int to = unit_holds(ev, unit) ? unit : ev;
       const float mn = fmaxf(m, bm);
       float corr = mn > m ? __builtin_amdgcn_exp2f(m - mn) : 1.0f;  // m = -inf: 0
       m = mn;
@@ -1072,17 +1082,11 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
     P[0] = (u32x4){pk_f16(e[0], e[1]), pk_f16(e[2], e[3]), pk_f16(e[8], e[9]), pk_f16(e[10], e[11])};
     P[1] = (u32x4){pk_f16(e[4], e[5]), pk_f16(e[6], e[7]), pk_f16(e[12], e[13]), pk_f16(e[14], e[15])};
     asm volatile("" : "+v"(P[0]), "+v"(P[1]));  // here, not behind the branches that follow
-    // the sum is of the rounded weights, two an instruction (which keeps f16's small numbers)
-    typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
-    const f16x2 ones = {(_Float16)1.f, (_Float16)1.f};
     float sum[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < 4; ++i)
 #pragma unroll
-      for (int k = 0; k < 2; ++k) {
-        const uint32_t two = P[k][i];
-        sum[k] = __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2, two), ones, sum[k], false);
-      }
+      for (int k = 0; k < 2; ++k) sum[k] = add_f16(P[k][i], sum[k]);
     l = fmaf(sum[0] + sum[1], pow2(-up), l);
   };
   // O += P V of half hb of the page in lv: fragments are read two ahead (the first two apart) and

@@ -239,3 +239,44 @@ def test_rows_that_run_into_each_other_are_refused(gpu):
         kv.step(i32([0]), i32([4]), i32([1]), 1)
         kv.append(0, one, one)
     kv.close()
+
+
+@pytest.mark.parametrize("most", [1, 20])
+def test_a_million_faint_keys(gpu, most):
+    """One key by 2^25.2 stronger than 2^20 others, which together weigh 2.6%, in one piece (the
+    bounds leave no more): where all values are the same, so is the output; where the strong
+    key's is zero, it is the others' weight."""
+    import gdn_amd
+    import torch
+    say("kv8 a million keys", most)
+    step, n = 262144, 1024
+    kv = gdn_amd.KV8Cache(1, 1024, 16400, 16400, 1, 1, 64, step)
+    k = torch.zeros(step, 1, 64, device="cuda:0", dtype=torch.bfloat16)
+    v = torch.full_like(k, 4.0)
+    slots = i32([0] + [-1] * (n - 1))
+    out = torch.zeros_like(k)
+    strong = 7.0 * 2.5
+    for first, want in ((4.0, 4.0), (0.0, 4.0 * 2 ** 20 / (2 ** 20 + np.exp(strong)))):
+        for i in range(4):
+            kk, vv = k.clone(), v.clone()
+            if i == 0:
+                kk[0, 0, 0] = 7.0
+                vv[0] = first
+            kv.step(i32([0]), i32([i * step]), i32([step]), step)
+            kv.append(0, kk, vv)
+        q = torch.zeros_like(k)
+        q[:most, 0, 0] = 2.5
+        kv.step(slots, i32([4 * step] + [0] * (n - 1)), i32([most] + [0] * (n - 1)),
+                n if most == 1 else step, most)
+        t = kv.tokens
+        kv.append(0, k[:t], v[:t])
+        kv.attention(0, q[:t], out[:t], scale=1.0)
+        assert kv.check() == 0
+        # each weight within 2^-11 of itself, or 2^-29 of the largest; f32 sums, of 2^20 / 32 additions
+        # to the weights' and 2^20 / 16 to the outputs', 2^-24 of a sum each; the result's rounding
+        got = num(out[:most])
+        tol = want * (2.0 ** -8 + 2.0 ** -10 + (2.0 ** 15 + 2.0 ** 16) * 2.0 ** -24)
+        tol += 2.0 ** 20 * 2.0 ** -29 * 4.0 if first == 0 else 0
+        say("kv8 a million keys", float(got.min()), float(got.max()), want, tol)
+        assert np.all(np.abs(got - want) <= tol)
+    kv.close()
