@@ -122,17 +122,45 @@ struct Score {
 };
 
 // cap * tanh(y), off by at most 2^-19 of itself. 1 - 2 / (1 + e^2y) is off by some 2^-21.3 of 1
-// everywhere, which is too much of a small y: below 1/4 the series y - y^3 / 3 + 2 y^5 / 15 - ..,
-// whose first term left out is 2^-26.8 of y there.
-__device__ __forceinline__ float capped(float y, float cap) {
-  const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);  // e^2y; inf: 1
-  const float far = fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+// everywhere, which is too much of a small y: below 1/2 the series y - y^3 / 3 + 2 y^5 / 15 - ..,
+// whose first term left out is 2^-23 of y there, and in fewer cycles.
+__device__ __forceinline__ float capped_near(float y, float cap) {
   const float z = y * y;
-  float c = fmaf(z, 62.0f / 2835.0f, -17.0f / 315.0f);
+  float c = fmaf(z, 21844.0f / 6081075.0f, -1382.0f / 155925.0f);
+  c = fmaf(z, c, 62.0f / 2835.0f);
+  c = fmaf(z, c, -17.0f / 315.0f);
   c = fmaf(z, c, 2.0f / 15.0f);
   c = fmaf(z, c, -1.0f / 3.0f);
-  const float near = fmaf(z * c, y, y);
-  return cap * (fabsf(y) < 0.25f ? near : far);
+  return cap * fmaf(z * c, y, y);
+}
+__device__ __forceinline__ float capped_any(float y, float cap) {
+  const float e = __builtin_amdgcn_exp2f(y * 2.8853900817779268f);  // e^2y; inf: 1
+  const float far = cap * fmaf(-2.0f, __builtin_amdgcn_rcpf(1.0f + e), 1.0f);
+  return fabsf(y) < 0.5f ? capped_near(y, cap) : far;
+}
+// N scores s times mul, capped. Where all of a wave's lie below half the cap, as they mostly do, they
+// take the series alone: 23 rows of 1,024 seen keys 21.0 us, 21.5 with both formed for each score.
+template <int N, typename T>
+__device__ __forceinline__ void cap_scores(T& s, float mul, float cap) {
+  float most = 0.f;
+#pragma unroll
+  for (int i = 0; i < N; ++i) {
+    s[i] *= mul;
+    most = fmaxf(most, fabsf(s[i]));
+  }
+  if (__all(most < 0.5f)) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s[i] = capped_near(s[i], cap);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);  // few registers at once
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+      s[i] = capped_any(s[i], cap);
+      if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+    }
+  }
 }
 
 // Inclusive sum over the wave's lanes.
@@ -340,12 +368,14 @@ struct Online {
     float s[8];
     const float mul = factor_of(sc.mul, e);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) s[i] = S[i >> 2][i & 3] * mul;
+    for (int i = 0; i < 8; ++i) s[i] = S[i >> 2][i & 3];
     const int k0 = key0 + 4 * g4;  // score i is of key k0 + 16 (i / 4) + i % 4
     if (__builtin_expect(sc.cap > 0.f, 0)) {
       asm volatile("");  // a branch: the caps are many instructions
+      cap_scores<8>(s, mul, sc.cap);
+    } else {
 #pragma unroll
-      for (int i = 0; i < 8; ++i) s[i] = capped(s[i], sc.cap);
+      for (int i = 0; i < 8; ++i) s[i] *= mul;
     }
     if (__builtin_expect(sc.sloped, 0)) {
       asm volatile("");
@@ -1022,11 +1052,7 @@ __global__ __launch_bounds__(64 * NW, D == 256 ? 2 : D == 128 ? 3 : 4) void attn
       asm volatile("");  // a branch, as below: rare and long
       const float cap = a.softcap * 1.4426950408889634f;
       if (cap > 0.f) {
-#pragma unroll
-        for (int i = 0; i < 16; ++i) {
-          S[i] = capped(S[i] * mk, cap);
-          if (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-        }
+        cap_scores<16>(S, mk, cap);
         mk = 1.f;
       }
       // slopes of zero where there are none: a scale that is small or negative comes here too

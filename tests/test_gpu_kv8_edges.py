@@ -139,9 +139,9 @@ def test_tokens_behind_a_replayed_plan_are_left_alone(gpu, new):
 
 def capped_reference(ref, q, cap, scale):
     """(out, tolerance) as Ref.attention's, but for a capped score, whose error is within 2^-19 of
-    itself: f32 roundings of its factors, and of the function, whose worst is near -1/4 where
-    2 / (1 + e^2y) is 1.25 with a relative error of 2 2^-23 (a reciprocal's and an exponential's
-    last places, two roundings), 10 2^-23 of the result."""
+    itself: f32 roundings of its factors, and of the function, whose worst is at -1/2 where
+    2 / (1 + e^2y) is 1.46 with a relative error of 2 2^-23 (a reciprocal's and an exponential's
+    last places, two roundings), 6.5 2^-23 of the result."""
     out, tol = np.zeros((2, ref.end) + q.shape[1:])
     G = q.shape[1] // ref.heads
     for s, a, b, c in ref.plan:
