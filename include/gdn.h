@@ -930,13 +930,13 @@ typedef struct gdn_kv8_attn_desc {
  * Products and sums are f32, a capped score within 2^-19 of itself; dimensions of q below
  * 2^-13 of its head's largest are rounded by at most 2^-21 of that, the softmax's weights
  * enter the product with the values, and their own sum, in f16 (11 bits, or by at most 2^-29
- * of the largest where they are small), and out is rounded once. The bits are the same every
- * time and do not depend on what the step's other rows are; the kernel and the places where
- * keys are split follow the row's tokens and the step's bounds (n, max_tokens,
- * max_row_tokens), so that steps of other bounds may differ by rounding. An infinity or NaN
- * in a head of q makes that head's output NaN. A NaN among the keys or values of a kv head
- * that a token sees makes its query heads there NaN; tokens that do not see it are
- * not touched. */
+ * of the largest where they are small), and out is rounded once. Values past 2^48 beside
+ * pages of zeros or of numbers below 2^-31 may overflow. The bits are the same every time and
+ * do not depend on what the step's other rows are; the kernel and the places where keys are
+ * split follow the row's tokens and the step's bounds (n, max_tokens, max_row_tokens), so
+ * that steps of other bounds may differ by rounding. An infinity or NaN in a head of q makes
+ * that head's output NaN. A NaN among the keys or values of a kv head that a token sees makes
+ * its query heads there NaN; tokens that do not see it are not touched. */
 gdn_status gdn_kv8_attention(gdn_kv8* kv, int32_t layer, const gdn_kv8_attn_desc* desc,
                              const uint16_t* q, int64_t q_stride, int64_t q_head_stride,
                              const float* slopes, const int32_t* prefix, const uint16_t* gate,

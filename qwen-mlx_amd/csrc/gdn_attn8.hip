@@ -522,8 +522,8 @@ __device__ __forceinline__ float* split_part(const Kv8Plan& p, float* part, cons
 // of a chunk each, and they join in LDS: one partial a chunk. A wave loads the next page's
 // keys as soon as this page's scores are formed, its values after this page's products: 32 KiB of
 // 256 dims in flight for each wave, which takes 512 registers and so a SIMD. Bound by HBM: 64
-// rows at 4,096 keys (279 MB of pages, 2 kv heads of 256 dims) 55 us, 5.1 TB/s where a large copy
-// reaches 5.2; 23 rows that see 1,024 keys each (49 MB, 8 of 128) 14.5 us. Bound by latency where
+// rows at 4,096 keys (279 MB of pages, 2 kv heads of 256 dims) 56 us, 5.0 TB/s where a large copy
+// reaches 5.2; 23 rows that see 1,024 keys each (49 MB, 8 of 128, capped) 15.0 us. Bound by latency where
 // a wave has a page or none: a row at 32,768 keys (34 MB) 15 us.
 template <int D, int W>
 __global__ __launch_bounds__(64 * W, D == 256 ? 1 : 2) void attn8_chunk_kernel(Kv8AttnArgs a, float* __restrict__ part) {
@@ -882,7 +882,7 @@ __global__ __launch_bounds__(256) void attn8_join_tiles_kernel(Kv8AttnArgs a, fl
 // As many waves a SIMD as the outputs and q's parts (128 + 64 registers at D = 256) leave room for,
 // 2, 3 and 4 at 256, 128 and 64 dims; one's products run beside the others' softmax, so that a
 // wave's own steps stay in order. 8,192 tokens of 16 query heads over 2 of 256 dims: one wave a
-// SIMD with the steps of two blocks side by side 665 us, two 483; products and softmax of half
+// SIMD with the steps of two blocks side by side 665 us, two 483 (483 to 523 by box); products and softmax of half
 // the waves in turn, by barriers, were as fast (508, where the rest took 500). At that rate (1.1
 // PFLOP/s, a quarter of the matrix time on top for the scores' second part) the clock, not a unit,
 // is what gives: the f16 products alone run at 1.6 GHz on such numbers, and at 2.2 on constants.

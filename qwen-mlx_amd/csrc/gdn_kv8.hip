@@ -134,8 +134,10 @@ __device__ __forceinline__ void map_token(const Kv8Plan& p, const int32_t* cu, i
 constexpr int kMapHere = 8192;
 
 // One work-group: prefix sums over the rows (R consecutive rows a thread), pages given
-// back, then pages taken, both in row order. Bound by latency: a load of the rows, five
-// scans and the tables' round trips; 64 rows 5 us, 700 rows 7.
+// back, then pages taken, both in row order. Bound by latency: a load of the rows, four or five
+// scans and the tables' round trips, and where pages move a load and a store for each row of a
+// wave in turn. 64 rows that move none 4.9 us, a page each 6.8, 16 each 18.6, 65 each 25.6; 700 rows
+// that move none 6.2, 4,185 pages 13.3.
 template <int TH, int R>
 __global__ __launch_bounds__(TH) void kv8_plan_kernel(Kv8Plan p, const int32_t* __restrict__ slots,
                                                       const int32_t* lens,
@@ -348,8 +350,9 @@ __device__ __forceinline__ uint32_t again4(uint32_t w, float f) {
 // whole; otherwise only the new rows' bytes are. An item is 4 keys x 8 dims: 8 bytes of each
 // key in K's order, a word of 4 keys for each dim in V's. Bound by latency: the tables, the exponent,
 // the old bytes and a barrier one after the other. 64 single tokens of 2 heads of 256 dims 8 us,
-// 2,899 tokens of 8 heads of 128 dims 12 us (18 MB). Element by element, every page written
-// whole, the 64 tokens took 27 us with a gather of them, where this takes 12.
+// 9.3 where every page is rewritten; 2,899 tokens of 8 heads of 128 dims 10 to 12 us (18 MB). Element
+// by element, every page written whole, the 64 tokens took 27 us with a gather of them, where this
+// takes 12.
 template <int D>
 __global__ __launch_bounds__(256) void kv8_append_kernel(Kv8AppendArgs a) {
   constexpr int kChunks = D / 8, kItems = 16 * kChunks, kPer = (kItems + 255) / 256;

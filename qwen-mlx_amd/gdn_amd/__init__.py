@@ -941,7 +941,8 @@ class KV8Cache:
                   window: int = 0, slopes=None, prefix=None, gate=None, stream=None):
         """Attention of the step's tokens over their sequences' keys (gdn_kv8_attention): q,
         out and gate [tokens, query heads, dim] bf16 (heads or columns of wider tensors are
-        fine), slopes f32 [query heads], prefix int32 [rows]. scale 0: 1 / sqrt(dim)."""
+        fine), slopes f32 [query heads], prefix int32 [rows]. scale 0: 1 / sqrt(dim); softcap 0
+        or 1e-30 .. 1e30."""
         dev = self.device
         size = (self.tokens, self.Hq, self.D)
         qp, qs, qh = _heads(q, dev, size, _IS_BF16, "q")
